@@ -568,6 +568,84 @@ int ll_unipc_step(const void* flow, const void* sample, const void* last, const 
                   const ll_unipc_scalars* corrector, const ll_unipc_scalars* predictor, void* converted, void* corrected, void* next,
                   void* stream);
 
+/*
+ * Several streams (requests) served in one batch.  Their new tokens lie one stream behind the other, stream b in rows
+ * q_starts[b] .. q_starts[b + 1] - 1; lengths, starts and page tables are device memory, read when the launch runs (a recorded
+ * launch follows what they hold at the replay).  None of the three has a counterpart in the reference, whose attention works on
+ * one sequence at a time (wan_5b/modules/causal_model.py:298-791).  dtype: LL_DTYPE_BF16 or LL_DTYPE_F16.
+ *
+ * ll_head_norm_rope: every head of q and k through its own RMS norm and the position rotation, K and V on to the rows of a paged
+ * cache, in one pass.  With y = x * rsqrt(mean(x^2) + eps) * weight (y = x without a weight) and the angles' row p =
+ * positions[t] (row t without positions), pairs (a, b) of the first rotary_dim columns become
+ *   (a cos[p, j] - b sin[p, j], b cos[p, j] + a sin[p, j]),  j < rotary_dim / 2;
+ * pair j is columns (2j, 2j + 1) when interleaved, else (j, j + rotary_dim / 2).  fp32 throughout, rounded once.  Rows whose p
+ * lies outside the table are normed and not rotated.  rotary_dim 0: no rotation.
+ */
+typedef struct ll_head_rows { /* the q, k or v of a batch of tokens */
+  const void* x;              /* [tokens, num_heads, head_dim]; strides in elements, the last dimension contiguous */
+  int64_t stride_token, stride_head;
+  int num_heads;              /* 0: there is none */
+  const void* weight;         /* [head_dim] or NULL: no norm.  Always NULL for v, which is copied */
+  int weight_f32;             /* the weight is fp32 rather than of the rows' type */
+  void* out;                  /* row t of the result goes to out + t * out_stride_token, with slots for k and v: slots[t] */
+  int64_t out_stride_token, out_stride_head;
+} ll_head_rows;
+/* tokens rows; head_dim a multiple of 8 up to 256, rotary_dim one up to head_dim; pointers 16-byte aligned, strides multiples of 8;
+ * cos, sin f32 [table_rows, rotary_dim / 2], contiguous; positions int64 [tokens] or NULL.  slots int64 [tokens] or NULL: where
+ * the k and v rows of token t go, nowhere if outside 0 .. n_slots - 1; two tokens with one slot leave either's values there.  q.out
+ * may be q.x, and without slots k.out k.x; apart from that outputs must not overlap inputs.  v.num_heads is 0 without slots. */
+int ll_head_norm_rope(int dtype, int64_t tokens, int head_dim, const ll_head_rows* q, const ll_head_rows* k, const ll_head_rows* v,
+                      float eps, const float* cos, const float* sin, int64_t table_rows, int rotary_dim, const int64_t* positions,
+                      int interleaved, const int64_t* slots, int64_t n_slots, void* stream);
+
+/*
+ * ll_ragged_attention: out[t, h] = sum_j w_j v_j / sum_j w_j,  w_j = exp(softmax_scale * (q[t, h] . k_j - max)), over the keys
+ * of t's stream that t may see; zeros for a row that sees none.  Head h reads kv head h / (num_heads / num_kv_heads).  Rows of q
+ * outside every stream get zeros (clear_rest) or stay as they are.  Keys:
+ *   page_table given: stream b's key j < kv_lens[b] is row j % page_size of page page_table[b, j / page_size]; entries outside
+ *     0 .. n_pages - 1 are holes, whose keys nobody sees, and so is what lies behind the table's width.  The stream's new tokens are
+ *     its last keys: row i of n sits at position p = kv_lens[b] - n + i and sees key j where (j <= p, if causal) and (j > p - window
+ *     or j < sink_keys, if window > 0).
+ *   else: rows k_starts[b] + j of k and v, j < k_lens[b], or without k_lens up to k_starts[b + 1]; within n_keys; key_mask (one
+ *     byte a row, or NULL) leaves out keys whose byte is zero.  Every row sees all of them; causal and window are 0.
+ * Whatever lies in K and V where no row of a launch's stream may look (unfilled rows of a page, masked states) has no part in
+ * the result, NaN included.
+ * max_q_len, max_kv_len: the longest stream's new tokens and keys as far as the host knows them, by which the launch is divided;
+ * right for any value, fast for true ones.  workspace: ll_ragged_attention_workspace bytes, 16-byte aligned, used by this launch
+ * alone while it runs (NULL where that is 0).
+ */
+typedef struct ll_ragged_attention_args {
+  int dtype, head_dim;        /* head_dim 64 or 128 */
+  int num_heads, num_kv_heads;
+  int64_t n_queries;
+  const void* q;              /* [n_queries, num_heads, head_dim], strides in elements */
+  int64_t q_stride_token, q_stride_head;
+  void* out;                  /* [n_queries, num_heads, head_dim] */
+  int64_t out_stride_token, out_stride_head;
+  int64_t streams;
+  const int32_t* q_starts;    /* [streams + 1] */
+  int clear_rest;
+  float softmax_scale;        /* > 0 */
+  const void *k, *v;          /* [n_pages, page_size, num_kv_heads, head_dim] or [n_keys, num_kv_heads, head_dim] */
+  int64_t k_stride_page, k_stride_row, k_stride_head, v_stride_page, v_stride_row, v_stride_head;
+  const int32_t* page_table;  /* [streams, table_width], rows table_stride apart; NULL: keys by k_starts */
+  int64_t table_stride, table_width, n_pages;
+  int page_size;
+  const int32_t* kv_lens;     /* [streams] */
+  int causal;
+  int64_t window, sink_keys;  /* window 0: none */
+  const int32_t *k_starts, *k_lens;
+  const uint8_t* key_mask;
+  int64_t n_keys;
+  int64_t max_q_len, max_kv_len;
+  void* workspace;
+  size_t workspace_bytes;
+} ll_ragged_attention_args;
+/* Bytes of workspace that ll_ragged_attention needs for these arguments (pointers are not looked at) on a device of
+ * `compute_units` (host arithmetic only), or, if 0, on the current device. */
+int ll_ragged_attention_workspace(const ll_ragged_attention_args* args, int compute_units, size_t* bytes);
+int ll_ragged_attention(const ll_ragged_attention_args* args, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

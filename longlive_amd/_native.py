@@ -115,6 +115,10 @@ _SIGNATURES = {
     "ll_kv_attention_reserve": (c_int, [c_int64, c_int, c_int64, c_void_p]),
     "ll_kv_attention_reserve_window": (c_int, [c_int64, c_int, c_int64, c_int64, c_void_p]),
     "ll_kv_attention_release": (c_int, [c_void_p]),
+    "ll_head_norm_rope": (c_int, [c_int, c_int64, c_int, c_void_p, c_void_p, c_void_p, c_float, c_void_p, c_void_p, c_int64, c_int, c_void_p,
+                                  c_int, c_void_p, c_int64, c_void_p]),
+    "ll_ragged_attention": (c_int, [c_void_p, c_void_p]),
+    "ll_ragged_attention_workspace": (c_int, [c_void_p, c_int, c_void_p]),
     "ll_nvfp4_quantize_noalloc_max_elements": (c_int64, []),
     "ll_nvfp4_quantize_noalloc": (c_int, [c_void_p, c_int64, c_int64, c_int64, c_int, c_void_p, c_void_p, c_void_p,
                                           c_void_p]),
@@ -994,3 +998,215 @@ def layer_norm(x, weight, bias, eps=1e-6, amax_out=None):
                                     ctypes.byref(sink), _stream())
     _check(code, "ll_layer_norm")
     return out.view(x.shape)
+
+
+# --------------------------------------------------------------------------- several streams in one batch
+class HeadRowsStruct(ctypes.Structure):
+    """struct ll_head_rows of include/ll_nvfp4.h."""
+    _fields_ = [("x", c_void_p), ("stride_token", c_int64), ("stride_head", c_int64), ("num_heads", c_int), ("weight", c_void_p),
+                ("weight_f32", c_int), ("out", c_void_p), ("out_stride_token", c_int64), ("out_stride_head", c_int64)]
+
+
+class RaggedAttentionStruct(ctypes.Structure):
+    """struct ll_ragged_attention_args of include/ll_nvfp4.h."""
+    _fields_ = [("dtype", c_int), ("head_dim", c_int), ("num_heads", c_int), ("num_kv_heads", c_int), ("n_queries", c_int64),
+                ("q", c_void_p), ("q_stride_token", c_int64), ("q_stride_head", c_int64),
+                ("out", c_void_p), ("out_stride_token", c_int64), ("out_stride_head", c_int64),
+                ("streams", c_int64), ("q_starts", c_void_p), ("clear_rest", c_int), ("softmax_scale", c_float),
+                ("k", c_void_p), ("v", c_void_p), ("k_stride_page", c_int64), ("k_stride_row", c_int64), ("k_stride_head", c_int64),
+                ("v_stride_page", c_int64), ("v_stride_row", c_int64), ("v_stride_head", c_int64),
+                ("page_table", c_void_p), ("table_stride", c_int64), ("table_width", c_int64), ("n_pages", c_int64), ("page_size", c_int),
+                ("kv_lens", c_void_p), ("causal", c_int), ("window", c_int64), ("sink_keys", c_int64),
+                ("k_starts", c_void_p), ("k_lens", c_void_p), ("key_mask", c_void_p), ("n_keys", c_int64),
+                ("max_q_len", c_int64), ("max_kv_len", c_int64), ("workspace", c_void_p), ("workspace_bytes", c_size_t)]
+
+
+def _one_device(what: str, *tensors) -> None:
+    """All of them on the GPU, and on the same one."""
+    _require_cuda(*tensors)
+    devices = {t.device for t in tensors if t is not None}
+    if len(devices) > 1:
+        raise ValueError(f"{what}: tensors on several devices: {sorted(map(str, devices))}")
+
+
+def _rows16(t: torch.Tensor) -> bool:
+    """Whether rows of 16-byte pieces can be read from a tensor of 16-bit values where it lies."""
+    return t.stride(-1) == 1 and t.data_ptr() % 16 == 0 and all(s % 8 == 0 for n, s in zip(t.shape[:-1], t.stride()) if n > 1)
+
+
+def _check_rows(what: str, name: str, t: torch.Tensor, dtype=None) -> None:
+    if t.ndim != 3 or t.dtype not in (torch.bfloat16, torch.float16) or (dtype is not None and t.dtype != dtype):
+        raise ValueError(f"{what}: {name} must be [rows, heads, head_dim] in bfloat16 or float16, all tensors in one type; got "
+                         f"{t.dtype} {tuple(t.shape)}")
+
+
+def _check_index(what: str, name: str, t: torch.Tensor, dtype, shape) -> None:
+    if t.dtype != dtype or tuple(t.shape) != tuple(shape) or not t.is_contiguous():
+        raise ValueError(f"{what}: {name} must be a contiguous {dtype} tensor of shape {tuple(shape)}; got {t.dtype} {tuple(t.shape)}")
+
+
+def _check_out(what: str, out: torch.Tensor, like: torch.Tensor) -> None:
+    if out.shape != like.shape or out.dtype != like.dtype or not _rows16(out):
+        raise ValueError(f"{what}: out must be a {like.dtype} tensor of shape {tuple(like.shape)} with whole, 16-byte aligned rows")
+
+
+def check_pages(what: str, cache: dict) -> tuple[torch.Tensor, torch.Tensor]:
+    """The K and V pages of a paged cache, which are used where they lie."""
+    k, v = cache["k_pages"], cache["v_pages"]
+    for name, t in (("k_pages", k), ("v_pages", v)):
+        if t.ndim != 4 or t.dtype not in (torch.bfloat16, torch.float16) or t.shape != k.shape or t.dtype != k.dtype:
+            raise ValueError(f"{what}: k_pages and v_pages must be [pages, page_size, heads, head_dim] in bfloat16 or float16, both alike")
+        if t.numel() and not _rows16(t):
+            raise ValueError(f"{what}: {name} must have contiguous, 16-byte aligned rows")
+    if k.shape[1] < 1:
+        raise ValueError(f"{what}: pages hold at least one row")
+    return k, v
+
+
+def _head_rows(x, weight, out, out_strides) -> HeadRowsStruct:
+    return HeadRowsStruct(x.data_ptr(), x.stride(0), x.stride(1), x.shape[1], _ptr(weight),
+                          int(weight is not None and weight.dtype == torch.float32), out.data_ptr(), *out_strides)
+
+
+def head_norm_rope(q, k, v, q_weight, k_weight, eps, cos, sin, positions, interleaved, cache=None, slots=None, q_out=None):
+    """q [T, Hq, D], k [T, Hk, D] through a norm per head and the rotation: (q, k) in fresh tensors, or with a paged ``cache`` q alone, k
+    and v [T, Hk, D] then going to the cache's rows ``slots``."""
+    what = "head_norm_rope"
+    paged = cache is not None
+    pages = check_pages(what, cache) if paged else ()
+    _one_device(what, q, k, v, q_weight, k_weight, cos, sin, positions, slots, q_out, *pages)
+    T, Hq, D = (*q.shape, 0, 0, 0)[:3]
+    for name, t in (("q", q), ("k", k)) + ((("v", v),) if paged else ()):
+        _check_rows(what, name, t, q.dtype)
+        if t.shape[0] != T or t.shape[2] != D or (name == "v" and t.shape != k.shape):
+            raise ValueError(f"{what}: q, k and v must have as many rows, one head_dim, and k and v as many heads; got {tuple(t.shape)} for {name} "
+                             f"beside q {tuple(q.shape)}, k {tuple(k.shape)}")
+    if D % 8 or not 8 <= D <= 256:
+        raise ValueError(f"{what}: head_dim {D} is not a multiple of 8 up to 256")
+    for name, w in (("q_weight", q_weight), ("k_weight", k_weight)):
+        if w is not None and (w.shape != (D,) or w.dtype not in (q.dtype, torch.float32)):
+            raise ValueError(f"{what}: {name} must be [{D}] in {q.dtype} or float32")
+    if (cos is None) != (sin is None):
+        raise ValueError(f"{what}: cos and sin go together")
+    R, table = 0, 0
+    if cos is not None:
+        if cos.ndim != 2 or cos.shape != sin.shape or cos.dtype != torch.float32 or sin.dtype != torch.float32:
+            raise ValueError(f"{what}: cos and sin must be float32 [positions, rotated columns / 2]")
+        table, R = cos.shape[0], 2 * cos.shape[1]
+        if R % 8 or R > D:
+            raise ValueError(f"{what}: {R} rotated columns are not a multiple of 8 up to head_dim {D}")
+        cos, sin = cos.contiguous(), sin.contiguous()
+        if cos.data_ptr() % 16 or sin.data_ptr() % 16:
+            cos, sin = cos.clone(), sin.clone()
+    if positions is not None:
+        _check_index(what, "positions", positions, torch.int64, (T,))
+    q, k = (t if _rows16(t) else t.contiguous().clone() for t in (q, k))
+    q_weight, k_weight = (w if w is None or (w.is_contiguous() and w.data_ptr() % 16 == 0) else w.contiguous().clone() for w in (q_weight, k_weight))
+    if q_out is None:
+        q_out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+    else:
+        _check_out(what, q_out, q)
+    v_rows, n_slots = None, 0
+    if paged:
+        k_pages, v_pages = pages
+        if k_pages.shape[2:] != k.shape[1:] or k_pages.dtype != q.dtype:
+            raise ValueError(f"{what}: pages of {k_pages.dtype} {tuple(k_pages.shape[2:])} do not take rows of {q.dtype} {tuple(k.shape[1:])}")
+        if any(t.numel() and t.stride(0) != t.shape[1] * t.stride(1) for t in pages):
+            raise ValueError(f"{what}: pages must lie one behind the other")
+        _check_index(what, "slots", slots, torch.int64, (T,))
+        v = v if _rows16(v) else v.contiguous().clone()
+        n_slots = k_pages.shape[0] * k_pages.shape[1]
+        k_rows = _head_rows(k, k_weight, k_pages, k_pages.stride()[1:3])
+        v_rows = _head_rows(v, None, v_pages, v_pages.stride()[1:3])
+        k_out = None
+    else:
+        k_out = torch.empty(k.shape, dtype=k.dtype, device=k.device)
+        k_rows = _head_rows(k, k_weight, k_out, k_out.stride()[:2])
+    if T == 0:
+        return q_out if paged else (q_out, k_out)
+    q_rows = _head_rows(q, q_weight, q_out, q_out.stride()[:2])
+    if n_slots == 0 and paged:   # a cache without pages: nothing to write to
+        k_rows.num_heads, v_rows = 0, None
+    with torch.cuda.device(q.device):
+        code = load().ll_head_norm_rope(DTYPE_CODES[q.dtype], T, D, ctypes.byref(q_rows), ctypes.byref(k_rows),
+                                        None if v_rows is None else ctypes.byref(v_rows), float(eps), _ptr(cos), _ptr(sin), table, R,
+                                        _ptr(positions), int(interleaved), _ptr(slots), n_slots, _stream())
+    _check(code, "ll_head_norm_rope")
+    return q_out if paged else (q_out, k_out)
+
+
+def ragged_attention(what, q, q_starts, softmax_scale, max_q_len, max_kv_len, out, *, cache=None, page_table=None, kv_lens=None, causal=False,
+                     window=None, sink_tokens=0, k=None, v=None, k_starts=None, k_lens=None, key_mask=None):
+    """The queries q [T, H, D] of several streams over the keys of a paged ``cache`` or over rows of k and v [n, Hk, D]
+    (``ll_ragged_attention``)."""
+    pages = check_pages(what, cache) if cache is not None else ()
+    _one_device(what, q, q_starts, out, page_table, kv_lens, k, v, k_starts, k_lens, key_mask, *pages)
+    _check_rows(what, "q", q)
+    T, H, D = q.shape
+    if D not in (64, 128):
+        raise ValueError(f"{what}: head_dim {D} is not 64 or 128")
+    streams = q_starts.numel() - 1
+    if streams < 0:
+        raise ValueError(f"{what}: q_starts must have one entry more than there are streams")
+    _check_index(what, "q_starts", q_starts, torch.int32, (streams + 1,))
+    scale = D ** -0.5 if softmax_scale is None else float(softmax_scale)
+    if not 0.0 < scale < float("inf"):
+        raise ValueError(f"{what}: softmax_scale {scale} is not a positive number")
+    for name, n in (("max_q_len", max_q_len), ("max_kv_len", max_kv_len), ("window", window), ("sink_tokens", sink_tokens)):
+        if n is not None and (int(n) != n or n < 0 or (name == "window" and n < 1)):
+            raise ValueError(f"{what}: {name} {n}")
+    a = RaggedAttentionStruct(dtype=DTYPE_CODES[q.dtype], head_dim=D, num_heads=H, n_queries=T, streams=streams, softmax_scale=scale,
+                              max_q_len=max_q_len or 0, max_kv_len=max_kv_len or 0)
+    q = q if _rows16(q) else q.contiguous().clone()
+    if cache is not None:
+        k, v = pages
+        _check_index(what, "kv_lens", kv_lens, torch.int32, (streams,))
+        if page_table.dtype != torch.int32 or page_table.ndim != 2 or page_table.shape[0] != streams or (page_table.numel() and page_table.stride(1) != 1):
+            raise ValueError(f"{what}: page_table must be int32 [{streams}, pages of the longest stream] with contiguous rows")
+        a.page_table, a.table_stride, a.table_width = page_table.data_ptr(), page_table.stride(0), page_table.shape[1]
+        a.n_pages, a.page_size, a.kv_lens, a.causal = k.shape[0], k.shape[1], kv_lens.data_ptr(), int(bool(causal))
+        a.window, a.sink_keys = window or 0, sink_tokens
+        a.k_stride_page, a.k_stride_row, a.k_stride_head = k.stride()[:3]
+        a.v_stride_page, a.v_stride_row, a.v_stride_head = v.stride()[:3]
+        if a.table_width * a.page_size >= 1 << 31:
+            raise ValueError(f"{what}: a table of {a.table_width} pages of {a.page_size} rows reaches beyond 2^31 keys")
+    else:
+        _check_rows(what, "k", k, q.dtype)
+        _check_rows(what, "v", v, q.dtype)
+        if k.shape != v.shape:
+            raise ValueError(f"{what}: k {tuple(k.shape)} and v {tuple(v.shape)} must be of one shape")
+        if k_lens is None:
+            _check_index(what, "k_starts", k_starts, torch.int32, (streams + 1,))
+        else:
+            if k_starts.ndim != 1 or k_starts.numel() < streams:
+                raise ValueError(f"{what}: k_starts must have an entry for each of {streams} streams")
+            _check_index(what, "k_starts", k_starts, torch.int32, k_starts.shape)
+            _check_index(what, "k_lens", k_lens, torch.int32, (streams,))
+        if key_mask is not None:
+            _check_index(what, "key_mask", key_mask, torch.bool, (k.shape[0],))
+        k, v = (t if _rows16(t) else t.contiguous().clone() for t in (k, v))
+        a.k_starts, a.k_lens, a.key_mask, a.n_keys = k_starts.data_ptr(), _ptr(k_lens), _ptr(key_mask), k.shape[0]
+        a.k_stride_row, a.k_stride_head = k.stride()[:2]
+        a.v_stride_row, a.v_stride_head = v.stride()[:2]
+    if k.shape[-1] != D or k.dtype != q.dtype or k.shape[-2] == 0 or H % k.shape[-2]:
+        raise ValueError(f"{what}: q of {q.dtype} {tuple(q.shape)} does not go with keys of {k.dtype} {tuple(k.shape)}")
+    a.num_kv_heads = k.shape[-2]
+    a.clear_rest = int(out is None)
+    if out is None:
+        out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+    else:
+        _check_out(what, out, q)
+    if T == 0 or H == 0:
+        return out
+    a.q, a.q_starts, a.out, a.k, a.v = q.data_ptr(), q_starts.data_ptr(), out.data_ptr(), k.data_ptr(), v.data_ptr()
+    a.q_stride_token, a.q_stride_head = q.stride()[:2]
+    a.out_stride_token, a.out_stride_head = out.stride()[:2]
+    with torch.cuda.device(q.device):
+        lib, need = load(), c_size_t()
+        _check(lib.ll_ragged_attention_workspace(ctypes.byref(a), 0, ctypes.byref(need)), what)
+        if need.value:
+            workspace = torch.empty(need.value, dtype=torch.uint8, device=q.device)
+            a.workspace, a.workspace_bytes = workspace.data_ptr(), need.value
+        code = lib.ll_ragged_attention(ctypes.byref(a), _stream())
+    _check(code, what)
+    return out

@@ -83,5 +83,20 @@ def rope_apply(x: torch.Tensor, cos_f32: torch.Tensor, sin_f32: torch.Tensor, se
     return _native.rope_apply(x, cos_f32, sin_f32, seq_len)
 
 
+def head_norm_rope(q: torch.Tensor, k: torch.Tensor, q_weight: torch.Tensor | None, k_weight: torch.Tensor | None, eps: float,
+                   cos_f32: torch.Tensor | None, sin_f32: torch.Tensor | None, positions: torch.Tensor | None = None,
+                   interleaved: bool = True) -> tuple[torch.Tensor, torch.Tensor]:
+    """RMS norm of every head of q [T, Hq, D] and k [T, Hk, D] and the rotation of its first ``2 * cos.shape[1]`` columns in one
+    pass: ``y = x * rsqrt(mean(x^2) + eps) * weight`` over the D columns of a head, then pairs (2j, 2j + 1), or with
+    ``interleaved=False`` (j, j + half the rotated columns), turned by the angles' row ``positions[t]`` (row t without positions).
+    fp32 throughout, rounded once.  Returns new (q, k).
+
+    bfloat16 or float16, D and the rotated columns multiples of 8, D up to 256; q and k may be views of one projection's rows.
+    A weight ([D], of the rows' type or float32) of None: no norm; cos and sin (float32 [positions, rotated / 2]) of None: no
+    rotation.  Rows whose position (int64) lies outside the table are normed and not rotated.  Where the norm runs over whole
+    rows of all heads, as in the reference's model, ``_native.qk_norm_rope_pair`` is the call."""
+    return _native.head_norm_rope(q, k, None, q_weight, k_weight, eps, cos_f32, sin_f32, positions, interleaved)
+
+
 # the reference's name for the same entry point
 rope_apply_triton = rope_apply
