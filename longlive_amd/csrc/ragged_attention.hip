@@ -3,15 +3,27 @@
 //
 //   out[t, h] = sum_j w_j v_j / sum_j w_j,   w_j = exp(scale * (q[t, h] . k_j - max)),   j over the keys that row t may see
 //
-// The rows of a kv head's queries, (token, head of the group) one behind the other, are cut into tiles of 128.  A workgroup of
-// four waves walks the keys of a tile 64 at a time: K and V come into LDS, every wave multiplies them with its own 32 rows,
+// The rows of a kv head's queries, (token, head of the group) one behind the other, are cut into tiles of 128; the launch has as
+// many workgroups of four waves per kv head as there can be tiles, and each finds its own by a prefix sum over the streams.  A
+// workgroup multiplies
 //   S^T = K Q^T  and  O^T = V^T P^T   (v_mfma_f32_32x32x16),
 // so that a lane owns one row: its maximum and sum need one exchange between the wave's halves, its mask two comparisons per
 // score with bounds of its own, and its rescaling is a multiplication by a scalar.  The probabilities leave the first product in
 // the registers in which the second one wants them, keys permuted; V^T is read permuted alike by the LDS read that transposes.
+//
+//   * Tiles of more than 32 rows: a wave owns 32 rows, and all four walk the same keys, 64 a step, through two stages in LDS.
+//   * Tiles of up to 32 rows (single tokens, drafts): all waves own the same rows, and each walks every fourth group of 32 keys
+//     with LDS of its own and no barrier, K of the next group on its way from the moment the scores are done, V from the moment
+//     they are used; the four results are merged at the end.
+//   * Long key ranges are cut into parts of p.part_steps steps, a workgroup each, whose results a second launch joins in order.
+//
+// K and V go straight from memory to LDS, 1024 bytes a load.  Where the rows lie is looked up one step ahead, an entry of the
+// page table per lane, also straight to LDS, so that no register load stands between the loads under way and their wait.
 #include "ll_types16.h"
 
+#include <algorithm>
 #include <cmath>
+#include <type_traits>
 
 namespace ll {
 
@@ -20,28 +32,39 @@ constexpr int kRaTileRows = 128;  // rows of a workgroup, 32 a wave
 constexpr int kRaKeys = 64;       // keys of a step
 constexpr int kRaClearGroups = 16;
 
+// Where keys lie: in the pages of a table, in rows one behind the other, in such rows with a mask.
+constexpr int kRaPaged = 0, kRaRows = 1, kRaMaskedRows = 2;
+
 struct RaParams {
   const uint16_t* q;
   uint16_t* out;
   int64_t q_stride_token, q_stride_head, out_stride_token, out_stride_head;
-  int64_t n_queries, streams;
+  int64_t n_queries;
+  int streams;
   const int32_t* q_starts;
   const uint16_t *k, *v;
-  int64_t k_stride_page, k_stride_row, k_stride_head, v_stride_page, v_stride_row, v_stride_head;
+  int64_t k_stride_head, v_stride_head;
+  uint32_t k_stride_page, k_stride_row, v_stride_page, v_stride_row;
   const int32_t* page_table;
-  int64_t table_stride, table_keys;  // keys that a stream's row of the table reaches
+  int64_t table_stride;
+  int64_t table_keys;  // keys that a stream's row of the table reaches
   uint32_t n_pages;
   Divisor page;
   const int32_t *kv_lens, *k_starts, *k_lens;
   const uint8_t* key_mask;
   int64_t n_keys;
   float scale_log2;
-  int causal, clear_rest;
+  int causal;
   int heads, kv_heads;
-  Divisor group;       // heads of a kv head
-  int64_t window, sink;
-  uint32_t tiles;      // workgroups of a (stream, kv head); each takes every tiles-th tile
-  uint32_t work_groups;
+  Divisor group;          // heads of a kv head
+  uint32_t window, sink;  // window 0: none
+  uint32_t tiles;         // workgroups per kv head and part: no fewer than there are tiles
+  uint32_t parts;         // workgroups that a tile's keys are cut for
+  uint32_t part_steps;    // steps of a part; the last takes what is left
+  uint32_t record_rows;   // tiles of more rows are not cut
+  uint32_t work_groups;   // tiles * parts * kv_heads
+  int by_head;            // an XCD's workgroups are neighbours in the order head, tile, part
+  float* records;         // [kv head][tile][part]: record_rows x (D + 2) floats
 };
 
 // Positions of 16-byte pieces in an LDS row of D columns.  The reads of a wave then go through all banks: 8 neighbouring rows of one
@@ -66,42 +89,145 @@ __device__ __forceinline__ float exchange_sum(float v) {
   return __uint_as_float(r[0]) + __uint_as_float(r[1]);
 }
 
-// The keys of a stream.
-struct Keys {
-  int64_t len;              // keys 0 .. len - 1
-  int64_t start;            // ragged: row of key 0
-  const int32_t* pages;     // paged: the stream's row of the table
+// 16 or 4 bytes per lane from memory straight into LDS at lds + 16 (4) * lane.  asm statements, so that the compiler does not wait
+// for them ahead of LDS reads of other data; wait_loads does.
+__device__ __forceinline__ void load16_to_lds(uint32_t offset, const void* base, uint32_t lds) {
+  asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %1" ::"v"(offset), "s"(base), "s"(__builtin_amdgcn_readfirstlane(lds)) : "memory");
+}
+__device__ __forceinline__ void load16_to_lds(const void* from, uint32_t lds) {
+  asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, off" ::"v"(from), "s"(__builtin_amdgcn_readfirstlane(lds)) : "memory");
+}
+__device__ __forceinline__ void load4_to_lds(const void* from, uint32_t lds) {
+  asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dword %0, off" ::"v"(from), "s"(__builtin_amdgcn_readfirstlane(lds)) : "memory");
+}
+// All but the last N loads of this wave have arrived.
+template <int N>
+__device__ __forceinline__ void wait_loads() {
+  asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory");
+}
+// This wave's LDS reads have their data: what they read may be overwritten.
+__device__ __forceinline__ void wait_lds_reads() { asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory"); }
+__device__ __forceinline__ uint32_t lds_at(const void* p) {
+  return __builtin_amdgcn_readfirstlane((uint32_t)(uintptr_t)(__attribute__((address_space(3))) const void*)p);
+}
+template <typename P>
+__device__ __forceinline__ const P* uniform_pointer(const P* p) {
+  const uint64_t v = (uint64_t)(uintptr_t)p;
+  const uint32_t lo = __builtin_amdgcn_readfirstlane((uint32_t)v), hi = __builtin_amdgcn_readfirstlane((uint32_t)(v >> 32));
+  return reinterpret_cast<const P*>((uintptr_t)(((uint64_t)hi << 32) | lo));
+}
+
+// What rows of keys that do not exist are read from.
+__device__ const uint4 kRaZeros[1] = {{0, 0, 0, 0}};
+
+__device__ __forceinline__ int64_t stream_start(const RaParams& p, int b) { return min(max((int64_t)p.q_starts[b], (int64_t)0), p.n_queries); }
+
+// The tile of a workgroup.
+struct RaTile {
+  int stream;
+  int64_t q0;           // first row of q of the stream
+  int n, rows, first;   // tokens of the stream; rows of the stream (token, head of the group), the tile's first
+  int len;              // keys of the stream
+  int64_t key0;         // rows of keys: row of key 0
+  const int32_t* pages; // paged: the stream's row of the table
+  // keys: steps 0 .. sink_steps - 1 and then from from_step on, n_steps in all
+  int sink_steps, from_step, n_steps;
+  int n_parts;          // workgroups that share the keys
 };
 
-// Whether key j exists and, if so, its row's offset in K and V.
-template <bool PAGED>
-__device__ __forceinline__ bool find_key(const RaParams& p, const Keys& keys, int64_t j, int64_t& k_at, int64_t& v_at) {
-  if (j < 0 || j >= keys.len) return false;
-  if constexpr (PAGED) {
-    const uint32_t page = (uint32_t)j / p.page, row = (uint32_t)j - page * p.page.d;
-    const uint32_t entry = (uint32_t)keys.pages[page];
-    if (entry >= p.n_pages) return false;
-    k_at = (int64_t)entry * p.k_stride_page + row * p.k_stride_row;
-    v_at = (int64_t)entry * p.v_stride_page + row * p.v_stride_row;
-  } else {
-    const int64_t row = keys.start + j;
-    if (p.key_mask && p.key_mask[row] == 0) return false;
-    k_at = row * p.k_stride_row;
-    v_at = row * p.v_stride_row;
+// Tile `index` of the tiles of a kv head: the streams' tiles one behind the other, the last of a stream (which sees most keys) first.
+// All lanes call it together.  False: there are fewer.
+template <int KIND>
+__device__ __forceinline__ bool find_tile(const RaParams& p, uint32_t index, RaTile& t) {
+  const int lane = threadIdx.x & 63;
+  t.stream = -1;
+  for (int b0 = 0; b0 < p.streams; b0 += 64) {
+    int mine = 0;
+    if (b0 + lane < p.streams) {
+      const int64_t n = stream_start(p, b0 + lane + 1) - stream_start(p, b0 + lane);
+      mine = n > 0 ? (int)((n * p.group.d + kRaTileRows - 1) / kRaTileRows) : 0;
+    }
+    int upto = mine;
+#pragma unroll
+    for (int d = 1; d < 64; d *= 2) {
+      const int other = __shfl_up(upto, d);
+      if (lane >= d) upto += other;
+    }
+    const uint64_t before = __builtin_amdgcn_ballot_w64((uint32_t)upto <= index);
+    if (before != ~0ull) {
+      const int at = __popcll(before);
+      t.stream = b0 + at;
+      t.first = (__builtin_amdgcn_readlane(upto, at) - 1 - (int)index) * kRaTileRows;
+      break;
+    }
+    index -= (uint32_t)__builtin_amdgcn_readlane(upto, 63);
   }
+  if (t.stream < 0) return false;
+  t.stream = __builtin_amdgcn_readfirstlane(t.stream);
+  t.first = __builtin_amdgcn_readfirstlane(t.first);
+  t.q0 = stream_start(p, t.stream);
+  t.n = (int)(stream_start(p, t.stream + 1) - t.q0);
+  t.rows = t.n * (int)p.group.d;
+  t.pages = nullptr;
+  t.key0 = 0;
+  if constexpr (KIND == kRaPaged) {
+    t.len = (int)min(max((int64_t)p.kv_lens[t.stream], (int64_t)0), p.table_keys);
+    t.pages = p.page_table + t.stream * p.table_stride;
+  } else {
+    t.key0 = min(max((int64_t)p.k_starts[t.stream], (int64_t)0), p.n_keys);
+    const int64_t len = p.k_lens ? (int64_t)p.k_lens[t.stream] : (int64_t)p.k_starts[t.stream + 1] - t.key0;
+    t.len = (int)min(max(len, (int64_t)0), p.n_keys - t.key0);
+  }
+  const int last_row = min(t.first + kRaTileRows, t.rows) - 1;
+  const int pos0 = t.len - t.n + (int)((uint32_t)t.first / p.group), pos1 = t.len - t.n + (int)((uint32_t)last_row / p.group);
+  const int end = p.causal ? min(pos1 + 1, t.len) : t.len;
+  const int from = p.window && pos0 >= (int)p.window ? pos0 - (int)p.window + 1 : 0;
+  const int end_step = end > 0 ? (end - 1) / kRaKeys + 1 : 0;
+  t.from_step = from / kRaKeys;
+  t.sink_steps = min((int)(((int64_t)min((int)p.sink, from) + kRaKeys - 1) / kRaKeys), t.from_step);
+  t.n_steps = min(t.sink_steps, end_step) + max(end_step - t.from_step, 0);
+  const bool cut = p.parts > 1 && last_row - t.first < (int)p.record_rows;
+  t.n_parts = cut ? max(min((int)((t.n_steps + p.part_steps - 1) / p.part_steps), (int)p.parts), 1) : 1;
   return true;
 }
 
-template <typename T, int D, bool PAGED>
-__global__ __launch_bounds__(kRaThreads) void ragged_attention_kernel(RaParams p) {
+// The number of workgroup `id` in the order head, tile, part or tile, part, head.
+struct RaPlace {
+  uint32_t head, tile, part;
+};
+__device__ __forceinline__ RaPlace place_of(const RaParams& p, uint32_t id) {
+  const uint32_t per_head = p.tiles * p.parts;
+  if (p.by_head) {  // consecutive workgroups go to different XCDs: each gets a contiguous range
+    id = p.work_groups % 8 == 0 ? (id & 7) * (p.work_groups / 8) + (id >> 3) : id;
+    const uint32_t head = id / per_head, rest = id - head * per_head;
+    return RaPlace{head, rest / p.parts, rest % p.parts};
+  }
+  const uint32_t rest = id / (uint32_t)p.kv_heads;
+  return RaPlace{id - rest * (uint32_t)p.kv_heads, rest / p.parts, rest % p.parts};
+}
+
+template <int D>
+__device__ __forceinline__ float* record_of(const RaParams& p, const RaPlace& at, uint32_t part) {
+  return p.records + ((int64_t)(at.head * p.tiles + at.tile) * p.parts + part) * p.record_rows * (D + 2);
+}
+
+template <int D>
+constexpr int kRaLds = 2 * 2 * kRaKeys * 2 * D + 4 * 2 * 256 + 4 * 32 * 8;  // stages, looked-up places, maxima and sums
+
+// The reference point of the exponentials follows the maximum once it is 2^2 ahead: fewer rescalings, no further from 64 bits.
+constexpr float kRaStep = 2.0f;
+
+template <typename T, int D, int KIND>
+__global__ __launch_bounds__(kRaThreads, 2) void ragged_attention_kernel(RaParams p) {
   constexpr int kRowBytes = 2 * D, kPieces = D / 8, kDTiles = D / 32, kSteps = D / 16;
-  __shared__ __attribute__((aligned(16))) uint8_t k_lds[kRaKeys * kRowBytes];
-  __shared__ __attribute__((aligned(16))) uint8_t v_lds[kRaKeys * kRowBytes];
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, l32 = lane & 31, lh = lane >> 5;
-  auto start_of = [&](int64_t b) { return min(max((int64_t)p.q_starts[b], (int64_t)0), p.n_queries); };
+  constexpr int kRowsPerLoad = 1024 / kRowBytes, kGroupLoads = 16 / kRowsPerLoad;  // loads of 16 rows
+  constexpr int kStepBytes = kRaKeys * kRowBytes;                                  // K or V of a step
+  constexpr bool kLooksUp = KIND != kRaRows;
+  extern __shared__ __attribute__((aligned(16))) uint8_t smem[];
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), l32 = lane & 31, lh = lane >> 5;
 
   if (blockIdx.x >= p.work_groups) {  // rows outside every stream
-    const int64_t first = p.streams ? start_of(0) : 0, end = p.streams ? max(start_of(p.streams), first) : 0;
+    const int64_t first = p.streams ? stream_start(p, 0) : 0, end = p.streams ? max(stream_start(p, p.streams), first) : 0;
     const int64_t outside = first + p.n_queries - end, pieces = outside * p.heads * kPieces;
     for (int64_t i = (int64_t)(blockIdx.x - p.work_groups) * kRaThreads + tid; i < pieces; i += (int64_t)kRaClearGroups * kRaThreads) {
       const int64_t row = i / (p.heads * kPieces);
@@ -112,147 +238,345 @@ __global__ __launch_bounds__(kRaThreads) void ragged_attention_kernel(RaParams p
     return;
   }
 
-  const uint32_t pair = blockIdx.x / p.tiles, hk = pair % p.kv_heads;
-  const int64_t b = pair / p.kv_heads;
-  const int64_t q0 = start_of(b), n = max(start_of(b + 1) - q0, (int64_t)0), rows = n * p.group.d;
-  Keys keys{};
-  if constexpr (PAGED) {
-    keys.len = min(max((int64_t)p.kv_lens[b], (int64_t)0), p.table_keys);
-    keys.pages = p.page_table + b * p.table_stride;
-  } else {
-    keys.start = min(max((int64_t)p.k_starts[b], (int64_t)0), p.n_keys);
-    const int64_t len = p.k_lens ? (int64_t)p.k_lens[b] : (int64_t)p.k_starts[b + 1] - keys.start;
-    keys.len = min(max(len, (int64_t)0), p.n_keys - keys.start);
+  const RaPlace place = place_of(p, blockIdx.x);
+  RaTile t;
+  if (!find_tile<KIND>(p, place.tile, t) || (int)place.part >= t.n_parts) return;
+  const int s_begin = t.n_parts > 1 ? (int)(place.part * p.part_steps) : 0;
+  const int s_end = (int)place.part + 1 == t.n_parts ? t.n_steps : s_begin + (int)p.part_steps;
+  const int tile_rows = min(kRaTileRows, t.rows - t.first);
+  const uint16_t *k_head = p.k + place.head * p.k_stride_head, *v_head = p.v + place.head * p.v_stride_head;
+  const bool narrow = tile_rows <= 32;
+  const int own = narrow ? 0 : wave * 32;  // the wave's first row in the tile
+
+  // this lane's row and what it sees: keys below `last`, from `from` on or below the sink
+  const int f = min(t.first + own + l32, t.rows - 1);
+  const int token = (uint32_t)f / p.group, pos = t.len - t.n + token;
+  const int head = place.head * p.group.d + (f - token * p.group.d);
+  const int last = p.causal ? min(pos + 1, t.len) : t.len;
+  const int from = p.window && pos >= (int)p.window ? pos - (int)p.window + 1 : 0;
+  // the same for the wave's first and last row, which bound the others
+  const int last0 = __builtin_amdgcn_readfirstlane(last), from1 = __builtin_amdgcn_readlane(from, 31);
+  const bool idle = own >= tile_rows;  // a wave without rows only moves keys
+
+  short8v qf[kSteps];
+  {
+    const uint16_t* src = p.q + (t.q0 + token) * p.q_stride_token + head * p.q_stride_head + 8 * lh;
+#pragma unroll
+    for (int ks = 0; ks < kSteps; ++ks) qf[ks] = *reinterpret_cast<const short8v*>(src + 16 * ks);
   }
-  const uint16_t *k_head = p.k + hk * p.k_stride_head, *v_head = p.v + hk * p.v_stride_head;
-
-  for (int64_t tile = blockIdx.x % p.tiles; tile * kRaTileRows < rows; tile += p.tiles) {
-    const int64_t f0 = tile * kRaTileRows, f1 = min(f0 + kRaTileRows, rows) - 1;
-    // this lane's row
-    const int64_t f = min(f0 + wave * 32 + l32, rows - 1);
-    const int64_t i = (uint32_t)f / p.group, pos = keys.len - n + i;
-    const int head = hk * p.group.d + (int)(f - i * p.group.d);
-    short8v qf[kSteps];
-    {
-      const uint16_t* src = p.q + (q0 + i) * p.q_stride_token + head * p.q_stride_head + 8 * lh;
+  float16v o[kDTiles];
 #pragma unroll
-      for (int ks = 0; ks < kSteps; ++ks) qf[ks] = *reinterpret_cast<const short8v*>(src + 16 * ks);
+  for (int dt = 0; dt < kDTiles; ++dt)
+#pragma unroll
+    for (int r = 0; r < 16; ++r) o[dt][r] = 0.0f;
+  float m = -INFINITY, l = 0.0f;
+
+  // ---- where the keys of 64 lanes lie
+  uint8_t* const looked_up = smem + 4 * kStepBytes + wave * 512;
+  const uint32_t looked_up_lds = lds_at(looked_up);
+  auto key_base = [&](int s) __attribute__((always_inline)) { return (s < t.sink_steps ? s : t.from_step + s - t.sink_steps) * kRaKeys; };
+  auto look_up = [&](int key, int slot) __attribute__((always_inline)) {
+    const uint32_t k = (uint32_t)min(key, t.len - 1);
+    if constexpr (KIND == kRaPaged) load4_to_lds(t.pages + k / p.page, looked_up_lds + slot * 256);
+    if constexpr (KIND == kRaMaskedRows) load4_to_lds(reinterpret_cast<const void*>((uintptr_t)(p.key_mask + t.key0 + k) & ~(uintptr_t)3), looked_up_lds + slot * 256);
+  };
+  uint32_t at_page = 0, at_row = 0;  // of this lane's key: page and row in it, or row
+  uint64_t there = 0;                // which of the 64 keys exist
+  auto take_places = [&](int key, int slot) __attribute__((always_inline)) {
+    bool ok = key < t.len;
+    if constexpr (KIND == kRaPaged) {
+      at_page = *reinterpret_cast<const uint32_t*>(looked_up + slot * 256 + lane * 4);
+      at_row = (uint32_t)key - ((uint32_t)key / p.page) * p.page.d;
+      ok = ok && at_page < p.n_pages;
+    } else {
+      at_row = (uint32_t)(t.key0 + key);
+      if constexpr (KIND == kRaMaskedRows) {
+        const uint32_t shift = 8 * ((uint32_t)(uintptr_t)(p.key_mask + t.key0 + min(key, t.len - 1)) & 3);
+        ok = ok && ((*reinterpret_cast<const uint32_t*>(looked_up + slot * 256 + lane * 4) >> shift) & 0xFF) != 0;
+      }
     }
-    // Keys that the row sees: those below `last`, from `from` on or below `sink`.
-    const int64_t pos0 = keys.len - n + (uint32_t)f0 / p.group, pos1 = keys.len - n + (uint32_t)f1 / p.group;
-    const int64_t last = p.causal ? min(pos + 1, keys.len) : keys.len;
-    const int64_t from = p.window ? max(pos - p.window + 1, (int64_t)0) : 0;
-    const int64_t last0 = p.causal ? min(pos0 + 1, keys.len) : keys.len, last1 = p.causal ? min(pos1 + 1, keys.len) : keys.len;
-    const int64_t from0 = p.window ? max(pos0 - p.window + 1, (int64_t)0) : 0, from1 = p.window ? max(pos1 - p.window + 1, (int64_t)0) : 0;
-    // Steps of 64 keys: those with kept first keys, then those from the first row's window on.
-    const int64_t end_step = max((last1 + kRaKeys - 1) / kRaKeys, (int64_t)0), from_step = from0 / kRaKeys;
-    const int64_t sink_steps = min((min(p.sink, from0) + kRaKeys - 1) / kRaKeys, from_step);
-    const int64_t n_steps = min(sink_steps, end_step) + max(end_step - from_step, (int64_t)0);
+    there = __builtin_amdgcn_ballot_w64(ok);
+  };
 
-    float16v o[kDTiles];
+  // ---- loads: 16 rows, the keys of lanes r0 .. r0 + 15, to 16 rows of LDS
+  uint32_t k_off[kGroupLoads], v_off[kGroupLoads];
+  int k_part[kGroupLoads], v_part[kGroupLoads];
 #pragma unroll
-    for (int dt = 0; dt < kDTiles; ++dt)
+  for (int i = 0; i < kGroupLoads; ++i) {
+    const int row = i * kRowsPerLoad + lane / kPieces;
+    k_part[i] = k_piece<D>(row, lane % kPieces) * 16;
+    v_part[i] = v_piece<D>(row, lane % kPieces) * 16;
+    k_off[i] = (uint32_t)row * p.k_stride_row * 2 + k_part[i];
+    v_off[i] = (uint32_t)row * p.v_stride_row * 2 + v_part[i];
+  }
+  const bool whole_groups = KIND != kRaPaged || p.page.d % 16 == 0;  // 16 rows lie one behind the other
+  auto load_rows = [&](bool values, int r0, uint32_t lds) __attribute__((always_inline)) {
+    const uint16_t* base = values ? v_head : k_head;
+    const uint32_t per_page = values ? p.v_stride_page : p.k_stride_page, per_row = values ? p.v_stride_row : p.k_stride_row;
+    if (whole_groups && ((uint32_t)(there >> r0) & 0xFFFFu) == 0xFFFFu) {
+      uint64_t at = (uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)at_row, r0) * per_row;
+      if constexpr (KIND == kRaPaged) at += (uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)at_page, r0) * per_page;
+      const uint16_t* from_here = uniform_pointer(base + at);
 #pragma unroll
-      for (int r = 0; r < 16; ++r) o[dt][r] = 0.0f;
-    float m = -INFINITY, l = 0.0f;
+      for (int i = 0; i < kGroupLoads; ++i) load16_to_lds(values ? v_off[i] : k_off[i], from_here, lds + i * 1024);
+    } else {
+#pragma unroll
+      for (int i = 0; i < kGroupLoads; ++i) {
+        const int row = r0 + i * kRowsPerLoad + lane / kPieces;
+        uint64_t at = (uint64_t)(uint32_t)__shfl((int)at_row, row) * per_row;
+        if constexpr (KIND == kRaPaged) at += (uint64_t)(uint32_t)__shfl((int)at_page, row) * per_page;
+        const uint8_t* src = reinterpret_cast<const uint8_t*>(base + at) + (values ? v_part[i] : k_part[i]);
+        load16_to_lds((there >> row) & 1 ? src : reinterpret_cast<const uint8_t*>(kRaZeros), lds + i * 1024);
+      }
+    }
+  };
 
-    for (int64_t s = 0; s < n_steps; ++s) {
-      const int64_t base = (s < sink_steps ? s : from_step + s - sink_steps) * kRaKeys;
-      __syncthreads();
+  // ---- scores and probabilities of NT groups of 32 keys from `base` on
+  // S^T: register r of sc[kt] is key 32 kt + 8 (r / 4) + 4 lh + r % 4
+  auto scores = [&](auto& sc, const uint8_t* k_rows) __attribute__((always_inline)) {
+    constexpr int NT = std::extent<std::remove_reference_t<decltype(sc)>>::value;
 #pragma unroll
-      for (int it = 0; it < kRaKeys * kPieces / kRaThreads; ++it) {
-        const int row = (it * kRaThreads + tid) / kPieces, c = tid % kPieces;
-        int64_t k_at, v_at;
-        uint4 kv = make_uint4(0, 0, 0, 0), vv = make_uint4(0, 0, 0, 0);
-        if (find_key<PAGED>(p, keys, base + row, k_at, v_at)) {
-          kv = *reinterpret_cast<const uint4*>(k_head + k_at + 8 * c);
-          vv = *reinterpret_cast<const uint4*>(v_head + v_at + 8 * c);
-        }
-        *reinterpret_cast<uint4*>(k_lds + row * kRowBytes + k_piece<D>(row, c) * 16) = kv;
-        *reinterpret_cast<uint4*>(v_lds + row * kRowBytes + v_piece<D>(row, c) * 16) = vv;
+    for (int kt = 0; kt < NT; ++kt) {
+#pragma unroll
+      for (int r = 0; r < 16; ++r) sc[kt][r] = 0.0f;
+#pragma unroll
+      for (int ks = 0; ks < kSteps; ++ks) {
+        const short8v a = *reinterpret_cast<const short8v*>(k_rows + (32 * kt + l32) * kRowBytes + k_piece<D>(l32, 2 * ks + lh) * 16);
+        sc[kt] = T::mfma(a, qf[ks], sc[kt]);
       }
-      int64_t k_at, v_at;
-      const uint64_t there = __builtin_amdgcn_ballot_w64(find_key<PAGED>(p, keys, base + lane, k_at, v_at));
-      __syncthreads();
-
-      // S^T: register r of sc[kt] is key 32 kt + 8 (r / 4) + 4 lh + r % 4
-      float16v sc[2];
+    }
+  };
+  auto mask = [&](auto& sc, int base, uint64_t exist) __attribute__((always_inline)) {
+    constexpr int NT = std::extent<std::remove_reference_t<decltype(sc)>>::value;
+    constexpr uint64_t kAll = NT == 2 ? ~0ull : 0xFFFFFFFFull;
+    const int end = base + 32 * NT;
+    if ((exist & kAll) == kAll && end <= last0 && (base >= from1 || end <= (int)p.sink)) return;
+    const uint64_t bits = exist >> (4 * lh);
+    const int first = base + 4 * lh;
 #pragma unroll
-      for (int kt = 0; kt < 2; ++kt) {
+    for (int kt = 0; kt < NT; ++kt)
 #pragma unroll
-        for (int r = 0; r < 16; ++r) sc[kt][r] = 0.0f;
-        const int row = 32 * kt + l32;
-#pragma unroll
-        for (int ks = 0; ks < kSteps; ++ks) {
-          const short8v a = *reinterpret_cast<const short8v*>(k_lds + row * kRowBytes + k_piece<D>(row, 2 * ks + lh) * 16);
-          sc[kt] = T::mfma(a, qf[ks], sc[kt]);
-        }
+      for (int r = 0; r < 16; ++r) {
+        const int at = 32 * kt + 8 * (r / 4) + r % 4, key = first + at;
+        const bool seen = key < last && (key >= from || key < (int)p.sink) && ((bits >> at) & 1);
+        sc[kt][r] = seen ? sc[kt][r] : -INFINITY;
       }
-      const bool all_seen = there == ~0ull && base + kRaKeys <= last0 && (base >= from1 || base + kRaKeys <= p.sink);
-      if (!all_seen) {
-        const uint64_t bits = there >> (4 * lh);
-        const int64_t first = base + 4 * lh;
+  };
+  auto attend = [&](auto& sc, const uint8_t* v_rows, auto v_arrived) __attribute__((always_inline)) {
+    constexpr int NT = std::extent<std::remove_reference_t<decltype(sc)>>::value;
+    float mx = sc[0][0];
 #pragma unroll
-        for (int kt = 0; kt < 2; ++kt)
+    for (int kt = 0; kt < NT; ++kt)
 #pragma unroll
-          for (int r = 0; r < 16; ++r) {
-            const int at = 32 * kt + 8 * (r / 4) + r % 4;
-            const int64_t key = first + at;
-            const bool seen = key < last && (key >= from || key < p.sink) && ((bits >> at) & 1);
-            sc[kt][r] = seen ? sc[kt][r] : -INFINITY;
-          }
-      }
-      float mx = -INFINITY;
-#pragma unroll
-      for (int kt = 0; kt < 2; ++kt)
-#pragma unroll
-        for (int r = 0; r < 16; ++r) mx = fmaxf(mx, sc[kt][r]);
-      mx = fmaxf(exchange_max(mx), m);
-      // a row that has seen nothing yet stays at -inf; 0 stands for it in the exponents, where -inf - -inf would be NaN
-      const float neg = mx == -INFINITY ? 0.0f : -mx * p.scale_log2;
-      const float alpha = m == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(fmaf(m, p.scale_log2, neg));
-      m = mx;
+      for (int r = 0; r < 16; ++r) mx = fmaxf(mx, sc[kt][r]);
+    mx = exchange_max(mx);
+    // a row that has seen nothing yet stays at -inf; 0 stands for it in the exponents, where -inf - -inf would be NaN
+    const bool raise = (mx - m) * p.scale_log2 > kRaStep;
+    if (__builtin_amdgcn_ballot_w64(raise) != 0) {
+      const float alpha = raise ? __builtin_amdgcn_exp2f((m - mx) * p.scale_log2) : 1.0f;
+      m = raise ? mx : m;
       l *= alpha;
 #pragma unroll
       for (int dt = 0; dt < kDTiles; ++dt)
 #pragma unroll
         for (int r = 0; r < 16; ++r) o[dt][r] *= alpha;
+    }
+    const float neg = m == -INFINITY ? 0.0f : -m * p.scale_log2;
+    v_arrived();
 #pragma unroll
-      for (int step = 0; step < 4; ++step) {
-        uint32_t w[4];
+    for (int step = 0; step < 2 * NT; ++step) {
+      uint32_t w[4];
 #pragma unroll
-        for (int u = 0; u < 4; ++u) {
-          const float p0 = __builtin_amdgcn_exp2f(fmaf(sc[step >> 1][8 * (step & 1) + 2 * u], p.scale_log2, neg));
-          const float p1 = __builtin_amdgcn_exp2f(fmaf(sc[step >> 1][8 * (step & 1) + 2 * u + 1], p.scale_log2, neg));
-          l += p0 + p1;
-          w[u] = T::pack2(p0, p1);
+      for (int u = 0; u < 4; ++u) {
+        const float p0 = __builtin_amdgcn_exp2f(fmaf(sc[step >> 1][8 * (step & 1) + 2 * u], p.scale_log2, neg));
+        const float p1 = __builtin_amdgcn_exp2f(fmaf(sc[step >> 1][8 * (step & 1) + 2 * u + 1], p.scale_log2, neg));
+        l += p0 + p1;
+        w[u] = T::pack2(p0, p1);  // at most 2^kRaStep: no overflow, and half a step's error each, as small as the result's own
+      }
+      const short8v pb = __builtin_bit_cast(short8v, make_uint4(w[0], w[1], w[2], w[3]));
+      typedef __attribute__((address_space(3))) short4v* lds_short4;
+#pragma unroll
+      for (int dt = 0; dt < kDTiles; ++dt) {
+        short4v part[2];
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+          const int row = 4 * lh + ((lane & 15) >> 2), piece = 4 * dt + 2 * ((lane >> 4) & 1) + ((lane & 3) >> 1);
+          part[j] = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+              (lds_short4)(v_rows + (row + 16 * step + 8 * j) * kRowBytes + v_piece<D>(row, piece) * 16 + (lane & 1) * 8));
         }
-        const short8v pb = __builtin_bit_cast(short8v, make_uint4(w[0], w[1], w[2], w[3]));
-        typedef __attribute__((address_space(3))) short4v* lds_short4;
-#pragma unroll
-        for (int dt = 0; dt < kDTiles; ++dt) {
-          short4v part[2];
-#pragma unroll
-          for (int j = 0; j < 2; ++j) {
-            const int row = 16 * step + 8 * j + 4 * lh + ((lane & 15) >> 2);
-            const int piece = 4 * dt + 2 * ((lane >> 4) & 1) + ((lane & 3) >> 1);
-            part[j] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_short4)(v_lds + row * kRowBytes + v_piece<D>(row, piece) * 16 + (lane & 1) * 8));
-          }
-          o[dt] = T::mfma(__builtin_shufflevector(part[0], part[1], 0, 1, 2, 3, 4, 5, 6, 7), pb, o[dt]);
-        }
+        o[dt] = T::mfma(__builtin_shufflevector(part[0], part[1], 0, 1, 2, 3, 4, 5, 6, 7), pb, o[dt]);
       }
     }
+  };
+
+  const int out_token = token;
+  auto write_row = [&](int row_in_tile, int tok, int hd, int column, const float (&v)[4], float mm, float ll) __attribute__((always_inline)) {
+    // four columns of a row: of the result, or of this part's record
+    if (t.n_parts == 1) {
+      const float inv = ll == 0.0f ? 0.0f : 1.0f / ll;
+      uint16_t* dst = p.out + (t.q0 + tok) * p.out_stride_token + hd * p.out_stride_head + column;
+      *reinterpret_cast<uint2*>(dst) = make_uint2(T::pack2(v[0] * inv, v[1] * inv), T::pack2(v[2] * inv, v[3] * inv));
+    } else {
+      float* rec = record_of<D>(p, place, place.part);
+      *reinterpret_cast<float4*>(rec + row_in_tile * D + column) = make_float4(v[0], v[1], v[2], v[3]);
+      if (column == 0) *reinterpret_cast<float2*>(rec + p.record_rows * D + 2 * row_in_tile) = make_float2(mm, ll);
+    }
+  };
+
+  if (!narrow) {
+    uint8_t* const stages = smem;
+    const uint32_t stages_lds = lds_at(smem);
+    auto load_step = [&](int stage) __attribute__((always_inline)) {  // each wave a quarter of the rows
+      load_rows(false, wave * 16, stages_lds + stage * 2 * kStepBytes + wave * 16 * kRowBytes);
+      load_rows(true, wave * 16, stages_lds + stage * 2 * kStepBytes + kStepBytes + wave * 16 * kRowBytes);
+    };
+    if (s_begin < s_end) {
+      if (kLooksUp) {
+        look_up(key_base(s_begin) + lane, s_begin & 1);
+        wait_loads<0>();
+      }
+      take_places(key_base(s_begin) + lane, s_begin & 1);
+      load_step(s_begin & 1);
+      if (kLooksUp && s_begin + 1 < s_end) look_up(key_base(s_begin + 1) + lane, (s_begin + 1) & 1);
+    }
+    for (int s = s_begin; s < s_end; ++s) {
+      const uint64_t exist = there;
+      wait_loads<0>();
+      __syncthreads();  // the step's keys are in LDS, and every wave is done with those of the step before
+      if (s + 1 < s_end) {
+        take_places(key_base(s + 1) + lane, (s + 1) & 1);
+        load_step((s + 1) & 1);
+        if (kLooksUp && s + 2 < s_end) look_up(key_base(s + 2) + lane, s & 1);
+      }
+      if (idle) continue;
+      const uint8_t* rows = stages + (s & 1) * 2 * kStepBytes;
+      float16v sc[2];
+      scores(sc, rows);
+      mask(sc, key_base(s), exist);
+      attend(sc, rows + kStepBytes, [] {});
+    }
+    if (idle) return;
     l = exchange_sum(l);
-    const float inv = l == 0.0f ? 0.0f : 1.0f / l;
-    if (f0 + wave * 32 + l32 < rows) {
-      uint16_t* dst = p.out + (q0 + i) * p.out_stride_token + head * p.out_stride_head + 4 * lh;
+    if (own + l32 < tile_rows) {
 #pragma unroll
       for (int dt = 0; dt < kDTiles; ++dt)
 #pragma unroll
-        for (int g = 0; g < 4; ++g)
-          *reinterpret_cast<uint2*>(dst + 32 * dt + 8 * g) =
-              make_uint2(T::pack2(o[dt][4 * g] * inv, o[dt][4 * g + 1] * inv), T::pack2(o[dt][4 * g + 2] * inv, o[dt][4 * g + 3] * inv));
+        for (int g = 0; g < 4; ++g) {
+          const float v[4] = {o[dt][4 * g], o[dt][4 * g + 1], o[dt][4 * g + 2], o[dt][4 * g + 3]};
+          write_row(own + l32, out_token, head, 32 * dt + 8 * g + 4 * lh, v, m, l);
+        }
     }
+    return;
+  }
+
+  // ---- up to 32 rows: groups of 32 keys u = 2 s + half, every fourth one this wave's
+  uint8_t* const rows = smem + wave * kStepBytes;  // 32 rows of K, 32 of V
+  const uint32_t rows_lds = lds_at(rows);
+  constexpr int kLoads = 2 * kGroupLoads;  // of K or of V
+  auto group_base = [&](int u) __attribute__((always_inline)) { return key_base(u >> 1) + 32 * (u & 1); };
+  auto load_group = [&](bool values) __attribute__((always_inline)) {
+    load_rows(values, 0, rows_lds + (values ? 32 * kRowBytes : 0));
+    load_rows(values, 16, rows_lds + (values ? 32 * kRowBytes : 0) + 16 * kRowBytes);
+  };
+  const int u_end = 2 * s_end;
+  int u = 2 * s_begin + wave;
+  if (u < u_end) {
+    if (kLooksUp) {
+      look_up(group_base(u) + l32, 0);
+      wait_loads<0>();
+    }
+    take_places(group_base(u) + l32, 0);
+    load_group(false);
+    if (kLooksUp) look_up(group_base(min(u + 4, u_end - 1)) + l32, 1);
+    load_group(true);
+    for (int slot = 1; u < u_end; u += 4, slot ^= 1) {
+      const uint64_t exist = there;
+      const bool more = u + 4 < u_end;
+      wait_loads<kLoads>();  // K, and the places of the next group; V may be on its way
+      float16v sc[1];
+      scores(sc, rows);
+      if (more) {
+        take_places(group_base(u + 4) + l32, slot);
+        wait_lds_reads();
+        load_group(false);
+        if (kLooksUp) look_up(group_base(min(u + 8, u_end - 1)) + l32, slot ^ 1);
+      }
+      mask(sc, group_base(u), exist);
+      attend(sc, rows + 32 * kRowBytes, [&]() __attribute__((always_inline)) {
+        if (more) wait_loads<kLoads + (kLooksUp ? 1 : 0)>();
+        else wait_loads<0>();
+      });
+      if (more) {
+        wait_lds_reads();
+        load_group(true);
+      }
+    }
+  }
+  // The four waves' results, joined: each wave takes a quarter of the columns.
+  l = exchange_sum(l);
+  float2* const ml = reinterpret_cast<float2*>(smem + 4 * kStepBytes + 4 * 512);
+  if (lh == 0) ml[wave * 32 + l32] = make_float2(m, l);
+  {
+    float4* mine = reinterpret_cast<float4*>(rows);
+#pragma unroll
+    for (int dt = 0; dt < kDTiles; ++dt)
+#pragma unroll
+      for (int g = 0; g < 4; ++g) mine[(dt * 4 + g) * 64 + lane] = make_float4(o[dt][4 * g], o[dt][4 * g + 1], o[dt][4 * g + 2], o[dt][4 * g + 3]);
+  }
+  __syncthreads();
+  float weight[4], all_l = 0.0f, all_m = -INFINITY;
+#pragma unroll
+  for (int w = 0; w < 4; ++w) all_m = fmaxf(all_m, ml[w * 32 + l32].x);
+#pragma unroll
+  for (int w = 0; w < 4; ++w) {
+    const float2 e = ml[w * 32 + l32];
+    weight[w] = e.x == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f((e.x - all_m) * p.scale_log2);
+    // a row without a maximum of which the sum is NaN has met NaN only
+    all_l += e.x == -INFINITY ? e.y : e.y * weight[w];
+  }
+#pragma unroll
+  for (int i = 0; i < kDTiles; ++i) {
+    const int piece = wave * kDTiles + i, dt = piece >> 2, g = piece & 3;
+    float v[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+    for (int w = 0; w < 4; ++w) {
+      const float4 e = reinterpret_cast<const float4*>(smem + w * kStepBytes)[piece * 64 + lane];
+      v[0] = fmaf(e.x, weight[w], v[0]);
+      v[1] = fmaf(e.y, weight[w], v[1]);
+      v[2] = fmaf(e.z, weight[w], v[2]);
+      v[3] = fmaf(e.w, weight[w], v[3]);
+    }
+    if (l32 < tile_rows) write_row(l32, out_token, head, 32 * dt + 8 * g + 4 * lh, v, all_m, all_l);
+  }
+}
+
+// Joins the parts of the tiles that were cut: a workgroup per (kv head, tile).
+template <typename T, int D, int KIND>
+__global__ __launch_bounds__(kRaThreads) void ragged_join_kernel(RaParams p) {
+  const RaPlace place{blockIdx.x % (uint32_t)p.kv_heads, blockIdx.x / (uint32_t)p.kv_heads, 0};
+  RaTile t;
+  if (!find_tile<KIND>(p, place.tile, t) || t.n_parts == 1) return;
+  const int rows = min(kRaTileRows, t.rows - t.first);
+  for (int i = threadIdx.x; i < rows * (D / 4); i += kRaThreads) {
+    const int row = i / (D / 4), column = i % (D / 4) * 4;
+    float m = -INFINITY, l = 0.0f;
+    for (int part = 0; part < t.n_parts; ++part) m = fmaxf(m, record_of<D>(p, place, part)[p.record_rows * D + 2 * row]);
+    float v[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+    for (int part = 0; part < t.n_parts; ++part) {
+      const float* rec = record_of<D>(p, place, part);
+      const float2 e = *reinterpret_cast<const float2*>(rec + p.record_rows * D + 2 * row);
+      const float4 x = *reinterpret_cast<const float4*>(rec + row * D + column);
+      const float w = e.x == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f((e.x - m) * p.scale_log2);
+      l += e.x == -INFINITY ? e.y : e.y * w;
+      v[0] = fmaf(x.x, w, v[0]);
+      v[1] = fmaf(x.y, w, v[1]);
+      v[2] = fmaf(x.z, w, v[2]);
+      v[3] = fmaf(x.w, w, v[3]);
+    }
+    const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+    const int f = t.first + row, token = (uint32_t)f / p.group, head = place.head * p.group.d + (f - token * p.group.d);
+    uint16_t* dst = p.out + (t.q0 + token) * p.out_stride_token + head * p.out_stride_head + column;
+    *reinterpret_cast<uint2*>(dst) = make_uint2(T::pack2(v[0] * inv, v[1] * inv), T::pack2(v[2] * inv, v[3] * inv));
   }
 }
 
@@ -265,7 +589,7 @@ static int check_ragged(const ll_ragged_attention_args* a) {
   LL_REQUIRE(a->n_queries >= 0 && a->streams >= 0, "ll_ragged_attention: %lld queries in %lld streams", (long long)a->n_queries, (long long)a->streams);
   LL_REQUIRE(a->n_queries <= 0x7fffffffll / a->num_heads, "ll_ragged_attention: %lld queries of %d heads are more than 2^31 rows",
              (long long)a->n_queries, a->num_heads);
-  LL_REQUIRE(a->streams <= 0x7fffffffll / a->num_kv_heads - 64, "ll_ragged_attention: %lld streams", (long long)a->streams);
+  LL_REQUIRE(a->streams <= 0xfffffff / a->num_kv_heads, "ll_ragged_attention: %lld streams", (long long)a->streams);
   LL_REQUIRE(a->softmax_scale > 0.0f && std::isfinite(a->softmax_scale), "ll_ragged_attention: softmax_scale has to be positive");
   LL_REQUIRE(a->max_q_len >= 0 && a->max_kv_len >= 0, "ll_ragged_attention: negative longest lengths");
   if (a->page_table || a->page_size) {
@@ -281,15 +605,85 @@ static int check_ragged(const ll_ragged_attention_args* a) {
   return LL_OK;
 }
 
+// Parts of the keys: at least 512 (a wave of a narrow tile walks a quarter of them), at most 4096; records of up to 256 MiB.
+constexpr int64_t kRaLeastSteps = 8, kRaMostSteps = 64;
+constexpr size_t kRaMostBytes = (size_t)256 << 20;
+
+// How a launch is divided (host arithmetic).  Tiles of up to 128 rows; their keys in parts where the tiles alone are few for the
+// device, and where a stream's keys are so many that one workgroup would still walk them when the others are done.
+struct RaPlan {
+  uint32_t tiles, parts, part_steps, record_rows;
+  size_t bytes;
+};
+static RaPlan plan_ragged(const ll_ragged_attention_args& a, int cus) {
+  RaPlan r{0, 1, 0, 0, 0};
+  const int64_t group = a.num_heads / a.num_kv_heads, rows = a.n_queries * group;
+  const int64_t longest = a.max_q_len > 0 && a.max_q_len < a.n_queries ? a.max_q_len : a.n_queries;
+  r.tiles = (uint32_t)(a.n_queries == 0 ? 0 : rows / kRaTileRows + a.streams);  // each stream one tile that is not full
+  if (r.tiles == 0) return r;
+  const bool paged = a.page_table || a.page_size;
+  const int64_t most_keys = paged ? a.table_width * a.page_size : a.n_keys;
+  int64_t keys = a.max_kv_len > 0 && a.max_kv_len < most_keys ? a.max_kv_len : most_keys;
+  if (a.window > 0 && a.window < keys && a.sink_keys < keys) keys = std::min(keys, a.window + a.sink_keys + longest + 2 * kRaKeys);
+  const int64_t steps = (keys + kRaKeys - 1) / kRaKeys;
+  const int64_t busy = std::min<int64_t>(r.tiles, a.streams * ((longest * group + kRaTileRows - 1) / kRaTileRows)) * a.num_kv_heads;
+  const int64_t want = busy >= 2 * cus ? 1 : (4 * cus + busy - 1) / busy;
+  int64_t per_part = std::min<int64_t>(std::max<int64_t>((steps + want - 1) / want, kRaLeastSteps), kRaMostSteps);
+  const uint32_t record_rows = (uint32_t)std::min<int64_t>((longest * group + 31) / 32 * 32, kRaTileRows);
+  const size_t record = (size_t)record_rows * (a.head_dim + 2) * sizeof(float);
+  for (; per_part < steps; per_part *= 2) {
+    const int64_t parts = (steps + per_part - 1) / per_part;
+    const size_t bytes = (size_t)r.tiles * a.num_kv_heads * parts * record;
+    if (bytes <= kRaMostBytes && (int64_t)r.tiles * a.num_kv_heads * parts < (1ll << 30)) {
+      r.parts = (uint32_t)parts;
+      r.part_steps = (uint32_t)per_part;
+      r.record_rows = record_rows;
+      r.bytes = bytes;
+      break;
+    }
+  }
+  return r;
+}
+
 }  // namespace ll
 
 extern "C" int ll_ragged_attention_workspace(const ll_ragged_attention_args* a, int compute_units, size_t* bytes) {
   using namespace ll;
   if (int rc = check_ragged(a)) return rc;
   LL_REQUIRE(bytes && compute_units >= 0, "ll_ragged_attention_workspace: nowhere to put the answer");
-  *bytes = 0;
+  if (compute_units == 0) {
+    int dev = 0;
+    if (hipError_t e = hipGetDevice(&dev)) {
+      set_error("ll_ragged_attention_workspace: hipGetDevice failed: %s", hipGetErrorString(e));
+      return LL_ELAUNCH;
+    }
+    if (int rc = compute_units_of(dev, compute_units, "ll_ragged_attention_workspace")) return rc;
+  }
+  *bytes = plan_ragged(*a, compute_units).bytes;
   return LL_OK;
 }
+
+namespace ll {
+template <typename T, int D, int KIND>
+static int launch_ragged(const RaParams& p, uint32_t grid, hipStream_t stream) {
+  static std::atomic<uint64_t> allowed{0};
+  const void* kernel = reinterpret_cast<const void*>(&ragged_attention_kernel<T, D, KIND>);
+  if (int rc = allow_dynamic_lds(kernel, kRaLds<D>, allowed, "ll_ragged_attention")) return rc;
+  ragged_attention_kernel<T, D, KIND><<<grid, kRaThreads, kRaLds<D>, stream>>>(p);
+  LL_CHECK_LAUNCH("ll_ragged_attention");
+  if (p.parts > 1) {
+    ragged_join_kernel<T, D, KIND><<<p.tiles * (uint32_t)p.kv_heads, kRaThreads, 0, stream>>>(p);
+    LL_CHECK_LAUNCH("ll_ragged_attention (join)");
+  }
+  return LL_OK;
+}
+template <typename T, int D>
+static int launch_ragged(const RaParams& p, int kind, uint32_t grid, hipStream_t stream) {
+  if (kind == kRaPaged) return launch_ragged<T, D, kRaPaged>(p, grid, stream);
+  if (kind == kRaRows) return launch_ragged<T, D, kRaRows>(p, grid, stream);
+  return launch_ragged<T, D, kRaMaskedRows>(p, grid, stream);
+}
+}  // namespace ll
 
 extern "C" int ll_ragged_attention(const ll_ragged_attention_args* a, void* stream) {
   using namespace ll;
@@ -306,6 +700,18 @@ extern "C" int ll_ragged_attention(const ll_ragged_attention_args* a, void* stre
   LL_REQUIRE((a->q_stride_token | a->q_stride_head | a->out_stride_token | a->out_stride_head | a->k_stride_page | a->k_stride_row |
               a->k_stride_head | a->v_stride_page | a->v_stride_row | a->v_stride_head) % 8 == 0,
              "ll_ragged_attention: strides must be multiples of 8 elements");
+  LL_REQUIRE(a->k_stride_page >= 0 && a->v_stride_page >= 0 && a->k_stride_page <= 0xffffffffll && a->v_stride_page <= 0xffffffffll &&
+                 a->k_stride_row >= 0 && a->v_stride_row >= 0 && a->k_stride_row < (1ll << 26) && a->v_stride_row < (1ll << 26),
+             "ll_ragged_attention: pages of k and v lie at most 2^32 elements apart, rows 2^26");
+  int dev = 0, cus = 0;
+  if (hipError_t e = hipGetDevice(&dev)) {
+    set_error("ll_ragged_attention: hipGetDevice failed: %s", hipGetErrorString(e));
+    return LL_ELAUNCH;
+  }
+  if (int rc = compute_units_of(dev, cus, "ll_ragged_attention")) return rc;
+  const RaPlan plan = plan_ragged(*a, cus);
+  LL_REQUIRE(plan.bytes == 0 || (a->workspace && (uintptr_t)a->workspace % 16 == 0 && a->workspace_bytes >= plan.bytes),
+             "ll_ragged_attention: a workspace of %zu bytes, 16-byte aligned, is needed", plan.bytes);
   RaParams p{};
   p.q = static_cast<const uint16_t*>(a->q);
   p.out = static_cast<uint16_t*>(a->out);
@@ -314,19 +720,19 @@ extern "C" int ll_ragged_attention(const ll_ragged_attention_args* a, void* stre
   p.out_stride_token = a->out_stride_token;
   p.out_stride_head = a->out_stride_head;
   p.n_queries = a->n_queries;
-  p.streams = a->streams;
+  p.streams = (int)a->streams;
   p.q_starts = a->q_starts;
   p.k = static_cast<const uint16_t*>(a->k);
   p.v = static_cast<const uint16_t*>(a->v);
-  p.k_stride_page = a->k_stride_page;
-  p.k_stride_row = a->k_stride_row;
+  p.k_stride_page = (uint32_t)a->k_stride_page;
+  p.k_stride_row = (uint32_t)a->k_stride_row;
   p.k_stride_head = a->k_stride_head;
-  p.v_stride_page = a->v_stride_page;
-  p.v_stride_row = a->v_stride_row;
+  p.v_stride_page = (uint32_t)a->v_stride_page;
+  p.v_stride_row = (uint32_t)a->v_stride_row;
   p.v_stride_head = a->v_stride_head;
   p.page_table = a->page_table;
   p.table_stride = a->table_stride;
-  p.table_keys = paged ? a->table_width * a->page_size : 0;
+  p.table_keys = paged && has_keys ? a->table_width * a->page_size : 0;
   p.n_pages = (uint32_t)a->n_pages;
   p.page = divisor(paged ? (uint32_t)a->page_size : 1u);
   p.kv_lens = a->kv_lens;
@@ -336,41 +742,24 @@ extern "C" int ll_ragged_attention(const ll_ragged_attention_args* a, void* stre
   p.n_keys = a->n_keys;
   p.scale_log2 = a->softmax_scale * 1.4426950408889634f;
   p.causal = a->causal;
-  p.clear_rest = a->clear_rest;
   p.heads = a->num_heads;
   p.kv_heads = a->num_kv_heads;
   p.group = divisor((uint32_t)(a->num_heads / a->num_kv_heads));
-  p.window = a->window;
-  p.sink = a->sink_keys;
-  const int64_t longest = a->max_q_len > 0 && a->max_q_len < a->n_queries ? a->max_q_len : a->n_queries;
-  int64_t tiles = (longest * p.group.d + kRaTileRows - 1) / kRaTileRows;
-  const int64_t pairs = a->streams * a->num_kv_heads;
-  if (pairs > 0 && tiles > 0x3fffffffll / pairs) tiles = 0x3fffffffll / pairs > 0 ? 0x3fffffffll / pairs : 1;
-  p.tiles = (uint32_t)tiles;
-  p.work_groups = (uint32_t)(pairs * tiles);
+  p.window = (uint32_t)std::min<int64_t>(a->window, 0x7fffffff);  // keys are fewer
+  p.sink = (uint32_t)std::min<int64_t>(a->sink_keys, 0x7fffffff);
+  p.tiles = plan.tiles;
+  p.parts = plan.parts;
+  p.part_steps = plan.part_steps ? plan.part_steps : 1;
+  p.record_rows = plan.record_rows;
+  p.work_groups = plan.tiles * plan.parts * (uint32_t)a->num_kv_heads;
+  // Workgroups that read the same keys on one XCD, if that leaves every XCD the same work: whole heads for each, or one stream.
+  p.by_head = a->num_kv_heads % 8 == 0 || a->streams == 1;
+  p.records = static_cast<float*>(a->workspace);
   const uint32_t grid = p.work_groups + (a->clear_rest ? kRaClearGroups : 0);
   if (grid == 0) return LL_OK;
+  const int kind = paged ? kRaPaged : a->key_mask ? kRaMaskedRows : kRaRows;
   const hipStream_t s = static_cast<hipStream_t>(stream);
-#define LL_LAUNCH(T, D)                                                                             \
-  if (paged) {                                                                                      \
-    ragged_attention_kernel<T, D, true><<<grid, kRaThreads, 0, s>>>(p);                             \
-  } else {                                                                                          \
-    ragged_attention_kernel<T, D, false><<<grid, kRaThreads, 0, s>>>(p);                            \
-  }
-  if (a->dtype == LL_DTYPE_BF16) {
-    if (a->head_dim == 128) {
-      LL_LAUNCH(Bf16, 128)
-    } else {
-      LL_LAUNCH(Bf16, 64)
-    }
-  } else {
-    if (a->head_dim == 128) {
-      LL_LAUNCH(F16, 128)
-    } else {
-      LL_LAUNCH(F16, 64)
-    }
-  }
-#undef LL_LAUNCH
-  LL_CHECK_LAUNCH("ll_ragged_attention");
-  return LL_OK;
+  if (a->dtype == LL_DTYPE_BF16)
+    return a->head_dim == 128 ? launch_ragged<Bf16, 128>(p, kind, grid, s) : launch_ragged<Bf16, 64>(p, kind, grid, s);
+  return a->head_dim == 128 ? launch_ragged<F16, 128>(p, kind, grid, s) : launch_ragged<F16, 64>(p, kind, grid, s);
 }
