@@ -6,7 +6,8 @@
 // D / 8 lanes hold a head, rounded up to 8, 16 or 32, eight columns each, as two groups of four that are each other's partners
 // in the rotation: 4 l and 4 l + R / 2 for pairs of halves, 8 l and 8 l + 4 for neighbouring pairs (and for columns that are not
 // rotated).  Either way pair j of lane l is j = 4 l .. 4 l + 3, so that the angles are one load of 16 bytes each and nothing
-// passes between lanes but the sum of squares.
+// passes between lanes but the sum of squares.  A wave takes heads of one token and one of q, k and v: position, slot, pointers and
+// strides are scalars, loaded once for up to kHeadsEach heads per lane, all of whose loads are under way before the first is used.
 #include "ll_types16.h"
 
 namespace ll {
@@ -22,8 +23,8 @@ struct HeadRows {
 struct HeadNormParams {
   HeadRows rows[3];  // q, k, v
   int64_t first_token;
-  uint32_t tokens;       // of this launch
-  uint32_t units_q, units_kv;  // units of kHeads heads: q's, and k's (and v's)
+  uint32_t tokens;             // of this launch
+  uint32_t units_q, units_kv;  // waves per token for q, and for k (and v)
   Divisor per_token;
   int D, R, interleaved;
   float eps, inv_D;
@@ -36,30 +37,37 @@ struct HeadNormParams {
 // Sum over LANES neighbouring lanes, in every one of them.
 template <int LANES>
 __device__ __forceinline__ float sum_over_lanes(float v) {
-#pragma unroll
-  for (int d = 1; d < LANES; d *= 2) v += __shfl_xor(v, d);
-  return v;
+  if constexpr (LANES == 8) {
+#define LL_DPP_ADD(v, ctrl) v += __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, v), ctrl, 0xF, 0xF, true))
+    LL_DPP_ADD(v, 0xB1);   // quad_perm [1, 0, 3, 2]
+    LL_DPP_ADD(v, 0x4E);   // quad_perm [2, 3, 0, 1]
+    LL_DPP_ADD(v, 0x141);  // row_half_mirror
+#undef LL_DPP_ADD
+    return v;
+  } else {
+    v = sum_over_16_lanes(v);
+    return LANES == 16 ? v : v + __shfl_xor(v, 16);
+  }
 }
 
 template <typename T>
-__device__ __forceinline__ void load4(const uint16_t* p, float* f) {
-  const uint2 w = *reinterpret_cast<const uint2*>(p);
+__device__ __forceinline__ void unpack4(uint2 w, float* f) {
   T::unpack2(w.x, f[0], f[1]);
   T::unpack2(w.y, f[2], f[3]);
 }
 
 constexpr int kHeadNormThreads = 256;
+constexpr int64_t kManyWaves = 8192;
 
-// LANES hold a head; a group of them takes HEADS heads of one token, one behind the other.
+// LANES hold a head, a wave 64 / LANES heads side by side, HEADS times.
 template <typename T, int LANES, int HEADS>
 __global__ __launch_bounds__(kHeadNormThreads) void head_norm_rope_kernel(HeadNormParams p) {
-  const uint32_t unit = blockIdx.x * (kHeadNormThreads / LANES) + threadIdx.x / LANES;
+  constexpr int kSide = 64 / LANES;
+  const uint32_t unit = __builtin_amdgcn_readfirstlane(blockIdx.x * (kHeadNormThreads / 64) + threadIdx.x / 64);
   const uint32_t local = unit / p.per_token;
-  if (local >= p.tokens) return;  // uniform over a group
+  if (local >= p.tokens) return;
   uint32_t at = unit - local * p.per_token.d;
   const int64_t t = p.first_token + local;
-  const int l = threadIdx.x % LANES;
-  const bool active = l * 8 < p.D;
   int kind = 0;
   if (at >= p.units_q) {
     at -= p.units_q;
@@ -69,84 +77,117 @@ __global__ __launch_bounds__(kHeadNormThreads) void head_norm_rope_kernel(HeadNo
       kind = 2;
     }
   }
-  const HeadRows& r = p.rows[kind];
-  const bool halves = !p.interleaved && 8 * l < p.R;
-  const int c0 = halves ? 4 * l : 8 * l, c1 = halves ? 4 * l + p.R / 2 : 8 * l + 4;
+  kind = __builtin_amdgcn_readfirstlane(kind);
+  const HeadRows r = p.rows[kind];
   int64_t row = t;
   if (kind != 0 && p.slots) {
     row = p.slots[t];
     if ((uint64_t)row >= (uint64_t)p.n_slots) return;
   }
-  float cs[4] = {1.0f, 1.0f, 1.0f, 1.0f}, sn[4] = {0.0f, 0.0f, 0.0f, 0.0f};
   const int64_t pos = p.positions ? p.positions[t] : t;
-  const bool rotate = kind != 2 && 8 * l < p.R && (uint64_t)pos < (uint64_t)p.table_rows;
-  if (rotate) {
-    const int64_t a = pos * (p.R / 2) + 4 * l;
+  const int l = threadIdx.x % LANES, h0 = (int)at * kSide * HEADS + (int)(threadIdx.x & 63) / LANES;
+  const bool active = l * 8 < p.D;
+  const bool halves = !p.interleaved && 8 * l < p.R;
+  const int c0 = halves ? 4 * l : 8 * l, c1 = halves ? 4 * l + p.R / 2 : 8 * l + 4;
+
+  uint2 x[HEADS][2], w[2] = {};
+  float4 wf[2] = {}, cs = make_float4(1.0f, 1.0f, 1.0f, 1.0f), sn = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+  const uint16_t* src = r.x + t * r.stride_token;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      cs[i] = p.cos[a + i];
-      sn[i] = p.sin[a + i];
+  for (int i = 0; i < HEADS; ++i) {
+    const int h = h0 + i * kSide;
+    if (active && h < r.heads) {
+      x[i][0] = *reinterpret_cast<const uint2*>(src + h * r.stride_head + c0);
+      x[i][1] = *reinterpret_cast<const uint2*>(src + h * r.stride_head + c1);
+    } else {
+      x[i][0] = x[i][1] = make_uint2(0, 0);
     }
   }
-  float w[8];
   if (r.weight && active) {
     if (r.weight_f32) {
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        w[i] = static_cast<const float*>(r.weight)[c0 + i];
-        w[4 + i] = static_cast<const float*>(r.weight)[c1 + i];
-      }
+      wf[0] = *reinterpret_cast<const float4*>(static_cast<const float*>(r.weight) + c0);
+      wf[1] = *reinterpret_cast<const float4*>(static_cast<const float*>(r.weight) + c1);
     } else {
-      load4<T>(static_cast<const uint16_t*>(r.weight) + c0, w);
-      load4<T>(static_cast<const uint16_t*>(r.weight) + c1, w + 4);
+      w[0] = *reinterpret_cast<const uint2*>(static_cast<const uint16_t*>(r.weight) + c0);
+      w[1] = *reinterpret_cast<const uint2*>(static_cast<const uint16_t*>(r.weight) + c1);
     }
   }
+  const bool rotate = kind != 2 && p.R != 0 && (uint64_t)pos < (uint64_t)p.table_rows;
+  if (rotate && 8 * l < p.R) {
+    cs = *reinterpret_cast<const float4*>(p.cos + pos * (p.R / 2) + 4 * l);
+    sn = *reinterpret_cast<const float4*>(p.sin + pos * (p.R / 2) + 4 * l);
+  }
+  float f[8] = {wf[0].x, wf[0].y, wf[0].z, wf[0].w, wf[1].x, wf[1].y, wf[1].z, wf[1].w};
+  if (r.weight && !r.weight_f32) {
+    unpack4<T>(w[0], f);
+    unpack4<T>(w[1], f + 4);
+  }
+  const float cc[4] = {cs.x, cs.y, cs.z, cs.w}, ss[4] = {sn.x, sn.y, sn.z, sn.w};
+  uint16_t* dst = r.out + row * r.out_stride_token;
+#pragma unroll
   for (int i = 0; i < HEADS; ++i) {
-    const int h = at * HEADS + i;
-    if (h >= r.heads) return;
-    float x[8] = {0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f};
-    const uint16_t* src = r.x + t * r.stride_token + h * r.stride_head;
-    if (active) {
-      load4<T>(src + c0, x);
-      load4<T>(src + c1, x + 4);
-    }
+    const int h = h0 + i * kSide;
+    float y[8];
+    unpack4<T>(x[i][0], y);
+    unpack4<T>(x[i][1], y + 4);
     if (r.weight) {
       float sum = 0.0f;
 #pragma unroll
-      for (int j = 0; j < 8; ++j) sum = fmaf(x[j], x[j], sum);
+      for (int j = 0; j < 8; ++j) sum = fmaf(y[j], y[j], sum);
       const float scale = rsqrtf(fmaf(sum_over_lanes<LANES>(sum), p.inv_D, p.eps));
 #pragma unroll
-      for (int j = 0; j < 8; ++j) x[j] = x[j] * scale * w[j];
+      for (int j = 0; j < 8; ++j) y[j] = y[j] * scale * f[j];
     }
-    if (rotate) {
-      if (halves) {
+    if (rotate && 8 * l < p.R) {  // nothing is turned by angles of zero, but a product with an infinity would be NaN
+      const bool apart = halves;
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          const float a = x[j], b = x[4 + j];
-          x[j] = a * cs[j] - b * sn[j];
-          x[4 + j] = b * cs[j] + a * sn[j];
-        }
-      } else {
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          const float a = x[2 * j], b = x[2 * j + 1];
-          x[2 * j] = a * cs[j] - b * sn[j];
-          x[2 * j + 1] = b * cs[j] + a * sn[j];
+      for (int j = 0; j < 4; ++j) {
+        const float a = apart ? y[j] : y[2 * j], b = apart ? y[4 + j] : y[2 * j + 1];
+        const float a2 = a * cc[j] - b * ss[j], b2 = b * cc[j] + a * ss[j];
+        if (apart) {
+          y[j] = a2;
+          y[4 + j] = b2;
+        } else {
+          y[2 * j] = a2;
+          y[2 * j + 1] = b2;
         }
       }
     }
-    uint16_t* dst = r.out + row * r.out_stride_token + h * r.out_stride_head;
-    if (active) {
-      *reinterpret_cast<uint2*>(dst + c0) = make_uint2(T::pack2(x[0], x[1]), T::pack2(x[2], x[3]));
-      *reinterpret_cast<uint2*>(dst + c1) = make_uint2(T::pack2(x[4], x[5]), T::pack2(x[6], x[7]));
+    if (active && h < r.heads) {
+      *reinterpret_cast<uint2*>(dst + h * r.out_stride_head + c0) = make_uint2(T::pack2(y[0], y[1]), T::pack2(y[2], y[3]));
+      *reinterpret_cast<uint2*>(dst + h * r.out_stride_head + c1) = make_uint2(T::pack2(y[4], y[5]), T::pack2(y[6], y[7]));
     }
   }
 }
 
+// Waves of LANES lanes a head and `heads` heads a lane that a token takes.
+static uint32_t waves_for(int num_heads, int lanes, int heads) {
+  const int each = 64 / lanes * heads;
+  return (uint32_t)((num_heads + each - 1) / each);
+}
+
+template <typename T, int LANES, int HEADS>
+static void launch_head_norm(HeadNormParams p, int64_t tokens, hipStream_t stream) {
+  p.units_q = waves_for(p.rows[0].heads, LANES, HEADS);
+  p.units_kv = waves_for(p.rows[1].heads, LANES, HEADS);
+  const uint32_t per_token = p.units_q + p.units_kv + waves_for(p.rows[2].heads, LANES, HEADS);
+  p.per_token = divisor(per_token);
+  const int64_t most = (1ll << 30) / per_token;  // waves are numbered in 32 bits
+  for (int64_t first = 0; first < tokens; first += most) {
+    p.first_token = first;
+    p.tokens = (uint32_t)(tokens - first < most ? tokens - first : most);
+    const uint32_t per_wg = kHeadNormThreads / 64, groups = (p.tokens * per_token + per_wg - 1) / per_wg;
+    head_norm_rope_kernel<T, LANES, HEADS><<<groups, kHeadNormThreads, 0, stream>>>(p);
+  }
+}
+
 template <typename T, int LANES>
-void launch_head_norm(const HeadNormParams& p, uint32_t units, hipStream_t stream) {
-  const uint32_t per_wg = kHeadNormThreads / LANES;
-  head_norm_rope_kernel<T, LANES, 1><<<(units + per_wg - 1) / per_wg, kHeadNormThreads, 0, stream>>>(p);
+static void launch_head_norm(const HeadNormParams& p, int64_t tokens, hipStream_t stream) {
+  const int64_t waves = tokens * (waves_for(p.rows[0].heads, LANES, 1) + 2 * waves_for(p.rows[1].heads, LANES, 1));
+  if (waves > kManyWaves)
+    launch_head_norm<T, LANES, 2>(p, tokens, stream);
+  else
+    launch_head_norm<T, LANES, 1>(p, tokens, stream);
 }
 
 static int check_rows(const ll_head_rows* r, const char* name, bool may_norm) {
@@ -199,32 +240,22 @@ extern "C" int ll_head_norm_rope(int dtype, int64_t tokens, int head_dim, const 
   p.positions = positions;
   p.slots = slots;
   p.n_slots = n_slots;
-  p.units_q = (uint32_t)q->num_heads;
-  p.units_kv = (uint32_t)k->num_heads;
-  const uint32_t per_token = p.units_q + p.units_kv + (uint32_t)v->num_heads;
-  if (per_token == 0 || tokens == 0) return LL_OK;
-  p.per_token = divisor(per_token);
-  const int64_t most = (1ll << 30) / per_token;  // units are numbered in 32 bits
-  for (int64_t first = 0; first < tokens; first += most) {
-    p.first_token = first;
-    p.tokens = (uint32_t)(tokens - first < most ? tokens - first : most);
-    const uint32_t units = p.tokens * per_token;
-    const hipStream_t s = static_cast<hipStream_t>(stream);
-#define LL_LAUNCH(T)                                            \
-  if (head_dim <= 64) {                                         \
-    launch_head_norm<T, 8>(p, units, s);                        \
-  } else if (head_dim <= 128) {                                 \
-    launch_head_norm<T, 16>(p, units, s);                       \
-  } else {                                                      \
-    launch_head_norm<T, 32>(p, units, s);                       \
+  if (tokens == 0 || q->num_heads + k->num_heads == 0) return LL_OK;
+  const hipStream_t s = static_cast<hipStream_t>(stream);
+#define LL_LAUNCH(T)                           \
+  if (head_dim <= 64) {                        \
+    launch_head_norm<T, 8>(p, tokens, s);      \
+  } else if (head_dim <= 128) {                \
+    launch_head_norm<T, 16>(p, tokens, s);     \
+  } else {                                     \
+    launch_head_norm<T, 32>(p, tokens, s);     \
   }
-    if (dtype == LL_DTYPE_BF16) {
-      LL_LAUNCH(Bf16)
-    } else {
-      LL_LAUNCH(F16)
-    }
+  if (dtype == LL_DTYPE_BF16) {
+    LL_LAUNCH(Bf16)
+  } else {
+    LL_LAUNCH(F16)
+  }
 #undef LL_LAUNCH
-    LL_CHECK_LAUNCH("ll_head_norm_rope");
-  }
+  LL_CHECK_LAUNCH("ll_head_norm_rope");
   return LL_OK;
 }

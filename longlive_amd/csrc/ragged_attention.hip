@@ -24,6 +24,7 @@
 #include <algorithm>
 #include <cmath>
 #include <type_traits>
+#include <utility>
 
 namespace ll {
 
@@ -214,6 +215,12 @@ __device__ __forceinline__ float* record_of(const RaParams& p, const RaPlace& at
 template <int D>
 constexpr int kRaLds = 2 * 2 * kRaKeys * 2 * D + 4 * 2 * 256 + 4 * 32 * 8;  // stages, looked-up places, maxima and sums
 
+// f(0), f(1), ... with every index a constant of its own type.
+template <typename F, int... I>
+__device__ __forceinline__ void each_index(F& f, std::integer_sequence<int, I...>) {
+  (f(std::integral_constant<int, I>{}), ...);
+}
+
 // The reference point of the exponentials follows the maximum once it is 2^2 ahead: fewer rescalings, no further from 64 bits.
 constexpr float kRaStep = 2.0f;
 
@@ -223,7 +230,7 @@ __global__ __launch_bounds__(kRaThreads, 2) void ragged_attention_kernel(RaParam
   constexpr int kRowsPerLoad = 1024 / kRowBytes, kGroupLoads = 16 / kRowsPerLoad;  // loads of 16 rows
   constexpr int kStepBytes = kRaKeys * kRowBytes;                                  // K or V of a step
   constexpr bool kLooksUp = KIND != kRaRows;
-  extern __shared__ __attribute__((aligned(16))) uint8_t smem[];
+  extern __shared__ __attribute__((aligned(1024))) uint8_t smem[];
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), l32 = lane & 31, lh = lane >> 5;
 
   if (blockIdx.x >= p.work_groups) {  // rows outside every stream
@@ -299,33 +306,31 @@ __global__ __launch_bounds__(kRaThreads, 2) void ragged_attention_kernel(RaParam
   };
 
   // ---- loads: 16 rows, the keys of lanes r0 .. r0 + 15, to 16 rows of LDS
-  uint32_t k_off[kGroupLoads], v_off[kGroupLoads];
-  int k_part[kGroupLoads], v_part[kGroupLoads];
-#pragma unroll
-  for (int i = 0; i < kGroupLoads; ++i) {
-    const int row = i * kRowsPerLoad + lane / kPieces;
-    k_part[i] = k_piece<D>(row, lane % kPieces) * 16;
-    v_part[i] = v_piece<D>(row, lane % kPieces) * 16;
-    k_off[i] = (uint32_t)row * p.k_stride_row * 2 + k_part[i];
-    v_off[i] = (uint32_t)row * p.v_stride_row * 2 + v_part[i];
-  }
   const bool whole_groups = KIND != kRaPaged || p.page.d % 16 == 0;  // 16 rows lie one behind the other
   auto load_rows = [&](bool values, int r0, uint32_t lds) __attribute__((always_inline)) {
     const uint16_t* base = values ? v_head : k_head;
     const uint32_t per_page = values ? p.v_stride_page : p.k_stride_page, per_row = values ? p.v_stride_row : p.k_stride_row;
+    int ln = lane;
+    asm volatile("" : "+v"(ln));  // the lane's offsets are formed here: kept over the loop they take registers it does not have
+    const int row0 = ln / kPieces, piece = ln % kPieces;
     if (whole_groups && ((uint32_t)(there >> r0) & 0xFFFFu) == 0xFFFFu) {
       uint64_t at = (uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)at_row, r0) * per_row;
       if constexpr (KIND == kRaPaged) at += (uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)at_page, r0) * per_page;
       const uint16_t* from_here = uniform_pointer(base + at);
+      const uint32_t first = (uint32_t)row0 * per_row * 2;
 #pragma unroll
-      for (int i = 0; i < kGroupLoads; ++i) load16_to_lds(values ? v_off[i] : k_off[i], from_here, lds + i * 1024);
+      for (int i = 0; i < kGroupLoads; ++i) {
+        const int row = i * kRowsPerLoad + row0;
+        const uint32_t part = (uint32_t)(values ? v_piece<D>(row, piece) : k_piece<D>(row, piece)) * 16;
+        load16_to_lds(first + (uint32_t)i * kRowsPerLoad * per_row * 2 + part, from_here, lds + i * 1024);
+      }
     } else {
 #pragma unroll
       for (int i = 0; i < kGroupLoads; ++i) {
-        const int row = r0 + i * kRowsPerLoad + lane / kPieces;
+        const int in_group = i * kRowsPerLoad + row0, row = r0 + in_group;
         uint64_t at = (uint64_t)(uint32_t)__shfl((int)at_row, row) * per_row;
         if constexpr (KIND == kRaPaged) at += (uint64_t)(uint32_t)__shfl((int)at_page, row) * per_page;
-        const uint8_t* src = reinterpret_cast<const uint8_t*>(base + at) + (values ? v_part[i] : k_part[i]);
+        const uint8_t* src = reinterpret_cast<const uint8_t*>(base + at) + (values ? v_piece<D>(in_group, piece) : k_piece<D>(in_group, piece)) * 16;
         load16_to_lds((there >> row) & 1 ? src : reinterpret_cast<const uint8_t*>(kRaZeros), lds + i * 1024);
       }
     }
@@ -333,7 +338,15 @@ __global__ __launch_bounds__(kRaThreads, 2) void ragged_attention_kernel(RaParam
 
   // ---- scores and probabilities of NT groups of 32 keys from `base` on
   // S^T: register r of sc[kt] is key 32 kt + 8 (r / 4) + 4 lh + r % 4
-  auto scores = [&](auto& sc, const uint8_t* k_rows) __attribute__((always_inline)) {
+  typedef const __attribute__((address_space(3))) short8v* lds_short8;
+  typedef __attribute__((address_space(3))) short4v* lds_short4;
+  const uint32_t lds0 = lds_at(smem);
+  // where the lane's fragments begin in LDS rows; a fragment's number turns bits of the piece's position
+  const uint32_t k_lane = (uint32_t)(l32 * kRowBytes + k_piece<D>(l32, lh) * 16);
+  auto read_k = [&](uint32_t k_rows, int kt, int ks) __attribute__((always_inline)) {
+    return *(lds_short8)(uintptr_t)(((k_rows + k_lane) ^ (uint32_t)(32 * ks)) + 32 * kt * kRowBytes);
+  };
+  auto scores = [&](auto& sc, uint32_t k_rows) __attribute__((always_inline)) {
     constexpr int NT = std::extent<std::remove_reference_t<decltype(sc)>>::value;
 #pragma unroll
     for (int kt = 0; kt < NT; ++kt) {
@@ -341,8 +354,7 @@ __global__ __launch_bounds__(kRaThreads, 2) void ragged_attention_kernel(RaParam
       for (int r = 0; r < 16; ++r) sc[kt][r] = 0.0f;
 #pragma unroll
       for (int ks = 0; ks < kSteps; ++ks) {
-        const short8v a = *reinterpret_cast<const short8v*>(k_rows + (32 * kt + l32) * kRowBytes + k_piece<D>(l32, 2 * ks + lh) * 16);
-        sc[kt] = T::mfma(a, qf[ks], sc[kt]);
+        sc[kt] = T::mfma(read_k(k_rows, kt, ks), qf[ks], sc[kt]);
       }
     }
   };
@@ -362,7 +374,8 @@ __global__ __launch_bounds__(kRaThreads, 2) void ragged_attention_kernel(RaParam
         sc[kt][r] = seen ? sc[kt][r] : -INFINITY;
       }
   };
-  auto attend = [&](auto& sc, const uint8_t* v_rows, auto v_arrived) __attribute__((always_inline)) {
+  float neg = 0.0f;
+  auto follow = [&](auto& sc) __attribute__((always_inline)) {  // the reference point for sc, which is masked
     constexpr int NT = std::extent<std::remove_reference_t<decltype(sc)>>::value;
     float mx = sc[0][0];
 #pragma unroll
@@ -370,19 +383,30 @@ __global__ __launch_bounds__(kRaThreads, 2) void ragged_attention_kernel(RaParam
 #pragma unroll
       for (int r = 0; r < 16; ++r) mx = fmaxf(mx, sc[kt][r]);
     mx = exchange_max(mx);
-    // a row that has seen nothing yet stays at -inf; 0 stands for it in the exponents, where -inf - -inf would be NaN
     const bool raise = (mx - m) * p.scale_log2 > kRaStep;
     if (__builtin_amdgcn_ballot_w64(raise) != 0) {
       const float alpha = raise ? __builtin_amdgcn_exp2f((m - mx) * p.scale_log2) : 1.0f;
       m = raise ? mx : m;
+      // a row that has seen nothing yet stays at -inf; 0 stands for it in the exponents, where -inf - -inf would be NaN
+      neg = m == -INFINITY ? 0.0f : -m * p.scale_log2;
       l *= alpha;
 #pragma unroll
       for (int dt = 0; dt < kDTiles; ++dt)
 #pragma unroll
         for (int r = 0; r < 16; ++r) o[dt][r] *= alpha;
     }
-    const float neg = m == -INFINITY ? 0.0f : -m * p.scale_log2;
-    v_arrived();
+  };
+  // V^T of 16 keys and 32 columns: a lane needs column 32 dt + l32 of the keys 8 j + 4 lh + 0 .. 3 (j = 0, 1: the order of the scores'
+  // registers).  A read serves 16 lanes: lane i points at row i / 4, columns 4 (i % 4) .. + 3, and each receives a column of the four rows.
+  const uint32_t v_lane = (uint32_t)((4 * lh + ((lane & 15) >> 2)) * kRowBytes +
+                                     v_piece<D>(4 * lh + ((lane & 15) >> 2), 2 * ((lane >> 4) & 1) + ((lane & 3) >> 1)) * 16 + (lane & 1) * 8);
+  auto read_v = [&](uint32_t v_rows, int step, int dt, short4v (&dst)[2]) __attribute__((always_inline)) {
+#pragma unroll
+    for (int j = 0; j < 2; ++j)
+      dst[j] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_short4)(uintptr_t)(((v_rows + v_lane) ^ (uint32_t)(64 * dt)) + (16 * step + 8 * j) * kRowBytes));
+  };
+  auto weigh = [&](auto& sc, uint32_t v_rows) __attribute__((always_inline)) {
+    constexpr int NT = std::extent<std::remove_reference_t<decltype(sc)>>::value;
 #pragma unroll
     for (int step = 0; step < 2 * NT; ++step) {
       uint32_t w[4];
@@ -394,19 +418,69 @@ __global__ __launch_bounds__(kRaThreads, 2) void ragged_attention_kernel(RaParam
         w[u] = T::pack2(p0, p1);  // at most 2^kRaStep: no overflow, and half a step's error each, as small as the result's own
       }
       const short8v pb = __builtin_bit_cast(short8v, make_uint4(w[0], w[1], w[2], w[3]));
-      typedef __attribute__((address_space(3))) short4v* lds_short4;
 #pragma unroll
       for (int dt = 0; dt < kDTiles; ++dt) {
         short4v part[2];
-#pragma unroll
-        for (int j = 0; j < 2; ++j) {
-          const int row = 4 * lh + ((lane & 15) >> 2), piece = 4 * dt + 2 * ((lane >> 4) & 1) + ((lane & 3) >> 1);
-          part[j] = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
-              (lds_short4)(v_rows + (row + 16 * step + 8 * j) * kRowBytes + v_piece<D>(row, piece) * 16 + (lane & 1) * 8));
-        }
+        read_v(v_rows, step, dt, part);
         o[dt] = T::mfma(__builtin_shufflevector(part[0], part[1], 0, 1, 2, 3, 4, 5, 6, 7), pb, o[dt]);
       }
     }
+  };
+  // One step of a tile of more than 32 rows and the scores of the next: every slot one MFMA (S^T of the next step, then O^T of this one) with
+  // what runs beside it, held in place by scheduling barriers: the LDS reads of MFMAs some slots later, and the probabilities, a pair
+  // of keys' multiply-adds, exponentials and packing in three slots in a row.
+  auto step_and_next = [&](float16v (&sc)[2], float16v (&nx)[2], uint32_t next_k, uint32_t v_rows) __attribute__((always_inline)) {
+    constexpr int kS = 2 * kSteps, kSlots = kS + 4 * kDTiles, kAhead = 4, kRing = kAhead + 1, kVAhead = 3, kVRing = kVAhead + 1;
+    short8v fk[kRing];
+    short4v fv[kVRing][2];
+    uint32_t pw[16];
+    float x[2][2], e[2][2];
+    auto fetch_k = [&](auto tag) __attribute__((always_inline)) {
+      constexpr int i = decltype(tag)::value;
+      fk[i % kRing] = read_k(next_k, i / kSteps, i % kSteps);
+    };
+    each_index(fetch_k, std::make_integer_sequence<int, kAhead>{});
+    __builtin_amdgcn_sched_barrier(0);
+    auto one_slot = [&](auto slot_tag) __attribute__((always_inline)) {
+      constexpr int slot = decltype(slot_tag)::value;
+      if constexpr (slot + kAhead < kS) fetch_k(std::integral_constant<int, slot + kAhead>{});
+      if constexpr (slot + kVAhead >= kS && slot + kVAhead < kSlots) {
+        constexpr int u = slot + kVAhead - kS;
+        read_v(v_rows, u / kDTiles, u % kDTiles, fv[u % kVRing]);
+      }
+      __builtin_amdgcn_sched_barrier(0);
+      if constexpr (slot < kS) {
+        constexpr int kt = slot / kSteps, ks = slot % kSteps;
+        const float16v zero = {0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f};
+        nx[kt] = T::mfma(fk[slot % kRing], qf[ks], ks == 0 ? zero : nx[kt]);
+      } else {
+        constexpr int u = slot - kS, step = u / kDTiles, dt = u % kDTiles;
+        const short4v(&v)[2] = fv[u % kVRing];
+        const short8v pb = __builtin_bit_cast(short8v, make_uint4(pw[4 * step], pw[4 * step + 1], pw[4 * step + 2], pw[4 * step + 3]));
+        o[dt] = T::mfma(__builtin_shufflevector(v[0], v[1], 0, 1, 2, 3, 4, 5, 6, 7), pb, o[dt]);
+      }
+      // pair i of the 16 pairs of keys begins in slot i * kSlots * 3 / 64
+      auto pairs = [&](auto pair_tag) __attribute__((always_inline)) {
+        constexpr int pair = decltype(pair_tag)::value, begin = pair * kSlots * 3 / 64;
+        if constexpr (slot == begin + 2) {
+          pw[pair] = T::pack2(e[pair & 1][0], e[pair & 1][1]);  // at most 2^kRaStep, see weigh
+          asm volatile("" : "+v"(pw[pair]));                    // here, and not sunk to the MFMA that reads it
+          l += e[pair & 1][0] + e[pair & 1][1];
+        }
+        if constexpr (slot == begin + 1) {
+          e[pair & 1][0] = __builtin_amdgcn_exp2f(x[pair & 1][0]);
+          e[pair & 1][1] = __builtin_amdgcn_exp2f(x[pair & 1][1]);
+        }
+        if constexpr (slot == begin) {
+          constexpr int kt = pair >> 3, r = 2 * (pair & 7);
+          x[pair & 1][0] = fmaf(sc[kt][r], p.scale_log2, neg);
+          x[pair & 1][1] = fmaf(sc[kt][r + 1], p.scale_log2, neg);
+        }
+      };
+      each_index(pairs, std::make_integer_sequence<int, 16>{});
+      __builtin_amdgcn_sched_barrier(0);
+    };
+    each_index(one_slot, std::make_integer_sequence<int, kSlots>{});
   };
 
   const int out_token = token;
@@ -424,36 +498,64 @@ __global__ __launch_bounds__(kRaThreads, 2) void ragged_attention_kernel(RaParam
   };
 
   if (!narrow) {
-    uint8_t* const stages = smem;
-    const uint32_t stages_lds = lds_at(smem);
-    auto load_step = [&](int stage) __attribute__((always_inline)) {  // each wave a quarter of the rows
-      load_rows(false, wave * 16, stages_lds + stage * 2 * kStepBytes + wave * 16 * kRowBytes);
-      load_rows(true, wave * 16, stages_lds + stage * 2 * kStepBytes + kStepBytes + wave * 16 * kRowBytes);
+    // K of step s is in buffer s & 1 an iteration before V of step s is: scores are a step ahead.
+    const uint32_t k_lds = lds0 + wave * 16 * kRowBytes, v_lds = k_lds + 2 * kStepBytes;
+    auto load_k = [&](int s) __attribute__((always_inline)) {
+      take_places(key_base(s) + lane, s & 1);
+      load_rows(false, wave * 16, k_lds + (s & 1) * kStepBytes);
+      if (kLooksUp && s + 1 < s_end) look_up(key_base(s + 1) + lane, (s + 1) & 1);
     };
+    auto load_v = [&](int s) __attribute__((always_inline)) { load_rows(true, wave * 16, v_lds + (s & 1) * kStepBytes); };
+    const uint32_t k_rows = lds0, v_rows = lds0 + 2 * kStepBytes;
+    float16v sc[2][2];
+    uint64_t exist = 0;
     if (s_begin < s_end) {
       if (kLooksUp) {
         look_up(key_base(s_begin) + lane, s_begin & 1);
         wait_loads<0>();
       }
-      take_places(key_base(s_begin) + lane, s_begin & 1);
-      load_step(s_begin & 1);
-      if (kLooksUp && s_begin + 1 < s_end) look_up(key_base(s_begin + 1) + lane, (s_begin + 1) & 1);
-    }
-    for (int s = s_begin; s < s_end; ++s) {
-      const uint64_t exist = there;
-      wait_loads<0>();
-      __syncthreads();  // the step's keys are in LDS, and every wave is done with those of the step before
-      if (s + 1 < s_end) {
-        take_places(key_base(s + 1) + lane, (s + 1) & 1);
-        load_step((s + 1) & 1);
-        if (kLooksUp && s + 2 < s_end) look_up(key_base(s + 2) + lane, s & 1);
+      load_k(s_begin);
+      exist = there;
+      load_v(s_begin);
+      wait_loads<kGroupLoads>();
+      __syncthreads();
+      if (s_begin + 1 < s_end) load_k(s_begin + 1);
+      if (!idle) {
+        scores(sc[0], k_rows + (s_begin & 1) * kStepBytes);
+        mask(sc[0], key_base(s_begin), exist);
+        follow(sc[0]);
       }
-      if (idle) continue;
-      const uint8_t* rows = stages + (s & 1) * 2 * kStepBytes;
-      float16v sc[2];
-      scores(sc, rows);
-      mask(sc, key_base(s), exist);
-      attend(sc, rows + kStepBytes, [] {});
+    }
+    auto iteration = [&](int s, auto from_tag) __attribute__((always_inline)) {
+      constexpr int from_buffer = decltype(from_tag)::value;
+      wait_loads<0>();
+      __syncthreads();  // K of step s + 1 and V of step s are in LDS, and every wave is done with K of step s and V of step s - 1
+      exist = there;    // of step s + 1
+      load_v(s + 1);    // from the places of the last load_k
+      if (s + 2 < s_end) load_k(s + 2);
+      if (idle) return;
+      step_and_next(sc[from_buffer], sc[from_buffer ^ 1], k_rows + ((s + 1) & 1) * kStepBytes, v_rows + (s & 1) * kStepBytes);
+      mask(sc[from_buffer ^ 1], key_base(s + 1), exist);
+      follow(sc[from_buffer ^ 1]);
+    };
+    int s = s_begin;
+    for (; s + 2 < s_end; s += 2) {
+      iteration(s, std::integral_constant<int, 0>{});
+      iteration(s + 1, std::integral_constant<int, 1>{});
+    }
+    bool second = false;
+    if (s + 1 < s_end) {
+      iteration(s, std::integral_constant<int, 0>{});
+      second = true;
+      ++s;
+    }
+    if (s < s_end) {
+      wait_loads<0>();
+      __syncthreads();
+      if (!idle) {
+        if (second) weigh(sc[1], v_rows + (s & 1) * kStepBytes);
+        else weigh(sc[0], v_rows + (s & 1) * kStepBytes);
+      }
     }
     if (idle) return;
     l = exchange_sum(l);
@@ -470,8 +572,7 @@ __global__ __launch_bounds__(kRaThreads, 2) void ragged_attention_kernel(RaParam
   }
 
   // ---- up to 32 rows: groups of 32 keys u = 2 s + half, every fourth one this wave's
-  uint8_t* const rows = smem + wave * kStepBytes;  // 32 rows of K, 32 of V
-  const uint32_t rows_lds = lds_at(rows);
+  const uint32_t rows_lds = lds0 + wave * kStepBytes;  // 32 rows of K, 32 of V
   constexpr int kLoads = 2 * kGroupLoads;  // of K or of V
   auto group_base = [&](int u) __attribute__((always_inline)) { return key_base(u >> 1) + 32 * (u & 1); };
   auto load_group = [&](bool values) __attribute__((always_inline)) {
@@ -494,7 +595,7 @@ __global__ __launch_bounds__(kRaThreads, 2) void ragged_attention_kernel(RaParam
       const bool more = u + 4 < u_end;
       wait_loads<kLoads>();  // K, and the places of the next group; V may be on its way
       float16v sc[1];
-      scores(sc, rows);
+      scores(sc, rows_lds);
       if (more) {
         take_places(group_base(u + 4) + l32, slot);
         wait_lds_reads();
@@ -502,10 +603,10 @@ __global__ __launch_bounds__(kRaThreads, 2) void ragged_attention_kernel(RaParam
         if (kLooksUp) look_up(group_base(min(u + 8, u_end - 1)) + l32, slot ^ 1);
       }
       mask(sc, group_base(u), exist);
-      attend(sc, rows + 32 * kRowBytes, [&]() __attribute__((always_inline)) {
-        if (more) wait_loads<kLoads + (kLooksUp ? 1 : 0)>();
-        else wait_loads<0>();
-      });
+      follow(sc);
+      if (more) wait_loads<kLoads + (kLooksUp ? 1 : 0)>();
+      else wait_loads<0>();
+      weigh(sc, rows_lds + 32 * kRowBytes);
       if (more) {
         wait_lds_reads();
         load_group(true);
@@ -517,7 +618,7 @@ __global__ __launch_bounds__(kRaThreads, 2) void ragged_attention_kernel(RaParam
   float2* const ml = reinterpret_cast<float2*>(smem + 4 * kStepBytes + 4 * 512);
   if (lh == 0) ml[wave * 32 + l32] = make_float2(m, l);
   {
-    float4* mine = reinterpret_cast<float4*>(rows);
+    float4* mine = reinterpret_cast<float4*>(smem + wave * kStepBytes);
 #pragma unroll
     for (int dt = 0; dt < kDTiles; ++dt)
 #pragma unroll
