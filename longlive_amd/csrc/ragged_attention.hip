@@ -123,6 +123,9 @@ __device__ const uint4 kRaZeros[1] = {{0, 0, 0, 0}};
 
 __device__ __forceinline__ int64_t stream_start(const RaParams& p, int b) { return min(max((int64_t)p.q_starts[b], (int64_t)0), p.n_queries); }
 
+// The lowest n of 64 bits, for any n.
+__device__ __forceinline__ uint64_t low_bits(int n) { return n <= 0 ? 0 : n >= 64 ? ~0ull : ~(~0ull << n); }
+
 // The tile of a workgroup.
 struct RaTile {
   int stream;
@@ -271,6 +274,9 @@ __global__ __launch_bounds__(kRaThreads, 2) void ragged_attention_kernel(RaParam
 #pragma unroll
     for (int ks = 0; ks < kSteps; ++ks) qf[ks] = *reinterpret_cast<const short8v*>(src + 16 * ks);
   }
+  // Here, where the compiler sees it: it would otherwise count the loads of the queries as under way for good, and wait for the keys'
+  // loads in their place ahead of every product.  0x0F70 = vmcnt(0), other counters untouched.
+  __builtin_amdgcn_s_waitcnt(0x0F70);
   float16v o[kDTiles];
 #pragma unroll
   for (int dt = 0; dt < kDTiles; ++dt)
@@ -358,30 +364,31 @@ __global__ __launch_bounds__(kRaThreads, 2) void ragged_attention_kernel(RaParam
       }
     }
   };
-  auto mask = [&](auto& sc, int base, uint64_t exist) __attribute__((always_inline)) {
+  auto mask = [&](auto& sc, int base, uint64_t exist) __attribute__((always_inline)) {  // whether it hides any
     constexpr int NT = std::extent<std::remove_reference_t<decltype(sc)>>::value;
     constexpr uint64_t kAll = NT == 2 ? ~0ull : 0xFFFFFFFFull;
     const int end = base + 32 * NT;
-    if ((exist & kAll) == kAll && end <= last0 && (base >= from1 || end <= (int)p.sink)) return;
-    const uint64_t bits = exist >> (4 * lh);
-    const int first = base + 4 * lh;
+    if ((exist & kAll) == kAll && end <= last0 && (base >= from1 || end <= (int)p.sink)) return false;
+    // one bit a key: it exists, it lies below `last`, and from `from` on or below the sink
+    const uint64_t seen = exist & low_bits(last - base) & (~low_bits(from - base) | low_bits((int)p.sink - base));
+    const uint32_t bits[2] = {(uint32_t)seen >> (4 * lh), (uint32_t)(seen >> 32) >> (4 * lh)};
 #pragma unroll
     for (int kt = 0; kt < NT; ++kt)
 #pragma unroll
-      for (int r = 0; r < 16; ++r) {
-        const int at = 32 * kt + 8 * (r / 4) + r % 4, key = first + at;
-        const bool seen = key < last && (key >= from || key < (int)p.sink) && ((bits >> at) & 1);
-        sc[kt][r] = seen ? sc[kt][r] : -INFINITY;
-      }
+      for (int r = 0; r < 16; ++r) sc[kt][r] = bits[kt] & (1u << (8 * (r / 4) + r % 4)) ? sc[kt][r] : -INFINITY;
+    return true;
   };
   float neg = 0.0f;
-  auto follow = [&](auto& sc) __attribute__((always_inline)) {  // the reference point for sc, which is masked
+  auto largest = [&](auto& sc) __attribute__((always_inline)) {
     constexpr int NT = std::extent<std::remove_reference_t<decltype(sc)>>::value;
     float mx = sc[0][0];
 #pragma unroll
     for (int kt = 0; kt < NT; ++kt)
 #pragma unroll
       for (int r = 0; r < 16; ++r) mx = fmaxf(mx, sc[kt][r]);
+    return mx;
+  };
+  auto follow = [&](float mx) __attribute__((always_inline)) {  // the reference point for scores of which this lane's largest is mx
     mx = exchange_max(mx);
     const bool raise = (mx - m) * p.scale_log2 > kRaStep;
     if (__builtin_amdgcn_ballot_w64(raise) != 0) {
@@ -434,7 +441,7 @@ __global__ __launch_bounds__(kRaThreads, 2) void ragged_attention_kernel(RaParam
     short8v fk[kRing];
     short4v fv[kVRing][2];
     uint32_t pw[16];
-    float x[2][2], e[2][2];
+    float x[2][2], e[2][2], mx = -INFINITY;
     auto fetch_k = [&](auto tag) __attribute__((always_inline)) {
       constexpr int i = decltype(tag)::value;
       fk[i % kRing] = read_k(next_k, i / kSteps, i % kSteps);
@@ -466,6 +473,7 @@ __global__ __launch_bounds__(kRaThreads, 2) void ragged_attention_kernel(RaParam
           pw[pair] = T::pack2(e[pair & 1][0], e[pair & 1][1]);  // at most 2^kRaStep, see weigh
           asm volatile("" : "+v"(pw[pair]));                    // here, and not sunk to the MFMA that reads it
           l += e[pair & 1][0] + e[pair & 1][1];
+          asm volatile("" : "+v"(l));
         }
         if constexpr (slot == begin + 1) {
           e[pair & 1][0] = __builtin_amdgcn_exp2f(x[pair & 1][0]);
@@ -478,9 +486,17 @@ __global__ __launch_bounds__(kRaThreads, 2) void ragged_attention_kernel(RaParam
         }
       };
       each_index(pairs, std::make_integer_sequence<int, 16>{});
+      // the next scores' largest, in the second half of the slots, two slots behind the last product of a group of keys
+      if constexpr (slot >= kSlots / 2 + 2) {
+        constexpr int first = (slot - kSlots / 2 - 2) * 32 / (kSlots / 2 - 2), end = (slot - kSlots / 2 - 1) * 32 / (kSlots / 2 - 2);
+#pragma unroll
+        for (int i = first; i < end; ++i) mx = fmaxf(mx, nx[i >> 4][i & 15]);
+        asm volatile("" : "+v"(mx));
+      }
       __builtin_amdgcn_sched_barrier(0);
     };
     each_index(one_slot, std::make_integer_sequence<int, kSlots>{});
+    return mx;
   };
 
   const int out_token = token;
@@ -523,7 +539,7 @@ __global__ __launch_bounds__(kRaThreads, 2) void ragged_attention_kernel(RaParam
       if (!idle) {
         scores(sc[0], k_rows + (s_begin & 1) * kStepBytes);
         mask(sc[0], key_base(s_begin), exist);
-        follow(sc[0]);
+        follow(largest(sc[0]));
       }
     }
     auto iteration = [&](int s, auto from_tag) __attribute__((always_inline)) {
@@ -534,9 +550,9 @@ __global__ __launch_bounds__(kRaThreads, 2) void ragged_attention_kernel(RaParam
       load_v(s + 1);    // from the places of the last load_k
       if (s + 2 < s_end) load_k(s + 2);
       if (idle) return;
-      step_and_next(sc[from_buffer], sc[from_buffer ^ 1], k_rows + ((s + 1) & 1) * kStepBytes, v_rows + (s & 1) * kStepBytes);
-      mask(sc[from_buffer ^ 1], key_base(s + 1), exist);
-      follow(sc[from_buffer ^ 1]);
+      float mx = step_and_next(sc[from_buffer], sc[from_buffer ^ 1], k_rows + ((s + 1) & 1) * kStepBytes, v_rows + (s & 1) * kStepBytes);
+      if (mask(sc[from_buffer ^ 1], key_base(s + 1), exist)) mx = largest(sc[from_buffer ^ 1]);
+      follow(mx);
     };
     int s = s_begin;
     for (; s + 2 < s_end; s += 2) {
@@ -603,7 +619,7 @@ __global__ __launch_bounds__(kRaThreads, 2) void ragged_attention_kernel(RaParam
         if (kLooksUp) look_up(group_base(min(u + 8, u_end - 1)) + l32, slot ^ 1);
       }
       mask(sc, group_base(u), exist);
-      follow(sc);
+      follow(largest(sc));
       if (more) wait_loads<kLoads + (kLooksUp ? 1 : 0)>();
       else wait_loads<0>();
       weigh(sc, rows_lds + 32 * kRowBytes);
@@ -651,34 +667,35 @@ __global__ __launch_bounds__(kRaThreads, 2) void ragged_attention_kernel(RaParam
   }
 }
 
-// Joins the parts of the tiles that were cut: a workgroup per (kv head, tile).
+// Joins the parts of the tiles that were cut: D / 4 lanes a row, kRaThreads * 4 / D rows of a tile a workgroup.
 template <typename T, int D, int KIND>
 __global__ __launch_bounds__(kRaThreads) void ragged_join_kernel(RaParams p) {
   const RaPlace place{blockIdx.x % (uint32_t)p.kv_heads, blockIdx.x / (uint32_t)p.kv_heads, 0};
   RaTile t;
   if (!find_tile<KIND>(p, place.tile, t) || t.n_parts == 1) return;
-  const int rows = min(kRaTileRows, t.rows - t.first);
-  for (int i = threadIdx.x; i < rows * (D / 4); i += kRaThreads) {
-    const int row = i / (D / 4), column = i % (D / 4) * 4;
-    float m = -INFINITY, l = 0.0f;
-    for (int part = 0; part < t.n_parts; ++part) m = fmaxf(m, record_of<D>(p, place, part)[p.record_rows * D + 2 * row]);
-    float v[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-    for (int part = 0; part < t.n_parts; ++part) {
-      const float* rec = record_of<D>(p, place, part);
-      const float2 e = *reinterpret_cast<const float2*>(rec + p.record_rows * D + 2 * row);
-      const float4 x = *reinterpret_cast<const float4*>(rec + row * D + column);
-      const float w = e.x == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f((e.x - m) * p.scale_log2);
-      l += e.x == -INFINITY ? e.y : e.y * w;
-      v[0] = fmaf(x.x, w, v[0]);
-      v[1] = fmaf(x.y, w, v[1]);
-      v[2] = fmaf(x.z, w, v[2]);
-      v[3] = fmaf(x.w, w, v[3]);
-    }
-    const float inv = l == 0.0f ? 0.0f : 1.0f / l;
-    const int f = t.first + row, token = (uint32_t)f / p.group, head = place.head * p.group.d + (f - token * p.group.d);
-    uint16_t* dst = p.out + (t.q0 + token) * p.out_stride_token + head * p.out_stride_head + column;
-    *reinterpret_cast<uint2*>(dst) = make_uint2(T::pack2(v[0] * inv, v[1] * inv), T::pack2(v[2] * inv, v[3] * inv));
+  const int row = blockIdx.y * (kRaThreads * 4 / D) + threadIdx.x / (D / 4), column = threadIdx.x % (D / 4) * 4;
+  if (row >= min(kRaTileRows, t.rows - t.first)) return;
+  const float* rec = record_of<D>(p, place, 0);
+  const int64_t next = (int64_t)p.record_rows * (D + 2);
+  const float *ml = rec + p.record_rows * D + 2 * row, *x = rec + row * D + column;
+  float m = -INFINITY, l = 0.0f, v[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll 4
+  for (int part = 0; part < t.n_parts; ++part) m = fmaxf(m, ml[part * next]);
+#pragma unroll 4
+  for (int part = 0; part < t.n_parts; ++part) {
+    const float2 e = *reinterpret_cast<const float2*>(ml + part * next);
+    const float4 y = *reinterpret_cast<const float4*>(x + part * next);
+    const float w = e.x == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f((e.x - m) * p.scale_log2);
+    l += e.x == -INFINITY ? e.y : e.y * w;  // a part without a maximum whose sum is NaN has met NaN only
+    v[0] = fmaf(y.x, w, v[0]);
+    v[1] = fmaf(y.y, w, v[1]);
+    v[2] = fmaf(y.z, w, v[2]);
+    v[3] = fmaf(y.w, w, v[3]);
   }
+  const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+  const int f = t.first + row, token = (uint32_t)f / p.group, head = place.head * p.group.d + (f - token * p.group.d);
+  uint16_t* dst = p.out + (t.q0 + token) * p.out_stride_token + head * p.out_stride_head + column;
+  *reinterpret_cast<uint2*>(dst) = make_uint2(T::pack2(v[0] * inv, v[1] * inv), T::pack2(v[2] * inv, v[3] * inv));
 }
 
 static int check_ragged(const ll_ragged_attention_args* a) {
@@ -728,8 +745,9 @@ static RaPlan plan_ragged(const ll_ragged_attention_args& a, int cus) {
   if (a.window > 0 && a.window < keys && a.sink_keys < keys) keys = std::min(keys, a.window + a.sink_keys + longest + 2 * kRaKeys);
   const int64_t steps = (keys + kRaKeys - 1) / kRaKeys;
   const int64_t busy = std::min<int64_t>(r.tiles, a.streams * ((longest * group + kRaTileRows - 1) / kRaTileRows)) * a.num_kv_heads;
-  const int64_t want = busy >= 2 * cus ? 1 : (4 * cus + busy - 1) / busy;
-  int64_t per_part = std::min<int64_t>(std::max<int64_t>((steps + want - 1) / want, kRaLeastSteps), kRaMostSteps);
+  const int64_t want = 2 * busy >= 3 * cus ? 1 : (4 * cus + busy - 1) / busy;
+  int64_t per_part = std::max<int64_t>((steps + want - 1) / want, kRaLeastSteps);
+  if (a.streams > 1) per_part = std::min(per_part, kRaMostSteps);
   const uint32_t record_rows = (uint32_t)std::min<int64_t>((longest * group + 31) / 32 * 32, kRaTileRows);
   const size_t record = (size_t)record_rows * (a.head_dim + 2) * sizeof(float);
   for (; per_part < steps; per_part *= 2) {
@@ -773,7 +791,8 @@ static int launch_ragged(const RaParams& p, uint32_t grid, hipStream_t stream) {
   ragged_attention_kernel<T, D, KIND><<<grid, kRaThreads, kRaLds<D>, stream>>>(p);
   LL_CHECK_LAUNCH("ll_ragged_attention");
   if (p.parts > 1) {
-    ragged_join_kernel<T, D, KIND><<<p.tiles * (uint32_t)p.kv_heads, kRaThreads, 0, stream>>>(p);
+    const uint32_t rows = kRaThreads * 4 / D;
+    ragged_join_kernel<T, D, KIND><<<dim3(p.tiles * (uint32_t)p.kv_heads, (p.record_rows + rows - 1) / rows), kRaThreads, 0, stream>>>(p);
     LL_CHECK_LAUNCH("ll_ragged_attention (join)");
   }
   return LL_OK;
