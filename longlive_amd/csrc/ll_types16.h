@@ -18,6 +18,11 @@ struct Bf16 {
   }
   // round to nearest even
   static __device__ __forceinline__ uint32_t pack2(float a, float b) { return pack_bf16x2(a, b); }
+  // c + the two values of w
+  static __device__ __forceinline__ float add2(uint32_t w, float c) {
+    const bf16x2_hw one = {(__bf16)1.0f, (__bf16)1.0f};
+    return __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(bf16x2_hw, w), one, c, false);
+  }
   static __device__ __forceinline__ float16v mfma(short8v a, short8v b, float16v c) {
     return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8_hw, a), __builtin_bit_cast(bf16x8_hw, b), c, 0, 0, 0);
   }
@@ -32,6 +37,10 @@ struct F16 {
   static __device__ __forceinline__ uint32_t pack2(float a, float b) {
     const f32x2_hw v = {a, b};
     return __builtin_bit_cast(uint32_t, __builtin_convertvector(v, f16x2_hw));
+  }
+  static __device__ __forceinline__ float add2(uint32_t w, float c) {
+    const f16x2_hw one = {(_Float16)1.0f, (_Float16)1.0f};
+    return __builtin_amdgcn_fdot2(__builtin_bit_cast(f16x2_hw, w), one, c, false);
   }
   static __device__ __forceinline__ float16v mfma(short8v a, short8v b, float16v c) {
     return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8_hw, a), __builtin_bit_cast(f16x8_hw, b), c, 0, 0, 0);

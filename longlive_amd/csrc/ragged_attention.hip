@@ -258,10 +258,19 @@ __global__ __launch_bounds__(kRaThreads, 2) void ragged_attention_kernel(RaParam
   const bool narrow = tile_rows <= 32;
   const int own = narrow ? 0 : wave * 32;  // the wave's first row in the tile
 
-  // this lane's row and what it sees: keys below `last`, from `from` on or below the sink
-  const int f = min(t.first + own + l32, t.rows - 1);
-  const int token = (uint32_t)f / p.group, pos = t.len - t.n + token;
-  const int head = place.head * p.group.d + (f - token * p.group.d);
+  // This lane's row.  Formed anew where it is needed at the end: over the loops it would take registers they do not have.
+  struct Row {
+    int token, head;
+  };
+  auto own_row = [&]() __attribute__((always_inline)) {
+    int f = min(t.first + own + l32, t.rows - 1);
+    asm volatile("" : "+v"(f));
+    const int token = (uint32_t)f / p.group;
+    return Row{token, (int)(place.head * p.group.d) + f - token * (int)p.group.d};
+  };
+  const Row row = own_row();
+  // what it sees: keys below `last`, from `from` on or below the sink
+  const int pos = t.len - t.n + row.token;
   const int last = p.causal ? min(pos + 1, t.len) : t.len;
   const int from = p.window && pos >= (int)p.window ? pos - (int)p.window + 1 : 0;
   // the same for the wave's first and last row, which bound the others
@@ -270,7 +279,7 @@ __global__ __launch_bounds__(kRaThreads, 2) void ragged_attention_kernel(RaParam
 
   short8v qf[kSteps];
   {
-    const uint16_t* src = p.q + (t.q0 + token) * p.q_stride_token + head * p.q_stride_head + 8 * lh;
+    const uint16_t* src = p.q + (t.q0 + row.token) * p.q_stride_token + row.head * p.q_stride_head + 8 * lh;
 #pragma unroll
     for (int ks = 0; ks < kSteps; ++ks) qf[ks] = *reinterpret_cast<const short8v*>(src + 16 * ks);
   }
@@ -288,9 +297,14 @@ __global__ __launch_bounds__(kRaThreads, 2) void ragged_attention_kernel(RaParam
   uint8_t* const looked_up = smem + 4 * kStepBytes + wave * 512;
   const uint32_t looked_up_lds = lds_at(looked_up);
   auto key_base = [&](int s) __attribute__((always_inline)) { return (s < t.sink_steps ? s : t.from_step + s - t.sink_steps) * kRaKeys; };
+  uint32_t next_row = 0;
   auto look_up = [&](int key, int slot) __attribute__((always_inline)) {
     const uint32_t k = (uint32_t)min(key, t.len - 1);
-    if constexpr (KIND == kRaPaged) load4_to_lds(t.pages + k / p.page, looked_up_lds + slot * 256);
+    if constexpr (KIND == kRaPaged) {
+      const uint32_t page = k / p.page;
+      next_row = k - page * p.page.d;
+      load4_to_lds(t.pages + page, looked_up_lds + slot * 256);
+    }
     if constexpr (KIND == kRaMaskedRows) load4_to_lds(reinterpret_cast<const void*>((uintptr_t)(p.key_mask + t.key0 + k) & ~(uintptr_t)3), looked_up_lds + slot * 256);
   };
   uint32_t at_page = 0, at_row = 0;  // of this lane's key: page and row in it, or row
@@ -299,7 +313,7 @@ __global__ __launch_bounds__(kRaThreads, 2) void ragged_attention_kernel(RaParam
     bool ok = key < t.len;
     if constexpr (KIND == kRaPaged) {
       at_page = *reinterpret_cast<const uint32_t*>(looked_up + slot * 256 + lane * 4);
-      at_row = (uint32_t)key - ((uint32_t)key / p.page) * p.page.d;
+      at_row = next_row;  // of the key that was looked up last, which is this one where it exists
       ok = ok && at_page < p.n_pages;
     } else {
       at_row = (uint32_t)(t.key0 + key);
@@ -312,31 +326,29 @@ __global__ __launch_bounds__(kRaThreads, 2) void ragged_attention_kernel(RaParam
   };
 
   // ---- loads: 16 rows, the keys of lanes r0 .. r0 + 15, to 16 rows of LDS
+  // The lane's piece of row lane / kPieces of a load, and how its position turns from load to load.
+  const uint32_t k_part = (uint32_t)k_piece<D>(lane / kPieces, lane % kPieces) * 16, v_part = (uint32_t)v_piece<D>(lane / kPieces, lane % kPieces) * 16;
+  const uint32_t k_row = (uint32_t)(lane / kPieces) * p.k_stride_row * 2, v_row = (uint32_t)(lane / kPieces) * p.v_stride_row * 2;
+  auto turn = [](bool values, int i) { return (values ? v_piece<D>(i * kRowsPerLoad, 0) : k_piece<D>(i * kRowsPerLoad, 0)) * 16; };
   const bool whole_groups = KIND != kRaPaged || p.page.d % 16 == 0;  // 16 rows lie one behind the other
   auto load_rows = [&](bool values, int r0, uint32_t lds) __attribute__((always_inline)) {
     const uint16_t* base = values ? v_head : k_head;
     const uint32_t per_page = values ? p.v_stride_page : p.k_stride_page, per_row = values ? p.v_stride_row : p.k_stride_row;
-    int ln = lane;
-    asm volatile("" : "+v"(ln));  // the lane's offsets are formed here: kept over the loop they take registers it does not have
-    const int row0 = ln / kPieces, piece = ln % kPieces;
     if (whole_groups && ((uint32_t)(there >> r0) & 0xFFFFu) == 0xFFFFu) {
       uint64_t at = (uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)at_row, r0) * per_row;
       if constexpr (KIND == kRaPaged) at += (uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)at_page, r0) * per_page;
       const uint16_t* from_here = uniform_pointer(base + at);
-      const uint32_t first = (uint32_t)row0 * per_row * 2;
 #pragma unroll
-      for (int i = 0; i < kGroupLoads; ++i) {
-        const int row = i * kRowsPerLoad + row0;
-        const uint32_t part = (uint32_t)(values ? v_piece<D>(row, piece) : k_piece<D>(row, piece)) * 16;
-        load16_to_lds(first + (uint32_t)i * kRowsPerLoad * per_row * 2 + part, from_here, lds + i * 1024);
-      }
+      for (int i = 0; i < kGroupLoads; ++i)
+        load16_to_lds(((values ? v_part : k_part) ^ (uint32_t)turn(values, i)) + (values ? v_row : k_row),
+                      uniform_pointer(from_here + (uint64_t)i * kRowsPerLoad * per_row), lds + i * 1024);
     } else {
 #pragma unroll
       for (int i = 0; i < kGroupLoads; ++i) {
-        const int in_group = i * kRowsPerLoad + row0, row = r0 + in_group;
+        const int row = r0 + i * kRowsPerLoad + lane / kPieces;
         uint64_t at = (uint64_t)(uint32_t)__shfl((int)at_row, row) * per_row;
         if constexpr (KIND == kRaPaged) at += (uint64_t)(uint32_t)__shfl((int)at_page, row) * per_page;
-        const uint8_t* src = reinterpret_cast<const uint8_t*>(base + at) + (values ? v_piece<D>(in_group, piece) : k_piece<D>(in_group, piece)) * 16;
+        const uint8_t* src = reinterpret_cast<const uint8_t*>(base + at) + ((values ? v_part : k_part) ^ (uint32_t)turn(values, i));
         load16_to_lds((there >> row) & 1 ? src : reinterpret_cast<const uint8_t*>(kRaZeros), lds + i * 1024);
       }
     }
@@ -416,13 +428,14 @@ __global__ __launch_bounds__(kRaThreads, 2) void ragged_attention_kernel(RaParam
     constexpr int NT = std::extent<std::remove_reference_t<decltype(sc)>>::value;
 #pragma unroll
     for (int step = 0; step < 2 * NT; ++step) {
+      __builtin_amdgcn_sched_barrier(0);  // no reads of later steps ahead of this one: they would take the registers
       uint32_t w[4];
 #pragma unroll
       for (int u = 0; u < 4; ++u) {
         const float p0 = __builtin_amdgcn_exp2f(fmaf(sc[step >> 1][8 * (step & 1) + 2 * u], p.scale_log2, neg));
         const float p1 = __builtin_amdgcn_exp2f(fmaf(sc[step >> 1][8 * (step & 1) + 2 * u + 1], p.scale_log2, neg));
-        l += p0 + p1;
         w[u] = T::pack2(p0, p1);  // at most 2^kRaStep: no overflow, and half a step's error each, as small as the result's own
+        l = T::add2(w[u], l);     // the sum, in fp32, is of what the product weighs with
       }
       const short8v pb = __builtin_bit_cast(short8v, make_uint4(w[0], w[1], w[2], w[3]));
 #pragma unroll
@@ -472,8 +485,7 @@ __global__ __launch_bounds__(kRaThreads, 2) void ragged_attention_kernel(RaParam
         if constexpr (slot == begin + 2) {
           pw[pair] = T::pack2(e[pair & 1][0], e[pair & 1][1]);  // at most 2^kRaStep, see weigh
           asm volatile("" : "+v"(pw[pair]));                    // here, and not sunk to the MFMA that reads it
-          l += e[pair & 1][0] + e[pair & 1][1];
-          asm volatile("" : "+v"(l));
+          l = T::add2(pw[pair], l);
         }
         if constexpr (slot == begin + 1) {
           e[pair & 1][0] = __builtin_amdgcn_exp2f(x[pair & 1][0]);
@@ -499,12 +511,11 @@ __global__ __launch_bounds__(kRaThreads, 2) void ragged_attention_kernel(RaParam
     return mx;
   };
 
-  const int out_token = token;
-  auto write_row = [&](int row_in_tile, int tok, int hd, int column, const float (&v)[4], float mm, float ll) __attribute__((always_inline)) {
+  auto write_row = [&](int row_in_tile, const Row& r, int column, const float (&v)[4], float mm, float ll) __attribute__((always_inline)) {
     // four columns of a row: of the result, or of this part's record
     if (t.n_parts == 1) {
       const float inv = ll == 0.0f ? 0.0f : 1.0f / ll;
-      uint16_t* dst = p.out + (t.q0 + tok) * p.out_stride_token + hd * p.out_stride_head + column;
+      uint16_t* dst = p.out + (t.q0 + r.token) * p.out_stride_token + r.head * p.out_stride_head + column;
       *reinterpret_cast<uint2*>(dst) = make_uint2(T::pack2(v[0] * inv, v[1] * inv), T::pack2(v[2] * inv, v[3] * inv));
     } else {
       float* rec = record_of<D>(p, place, place.part);
@@ -559,29 +570,27 @@ __global__ __launch_bounds__(kRaThreads, 2) void ragged_attention_kernel(RaParam
       iteration(s, std::integral_constant<int, 0>{});
       iteration(s + 1, std::integral_constant<int, 1>{});
     }
-    bool second = false;
     if (s + 1 < s_end) {
       iteration(s, std::integral_constant<int, 0>{});
-      second = true;
+      sc[0][0] = sc[1][0];
+      sc[0][1] = sc[1][1];
       ++s;
     }
     if (s < s_end) {
       wait_loads<0>();
       __syncthreads();
-      if (!idle) {
-        if (second) weigh(sc[1], v_rows + (s & 1) * kStepBytes);
-        else weigh(sc[0], v_rows + (s & 1) * kStepBytes);
-      }
+      if (!idle) weigh(sc[0], v_rows + (s & 1) * kStepBytes);
     }
     if (idle) return;
     l = exchange_sum(l);
+    const Row to = own_row();
     if (own + l32 < tile_rows) {
 #pragma unroll
       for (int dt = 0; dt < kDTiles; ++dt)
 #pragma unroll
         for (int g = 0; g < 4; ++g) {
           const float v[4] = {o[dt][4 * g], o[dt][4 * g + 1], o[dt][4 * g + 2], o[dt][4 * g + 3]};
-          write_row(own + l32, out_token, head, 32 * dt + 8 * g + 4 * lh, v, m, l);
+          write_row(own + l32, to, 32 * dt + 8 * g + 4 * lh, v, m, l);
         }
     }
     return;
@@ -641,6 +650,7 @@ __global__ __launch_bounds__(kRaThreads, 2) void ragged_attention_kernel(RaParam
       for (int g = 0; g < 4; ++g) mine[(dt * 4 + g) * 64 + lane] = make_float4(o[dt][4 * g], o[dt][4 * g + 1], o[dt][4 * g + 2], o[dt][4 * g + 3]);
   }
   __syncthreads();
+  const Row to = own_row();
   float weight[4], all_l = 0.0f, all_m = -INFINITY;
 #pragma unroll
   for (int w = 0; w < 4; ++w) all_m = fmaxf(all_m, ml[w * 32 + l32].x);
@@ -663,7 +673,7 @@ __global__ __launch_bounds__(kRaThreads, 2) void ragged_attention_kernel(RaParam
       v[2] = fmaf(e.z, weight[w], v[2]);
       v[3] = fmaf(e.w, weight[w], v[3]);
     }
-    if (l32 < tile_rows) write_row(l32, out_token, head, 32 * dt + 8 * g + 4 * lh, v, all_m, all_l);
+    if (l32 < tile_rows) write_row(l32, to, 32 * dt + 8 * g + 4 * lh, v, all_m, all_l);
   }
 }
 
