@@ -1034,6 +1034,18 @@ def _rows16(t: torch.Tensor) -> bool:
     return t.stride(-1) == 1 and t.data_ptr() % 16 == 0 and all(s % 8 == 0 for n, s in zip(t.shape[:-1], t.stride()) if n > 1)
 
 
+def _stride(t: torch.Tensor, dim: int) -> int:
+    """The stride of a dimension, 0 where it is never taken (torch leaves anything there)."""
+    return t.stride(dim) if t.shape[dim] > 1 else 0
+
+
+def _page_rows(pages: torch.Tensor) -> int | None:
+    """How far the rows of a cache's pages lie apart, None if not all as far."""
+    if pages.shape[0] > 1 and pages.shape[1] > 1:
+        return pages.stride(1) if pages.stride(0) == pages.shape[1] * pages.stride(1) else None
+    return _stride(pages, 1) or _stride(pages, 0)
+
+
 def _check_rows(what: str, name: str, t: torch.Tensor, dtype=None) -> None:
     if t.ndim != 3 or t.dtype not in (torch.bfloat16, torch.float16) or (dtype is not None and t.dtype != dtype):
         raise ValueError(f"{what}: {name} must be [rows, heads, head_dim] in bfloat16 or float16, all tensors in one type; got "
@@ -1064,7 +1076,7 @@ def check_pages(what: str, cache: dict) -> tuple[torch.Tensor, torch.Tensor]:
 
 
 def _head_rows(x, weight, out, out_strides) -> HeadRowsStruct:
-    return HeadRowsStruct(x.data_ptr(), x.stride(0), x.stride(1), x.shape[1], _ptr(weight),
+    return HeadRowsStruct(x.data_ptr(), _stride(x, 0), _stride(x, 1), x.shape[1], _ptr(weight),
                           int(weight is not None and weight.dtype == torch.float32), out.data_ptr(), *out_strides)
 
 
@@ -1073,6 +1085,11 @@ def head_norm_rope(q, k, v, q_weight, k_weight, eps, cos, sin, positions, interl
     and v [T, Hk, D] then going to the cache's rows ``slots``."""
     what = "head_norm_rope"
     paged = cache is not None
+    if q.is_cuda:
+        pages = (cache["k_pages"], cache["v_pages"]) if paged else (None, None)
+        done = host().head_norm_rope(q, k, v, q_weight, k_weight, float(eps), cos, sin, positions, bool(interleaved), *pages, slots, q_out)
+        if done is not None:
+            return done
     pages = check_pages(what, cache) if paged else ()
     _one_device(what, q, k, v, q_weight, k_weight, cos, sin, positions, slots, q_out, *pages)
     T, Hq, D = (*q.shape, 0, 0, 0)[:3]
@@ -1111,20 +1128,20 @@ def head_norm_rope(q, k, v, q_weight, k_weight, eps, cos, sin, positions, interl
         k_pages, v_pages = pages
         if k_pages.shape[2:] != k.shape[1:] or k_pages.dtype != q.dtype:
             raise ValueError(f"{what}: pages of {k_pages.dtype} {tuple(k_pages.shape[2:])} do not take rows of {q.dtype} {tuple(k.shape[1:])}")
-        if any(t.numel() and t.stride(0) != t.shape[1] * t.stride(1) for t in pages):
+        if any(t.numel() and _page_rows(t) is None for t in pages):
             raise ValueError(f"{what}: pages must lie one behind the other")
         _check_index(what, "slots", slots, torch.int64, (T,))
         v = v if _rows16(v) else v.contiguous().clone()
         n_slots = k_pages.shape[0] * k_pages.shape[1]
-        k_rows = _head_rows(k, k_weight, k_pages, k_pages.stride()[1:3])
-        v_rows = _head_rows(v, None, v_pages, v_pages.stride()[1:3])
+        k_rows = _head_rows(k, k_weight, k_pages, (_page_rows(k_pages), _stride(k_pages, 2)))
+        v_rows = _head_rows(v, None, v_pages, (_page_rows(v_pages), _stride(v_pages, 2)))
         k_out = None
     else:
         k_out = torch.empty(k.shape, dtype=k.dtype, device=k.device)
-        k_rows = _head_rows(k, k_weight, k_out, k_out.stride()[:2])
+        k_rows = _head_rows(k, k_weight, k_out, (_stride(k_out, 0), _stride(k_out, 1)))
     if T == 0:
         return q_out if paged else (q_out, k_out)
-    q_rows = _head_rows(q, q_weight, q_out, q_out.stride()[:2])
+    q_rows = _head_rows(q, q_weight, q_out, (_stride(q_out, 0), _stride(q_out, 1)))
     if n_slots == 0 and paged:   # a cache without pages: nothing to write to
         k_rows.num_heads, v_rows = 0, None
     with torch.cuda.device(q.device):
@@ -1139,6 +1156,12 @@ def ragged_attention(what, q, q_starts, softmax_scale, max_q_len, max_kv_len, ou
                      window=None, sink_tokens=0, k=None, v=None, k_starts=None, k_lens=None, key_mask=None):
     """The queries q [T, H, D] of several streams over the keys of a paged ``cache`` or over rows of k and v [n, Hk, D]
     (``ll_ragged_attention``)."""
+    if q.is_cuda and (window is None or window):
+        keys = (k, v) if cache is None else (cache["k_pages"], cache["v_pages"])
+        done = host().ragged_attention(q, q_starts, q.shape[-1] ** -0.5 if softmax_scale is None else float(softmax_scale), max_q_len or 0, max_kv_len or 0,
+                                       out, *keys, page_table, kv_lens, bool(causal), window or 0, sink_tokens, k_starts, k_lens, key_mask)
+        if done is not None:
+            return done
     pages = check_pages(what, cache) if cache is not None else ()
     _one_device(what, q, q_starts, out, page_table, kv_lens, k, v, k_starts, k_lens, key_mask, *pages)
     _check_rows(what, "q", q)
@@ -1163,11 +1186,11 @@ def ragged_attention(what, q, q_starts, softmax_scale, max_q_len, max_kv_len, ou
         _check_index(what, "kv_lens", kv_lens, torch.int32, (streams,))
         if page_table.dtype != torch.int32 or page_table.ndim != 2 or page_table.shape[0] != streams or (page_table.numel() and page_table.stride(1) != 1):
             raise ValueError(f"{what}: page_table must be int32 [{streams}, pages of the longest stream] with contiguous rows")
-        a.page_table, a.table_stride, a.table_width = page_table.data_ptr(), page_table.stride(0), page_table.shape[1]
+        a.page_table, a.table_stride, a.table_width = page_table.data_ptr(), _stride(page_table, 0), page_table.shape[1]
         a.n_pages, a.page_size, a.kv_lens, a.causal = k.shape[0], k.shape[1], kv_lens.data_ptr(), int(bool(causal))
         a.window, a.sink_keys = window or 0, sink_tokens
-        a.k_stride_page, a.k_stride_row, a.k_stride_head = k.stride()[:3]
-        a.v_stride_page, a.v_stride_row, a.v_stride_head = v.stride()[:3]
+        a.k_stride_page, a.k_stride_row, a.k_stride_head = (_stride(k, i) for i in range(3))
+        a.v_stride_page, a.v_stride_row, a.v_stride_head = (_stride(v, i) for i in range(3))
         if a.table_width * a.page_size >= 1 << 31:
             raise ValueError(f"{what}: a table of {a.table_width} pages of {a.page_size} rows reaches beyond 2^31 keys")
     else:
@@ -1186,8 +1209,8 @@ def ragged_attention(what, q, q_starts, softmax_scale, max_q_len, max_kv_len, ou
             _check_index(what, "key_mask", key_mask, torch.bool, (k.shape[0],))
         k, v = (t if _rows16(t) else t.contiguous().clone() for t in (k, v))
         a.k_starts, a.k_lens, a.key_mask, a.n_keys = k_starts.data_ptr(), _ptr(k_lens), _ptr(key_mask), k.shape[0]
-        a.k_stride_row, a.k_stride_head = k.stride()[:2]
-        a.v_stride_row, a.v_stride_head = v.stride()[:2]
+        a.k_stride_row, a.k_stride_head = _stride(k, 0), _stride(k, 1)
+        a.v_stride_row, a.v_stride_head = _stride(v, 0), _stride(v, 1)
     if k.shape[-1] != D or k.dtype != q.dtype or k.shape[-2] == 0 or H % k.shape[-2]:
         raise ValueError(f"{what}: q of {q.dtype} {tuple(q.shape)} does not go with keys of {k.dtype} {tuple(k.shape)}")
     a.num_kv_heads = k.shape[-2]
@@ -1199,8 +1222,8 @@ def ragged_attention(what, q, q_starts, softmax_scale, max_q_len, max_kv_len, ou
     if T == 0 or H == 0:
         return out
     a.q, a.q_starts, a.out, a.k, a.v = q.data_ptr(), q_starts.data_ptr(), out.data_ptr(), k.data_ptr(), v.data_ptr()
-    a.q_stride_token, a.q_stride_head = q.stride()[:2]
-    a.out_stride_token, a.out_stride_head = out.stride()[:2]
+    a.q_stride_token, a.q_stride_head = _stride(q, 0), _stride(q, 1)
+    a.out_stride_token, a.out_stride_head = _stride(out, 0), _stride(out, 1)
     with torch.cuda.device(q.device):
         lib, need = load(), c_size_t()
         _check(lib.ll_ragged_attention_workspace(ctypes.byref(a), 0, ctypes.byref(need)), what)

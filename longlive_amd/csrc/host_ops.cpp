@@ -1008,6 +1008,215 @@ PyObject* py_release_stream_sink(PyObject*, PyObject*) {
   END_HANDLE_TH_ERRORS
 }
 
+// ------------------------------------------------------------------------------------------------ several streams in one batch
+inline bool is_half(const Tensor& t) { return t.scalar_type() == at::kBFloat16 || t.scalar_type() == at::kHalf; }
+inline int half_code(const Tensor& t) { return t.scalar_type() == at::kBFloat16 ? LL_DTYPE_BF16 : LL_DTYPE_F16; }
+// A tensor of 16-bit values of `like`'s type on the device whose rows can be read 16 bytes at a time where they lie.
+const Tensor* as_rows(PyObject* o, int dev, int64_t dims, const Tensor* like) {
+  const Tensor* t = plain(o) ? &THPVariable_Unpack(o) : nullptr;
+  if (!t || !on_device(*t, dev) || t->layout() != at::kStrided || t->dim() != dims || !is_half(*t) || (like && t->scalar_type() != like->scalar_type()))
+    return nullptr;
+  if (t->numel() == 0 || t->stride(dims - 1) != 1 || !aligned16(t->data_ptr())) return nullptr;
+  for (int64_t i = 0; i + 1 < dims; ++i)
+    if (t->size(i) > 1 && t->stride(i) % 8 != 0) return nullptr;
+  return t;
+}
+// The stride of a dimension, 0 where it is never taken.
+inline int64_t stride_of(const Tensor* t, int64_t d) { return t->size(d) > 1 ? t->stride(d) : 0; }
+// A contiguous tensor of a type and so many elements.
+const Tensor* as_list(PyObject* o, int dev, at::ScalarType type, int64_t numel) {
+  const Tensor* t = plain(o) ? &THPVariable_Unpack(o) : nullptr;
+  return t && on_device(*t, dev) && t->scalar_type() == type && t->dim() == 1 && t->numel() == numel && t->is_contiguous() ? t : nullptr;
+}
+inline bool as_count(PyObject* o, int64_t& n) {
+  if (!PyLong_Check(o)) return false;
+  n = PyLong_AsLongLong(o);
+  if (n == -1 && PyErr_Occurred()) PyErr_Clear();
+  return n >= 0;
+}
+
+// ragged_attention(q, q_starts, scale, max_q_len, max_kv_len, out or None, k, v, page_table, kv_lens, causal, window, sink, k_starts, k_lens,
+// key_mask) -> [T, H, D]: over pages k, v [pages, page_size, Hk, D] with a page table, else over rows k, v [n, Hk, D] (page_table None).
+PyObject* py_ragged_attention(PyObject*, PyObject* const* args, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  if (n != 16 || !plain(args[0])) Py_RETURN_NONE;
+  const int dev = current_device_of(THPVariable_Unpack(args[0]));
+  if (dev < 0) Py_RETURN_NONE;
+  const Tensor* q = as_rows(args[0], dev, 3, nullptr);
+  const bool paged = args[8] != Py_None;
+  const Tensor *k = q ? as_rows(args[6], dev, paged ? 4 : 3, q) : nullptr, *v = q ? as_rows(args[7], dev, paged ? 4 : 3, q) : nullptr;
+  if (!q || !k || !v || k->sizes() != v->sizes()) Py_RETURN_NONE;
+  const int64_t T = q->size(0), H = q->size(1), D = q->size(2), last = paged ? 3 : 2;
+  if ((D != 64 && D != 128) || k->size(last) != D || H % k->size(last - 1) != 0) Py_RETURN_NONE;
+  const Tensor* starts = plain(args[1]) ? &THPVariable_Unpack(args[1]) : nullptr;
+  if (!starts || !as_list(args[1], dev, at::kInt, starts->numel()) || starts->numel() < 2) Py_RETURN_NONE;
+  ll_ragged_attention_args a{};
+  a.streams = starts->numel() - 1;
+  if (!PyFloat_Check(args[2]) || !as_count(args[3], a.max_q_len) || !as_count(args[4], a.max_kv_len) || !as_count(args[11], a.window) ||
+      !as_count(args[12], a.sink_keys))
+    Py_RETURN_NONE;
+  a.softmax_scale = (float)PyFloat_AsDouble(args[2]);
+  if (paged) {
+    const Tensor* table = plain(args[8]) ? &THPVariable_Unpack(args[8]) : nullptr;
+    const Tensor* lens = as_list(args[9], dev, at::kInt, a.streams);
+    if (!table || !lens || !on_device(*table, dev) || table->scalar_type() != at::kInt || table->dim() != 2 || table->size(0) != a.streams ||
+        table->numel() == 0 || table->stride(1) != 1)
+      Py_RETURN_NONE;
+    a.page_table = table->data_ptr<int32_t>();
+    a.table_stride = table->stride(0);
+    a.table_width = table->size(1);
+    a.n_pages = k->size(0);
+    if (k->size(1) > 0x7fffffff) Py_RETURN_NONE;
+    a.page_size = (int)k->size(1);
+    a.kv_lens = lens->data_ptr<int32_t>();
+    a.causal = args[10] == Py_True;
+    a.k_stride_page = stride_of(k, 0);
+    a.v_stride_page = stride_of(v, 0);
+  } else {
+    const Tensor* k_starts = args[14] == Py_None ? as_list(args[13], dev, at::kInt, a.streams + 1)
+                                                 : plain(args[13]) ? &THPVariable_Unpack(args[13]) : nullptr;
+    if (!k_starts || k_starts->numel() < a.streams || !as_list(args[13], dev, at::kInt, k_starts->numel())) Py_RETURN_NONE;
+    a.k_starts = k_starts->data_ptr<int32_t>();
+    if (args[14] != Py_None) {
+      const Tensor* lens = as_list(args[14], dev, at::kInt, a.streams);
+      if (!lens) Py_RETURN_NONE;
+      a.k_lens = lens->data_ptr<int32_t>();
+    }
+    a.n_keys = k->size(0);
+    if (args[15] != Py_None) {
+      const Tensor* mask = as_list(args[15], dev, at::kBool, a.n_keys);
+      if (!mask) Py_RETURN_NONE;
+      a.key_mask = static_cast<const uint8_t*>(mask->data_ptr());
+    }
+  }
+  Tensor out;
+  if (args[5] == Py_None) {
+    out = empty(q->sizes(), q->scalar_type(), dev);
+    a.clear_rest = 1;
+  } else {
+    const Tensor* given = as_rows(args[5], dev, 3, q);
+    if (!given || given->sizes() != q->sizes()) Py_RETURN_NONE;
+    out = *given;
+  }
+  a.dtype = half_code(*q);
+  a.head_dim = (int)D;
+  a.num_heads = (int)H;
+  a.num_kv_heads = (int)k->size(last - 1);
+  a.n_queries = T;
+  a.q = q->data_ptr();
+  a.q_stride_token = stride_of(q, 0);
+  a.q_stride_head = stride_of(q, 1);
+  a.out = out.data_ptr();
+  a.out_stride_token = stride_of(&out, 0);
+  a.out_stride_head = stride_of(&out, 1);
+  a.q_starts = starts->data_ptr<int32_t>();
+  a.k = k->data_ptr();
+  a.v = v->data_ptr();
+  a.k_stride_row = stride_of(k, last - 2);
+  a.v_stride_row = stride_of(v, last - 2);
+  a.k_stride_head = stride_of(k, last - 1);
+  a.v_stride_head = stride_of(v, last - 1);
+  size_t need = 0;
+  const char* what = paged ? "paged_attention" : "ragged_cross_attention";
+  if (failed(ll_ragged_attention_workspace(&a, 0, &need), what)) return nullptr;
+  Tensor workspace;  // freed for work behind this call's launches on the stream
+  if (need) {
+    workspace = empty({(int64_t)need}, at::kByte, dev);
+    a.workspace = workspace.data_ptr();
+    a.workspace_bytes = need;
+  }
+  if (failed(ll_ragged_attention(&a, stream_of(dev)), what)) return nullptr;
+  if (args[5] != Py_None) {
+    Py_INCREF(args[5]);
+    return args[5];
+  }
+  return THPVariable_Wrap(out);
+  END_HANDLE_TH_ERRORS
+}
+
+// head_norm_rope(q, k, v or None, q_weight, k_weight, eps, cos, sin, positions, interleaved, k_pages, v_pages, slots, q_out) -> (q, k), or with
+// pages q; the weights, cos and sin, positions, pages (with v and slots) and q_out may be None.
+PyObject* py_head_norm_rope(PyObject*, PyObject* const* args, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  if (n != 14 || !plain(args[0])) Py_RETURN_NONE;
+  const int dev = current_device_of(THPVariable_Unpack(args[0]));
+  if (dev < 0) Py_RETURN_NONE;
+  const Tensor* q = as_rows(args[0], dev, 3, nullptr);
+  const Tensor* k = q ? as_rows(args[1], dev, 3, q) : nullptr;
+  if (!q || !k || k->size(0) != q->size(0) || k->size(2) != q->size(2) || !PyFloat_Check(args[5])) Py_RETURN_NONE;
+  const int64_t T = q->size(0), D = q->size(2);
+  if (D % 8 != 0 || D > 256) Py_RETURN_NONE;
+  const bool paged = args[10] != Py_None;
+  const Tensor *cos = nullptr, *sin = nullptr, *positions = nullptr, *weights[2] = {nullptr, nullptr};
+  for (int i = 0; i < 2; ++i) {
+    if (args[3 + i] == Py_None) continue;
+    const Tensor* w = as_tensor(args[3 + i]);
+    if (!w || !as_list(args[3 + i], dev, w->scalar_type(), D) || (w->scalar_type() != q->scalar_type() && w->scalar_type() != at::kFloat) || !aligned16(w->data_ptr()))
+      Py_RETURN_NONE;
+    weights[i] = w;
+  }
+  if (args[6] != Py_None || args[7] != Py_None) {
+    cos = as_tensor(args[6]);
+    sin = as_tensor(args[7]);
+    for (const Tensor* t : {cos, sin})
+      if (!t || !on_device(*t, dev) || t->scalar_type() != at::kFloat || t->dim() != 2 || t->sizes() != cos->sizes() || !t->is_contiguous() || !aligned16(t->data_ptr()))
+        Py_RETURN_NONE;
+    if (2 * cos->size(1) % 8 != 0 || 2 * cos->size(1) > D || cos->numel() == 0) Py_RETURN_NONE;
+  }
+  if (args[8] != Py_None && !(positions = as_list(args[8], dev, at::kLong, T))) Py_RETURN_NONE;
+  Tensor q_out, k_out;
+  if (args[13] == Py_None) {
+    q_out = empty(q->sizes(), q->scalar_type(), dev);
+  } else {
+    const Tensor* given = as_rows(args[13], dev, 3, q);
+    if (!given || given->sizes() != q->sizes()) Py_RETURN_NONE;
+    q_out = *given;
+  }
+  const auto rows = [](const Tensor* x, const Tensor* weight, void* out, int64_t out_token, int64_t out_head) {
+    return ll_head_rows{x->data_ptr(), stride_of(x, 0), stride_of(x, 1), (int)x->size(1), weight ? weight->data_ptr() : nullptr,
+                        weight && weight->scalar_type() == at::kFloat, out, out_token, out_head};
+  };
+  const ll_head_rows q_rows = rows(q, weights[0], q_out.data_ptr(), stride_of(&q_out, 0), stride_of(&q_out, 1));
+  ll_head_rows k_rows{}, v_rows{};
+  const int64_t* slots = nullptr;
+  int64_t n_slots = 0;
+  if (paged) {
+    const Tensor *kp = as_rows(args[10], dev, 4, q), *vp = as_rows(args[11], dev, 4, q), *v = as_rows(args[2], dev, 3, q);
+    const Tensor* at = as_list(args[12], dev, at::kLong, T);
+    if (!kp || !vp || !v || !at || v->sizes() != k->sizes() || kp->sizes() != vp->sizes() || kp->size(2) != k->size(1) || kp->size(3) != D) Py_RETURN_NONE;
+    for (const Tensor* t : {kp, vp})  // the cache's rows all as far apart
+      if (t->size(0) > 1 && t->size(1) > 1 && t->stride(0) != t->size(1) * t->stride(1)) Py_RETURN_NONE;
+    const auto apart = [](const Tensor* t) { return t->size(1) > 1 ? t->stride(1) : stride_of(t, 0); };
+    k_rows = rows(k, weights[1], kp->data_ptr(), apart(kp), stride_of(kp, 2));
+    v_rows = rows(v, nullptr, vp->data_ptr(), apart(vp), stride_of(vp, 2));
+    slots = at->data_ptr<int64_t>();
+    n_slots = kp->size(0) * kp->size(1);
+  } else {
+    k_out = empty(k->sizes(), k->scalar_type(), dev);
+    k_rows = rows(k, weights[1], k_out.data_ptr(), stride_of(&k_out, 0), stride_of(&k_out, 1));
+  }
+  if (failed(ll_head_norm_rope(half_code(*q), T, (int)D, &q_rows, &k_rows, paged ? &v_rows : nullptr, (float)PyFloat_AsDouble(args[5]),
+                               cos ? cos->data_ptr<float>() : nullptr, sin ? sin->data_ptr<float>() : nullptr, cos ? cos->size(0) : 0,
+                               cos ? (int)(2 * cos->size(1)) : 0, positions ? positions->data_ptr<int64_t>() : nullptr, args[9] == Py_True, slots, n_slots,
+                               stream_of(dev)),
+             "head_norm_rope"))
+    return nullptr;
+  PyObject* first;
+  if (args[13] != Py_None) {
+    Py_INCREF(args[13]);
+    first = args[13];
+  } else {
+    first = THPVariable_Wrap(q_out);
+  }
+  if (paged) return first;
+  PyObject* both = PyTuple_New(2);
+  if (!both) return nullptr;
+  PyTuple_SET_ITEM(both, 0, first);
+  PyTuple_SET_ITEM(both, 1, THPVariable_Wrap(k_out));
+  return both;
+  END_HANDLE_TH_ERRORS
+}
+
 PyMethodDef methods[] = {
     {"block_forward", (PyCFunction)(void (*)(void))py_block_forward, METH_FASTCALL, nullptr},
     {"slot_addresses", (PyCFunction)(void (*)(void))py_slot_addresses, METH_FASTCALL, nullptr},
@@ -1017,6 +1226,8 @@ PyMethodDef methods[] = {
     {"patch_embed", (PyCFunction)(void (*)(void))py_patch_embed, METH_FASTCALL, nullptr},
     {"head", (PyCFunction)(void (*)(void))py_head, METH_FASTCALL, nullptr},
     {"unipc_step", (PyCFunction)(void (*)(void))py_unipc_step, METH_FASTCALL, nullptr},
+    {"ragged_attention", (PyCFunction)(void (*)(void))py_ragged_attention, METH_FASTCALL, nullptr},
+    {"head_norm_rope", (PyCFunction)(void (*)(void))py_head_norm_rope, METH_FASTCALL, nullptr},
     {"recording", py_recording, METH_O, nullptr},
     {"current_stream", py_current_stream, METH_NOARGS, nullptr},
     {"release_stream_sink", py_release_stream_sink, METH_NOARGS, nullptr},

@@ -265,6 +265,53 @@ def test_queries_outputs_and_pages_with_strides(gpu):
     assert torch.equal(paged_attention(odd, paged, tables, lens.to(gpu), q_starts.to(gpu)), want)
 
 
+def test_dimensions_of_one_with_any_stride(gpu):
+    """Torch leaves anything in the stride of a dimension of size one: one row, one head, one page, pages of one row."""
+    def odd(t, *dims):
+        return t.as_strided(t.shape, [7 if d in dims else s for d, s in enumerate(t.stride())])
+
+    q, cache, table, lens, q_starts = (t if isinstance(t, dict) else t.to(gpu) for t in batch(105, [1], [1], 1, 1, 64, 1, BF16, spare=0))
+    cache = {n: t.to(gpu) for n, t in cache.items()}
+    want = paged_attention(q, cache, table, lens, q_starts)
+    pages = {n: odd(t, 0, 1, 2) for n, t in cache.items()}
+    assert torch.equal(paged_attention(odd(q, 0, 1), pages, odd(table, 0), lens, q_starts), want)
+    assert torch.equal(ragged_cross_attention(odd(q, 0, 1), odd(cache["k_pages"][0], 0, 1), odd(cache["v_pages"][0], 0, 1), q_starts, q_starts), want)
+    k, w = randn(3, 1, 1, 64).to(gpu), randn(4, 64).to(gpu)
+    first, _ = head_norm_rope(q, k, w, w, 1e-6, None, None)
+    assert torch.equal(head_norm_rope(odd(q, 0, 1), odd(k, 0, 1), w, w, 1e-6, None, None)[0], first)
+    cache = {n: torch.zeros(5, 1, 1, 64, dtype=BF16, device=gpu) for n in cache}
+    head_norm_rope_paged(q, k, k, {n: odd(t, 1, 2) for n, t in cache.items()}, torch.tensor([3], device=gpu), None, None, 1e-6, None, None)
+    assert torch.equal(cache["k_pages"][3, 0], k[0]) and torch.equal(cache["v_pages"][3, 0], k[0]) and not cache["k_pages"][:3].any()
+
+
+@pytest.mark.parametrize("native", [True, False])
+def test_both_host_paths_give_the_same(gpu, native, monkeypatch):
+    from longlive_amd import _native
+
+    q, cache, table, lens, q_starts = (t if isinstance(t, dict) else t.to(gpu) for t in batch(106, [3, 1], [100, 700], 4, 2, 64, 16, F16))
+    cache = {n: t.to(gpu) for n, t in cache.items()}
+    cos, sin = (t.to(gpu) for t in angles(4, 64))
+    slots = paged_slots(table, lens, q_starts, 4, 16)
+    k = randn(3, 4, 2, 64, dtype=F16).to(gpu)
+
+    def everything():
+        pages = {n: t.clone() for n, t in cache.items()}
+        roped = head_norm_rope_paged(q, k, k, pages, slots, None, None, 1e-6, cos, sin, interleaved=False)
+        rows = pages["k_pages"].flatten(0, 1)
+        return (roped, *pages.values(), *head_norm_rope(q, k, None, None, 1e-6, cos, sin), paged_attention(roped, pages, table, lens, q_starts, window=50),
+                ragged_cross_attention(roped, rows, rows, q_starts, q_starts, k_lens=lens, key_mask=torch.arange(len(rows), device=gpu) % 3 > 0))
+
+    want = everything()
+    if not native:
+        monkeypatch.setattr(_native, "_host", _native._NoHostPath())
+    for a, b in zip(everything(), want):
+        assert torch.equal(a, b)
+    taken = _native.host().ragged_attention(q, q_starts, 0.125, 0, 0, None, cache["k_pages"], cache["v_pages"], table, lens, True, 0, 0, None, None, None)
+    assert (taken is not None) == native
+    taken = _native.host().head_norm_rope(q, k, None, None, None, 1e-6, cos, sin, None, True, None, None, None, None)
+    assert (taken is not None) == native
+
+
 def test_pages_beyond_4_gib(gpu):
     pages, page, Hk, D = 70000, 64, 4, 128     # 4.3 GiB of K and as much of V
     cache = initialize_paged_kv_cache(1, pages, page, Hk, D, gpu)[0]
