@@ -32,6 +32,7 @@ constexpr int kRaThreads = 256;
 constexpr int kRaTileRows = 128;  // rows of a workgroup, 32 a wave
 constexpr int kRaKeys = 64;       // keys of a step
 constexpr int kRaClearGroups = 16;
+constexpr uint32_t kRaJoinGroups = 8192;
 
 // Where keys lie: in the pages of a table, in rows one behind the other, in such rows with a mask.
 constexpr int kRaPaged = 0, kRaRows = 1, kRaMaskedRows = 2;
@@ -61,10 +62,10 @@ struct RaParams {
   uint32_t window, sink;  // window 0: none
   uint32_t tiles;         // workgroups per kv head and part: no fewer than there are tiles
   uint32_t parts;         // workgroups that a tile's keys are cut for
-  uint32_t part_steps;    // steps of a part; the last takes what is left
+  uint32_t part_steps;    // a tile is cut into as many parts as it has that many steps
   uint32_t record_rows;   // tiles of more rows are not cut
   uint32_t work_groups;   // tiles * parts * kv_heads
-  int by_head;            // an XCD's workgroups are neighbours in the order head, tile, part
+  int by_head;            // an XCD's workgroups are neighbours in the order head, part, tile
   float* records;         // [kv head][tile][part]: record_rows x (D + 2) floats
 };
 
@@ -132,26 +133,31 @@ struct RaTile {
   int64_t q0;           // first row of q of the stream
   int n, rows, first;   // tokens of the stream; rows of the stream (token, head of the group), the tile's first
   int len;              // keys of the stream
-  int64_t key0;         // rows of keys: row of key 0
+  int key0;             // rows of keys: row of key 0
   const int32_t* pages; // paged: the stream's row of the table
   // keys: steps 0 .. sink_steps - 1 and then from from_step on, n_steps in all
   int sink_steps, from_step, n_steps;
-  int n_parts;          // workgroups that share the keys
+  int n_parts, part_steps;  // workgroups that share the keys, steps of each
 };
 
 // Tile `index` of the tiles of a kv head: the streams' tiles one behind the other, the last of a stream (which sees most keys) first.
-// All lanes call it together.  False: there are fewer.
+// All lanes call it together, a stream a lane; what is known of the streams is loaded at once.  False: there are fewer tiles.
 template <int KIND>
 __device__ __forceinline__ bool find_tile(const RaParams& p, uint32_t index, RaTile& t) {
   const int lane = threadIdx.x & 63;
   t.stream = -1;
   for (int b0 = 0; b0 < p.streams; b0 += 64) {
-    int mine = 0;
-    if (b0 + lane < p.streams) {
-      const int64_t n = stream_start(p, b0 + lane + 1) - stream_start(p, b0 + lane);
-      mine = n > 0 ? (int)((n * p.group.d + kRaTileRows - 1) / kRaTileRows) : 0;
+    const int b = min(b0 + lane, p.streams - 1);
+    const int start = p.q_starts[b], next = p.q_starts[b + 1];
+    int key0 = 0, len;
+    if constexpr (KIND == kRaPaged) {
+      len = p.kv_lens[b];
+    } else {
+      key0 = p.k_starts[b];
+      len = p.k_lens ? p.k_lens[b] : p.k_starts[b + 1];
     }
-    int upto = mine;
+    const int limit = (int)p.n_queries, q0 = min(max(start, 0), limit), n = max(min(max(next, 0), limit) - q0, 0);
+    int upto = b0 + lane < p.streams ? (int)(((int64_t)n * p.group.d + kRaTileRows - 1) / kRaTileRows) : 0;
 #pragma unroll
     for (int d = 1; d < 64; d *= 2) {
       const int other = __shfl_up(upto, d);
@@ -159,28 +165,29 @@ __device__ __forceinline__ bool find_tile(const RaParams& p, uint32_t index, RaT
     }
     const uint64_t before = __builtin_amdgcn_ballot_w64((uint32_t)upto <= index);
     if (before != ~0ull) {
-      const int at = __popcll(before);
+      const int at = __builtin_amdgcn_readfirstlane(__popcll(before));
       t.stream = b0 + at;
       t.first = (__builtin_amdgcn_readlane(upto, at) - 1 - (int)index) * kRaTileRows;
+      t.q0 = __builtin_amdgcn_readlane(q0, at);
+      t.n = __builtin_amdgcn_readlane(n, at);
+      t.len = __builtin_amdgcn_readlane(len, at);
+      t.key0 = __builtin_amdgcn_readlane(key0, at);
       break;
     }
     index -= (uint32_t)__builtin_amdgcn_readlane(upto, 63);
   }
   if (t.stream < 0) return false;
-  t.stream = __builtin_amdgcn_readfirstlane(t.stream);
-  t.first = __builtin_amdgcn_readfirstlane(t.first);
-  t.q0 = stream_start(p, t.stream);
-  t.n = (int)(stream_start(p, t.stream + 1) - t.q0);
   t.rows = t.n * (int)p.group.d;
   t.pages = nullptr;
-  t.key0 = 0;
   if constexpr (KIND == kRaPaged) {
-    t.len = (int)min(max((int64_t)p.kv_lens[t.stream], (int64_t)0), p.table_keys);
+    t.len = (int)min(max((int64_t)t.len, (int64_t)0), p.table_keys);
+    t.key0 = 0;
     t.pages = p.page_table + t.stream * p.table_stride;
   } else {
-    t.key0 = min(max((int64_t)p.k_starts[t.stream], (int64_t)0), p.n_keys);
-    const int64_t len = p.k_lens ? (int64_t)p.k_lens[t.stream] : (int64_t)p.k_starts[t.stream + 1] - t.key0;
-    t.len = (int)min(max(len, (int64_t)0), p.n_keys - t.key0);
+    const int64_t first = min(max((int64_t)t.key0, (int64_t)0), p.n_keys);
+    const int64_t len = p.k_lens ? (int64_t)t.len : (int64_t)t.len - first;
+    t.key0 = (int)first;
+    t.len = (int)min(max(len, (int64_t)0), p.n_keys - first);
   }
   const int last_row = min(t.first + kRaTileRows, t.rows) - 1;
   const int pos0 = t.len - t.n + (int)((uint32_t)t.first / p.group), pos1 = t.len - t.n + (int)((uint32_t)last_row / p.group);
@@ -192,22 +199,24 @@ __device__ __forceinline__ bool find_tile(const RaParams& p, uint32_t index, RaT
   t.n_steps = min(t.sink_steps, end_step) + max(end_step - t.from_step, 0);
   const bool cut = p.parts > 1 && last_row - t.first < (int)p.record_rows;
   t.n_parts = cut ? max(min((int)((t.n_steps + p.part_steps - 1) / p.part_steps), (int)p.parts), 1) : 1;
+  t.part_steps = (t.n_steps + t.n_parts - 1) / t.n_parts;  // equal parts
   return true;
 }
 
-// The number of workgroup `id` in the order head, tile, part or tile, part, head.
+// What workgroup `id` does.  Last parts come first, which only the tiles of the most keys have, and first parts, which all have, at the
+// end: what is long begins early.
 struct RaPlace {
   uint32_t head, tile, part;
 };
 __device__ __forceinline__ RaPlace place_of(const RaParams& p, uint32_t id) {
-  const uint32_t per_head = p.tiles * p.parts;
-  if (p.by_head) {  // consecutive workgroups go to different XCDs: each gets a contiguous range
+  if (p.by_head) {  // consecutive workgroups go to different XCDs: each gets a contiguous range of head, part, tile
+    const uint32_t per_head = p.tiles * p.parts;
     id = p.work_groups % 8 == 0 ? (id & 7) * (p.work_groups / 8) + (id >> 3) : id;
-    const uint32_t head = id / per_head, rest = id - head * per_head;
-    return RaPlace{head, rest / p.parts, rest % p.parts};
+    const uint32_t head = id / per_head, rest = id - head * per_head, part = rest / p.tiles;
+    return RaPlace{head, rest - part * p.tiles, p.parts - 1 - part};
   }
-  const uint32_t rest = id / (uint32_t)p.kv_heads;
-  return RaPlace{id - rest * (uint32_t)p.kv_heads, rest / p.parts, rest % p.parts};
+  const uint32_t per_part = p.tiles * (uint32_t)p.kv_heads, part = id / per_part, rest = id - part * per_part, tile = rest / (uint32_t)p.kv_heads;
+  return RaPlace{rest - tile * (uint32_t)p.kv_heads, tile, p.parts - 1 - part};
 }
 
 template <int D>
@@ -251,8 +260,7 @@ __global__ __launch_bounds__(kRaThreads, 2) void ragged_attention_kernel(RaParam
   const RaPlace place = place_of(p, blockIdx.x);
   RaTile t;
   if (!find_tile<KIND>(p, place.tile, t) || (int)place.part >= t.n_parts) return;
-  const int s_begin = t.n_parts > 1 ? (int)(place.part * p.part_steps) : 0;
-  const int s_end = (int)place.part + 1 == t.n_parts ? t.n_steps : s_begin + (int)p.part_steps;
+  const int s_begin = min((int)place.part * t.part_steps, t.n_steps), s_end = min(s_begin + t.part_steps, t.n_steps);
   const int tile_rows = min(kRaTileRows, t.rows - t.first);
   const uint16_t *k_head = p.k + place.head * p.k_stride_head, *v_head = p.v + place.head * p.v_stride_head;
   const bool narrow = tile_rows <= 32;
@@ -283,9 +291,9 @@ __global__ __launch_bounds__(kRaThreads, 2) void ragged_attention_kernel(RaParam
 #pragma unroll
     for (int ks = 0; ks < kSteps; ++ks) qf[ks] = *reinterpret_cast<const short8v*>(src + 16 * ks);
   }
-  // Here, where the compiler sees it: it would otherwise count the loads of the queries as under way for good, and wait for the keys'
-  // loads in their place ahead of every product.  0x0F70 = vmcnt(0), other counters untouched.
-  __builtin_amdgcn_s_waitcnt(0x0F70);
+  // Ahead of the loops and where the compiler sees it: it would otherwise count the loads of the queries as under way for good, and wait
+  // for the keys' loads in their place ahead of every product.  0x0F70 = vmcnt(0), other counters untouched.
+  auto wait_for_queries = [] { __builtin_amdgcn_s_waitcnt(0x0F70); };
   float16v o[kDTiles];
 #pragma unroll
   for (int dt = 0; dt < kDTiles; ++dt)
@@ -307,20 +315,22 @@ __global__ __launch_bounds__(kRaThreads, 2) void ragged_attention_kernel(RaParam
     }
     if constexpr (KIND == kRaMaskedRows) load4_to_lds(reinterpret_cast<const void*>((uintptr_t)(p.key_mask + t.key0 + k) & ~(uintptr_t)3), looked_up_lds + slot * 256);
   };
-  uint32_t at_page = 0, at_row = 0;  // of this lane's key: page and row in it, or row
+  uint32_t at_page = 0, at_row = 0;  // paged: page and row in it of this lane's key
+  int first_key = 0;                 // the key of lane 0
   uint64_t there = 0;                // which of the 64 keys exist
-  auto take_places = [&](int key, int slot) __attribute__((always_inline)) {
+  // The keys of the lanes: base + lane, or twice base + lane % 32.
+  auto take_places = [&](int base, int at, int slot) __attribute__((always_inline)) {
+    const int key = base + at;
     bool ok = key < t.len;
+    first_key = base;
     if constexpr (KIND == kRaPaged) {
       at_page = *reinterpret_cast<const uint32_t*>(looked_up + slot * 256 + lane * 4);
       at_row = next_row;  // of the key that was looked up last, which is this one where it exists
       ok = ok && at_page < p.n_pages;
-    } else {
-      at_row = (uint32_t)(t.key0 + key);
-      if constexpr (KIND == kRaMaskedRows) {
-        const uint32_t shift = 8 * ((uint32_t)(uintptr_t)(p.key_mask + t.key0 + min(key, t.len - 1)) & 3);
-        ok = ok && ((*reinterpret_cast<const uint32_t*>(looked_up + slot * 256 + lane * 4) >> shift) & 0xFF) != 0;
-      }
+    }
+    if constexpr (KIND == kRaMaskedRows) {
+      const uint32_t shift = 8 * ((uint32_t)(uintptr_t)(p.key_mask + t.key0 + min(key, t.len - 1)) & 3);
+      ok = ok && ((*reinterpret_cast<const uint32_t*>(looked_up + slot * 256 + lane * 4) >> shift) & 0xFF) != 0;
     }
     there = __builtin_amdgcn_ballot_w64(ok);
   };
@@ -330,25 +340,55 @@ __global__ __launch_bounds__(kRaThreads, 2) void ragged_attention_kernel(RaParam
   const uint32_t k_part = (uint32_t)k_piece<D>(lane / kPieces, lane % kPieces) * 16, v_part = (uint32_t)v_piece<D>(lane / kPieces, lane % kPieces) * 16;
   const uint32_t k_row = (uint32_t)(lane / kPieces) * p.k_stride_row * 2, v_row = (uint32_t)(lane / kPieces) * p.v_stride_row * 2;
   auto turn = [](bool values, int i) { return (values ? v_piece<D>(i * kRowsPerLoad, 0) : k_piece<D>(i * kRowsPerLoad, 0)) * 16; };
-  const bool whole_groups = KIND != kRaPaged || p.page.d % 16 == 0;  // 16 rows lie one behind the other
-  auto load_rows = [&](bool values, int r0, uint32_t lds) __attribute__((always_inline)) {
+  typedef __attribute__((address_space(3))) u32x4* lds_uint4;
+  const bool whole_pages = KIND == kRaPaged && p.page.d % 16 == 0;  // 16 rows from a multiple of 16 on lie one behind the other
+  // counted: as many loads whatever keys there are, for waits that leave some under way.
+  auto load_rows = [&](bool values, int r0, uint32_t lds, bool counted) __attribute__((always_inline)) {
     const uint16_t* base = values ? v_head : k_head;
     const uint32_t per_page = values ? p.v_stride_page : p.k_stride_page, per_row = values ? p.v_stride_row : p.k_stride_row;
-    if (whole_groups && ((uint32_t)(there >> r0) & 0xFFFFu) == 0xFFFFu) {
-      uint64_t at = (uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)at_row, r0) * per_row;
-      if constexpr (KIND == kRaPaged) at += (uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)at_page, r0) * per_page;
-      const uint16_t* from_here = uniform_pointer(base + at);
+    const uint32_t part = values ? v_part : k_part, in_row = values ? v_row : k_row;
+    const uint32_t exist = (uint32_t)(there >> r0) & 0xFFFFu;
+    // 16 rows one behind the other that may be read, whether they hold keys or not.
+    bool in_line;
+    uint64_t at;
+    if constexpr (KIND == kRaPaged) {
+      in_line = whole_pages && (exist & 1);
+      at = (uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)at_page, r0) * per_page + (uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)at_row, r0) * per_row;
+    } else {
+      in_line = first_key + r0 < t.len && (int64_t)t.key0 + first_key + r0 + 15 < p.n_keys;
+      at = (uint64_t)(uint32_t)(t.key0 + first_key + r0) * per_row;
+    }
+    if (in_line && (!values || exist == 0xFFFFu)) {  // K of keys that do not exist is read and not looked at
 #pragma unroll
       for (int i = 0; i < kGroupLoads; ++i)
-        load16_to_lds(((values ? v_part : k_part) ^ (uint32_t)turn(values, i)) + (values ? v_row : k_row),
-                      uniform_pointer(from_here + (uint64_t)i * kRowsPerLoad * per_row), lds + i * 1024);
+        load16_to_lds((part ^ (uint32_t)turn(values, i)) + in_row, uniform_pointer(base + at + (uint64_t)i * kRowsPerLoad * per_row), lds + i * 1024);
+      return;
+    }
+    // What follows is rare enough to form the lane's places anew: kept over the loops they would take registers these do not have.
+    int ln = lane;
+    asm volatile("" : "+v"(ln));
+    const int row0 = ln / kPieces, piece = ln % kPieces;
+    if (in_line && !counted) {  // of V, zeros take the place of rows that hold no key
+#pragma unroll
+      for (int i = 0; i < kGroupLoads; ++i) {
+        const int row = i * kRowsPerLoad + row0;
+        if ((exist >> row) & 1) {  // lanes that take no part write nothing
+          const uint32_t off = (uint32_t)row0 * per_row * 2 + (uint32_t)(values ? v_piece<D>(row, piece) : k_piece<D>(row, piece)) * 16;
+          load16_to_lds(off, uniform_pointer(base + at + (uint64_t)i * kRowsPerLoad * per_row), lds + i * 1024);
+        } else {
+          *(lds_uint4)(uintptr_t)(lds + i * 1024 + ln * 16) = u32x4{0, 0, 0, 0};
+        }
+      }
     } else {
 #pragma unroll
       for (int i = 0; i < kGroupLoads; ++i) {
-        const int row = r0 + i * kRowsPerLoad + lane / kPieces;
-        uint64_t at = (uint64_t)(uint32_t)__shfl((int)at_row, row) * per_row;
-        if constexpr (KIND == kRaPaged) at += (uint64_t)(uint32_t)__shfl((int)at_page, row) * per_page;
-        const uint8_t* src = reinterpret_cast<const uint8_t*>(base + at) + ((values ? v_part : k_part) ^ (uint32_t)turn(values, i));
+        const int in_group = i * kRowsPerLoad + row0, row = r0 + in_group;
+        if constexpr (KIND == kRaPaged) {
+          at = (uint64_t)(uint32_t)__shfl((int)at_page, row) * per_page + (uint64_t)(uint32_t)__shfl((int)at_row, row) * per_row;
+        } else {
+          at = (uint64_t)(uint32_t)(t.key0 + first_key + row) * per_row;
+        }
+        const uint8_t* src = reinterpret_cast<const uint8_t*>(base + at) + (values ? v_piece<D>(in_group, piece) : k_piece<D>(in_group, piece)) * 16;
         load16_to_lds((there >> row) & 1 ? src : reinterpret_cast<const uint8_t*>(kRaZeros), lds + i * 1024);
       }
     }
@@ -387,7 +427,10 @@ __global__ __launch_bounds__(kRaThreads, 2) void ragged_attention_kernel(RaParam
 #pragma unroll
     for (int kt = 0; kt < NT; ++kt)
 #pragma unroll
-      for (int r = 0; r < 16; ++r) sc[kt][r] = bits[kt] & (1u << (8 * (r / 4) + r % 4)) ? sc[kt][r] : -INFINITY;
+      for (int r = 0; r < 16; ++r) {
+        const uint32_t keep = (uint32_t)__builtin_amdgcn_sbfe((int)bits[kt], 8 * (r / 4) + r % 4, 1);
+        sc[kt][r] = __uint_as_float((keep & __float_as_uint(sc[kt][r])) | (~keep & 0xFF800000u));
+      }
     return true;
   };
   float neg = 0.0f;
@@ -511,28 +554,22 @@ __global__ __launch_bounds__(kRaThreads, 2) void ragged_attention_kernel(RaParam
     return mx;
   };
 
-  auto write_row = [&](int row_in_tile, const Row& r, int column, const float (&v)[4], float mm, float ll) __attribute__((always_inline)) {
-    // four columns of a row: of the result, or of this part's record
-    if (t.n_parts == 1) {
-      const float inv = ll == 0.0f ? 0.0f : 1.0f / ll;
-      uint16_t* dst = p.out + (t.q0 + r.token) * p.out_stride_token + r.head * p.out_stride_head + column;
-      *reinterpret_cast<uint2*>(dst) = make_uint2(T::pack2(v[0] * inv, v[1] * inv), T::pack2(v[2] * inv, v[3] * inv));
-    } else {
-      float* rec = record_of<D>(p, place, place.part);
-      *reinterpret_cast<float4*>(rec + row_in_tile * D + column) = make_float4(v[0], v[1], v[2], v[3]);
-      if (column == 0) *reinterpret_cast<float2*>(rec + p.record_rows * D + 2 * row_in_tile) = make_float2(mm, ll);
-    }
+  auto write_record = [&](int row_in_tile, int column, const float (&v)[4], float mm, float ll) __attribute__((always_inline)) {
+    // four columns of a row of this part's record
+    float* rec = record_of<D>(p, place, place.part);
+    *reinterpret_cast<float4*>(rec + row_in_tile * D + column) = make_float4(v[0], v[1], v[2], v[3]);
+    if (column == 0) *reinterpret_cast<float2*>(rec + p.record_rows * D + 2 * row_in_tile) = make_float2(mm, ll);
   };
 
   if (!narrow) {
     // K of step s is in buffer s & 1 an iteration before V of step s is: scores are a step ahead.
     const uint32_t k_lds = lds0 + wave * 16 * kRowBytes, v_lds = k_lds + 2 * kStepBytes;
     auto load_k = [&](int s) __attribute__((always_inline)) {
-      take_places(key_base(s) + lane, s & 1);
-      load_rows(false, wave * 16, k_lds + (s & 1) * kStepBytes);
+      take_places(key_base(s), lane, s & 1);
+      load_rows(false, wave * 16, k_lds + (s & 1) * kStepBytes, false);
       if (kLooksUp && s + 1 < s_end) look_up(key_base(s + 1) + lane, (s + 1) & 1);
     };
-    auto load_v = [&](int s) __attribute__((always_inline)) { load_rows(true, wave * 16, v_lds + (s & 1) * kStepBytes); };
+    auto load_v = [&](int s) __attribute__((always_inline)) { load_rows(true, wave * 16, v_lds + (s & 1) * kStepBytes, false); };
     const uint32_t k_rows = lds0, v_rows = lds0 + 2 * kStepBytes;
     float16v sc[2][2];
     uint64_t exist = 0;
@@ -544,7 +581,9 @@ __global__ __launch_bounds__(kRaThreads, 2) void ragged_attention_kernel(RaParam
       load_k(s_begin);
       exist = there;
       load_v(s_begin);
-      wait_loads<kGroupLoads>();
+    }
+    wait_for_queries();
+    if (s_begin < s_end) {
       __syncthreads();
       if (s_begin + 1 < s_end) load_k(s_begin + 1);
       if (!idle) {
@@ -583,15 +622,38 @@ __global__ __launch_bounds__(kRaThreads, 2) void ragged_attention_kernel(RaParam
     }
     if (idle) return;
     l = exchange_sum(l);
-    const Row to = own_row();
-    if (own + l32 < tile_rows) {
+    if (t.n_parts > 1) {
+      if (own + l32 < tile_rows) {
 #pragma unroll
-      for (int dt = 0; dt < kDTiles; ++dt)
+        for (int dt = 0; dt < kDTiles; ++dt)
 #pragma unroll
-        for (int g = 0; g < 4; ++g) {
-          const float v[4] = {o[dt][4 * g], o[dt][4 * g + 1], o[dt][4 * g + 2], o[dt][4 * g + 3]};
-          write_row(own + l32, to, 32 * dt + 8 * g + 4 * lh, v, m, l);
-        }
+          for (int g = 0; g < 4; ++g) {
+            const float v[4] = {o[dt][4 * g], o[dt][4 * g + 1], o[dt][4 * g + 2], o[dt][4 * g + 3]};
+            write_record(own + l32, 32 * dt + 8 * g + 4 * lh, v, m, l);
+          }
+      }
+      return;
+    }
+    // Whole rows per store, through the buffers of K, which every wave left ahead of the last step's barrier: straight from the registers a
+    // store reaches 16 bytes of each of 32 rows.
+    const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+    uint8_t* patch = smem + wave * 32 * kRowBytes;
+#pragma unroll
+    for (int dt = 0; dt < kDTiles; ++dt)
+#pragma unroll
+      for (int g = 0; g < 4; ++g)
+        *reinterpret_cast<uint2*>(patch + l32 * kRowBytes + k_piece<D>(l32, 4 * dt + g) * 16 + lh * 8) =
+            make_uint2(T::pack2(o[dt][4 * g] * inv, o[dt][4 * g + 1] * inv), T::pack2(o[dt][4 * g + 2] * inv, o[dt][4 * g + 3] * inv));
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+#pragma unroll
+    for (int it = 0; it < 32 / kRowsPerLoad; ++it) {
+      const int r = it * kRowsPerLoad + lane / kPieces, piece = lane % kPieces;
+      const uint4 v = *reinterpret_cast<const uint4*>(patch + r * kRowBytes + k_piece<D>(r, piece) * 16);
+      if (own + r < tile_rows) {
+        const int f = t.first + own + r, token = (uint32_t)f / p.group, head = place.head * p.group.d + (f - token * p.group.d);
+        *reinterpret_cast<uint4*>(p.out + (t.q0 + token) * p.out_stride_token + head * p.out_stride_head + 8 * piece) = v;
+      }
     }
     return;
   }
@@ -601,8 +663,8 @@ __global__ __launch_bounds__(kRaThreads, 2) void ragged_attention_kernel(RaParam
   constexpr int kLoads = 2 * kGroupLoads;  // of K or of V
   auto group_base = [&](int u) __attribute__((always_inline)) { return key_base(u >> 1) + 32 * (u & 1); };
   auto load_group = [&](bool values) __attribute__((always_inline)) {
-    load_rows(values, 0, rows_lds + (values ? 32 * kRowBytes : 0));
-    load_rows(values, 16, rows_lds + (values ? 32 * kRowBytes : 0) + 16 * kRowBytes);
+    load_rows(values, 0, rows_lds + (values ? 32 * kRowBytes : 0), true);
+    load_rows(values, 16, rows_lds + (values ? 32 * kRowBytes : 0) + 16 * kRowBytes, true);
   };
   const int u_end = 2 * s_end;
   int u = 2 * s_begin + wave;
@@ -611,10 +673,13 @@ __global__ __launch_bounds__(kRaThreads, 2) void ragged_attention_kernel(RaParam
       look_up(group_base(u) + l32, 0);
       wait_loads<0>();
     }
-    take_places(group_base(u) + l32, 0);
+    take_places(group_base(u), l32, 0);
     load_group(false);
     if (kLooksUp) look_up(group_base(min(u + 4, u_end - 1)) + l32, 1);
     load_group(true);
+  }
+  wait_for_queries();
+  if (u < u_end) {
     for (int slot = 1; u < u_end; u += 4, slot ^= 1) {
       const uint64_t exist = there;
       const bool more = u + 4 < u_end;
@@ -622,7 +687,7 @@ __global__ __launch_bounds__(kRaThreads, 2) void ragged_attention_kernel(RaParam
       float16v sc[1];
       scores(sc, rows_lds);
       if (more) {
-        take_places(group_base(u + 4) + l32, slot);
+        take_places(group_base(u + 4), l32, slot);
         wait_lds_reads();
         load_group(false);
         if (kLooksUp) look_up(group_base(min(u + 8, u_end - 1)) + l32, slot ^ 1);
@@ -661,6 +726,7 @@ __global__ __launch_bounds__(kRaThreads, 2) void ragged_attention_kernel(RaParam
     // a row without a maximum of which the sum is NaN has met NaN only
     all_l += e.x == -INFINITY ? e.y : e.y * weight[w];
   }
+  const float inv = all_l == 0.0f ? 0.0f : 1.0f / all_l;
 #pragma unroll
   for (int i = 0; i < kDTiles; ++i) {
     const int piece = wave * kDTiles + i, dt = piece >> 2, g = piece & 3;
@@ -673,7 +739,11 @@ __global__ __launch_bounds__(kRaThreads, 2) void ragged_attention_kernel(RaParam
       v[2] = fmaf(e.z, weight[w], v[2]);
       v[3] = fmaf(e.w, weight[w], v[3]);
     }
-    if (l32 < tile_rows) write_row(l32, to, 32 * dt + 8 * g + 4 * lh, v, all_m, all_l);
+    const int column = 32 * dt + 8 * g + 4 * lh;
+    if (l32 < tile_rows && t.n_parts > 1) write_record(l32, column, v, all_m, all_l);
+    if (l32 < tile_rows && t.n_parts == 1)
+      *reinterpret_cast<uint2*>(p.out + (t.q0 + to.token) * p.out_stride_token + to.head * p.out_stride_head + column) =
+          make_uint2(T::pack2(v[0] * inv, v[1] * inv), T::pack2(v[2] * inv, v[3] * inv));
   }
 }
 
@@ -683,29 +753,33 @@ __global__ __launch_bounds__(kRaThreads) void ragged_join_kernel(RaParams p) {
   const RaPlace place{blockIdx.x % (uint32_t)p.kv_heads, blockIdx.x / (uint32_t)p.kv_heads, 0};
   RaTile t;
   if (!find_tile<KIND>(p, place.tile, t) || t.n_parts == 1) return;
-  const int row = blockIdx.y * (kRaThreads * 4 / D) + threadIdx.x / (D / 4), column = threadIdx.x % (D / 4) * 4;
-  if (row >= min(kRaTileRows, t.rows - t.first)) return;
+  constexpr int kRows = kRaThreads * 4 / D;
+  const int column = threadIdx.x % (D / 4) * 4, rows = min(kRaTileRows, t.rows - t.first);
   const float* rec = record_of<D>(p, place, 0);
   const int64_t next = (int64_t)p.record_rows * (D + 2);
-  const float *ml = rec + p.record_rows * D + 2 * row, *x = rec + row * D + column;
-  float m = -INFINITY, l = 0.0f, v[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+  for (int row = blockIdx.y * kRows + threadIdx.x / (D / 4); row < rows; row += gridDim.y * kRows) {
+    const float *ml = rec + p.record_rows * D + 2 * row, *x = rec + row * D + column;
+    float m = -INFINITY, l = 0.0f, v[4] = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll 4
-  for (int part = 0; part < t.n_parts; ++part) m = fmaxf(m, ml[part * next]);
-#pragma unroll 4
-  for (int part = 0; part < t.n_parts; ++part) {
-    const float2 e = *reinterpret_cast<const float2*>(ml + part * next);
-    const float4 y = *reinterpret_cast<const float4*>(x + part * next);
-    const float w = e.x == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f((e.x - m) * p.scale_log2);
-    l += e.x == -INFINITY ? e.y : e.y * w;  // a part without a maximum whose sum is NaN has met NaN only
-    v[0] = fmaf(y.x, w, v[0]);
-    v[1] = fmaf(y.y, w, v[1]);
-    v[2] = fmaf(y.z, w, v[2]);
-    v[3] = fmaf(y.w, w, v[3]);
+    for (int part = 0; part < t.n_parts; ++part) {
+      const float2 e = *reinterpret_cast<const float2*>(ml + part * next);
+      const float4 y = *reinterpret_cast<const float4*>(x + part * next);
+      const float top = fmaxf(m, e.x);
+      const float a = m == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f((m - top) * p.scale_log2);
+      const float b = e.x == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f((e.x - top) * p.scale_log2);
+      // a sum beside a maximum of -inf is zero, or NaN where NaN was all that was met
+      l = (m == -INFINITY ? l : l * a) + (e.x == -INFINITY ? e.y : e.y * b);
+      v[0] = fmaf(y.x, b, v[0] * a);
+      v[1] = fmaf(y.y, b, v[1] * a);
+      v[2] = fmaf(y.z, b, v[2] * a);
+      v[3] = fmaf(y.w, b, v[3] * a);
+      m = top;
+    }
+    const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+    const int f = t.first + row, token = (uint32_t)f / p.group, head = place.head * p.group.d + (f - token * p.group.d);
+    uint16_t* dst = p.out + (t.q0 + token) * p.out_stride_token + head * p.out_stride_head + column;
+    *reinterpret_cast<uint2*>(dst) = make_uint2(T::pack2(v[0] * inv, v[1] * inv), T::pack2(v[2] * inv, v[3] * inv));
   }
-  const float inv = l == 0.0f ? 0.0f : 1.0f / l;
-  const int f = t.first + row, token = (uint32_t)f / p.group, head = place.head * p.group.d + (f - token * p.group.d);
-  uint16_t* dst = p.out + (t.q0 + token) * p.out_stride_token + head * p.out_stride_head + column;
-  *reinterpret_cast<uint2*>(dst) = make_uint2(T::pack2(v[0] * inv, v[1] * inv), T::pack2(v[2] * inv, v[3] * inv));
 }
 
 static int check_ragged(const ll_ragged_attention_args* a) {
@@ -733,8 +807,8 @@ static int check_ragged(const ll_ragged_attention_args* a) {
   return LL_OK;
 }
 
-// Parts of the keys: at least 512 (a wave of a narrow tile walks a quarter of them), at most 4096; records of up to 256 MiB.
-constexpr int64_t kRaLeastSteps = 8, kRaMostSteps = 64;
+// Parts of the keys, in steps of 64: at least 512 (a wave of a narrow tile walks a quarter of them); records of up to 256 MiB.
+constexpr int64_t kRaLeastSteps = 8, kRaMostNarrowSteps = 16, kRaLeastWideSteps = 12;
 constexpr size_t kRaMostBytes = (size_t)256 << 20;
 
 // How a launch is divided (host arithmetic).  Tiles of up to 128 rows; their keys in parts where the tiles alone are few for the
@@ -752,12 +826,22 @@ static RaPlan plan_ragged(const ll_ragged_attention_args& a, int cus) {
   const bool paged = a.page_table || a.page_size;
   const int64_t most_keys = paged ? a.table_width * a.page_size : a.n_keys;
   int64_t keys = a.max_kv_len > 0 && a.max_kv_len < most_keys ? a.max_kv_len : most_keys;
-  if (a.window > 0 && a.window < keys && a.sink_keys < keys) keys = std::min(keys, a.window + a.sink_keys + longest + 2 * kRaKeys);
+  if (a.window > 0 && a.window < keys && a.sink_keys < keys)  // what a tile's tokens see
+    keys = std::min(keys, a.window + a.sink_keys + kRaTileRows / group + 2 * kRaKeys);
   const int64_t steps = (keys + kRaKeys - 1) / kRaKeys;
   const int64_t busy = std::min<int64_t>(r.tiles, a.streams * ((longest * group + kRaTileRows - 1) / kRaTileRows)) * a.num_kv_heads;
-  const int64_t want = 2 * busy >= 3 * cus ? 1 : (4 * cus + busy - 1) / busy;
-  int64_t per_part = std::max<int64_t>((steps + want - 1) / want, kRaLeastSteps);
-  if (a.streams > 1) per_part = std::min(per_part, kRaMostSteps);
+  // Streams of the most keys take longest, and how many keys the others have is known on the device only: half of the most is assumed.
+  const int64_t shared = paged ? a.n_pages * a.page_size : a.n_keys;  // pages may be shared, and states too, but rarely
+  const int64_t mean_steps = a.streams > 1 ? std::min(steps, (shared / a.streams + kRaKeys - 1) / kRaKeys + 1) / 2 + 1 : steps;
+  int64_t per_part;
+  if (longest * group <= 32) {  // bound by memory: short parts keep the device busy to the end
+    per_part = std::min(std::max((steps * busy + 8 * cus - 1) / (8 * cus), kRaLeastSteps), kRaMostNarrowSteps);
+  } else if (a.streams > 1) {  // a third of what a workgroup that runs beside one other on each unit has to do in all
+    per_part = std::max(busy * mean_steps / (3 * 2 * cus), kRaLeastWideSteps);
+  } else {
+    const int64_t want = 2 * busy >= 3 * cus ? 1 : (4 * cus + busy - 1) / busy;
+    per_part = std::max((steps + want - 1) / want, kRaLeastSteps);
+  }
   const uint32_t record_rows = (uint32_t)std::min<int64_t>((longest * group + 31) / 32 * 32, kRaTileRows);
   const size_t record = (size_t)record_rows * (a.head_dim + 2) * sizeof(float);
   for (; per_part < steps; per_part *= 2) {
@@ -801,8 +885,9 @@ static int launch_ragged(const RaParams& p, uint32_t grid, hipStream_t stream) {
   ragged_attention_kernel<T, D, KIND><<<grid, kRaThreads, kRaLds<D>, stream>>>(p);
   LL_CHECK_LAUNCH("ll_ragged_attention");
   if (p.parts > 1) {
-    const uint32_t rows = kRaThreads * 4 / D;
-    ragged_join_kernel<T, D, KIND><<<dim3(p.tiles * (uint32_t)p.kv_heads, (p.record_rows + rows - 1) / rows), kRaThreads, 0, stream>>>(p);
+    // No more workgroups than a few rounds: most of them find a tile that was not cut, and that is all that they do.
+    const uint32_t tiles = p.tiles * (uint32_t)p.kv_heads, each = kRaThreads * 4 / D, most = std::max(1u, kRaJoinGroups / tiles);
+    ragged_join_kernel<T, D, KIND><<<dim3(tiles, std::min((p.record_rows + each - 1) / each, most)), kRaThreads, 0, stream>>>(p);
     LL_CHECK_LAUNCH("ll_ragged_attention (join)");
   }
   return LL_OK;
