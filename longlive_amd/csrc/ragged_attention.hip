@@ -3,9 +3,10 @@
 //
 //   out[t, h] = sum_j w_j v_j / sum_j w_j,   w_j = exp(scale * (q[t, h] . k_j - max)),   j over the keys that row t may see
 //
-// The rows of a kv head's queries, (token, head of the group) one behind the other, are cut into tiles of 128; the launch has as
-// many workgroups of four waves per kv head as there can be tiles, and each finds its own by a prefix sum over the streams.  A
-// workgroup multiplies
+// The rows of a kv head's queries, (token, head of the group) one behind the other, are cut into tiles of 128, and the keys of a tile
+// into parts of about as many steps as the plan says; the workgroups of the launch, as many as the device holds at once, take
+// these items in turn and find them by prefix sums over the streams, whose lengths only the device knows.  A workgroup of four
+// waves multiplies
 //   S^T = K Q^T  and  O^T = V^T P^T   (v_mfma_f32_32x32x16),
 // so that a lane owns one row: its maximum and sum need one exchange between the wave's halves, its mask two comparisons per
 // score with bounds of its own, and its rescaling is a multiplication by a scalar.  The probabilities leave the first product in
@@ -15,7 +16,7 @@
 //   * Tiles of up to 32 rows (single tokens, drafts): all waves own the same rows, and each walks every fourth group of 32 keys
 //     with LDS of its own and no barrier, K of the next group on its way from the moment the scores are done, V from the moment
 //     they are used; the four results are merged at the end.
-//   * Long key ranges are cut into parts of p.part_steps steps, a workgroup each, whose results a second launch joins in order.
+//   * The results of a tile's parts go to memory as they are, and a second launch joins them in order.
 //
 // K and V go straight from memory to LDS, 1024 bytes a load.  Where the rows lie is looked up one step ahead, an entry of the
 // page table per lane, also straight to LDS, so that no register load stands between the loads under way and their wait.
@@ -32,7 +33,7 @@ constexpr int kRaThreads = 256;
 constexpr int kRaTileRows = 128;  // rows of a workgroup, 32 a wave
 constexpr int kRaKeys = 64;       // keys of a step
 constexpr int kRaClearGroups = 16;
-constexpr uint32_t kRaJoinGroups = 8192;
+constexpr uint32_t kRaJoinGroups = 512;
 
 // Where keys lie: in the pages of a table, in rows one behind the other, in such rows with a mask.
 constexpr int kRaPaged = 0, kRaRows = 1, kRaMaskedRows = 2;
@@ -60,13 +61,11 @@ struct RaParams {
   int heads, kv_heads;
   Divisor group;          // heads of a kv head
   uint32_t window, sink;  // window 0: none
-  uint32_t tiles;         // workgroups per kv head and part: no fewer than there are tiles
-  uint32_t parts;         // workgroups that a tile's keys are cut for
-  uint32_t part_steps;    // a tile is cut into as many parts as it has that many steps
-  uint32_t record_rows;   // tiles of more rows are not cut
-  uint32_t work_groups;   // tiles * parts * kv_heads
-  int by_head;            // an XCD's workgroups are neighbours in the order head, part, tile
-  float* records;         // [kv head][tile][part]: record_rows x (D + 2) floats
+  uint32_t groups;        // workgroups that take the items
+  // Steps of a part, for tiles of more rows and for streams of up to 32 rows.  0 records: nothing is cut.
+  uint32_t part_steps, narrow_part_steps;
+  uint32_t records;       // of a kv head, 32 rows each
+  float* record_mem;      // [kv head][records]: 32 x D columns, then maximum and sum of each row
 };
 
 // Positions of 16-byte pieces in an LDS row of D columns.  The reads of a wave then go through all banks: 8 neighbouring rows of one
@@ -127,101 +126,160 @@ __device__ __forceinline__ int64_t stream_start(const RaParams& p, int b) { retu
 // The lowest n of 64 bits, for any n.
 __device__ __forceinline__ uint64_t low_bits(int n) { return n <= 0 ? 0 : n >= 64 ? ~0ull : ~(~0ull << n); }
 
-// The tile of a workgroup.
-struct RaTile {
-  int stream;
-  int64_t q0;           // first row of q of the stream
-  int n, rows, first;   // tokens of the stream; rows of the stream (token, head of the group), the tile's first
-  int len;              // keys of the stream
-  int key0;             // rows of keys: row of key 0
-  const int32_t* pages; // paged: the stream's row of the table
-  // keys: steps 0 .. sink_steps - 1 and then from from_step on, n_steps in all
-  int sink_steps, from_step, n_steps;
-  int n_parts, part_steps;  // workgroups that share the keys, steps of each
+// What a workgroup does next: a part of a tile.
+struct RaItem {
+  int64_t q0;               // first row of q of the stream
+  int n, rows, first;       // tokens of the stream; rows of the stream (token, head of the group), the tile's first
+  int len;                  // keys of the stream
+  int key0;                 // rows of keys: row of key 0
+  const int32_t* pages;     // paged: the stream's row of the table
+  int sink_steps, from_step;  // the tile's steps: 0 .. sink_steps - 1, and then from from_step on
+  int s_begin, s_end;       // of these, the part's
+  int n_parts, part;
+  uint32_t record;          // of part 0; the others follow, each as many records as the tile has groups of 32 rows
 };
 
-// Tile `index` of the tiles of a kv head: the streams' tiles one behind the other, the last of a stream (which sees most keys) first.
-// All lanes call it together, a stream a lane; what is known of the streams is loaded at once.  False: there are fewer tiles.
-template <int KIND>
-__device__ __forceinline__ bool find_tile(const RaParams& p, uint32_t index, RaTile& t) {
-  const int lane = threadIdx.x & 63;
-  t.stream = -1;
-  for (int b0 = 0; b0 < p.streams; b0 += 64) {
-    const int b = min(b0 + lane, p.streams - 1);
-    const int start = p.q_starts[b], next = p.q_starts[b + 1];
-    int key0 = 0, len;
-    if constexpr (KIND == kRaPaged) {
-      len = p.kv_lens[b];
-    } else {
-      key0 = p.k_starts[b];
-      len = p.k_lens ? p.k_lens[b] : p.k_starts[b + 1];
-    }
-    const int limit = (int)p.n_queries, q0 = min(max(start, 0), limit), n = max(min(max(next, 0), limit) - q0, 0);
-    int upto = b0 + lane < p.streams ? (int)(((int64_t)n * p.group.d + kRaTileRows - 1) / kRaTileRows) : 0;
-#pragma unroll
-    for (int d = 1; d < 64; d *= 2) {
-      const int other = __shfl_up(upto, d);
-      if (lane >= d) upto += other;
-    }
-    const uint64_t before = __builtin_amdgcn_ballot_w64((uint32_t)upto <= index);
-    if (before != ~0ull) {
-      const int at = __builtin_amdgcn_readfirstlane(__popcll(before));
-      t.stream = b0 + at;
-      t.first = (__builtin_amdgcn_readlane(upto, at) - 1 - (int)index) * kRaTileRows;
-      t.q0 = __builtin_amdgcn_readlane(q0, at);
-      t.n = __builtin_amdgcn_readlane(n, at);
-      t.len = __builtin_amdgcn_readlane(len, at);
-      t.key0 = __builtin_amdgcn_readlane(key0, at);
-      break;
-    }
-    index -= (uint32_t)__builtin_amdgcn_readlane(upto, 63);
-  }
-  if (t.stream < 0) return false;
-  t.rows = t.n * (int)p.group.d;
-  t.pages = nullptr;
-  if constexpr (KIND == kRaPaged) {
-    t.len = (int)min(max((int64_t)t.len, (int64_t)0), p.table_keys);
-    t.key0 = 0;
-    t.pages = p.page_table + t.stream * p.table_stride;
-  } else {
-    const int64_t first = min(max((int64_t)t.key0, (int64_t)0), p.n_keys);
-    const int64_t len = p.k_lens ? (int64_t)t.len : (int64_t)t.len - first;
-    t.key0 = (int)first;
-    t.len = (int)min(max(len, (int64_t)0), p.n_keys - first);
-  }
-  const int last_row = min(t.first + kRaTileRows, t.rows) - 1;
-  const int pos0 = t.len - t.n + (int)((uint32_t)t.first / p.group), pos1 = t.len - t.n + (int)((uint32_t)last_row / p.group);
-  const int end = p.causal ? min(pos1 + 1, t.len) : t.len;
+// The streams b0 .. b0 + 63, one a lane.
+struct RaStreams {
+  int q0, n, len, key0;
+  int tiles, parts;                  // parts at most: of the tile that sees most keys
+  uint32_t items_upto, records_upto;  // of these and the streams before
+};
+
+// Steps of a tile whose first and last token sit at pos0 and pos1, of a stream of len keys.
+struct RaSpan {
+  int sink_steps, from_step, n_steps;
+};
+__device__ __forceinline__ RaSpan span_of(const RaParams& p, int len, int pos0, int pos1) {
+  const int end = p.causal ? min(pos1 + 1, len) : len;
   const int from = p.window && pos0 >= (int)p.window ? pos0 - (int)p.window + 1 : 0;
   const int end_step = end > 0 ? (end - 1) / kRaKeys + 1 : 0;
-  t.from_step = from / kRaKeys;
-  t.sink_steps = min((int)(((int64_t)min((int)p.sink, from) + kRaKeys - 1) / kRaKeys), t.from_step);
-  t.n_steps = min(t.sink_steps, end_step) + max(end_step - t.from_step, 0);
-  const bool cut = p.parts > 1 && last_row - t.first < (int)p.record_rows;
-  t.n_parts = cut ? max(min((int)((t.n_steps + p.part_steps - 1) / p.part_steps), (int)p.parts), 1) : 1;
-  t.part_steps = (t.n_steps + t.n_parts - 1) / t.n_parts;  // equal parts
-  return true;
+  RaSpan s;
+  s.from_step = from / kRaKeys;
+  s.sink_steps = min((int)(((int64_t)min((int)p.sink, from) + kRaKeys - 1) / kRaKeys), s.from_step);
+  s.n_steps = min(s.sink_steps, end_step) + max(end_step - s.from_step, 0);
+  return s;
 }
+__device__ __forceinline__ uint32_t part_steps_of(const RaParams& p, int rows) { return rows <= 32 ? p.narrow_part_steps : p.part_steps; }
+// Records of a tile's part.
+__device__ __forceinline__ int record_groups(int rows) { return rows <= 32 ? 1 : kRaTileRows / 32; }
 
-// What workgroup `id` does.  Last parts come first, which only the tiles of the most keys have, and first parts, which all have, at the
-// end: what is long begins early.
-struct RaPlace {
-  uint32_t head, tile, part;
-};
-__device__ __forceinline__ RaPlace place_of(const RaParams& p, uint32_t id) {
-  if (p.by_head) {  // consecutive workgroups go to different XCDs: each gets a contiguous range of head, part, tile
-    const uint32_t per_head = p.tiles * p.parts;
-    id = p.work_groups % 8 == 0 ? (id & 7) * (p.work_groups / 8) + (id >> 3) : id;
-    const uint32_t head = id / per_head, rest = id - head * per_head, part = rest / p.tiles;
-    return RaPlace{head, rest - part * p.tiles, p.parts - 1 - part};
+// The sum over this lane and those before it, by moves between the lanes of a row of 16 and then from row to row.
+#define LL_DPP_ADD(v, ctrl, row_mask) v += (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, ctrl, row_mask, 0xF, true)
+__device__ __forceinline__ uint32_t sum_upto(uint32_t v) {
+  LL_DPP_ADD(v, 0x111, 0xF);  // row_shr:1
+  LL_DPP_ADD(v, 0x112, 0xF);  // row_shr:2
+  LL_DPP_ADD(v, 0x114, 0xF);  // row_shr:4
+  LL_DPP_ADD(v, 0x118, 0xF);  // row_shr:8
+  LL_DPP_ADD(v, 0x142, 0xA);  // row_bcast:15 into rows 1 and 3
+  LL_DPP_ADD(v, 0x143, 0xC);  // row_bcast:31 into rows 2 and 3
+  return v;
+}
+#undef LL_DPP_ADD
+
+// What is known of 64 streams, loaded at once; `items` and `records`: of the streams before.  A stream whose records would go beyond
+// what there is stays whole.  COUNT_TILES: the items are the tiles that were cut.
+template <int KIND, bool COUNT_TILES>
+__device__ __forceinline__ RaStreams load_streams(const RaParams& p, int b0, uint32_t items, uint32_t records) {
+  const int lane = threadIdx.x & 63, b = min(b0 + lane, p.streams - 1);
+  const int start = p.q_starts[b], next = p.q_starts[b + 1];
+  int64_t key0 = 0, len;
+  if constexpr (KIND == kRaPaged) {
+    len = min(max((int64_t)p.kv_lens[b], (int64_t)0), p.table_keys);
+  } else {
+    const int64_t first = p.k_starts[b], given = p.k_lens ? p.k_lens[b] : p.k_starts[b + 1];
+    key0 = min(max(first, (int64_t)0), p.n_keys);
+    len = min(max(p.k_lens ? given : given - key0, (int64_t)0), p.n_keys - key0);
   }
-  const uint32_t per_part = p.tiles * (uint32_t)p.kv_heads, part = id / per_part, rest = id - part * per_part, tile = rest / (uint32_t)p.kv_heads;
-  return RaPlace{rest - tile * (uint32_t)p.kv_heads, tile, p.parts - 1 - part};
+  const int limit = (int)p.n_queries;
+  RaStreams s;
+  s.q0 = min(max(start, 0), limit);
+  s.n = b0 + lane < p.streams ? max(min(max(next, 0), limit) - s.q0, 0) : 0;
+  s.len = (int)len;
+  s.key0 = (int)key0;
+  const int rows = s.n * (int)p.group.d;
+  s.tiles = (int)(((int64_t)rows + kRaTileRows - 1) / kRaTileRows);
+  s.parts = 1;
+  s.records_upto = 0;
+  if (p.records) {
+    uint32_t mine = 0;
+    if (s.tiles) {
+      // the first tile that sees the stream's last key sees most: where there is a window, up to a tile's tokens more than it
+      const int pos1 = s.len - 1, pos0 = pos1 - min(s.n - 1, (int)((uint32_t)(kRaTileRows - 1) / p.group) + 1);
+      const int steps = p.window ? span_of(p, s.len, pos0, pos1).n_steps + 1 : (s.len + kRaKeys - 1) / kRaKeys;
+      const uint32_t per_part = part_steps_of(p, rows);
+      s.parts = max((int)((steps + per_part - 1) / per_part), 1);
+      if (s.parts > 1) mine = (uint32_t)min((int64_t)s.tiles * s.parts * record_groups(rows), (int64_t)p.records + 1);
+    }
+    // sums that do not pass 32 bits: a stream adds at most records + 1, the streams before at most as much
+    s.records_upto = records + sum_upto(mine);
+    if (s.records_upto > p.records) s.parts = 1;
+  }
+  s.items_upto = items + sum_upto(COUNT_TILES ? (s.parts > 1 ? s.tiles : 0) : s.tiles * s.parts);
+  return s;
 }
 
+// Finds items one behind the other.
+template <int KIND, bool COUNT_TILES>
+struct RaCursor {
+  int b0 = 0;
+  uint32_t items = 0, records = 0;  // of the streams before b0
+  RaStreams s;                      // streams from b0 on
+  __device__ __forceinline__ void start(const RaParams& p) {
+    if (p.streams > 0) s = load_streams<KIND, COUNT_TILES>(p, 0, 0, 0);
+  }
+  // Item `index` of a kv head, which is no smaller than the last one asked for.  All lanes call it together.  False: there are fewer.
+  __device__ __forceinline__ bool find(const RaParams& p, uint32_t index, RaItem& t) {
+    if (p.streams <= 0) return false;
+    for (;;) {
+      const uint64_t before = __builtin_amdgcn_ballot_w64(s.items_upto <= index);
+      if (before != ~0ull) {
+        const int at = __builtin_amdgcn_readfirstlane(__popcll(before));
+        auto of = [&](int v) { return __builtin_amdgcn_readlane(v, at); };
+        const int tiles = of(s.tiles), parts = of(s.parts);
+        const uint32_t records_end = (uint32_t)of((int)s.records_upto);
+        // the last tile of a stream, which sees most keys, first, and all its parts
+        uint32_t left = (uint32_t)of((int)s.items_upto) - 1 - index;
+        const uint32_t tile = COUNT_TILES ? left : left / (uint32_t)parts;
+        t.part = COUNT_TILES ? 0 : (int)(left - tile * (uint32_t)parts);
+        t.q0 = of(s.q0);
+        t.n = of(s.n);
+        t.rows = t.n * (int)p.group.d;
+        t.first = (int)tile * kRaTileRows;
+        t.len = of(s.len);
+        t.key0 = of(s.key0);
+        t.pages = KIND == kRaPaged ? p.page_table + (int64_t)(b0 + at) * p.table_stride : nullptr;
+        const int last_row = min(t.first + kRaTileRows, t.rows) - 1, base = t.len - t.n;
+        const RaSpan span = span_of(p, t.len, base + (int)((uint32_t)t.first / p.group), base + (int)((uint32_t)last_row / p.group));
+        t.sink_steps = span.sink_steps;
+        t.from_step = span.from_step;
+        const uint32_t per_part = part_steps_of(p, t.rows);
+        t.n_parts = parts > 1 ? max(min((int)((span.n_steps + per_part - 1) / per_part), parts), 1) : 1;
+        const int each = (span.n_steps + t.n_parts - 1) / t.n_parts;  // equal parts
+        t.s_begin = min(t.part * each, span.n_steps);
+        t.s_end = min(t.s_begin + each, span.n_steps);
+        t.record = records_end - (uint32_t)((tiles - (int)tile) * parts * record_groups(t.rows));
+        return true;
+      }
+      b0 += 64;
+      if (b0 >= p.streams) return false;
+      items = (uint32_t)__builtin_amdgcn_readlane((int)s.items_upto, 63);
+      records = min((uint32_t)__builtin_amdgcn_readlane((int)s.records_upto, 63), p.records + 1);
+      s = load_streams<KIND, COUNT_TILES>(p, b0, items, records);
+    }
+  }
+};
+
+// Where part `part` of an item's tile has the four columns from `column` on of a row, and the row's maximum and sum.
 template <int D>
-__device__ __forceinline__ float* record_of(const RaParams& p, const RaPlace& at, uint32_t part) {
-  return p.records + ((int64_t)(at.head * p.tiles + at.tile) * p.parts + part) * p.record_rows * (D + 2);
+__device__ __forceinline__ float* record_of(const RaParams& p, uint32_t head, const RaItem& t, int part, int row) {
+  const int64_t at = (int64_t)head * p.records + t.record + (uint32_t)(part * record_groups(t.rows) + row / 32);
+  return p.record_mem + at * 32 * (D + 2) + row % 32 * D;
+}
+template <int D>
+__device__ __forceinline__ float2* record_sums(const RaParams& p, uint32_t head, const RaItem& t, int part, int row) {
+  const int64_t at = (int64_t)head * p.records + t.record + (uint32_t)(part * record_groups(t.rows) + row / 32);
+  return reinterpret_cast<float2*>(p.record_mem + at * 32 * (D + 2) + 32 * D) + row % 32;
 }
 
 template <int D>
@@ -237,18 +295,16 @@ __device__ __forceinline__ void each_index(F& f, std::integer_sequence<int, I...
 constexpr float kRaStep = 2.0f;
 
 template <typename T, int D, int KIND>
-__global__ __launch_bounds__(kRaThreads, 2) void ragged_attention_kernel(RaParams p) {
+__global__ __launch_bounds__(kRaThreads, D == 64 ? 3 : 2) void ragged_attention_kernel(RaParams p) {
   constexpr int kRowBytes = 2 * D, kPieces = D / 8, kDTiles = D / 32, kSteps = D / 16;
   constexpr int kRowsPerLoad = 1024 / kRowBytes, kGroupLoads = 16 / kRowsPerLoad;  // loads of 16 rows
   constexpr int kStepBytes = kRaKeys * kRowBytes;                                  // K or V of a step
   constexpr bool kLooksUp = KIND != kRaRows;
   extern __shared__ __attribute__((aligned(1024))) uint8_t smem[];
-  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), l32 = lane & 31, lh = lane >> 5;
-
-  if (blockIdx.x >= p.work_groups) {  // rows outside every stream
+  if (blockIdx.x >= p.groups) {  // rows outside every stream
     const int64_t first = p.streams ? stream_start(p, 0) : 0, end = p.streams ? max(stream_start(p, p.streams), first) : 0;
     const int64_t outside = first + p.n_queries - end, pieces = outside * p.heads * kPieces;
-    for (int64_t i = (int64_t)(blockIdx.x - p.work_groups) * kRaThreads + tid; i < pieces; i += (int64_t)kRaClearGroups * kRaThreads) {
+    for (int64_t i = (int64_t)(blockIdx.x - p.groups) * kRaThreads + threadIdx.x; i < pieces; i += (int64_t)kRaClearGroups * kRaThreads) {
       const int64_t row = i / (p.heads * kPieces);
       const int at = (int)(i - row * (p.heads * kPieces)), h = at / kPieces, c = at % kPieces;
       uint16_t* dst = p.out + (row < first ? row : row - first + end) * p.out_stride_token + h * p.out_stride_head + 8 * c;
@@ -257,12 +313,25 @@ __global__ __launch_bounds__(kRaThreads, 2) void ragged_attention_kernel(RaParam
     return;
   }
 
-  const RaPlace place = place_of(p, blockIdx.x);
-  RaTile t;
-  if (!find_tile<KIND>(p, place.tile, t) || (int)place.part >= t.n_parts) return;
-  const int s_begin = min((int)place.part * t.part_steps, t.n_steps), s_end = min(s_begin + t.part_steps, t.n_steps);
+  // Item after item: a kv head after the other, so that with a multiple of eight heads the workgroups of an XCD (consecutive ones go to
+  // different XCDs) read the same, and neighbouring tiles of a stream run side by side.  (Items handed to whoever asks first, by a counter
+  // of each XCD that a launch ahead clears: 12 streams of 1 to 700 tokens over 300 to 9000 keys 176 us in turn, 199 so.)
+  RaCursor<KIND, false> cursor;
+  cursor.start(p);
+  for (uint32_t id = blockIdx.x;; id += p.groups) {
+  const uint32_t index = id / (uint32_t)p.kv_heads, kv_head = id - index * (uint32_t)p.kv_heads;
+  RaItem t;
+  if (!cursor.find(p, index, t)) return;
+  if (t.part >= t.n_parts) continue;  // a tile that sees fewer keys than the stream's last
+  __syncthreads();                    // no wave is at the item before any more
+  // The thread's coordinates, formed anew for every item: what is derived from them would otherwise be formed ahead of the loop over the
+  // items and take registers throughout.
+  int tid = threadIdx.x;
+  asm volatile("" : "+v"(tid));
+  const int lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), l32 = lane & 31, lh = lane >> 5;
+  const int s_begin = t.s_begin, s_end = t.s_end;
   const int tile_rows = min(kRaTileRows, t.rows - t.first);
-  const uint16_t *k_head = p.k + place.head * p.k_stride_head, *v_head = p.v + place.head * p.v_stride_head;
+  const uint16_t *k_head = p.k + kv_head * p.k_stride_head, *v_head = p.v + kv_head * p.v_stride_head;
   const bool narrow = tile_rows <= 32;
   const int own = narrow ? 0 : wave * 32;  // the wave's first row in the tile
 
@@ -274,7 +343,7 @@ __global__ __launch_bounds__(kRaThreads, 2) void ragged_attention_kernel(RaParam
     int f = min(t.first + own + l32, t.rows - 1);
     asm volatile("" : "+v"(f));
     const int token = (uint32_t)f / p.group;
-    return Row{token, (int)(place.head * p.group.d) + f - token * (int)p.group.d};
+    return Row{token, (int)(kv_head * p.group.d) + f - token * (int)p.group.d};
   };
   const Row row = own_row();
   // what it sees: keys below `last`, from `from` on or below the sink
@@ -493,7 +562,7 @@ __global__ __launch_bounds__(kRaThreads, 2) void ragged_attention_kernel(RaParam
   // what runs beside it, held in place by scheduling barriers: the LDS reads of MFMAs some slots later, and the probabilities, a pair
   // of keys' multiply-adds, exponentials and packing in three slots in a row.
   auto step_and_next = [&](float16v (&sc)[2], float16v (&nx)[2], uint32_t next_k, uint32_t v_rows) __attribute__((always_inline)) {
-    constexpr int kS = 2 * kSteps, kSlots = kS + 4 * kDTiles, kAhead = 4, kRing = kAhead + 1, kVAhead = 3, kVRing = kVAhead + 1;
+    constexpr int kS = 2 * kSteps, kSlots = kS + 4 * kDTiles, kAhead = D == 64 ? 2 : 4, kRing = kAhead + 1, kVAhead = D == 64 ? 2 : 3, kVRing = kVAhead + 1;
     short8v fk[kRing];
     short4v fv[kVRing][2];
     uint32_t pw[16];
@@ -556,9 +625,8 @@ __global__ __launch_bounds__(kRaThreads, 2) void ragged_attention_kernel(RaParam
 
   auto write_record = [&](int row_in_tile, int column, const float (&v)[4], float mm, float ll) __attribute__((always_inline)) {
     // four columns of a row of this part's record
-    float* rec = record_of<D>(p, place, place.part);
-    *reinterpret_cast<float4*>(rec + row_in_tile * D + column) = make_float4(v[0], v[1], v[2], v[3]);
-    if (column == 0) *reinterpret_cast<float2*>(rec + p.record_rows * D + 2 * row_in_tile) = make_float2(mm, ll);
+    *reinterpret_cast<float4*>(record_of<D>(p, kv_head, t, t.part, row_in_tile) + column) = make_float4(v[0], v[1], v[2], v[3]);
+    if (column == 0) *record_sums<D>(p, kv_head, t, t.part, row_in_tile) = make_float2(mm, ll);
   };
 
   if (!narrow) {
@@ -571,7 +639,6 @@ __global__ __launch_bounds__(kRaThreads, 2) void ragged_attention_kernel(RaParam
     };
     auto load_v = [&](int s) __attribute__((always_inline)) { load_rows(true, wave * 16, v_lds + (s & 1) * kStepBytes, false); };
     const uint32_t k_rows = lds0, v_rows = lds0 + 2 * kStepBytes;
-    float16v sc[2][2];
     uint64_t exist = 0;
     if (s_begin < s_end) {
       if (kLooksUp) {
@@ -586,41 +653,50 @@ __global__ __launch_bounds__(kRaThreads, 2) void ragged_attention_kernel(RaParam
     if (s_begin < s_end) {
       __syncthreads();
       if (s_begin + 1 < s_end) load_k(s_begin + 1);
-      if (!idle) {
-        scores(sc[0], k_rows + (s_begin & 1) * kStepBytes);
-        mask(sc[0], key_base(s_begin), exist);
-        follow(largest(sc[0]));
-      }
     }
-    auto iteration = [&](int s, auto from_tag) __attribute__((always_inline)) {
-      constexpr int from_buffer = decltype(from_tag)::value;
-      wait_loads<0>();
-      __syncthreads();  // K of step s + 1 and V of step s are in LDS, and every wave is done with K of step s and V of step s - 1
-      exist = there;    // of step s + 1
-      load_v(s + 1);    // from the places of the last load_k
-      if (s + 2 < s_end) load_k(s + 2);
-      if (idle) return;
-      float mx = step_and_next(sc[from_buffer], sc[from_buffer ^ 1], k_rows + ((s + 1) & 1) * kStepBytes, v_rows + (s & 1) * kStepBytes);
-      if (mask(sc[from_buffer ^ 1], key_base(s + 1), exist)) mx = largest(sc[from_buffer ^ 1]);
-      follow(mx);
-    };
-    int s = s_begin;
-    for (; s + 2 < s_end; s += 2) {
-      iteration(s, std::integral_constant<int, 0>{});
-      iteration(s + 1, std::integral_constant<int, 1>{});
-    }
-    if (s + 1 < s_end) {
-      iteration(s, std::integral_constant<int, 0>{});
-      sc[0][0] = sc[1][0];
-      sc[0][1] = sc[1][1];
-      ++s;
-    }
-    if (s < s_end) {
+    // An iteration's loads: K of step s + 1 and V of step s are in LDS, and every wave is done with K of step s and V of step s - 1.
+    auto move_keys = [&](int s) __attribute__((always_inline)) {
       wait_loads<0>();
       __syncthreads();
-      if (!idle) weigh(sc[0], v_rows + (s & 1) * kStepBytes);
+      exist = there;  // of step s + 1
+      load_v(s + 1);  // from the places of the last load_k
+      if (s + 2 < s_end) load_k(s + 2);
+    };
+    if (idle) {
+      if (s_begin < s_end) {
+        for (int s = s_begin; s + 1 < s_end; ++s) move_keys(s);
+        wait_loads<0>();
+        __syncthreads();
+      }
+      continue;
     }
-    if (idle) return;
+    if (s_begin < s_end) {
+      float16v sc[2][2];
+      scores(sc[0], k_rows + (s_begin & 1) * kStepBytes);
+      mask(sc[0], key_base(s_begin), exist);
+      follow(largest(sc[0]));
+      auto iteration = [&](int s, auto from_tag) __attribute__((always_inline)) {
+        constexpr int from_buffer = decltype(from_tag)::value;
+        move_keys(s);
+        float mx = step_and_next(sc[from_buffer], sc[from_buffer ^ 1], k_rows + ((s + 1) & 1) * kStepBytes, v_rows + (s & 1) * kStepBytes);
+        if (mask(sc[from_buffer ^ 1], key_base(s + 1), exist)) mx = largest(sc[from_buffer ^ 1]);
+        follow(mx);
+      };
+      int s = s_begin;
+      for (; s + 2 < s_end; s += 2) {
+        iteration(s, std::integral_constant<int, 0>{});
+        iteration(s + 1, std::integral_constant<int, 1>{});
+      }
+      if (s + 1 < s_end) {
+        iteration(s, std::integral_constant<int, 0>{});
+        sc[0][0] = sc[1][0];
+        sc[0][1] = sc[1][1];
+        ++s;
+      }
+      wait_loads<0>();
+      __syncthreads();
+      weigh(sc[0], v_rows + (s & 1) * kStepBytes);
+    }
     l = exchange_sum(l);
     if (t.n_parts > 1) {
       if (own + l32 < tile_rows) {
@@ -632,7 +708,7 @@ __global__ __launch_bounds__(kRaThreads, 2) void ragged_attention_kernel(RaParam
             write_record(own + l32, 32 * dt + 8 * g + 4 * lh, v, m, l);
           }
       }
-      return;
+      continue;
     }
     // Whole rows per store, through the buffers of K, which every wave left ahead of the last step's barrier: straight from the registers a
     // store reaches 16 bytes of each of 32 rows.
@@ -651,11 +727,11 @@ __global__ __launch_bounds__(kRaThreads, 2) void ragged_attention_kernel(RaParam
       const int r = it * kRowsPerLoad + lane / kPieces, piece = lane % kPieces;
       const uint4 v = *reinterpret_cast<const uint4*>(patch + r * kRowBytes + k_piece<D>(r, piece) * 16);
       if (own + r < tile_rows) {
-        const int f = t.first + own + r, token = (uint32_t)f / p.group, head = place.head * p.group.d + (f - token * p.group.d);
+        const int f = t.first + own + r, token = (uint32_t)f / p.group, head = kv_head * p.group.d + (f - token * p.group.d);
         *reinterpret_cast<uint4*>(p.out + (t.q0 + token) * p.out_stride_token + head * p.out_stride_head + 8 * piece) = v;
       }
     }
-    return;
+    continue;
   }
 
   // ---- up to 32 rows: groups of 32 keys u = 2 s + half, every fourth one this wave's
@@ -745,40 +821,44 @@ __global__ __launch_bounds__(kRaThreads, 2) void ragged_attention_kernel(RaParam
       *reinterpret_cast<uint2*>(p.out + (t.q0 + to.token) * p.out_stride_token + to.head * p.out_stride_head + column) =
           make_uint2(T::pack2(v[0] * inv, v[1] * inv), T::pack2(v[2] * inv, v[3] * inv));
   }
+  }
 }
 
-// Joins the parts of the tiles that were cut: D / 4 lanes a row, kRaThreads * 4 / D rows of a tile a workgroup.
+// Joins the parts of the tiles that were cut, item by item: D / 4 lanes a row.
 template <typename T, int D, int KIND>
 __global__ __launch_bounds__(kRaThreads) void ragged_join_kernel(RaParams p) {
-  const RaPlace place{blockIdx.x % (uint32_t)p.kv_heads, blockIdx.x / (uint32_t)p.kv_heads, 0};
-  RaTile t;
-  if (!find_tile<KIND>(p, place.tile, t) || t.n_parts == 1) return;
   constexpr int kRows = kRaThreads * 4 / D;
-  const int column = threadIdx.x % (D / 4) * 4, rows = min(kRaTileRows, t.rows - t.first);
-  const float* rec = record_of<D>(p, place, 0);
-  const int64_t next = (int64_t)p.record_rows * (D + 2);
-  for (int row = blockIdx.y * kRows + threadIdx.x / (D / 4); row < rows; row += gridDim.y * kRows) {
-    const float *ml = rec + p.record_rows * D + 2 * row, *x = rec + row * D + column;
-    float m = -INFINITY, l = 0.0f, v[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+  const int column = threadIdx.x % (D / 4) * 4;
+  RaCursor<KIND, true> cursor;
+  cursor.start(p);
+  for (uint32_t id = blockIdx.x;; id += gridDim.x) {
+    const uint32_t index = id / (uint32_t)p.kv_heads, kv_head = id - index * (uint32_t)p.kv_heads;
+    RaItem t;
+    if (!cursor.find(p, index, t)) return;
+    if (t.n_parts == 1) continue;
+    const int rows = min(kRaTileRows, t.rows - t.first);
+    for (int row = blockIdx.y * kRows + threadIdx.x / (D / 4); row < rows; row += gridDim.y * kRows) {
+      float m = -INFINITY, l = 0.0f, v[4] = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll 4
-    for (int part = 0; part < t.n_parts; ++part) {
-      const float2 e = *reinterpret_cast<const float2*>(ml + part * next);
-      const float4 y = *reinterpret_cast<const float4*>(x + part * next);
-      const float top = fmaxf(m, e.x);
-      const float a = m == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f((m - top) * p.scale_log2);
-      const float b = e.x == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f((e.x - top) * p.scale_log2);
-      // a sum beside a maximum of -inf is zero, or NaN where NaN was all that was met
-      l = (m == -INFINITY ? l : l * a) + (e.x == -INFINITY ? e.y : e.y * b);
-      v[0] = fmaf(y.x, b, v[0] * a);
-      v[1] = fmaf(y.y, b, v[1] * a);
-      v[2] = fmaf(y.z, b, v[2] * a);
-      v[3] = fmaf(y.w, b, v[3] * a);
-      m = top;
+      for (int part = 0; part < t.n_parts; ++part) {
+        const float2 e = *record_sums<D>(p, kv_head, t, part, row);
+        const float4 y = *reinterpret_cast<const float4*>(record_of<D>(p, kv_head, t, part, row) + column);
+        const float top = fmaxf(m, e.x);
+        const float a = m == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f((m - top) * p.scale_log2);
+        const float b = e.x == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f((e.x - top) * p.scale_log2);
+        // a sum beside a maximum of -inf is zero, or NaN where NaN was all that was met
+        l = (m == -INFINITY ? l : l * a) + (e.x == -INFINITY ? e.y : e.y * b);
+        v[0] = fmaf(y.x, b, v[0] * a);
+        v[1] = fmaf(y.y, b, v[1] * a);
+        v[2] = fmaf(y.z, b, v[2] * a);
+        v[3] = fmaf(y.w, b, v[3] * a);
+        m = top;
+      }
+      const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+      const int f = t.first + row, token = (uint32_t)f / p.group, head = kv_head * p.group.d + (f - token * p.group.d);
+      uint16_t* dst = p.out + (t.q0 + token) * p.out_stride_token + head * p.out_stride_head + column;
+      *reinterpret_cast<uint2*>(dst) = make_uint2(T::pack2(v[0] * inv, v[1] * inv), T::pack2(v[2] * inv, v[3] * inv));
     }
-    const float inv = l == 0.0f ? 0.0f : 1.0f / l;
-    const int f = t.first + row, token = (uint32_t)f / p.group, head = place.head * p.group.d + (f - token * p.group.d);
-    uint16_t* dst = p.out + (t.q0 + token) * p.out_stride_token + head * p.out_stride_head + column;
-    *reinterpret_cast<uint2*>(dst) = make_uint2(T::pack2(v[0] * inv, v[1] * inv), T::pack2(v[2] * inv, v[3] * inv));
   }
 }
 
@@ -807,54 +887,63 @@ static int check_ragged(const ll_ragged_attention_args* a) {
   return LL_OK;
 }
 
-// Parts of the keys, in steps of 64: at least 512 (a wave of a narrow tile walks a quarter of them); records of up to 256 MiB.
-constexpr int64_t kRaLeastSteps = 8, kRaMostNarrowSteps = 16, kRaLeastWideSteps = 12;
-constexpr size_t kRaMostBytes = (size_t)256 << 20;
-
-// How a launch is divided (host arithmetic).  Tiles of up to 128 rows; their keys in parts where the tiles alone are few for the
-// device, and where a stream's keys are so many that one workgroup would still walk them when the others are done.
+// How a launch is divided (host arithmetic): as many workgroups as the device holds, and the steps of a part.  Only the device knows
+// the streams' lengths; the host knows the longest, if it is told, and how many rows there are in all.
 struct RaPlan {
-  uint32_t tiles, parts, part_steps, record_rows;
+  uint32_t groups, part_steps, narrow_part_steps, records;
   size_t bytes;
 };
+constexpr int64_t kRaPartCost = 3;          // what an item costs beside its steps, in steps
+constexpr int64_t kRaCutCost = 7;           // ... and where it leaves a record, with the joining of it
+constexpr int64_t kRaLeastWideSteps = 10, kRaLeastNarrowSteps = 8, kRaMostNarrowSteps = 16;
+constexpr size_t kRaMostBytes = (size_t)256 << 20;  // of records
+
 static RaPlan plan_ragged(const ll_ragged_attention_args& a, int cus) {
-  RaPlan r{0, 1, 0, 0, 0};
-  const int64_t group = a.num_heads / a.num_kv_heads, rows = a.n_queries * group;
-  const int64_t longest = a.max_q_len > 0 && a.max_q_len < a.n_queries ? a.max_q_len : a.n_queries;
-  r.tiles = (uint32_t)(a.n_queries == 0 ? 0 : rows / kRaTileRows + a.streams);  // each stream one tile that is not full
-  if (r.tiles == 0) return r;
+  RaPlan r{0, 0, 0, 0, 0};
+  if (a.n_queries == 0 || a.streams == 0) return r;
   const bool paged = a.page_table || a.page_size;
-  const int64_t most_keys = paged ? a.table_width * a.page_size : a.n_keys;
-  int64_t keys = a.max_kv_len > 0 && a.max_kv_len < most_keys ? a.max_kv_len : most_keys;
-  if (a.window > 0 && a.window < keys && a.sink_keys < keys)  // what a tile's tokens see
-    keys = std::min(keys, a.window + a.sink_keys + kRaTileRows / group + 2 * kRaKeys);
-  const int64_t steps = (keys + kRaKeys - 1) / kRaKeys;
-  const int64_t busy = std::min<int64_t>(r.tiles, a.streams * ((longest * group + kRaTileRows - 1) / kRaTileRows)) * a.num_kv_heads;
-  // Streams of the most keys take longest, and how many keys the others have is known on the device only: half of the most is assumed.
-  const int64_t shared = paged ? a.n_pages * a.page_size : a.n_keys;  // pages may be shared, and states too, but rarely
-  const int64_t mean_steps = a.streams > 1 ? std::min(steps, (shared / a.streams + kRaKeys - 1) / kRaKeys + 1) / 2 + 1 : steps;
-  int64_t per_part;
-  if (longest * group <= 32) {  // bound by memory: short parts keep the device busy to the end
-    per_part = std::min(std::max((steps * busy + 8 * cus - 1) / (8 * cus), kRaLeastSteps), kRaMostNarrowSteps);
-  } else if (a.streams > 1) {  // a third of what a workgroup that runs beside one other on each unit has to do in all
-    per_part = std::max(busy * mean_steps / (3 * 2 * cus), kRaLeastWideSteps);
-  } else {
-    const int64_t want = 2 * busy >= 3 * cus ? 1 : (4 * cus + busy - 1) / busy;
-    per_part = std::max((steps + want - 1) / want, kRaLeastSteps);
+  const int64_t group = a.num_heads / a.num_kv_heads, slots = (a.head_dim == 64 ? 3 : 2) * cus;
+  const int64_t longest = a.max_q_len > 0 && a.max_q_len < a.n_queries ? a.max_q_len : a.n_queries;
+  const int64_t tiles = std::min(a.n_queries * group / kRaTileRows + a.streams, a.streams * ((longest * group + kRaTileRows - 1) / kRaTileRows));
+  const int64_t all_keys = paged ? a.table_width * a.page_size : a.n_keys, rows_of_keys = paged ? a.n_pages * a.page_size : a.n_keys;
+  int64_t keys = a.max_kv_len > 0 && a.max_kv_len < all_keys ? a.max_kv_len : all_keys;
+  bool alike = a.streams == 1;  // whether all tiles see about as many keys
+  if (a.window > 0 && a.window < keys && a.sink_keys < keys) {
+    const int64_t seen = a.window + a.sink_keys + kRaTileRows / group + kRaKeys;
+    alike = alike || 2 * seen < keys;
+    keys = std::min(keys, seen);
   }
-  const uint32_t record_rows = (uint32_t)std::min<int64_t>((longest * group + 31) / 32 * 32, kRaTileRows);
-  const size_t record = (size_t)record_rows * (a.head_dim + 2) * sizeof(float);
-  for (; per_part < steps; per_part *= 2) {
-    const int64_t parts = (steps + per_part - 1) / per_part;
-    const size_t bytes = (size_t)r.tiles * a.num_kv_heads * parts * record;
-    if (bytes <= kRaMostBytes && (int64_t)r.tiles * a.num_kv_heads * parts < (1ll << 30)) {
-      r.parts = (uint32_t)parts;
-      r.part_steps = (uint32_t)per_part;
-      r.record_rows = record_rows;
-      r.bytes = bytes;
-      break;
+  const int64_t steps = std::max<int64_t>((keys + kRaKeys - 1) / kRaKeys, 1), busy = tiles * a.num_kv_heads;
+  // Narrow tiles are bound by memory: parts short enough to keep the device busy to the end whatever the lengths are.
+  r.narrow_part_steps = (uint32_t)std::min(std::max((steps * busy + 4 * slots - 1) / (4 * slots), kRaLeastNarrowSteps), kRaMostNarrowSteps);
+  if (alike) {  // the number of parts for which the rounds of all of them, one behind the other, are shortest
+    int64_t best = 1, least = -1;
+    for (int64_t parts = 1; parts <= 64 && (parts == 1 || steps / parts >= kRaLeastNarrowSteps); ++parts) {
+      const int64_t each = (steps + parts - 1) / parts, cost = (busy * parts + slots - 1) / slots * (each + (parts > 1 ? kRaCutCost : kRaPartCost)) + (parts > 1 ? kRaCutCost : 0);
+      if (least < 0 || cost < least) {
+        least = cost;
+        best = parts;
+      }
     }
+    r.part_steps = best == 1 ? 1u << 24 : (uint32_t)((steps + best - 1) / best);
+  } else {  // about what a workgroup has to do in all, if the mean stream has half of the keys that there is room for
+    const int64_t mean = std::min(steps, (rows_of_keys / a.streams + kRaKeys - 1) / kRaKeys + 1) / 2 + 1;
+    r.part_steps = (uint32_t)std::min<int64_t>(std::max(busy * mean * 5 / (4 * slots), kRaLeastWideSteps), 1 << 24);
   }
+  const bool all_narrow = longest * group <= 32;
+  // Beside wider tiles, streams of few rows are worth a second launch only where they are long.
+  if (!all_narrow && (a.streams == 1 || steps <= 2 * kRaMostNarrowSteps)) r.narrow_part_steps = 1u << 24;
+  const int64_t part = all_narrow ? r.narrow_part_steps : std::min(r.part_steps, r.narrow_part_steps);
+  const int64_t parts = (steps + part - 1) / part;
+  if (parts > 1) {
+    // Every tile in as many parts, or what is allowed; streams that find no records left stay whole.
+    const size_t record = 32 * (size_t)(a.head_dim + 2) * sizeof(float);
+    const int64_t want = tiles * parts * (all_narrow ? 1 : kRaTileRows / 32);
+    r.records = (uint32_t)std::min<int64_t>(want, (int64_t)(kRaMostBytes / record) / a.num_kv_heads);
+    r.bytes = r.records * record * a.num_kv_heads;
+  }
+  const int64_t items = (a.n_queries * group / kRaTileRows + a.streams) * a.num_kv_heads * (r.records ? parts : 1);
+  r.groups = (uint32_t)std::min(slots, items);
   return r;
 }
 
@@ -884,10 +973,9 @@ static int launch_ragged(const RaParams& p, uint32_t grid, hipStream_t stream) {
   if (int rc = allow_dynamic_lds(kernel, kRaLds<D>, allowed, "ll_ragged_attention")) return rc;
   ragged_attention_kernel<T, D, KIND><<<grid, kRaThreads, kRaLds<D>, stream>>>(p);
   LL_CHECK_LAUNCH("ll_ragged_attention");
-  if (p.parts > 1) {
-    // No more workgroups than a few rounds: most of them find a tile that was not cut, and that is all that they do.
-    const uint32_t tiles = p.tiles * (uint32_t)p.kv_heads, each = kRaThreads * 4 / D, most = std::max(1u, kRaJoinGroups / tiles);
-    ragged_join_kernel<T, D, KIND><<<dim3(tiles, std::min((p.record_rows + each - 1) / each, most)), kRaThreads, 0, stream>>>(p);
+  if (p.records) {
+    const uint32_t each = kRaThreads * 4 / D;
+    ragged_join_kernel<T, D, KIND><<<dim3(kRaJoinGroups, kRaTileRows / each / 4), kRaThreads, 0, stream>>>(p);
     LL_CHECK_LAUNCH("ll_ragged_attention (join)");
   }
   return LL_OK;
@@ -962,15 +1050,12 @@ extern "C" int ll_ragged_attention(const ll_ragged_attention_args* a, void* stre
   p.group = divisor((uint32_t)(a->num_heads / a->num_kv_heads));
   p.window = (uint32_t)std::min<int64_t>(a->window, 0x7fffffff);  // keys are fewer
   p.sink = (uint32_t)std::min<int64_t>(a->sink_keys, 0x7fffffff);
-  p.tiles = plan.tiles;
-  p.parts = plan.parts;
-  p.part_steps = plan.part_steps ? plan.part_steps : 1;
-  p.record_rows = plan.record_rows;
-  p.work_groups = plan.tiles * plan.parts * (uint32_t)a->num_kv_heads;
-  // Workgroups that read the same keys on one XCD, if that leaves every XCD the same work: whole heads for each, or one stream.
-  p.by_head = a->num_kv_heads % 8 == 0 || a->streams == 1;
-  p.records = static_cast<float*>(a->workspace);
-  const uint32_t grid = p.work_groups + (a->clear_rest ? kRaClearGroups : 0);
+  p.groups = plan.groups;
+  p.part_steps = plan.part_steps;
+  p.narrow_part_steps = plan.narrow_part_steps;
+  p.records = plan.records;
+  p.record_mem = static_cast<float*>(a->workspace);
+  const uint32_t grid = p.groups + (a->clear_rest ? kRaClearGroups : 0);
   if (grid == 0) return LL_OK;
   const int kind = paged ? kRaPaged : a->key_mask ? kRaMaskedRows : kRaRows;
   const hipStream_t s = static_cast<hipStream_t>(stream);
