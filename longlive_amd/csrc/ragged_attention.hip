@@ -355,14 +355,6 @@ __global__ __launch_bounds__(kRaThreads, D == 64 ? 3 : 2) void ragged_attention_
   const bool idle = own >= tile_rows;  // a wave without rows only moves keys
 
   short8v qf[kSteps];
-  {
-    const uint16_t* src = p.q + (t.q0 + row.token) * p.q_stride_token + row.head * p.q_stride_head + 8 * lh;
-#pragma unroll
-    for (int ks = 0; ks < kSteps; ++ks) qf[ks] = *reinterpret_cast<const short8v*>(src + 16 * ks);
-  }
-  // Ahead of the loops and where the compiler sees it: it would otherwise count the loads of the queries as under way for good, and wait
-  // for the keys' loads in their place ahead of every product.  0x0F70 = vmcnt(0), other counters untouched.
-  auto wait_for_queries = [] { __builtin_amdgcn_s_waitcnt(0x0F70); };
   float16v o[kDTiles];
 #pragma unroll
   for (int dt = 0; dt < kDTiles; ++dt)
@@ -641,6 +633,17 @@ __global__ __launch_bounds__(kRaThreads, D == 64 ? 3 : 2) void ragged_attention_
     const uint32_t k_rows = lds0, v_rows = lds0 + 2 * kStepBytes;
     uint64_t exist = 0;
     if (s_begin < s_end) {
+      // The wave's queries, whole rows per load, by way of the buffers that the first step leaves alone: straight into the fragments a load
+      // reaches 32 bytes of each of 32 rows.
+      const uint32_t q_lds = (wave < 2 ? k_rows : v_rows) + ((s_begin & 1) ^ 1) * kStepBytes + (wave & 1) * 32 * kRowBytes;
+      if (!idle) {
+#pragma unroll
+        for (int i = 0; i < 2 * kGroupLoads; ++i) {
+          const int r = i * kRowsPerLoad + lane / kPieces, f = min(t.first + own + r, t.rows - 1);
+          const int token = (uint32_t)f / p.group, head = (int)(kv_head * p.group.d) + f - token * (int)p.group.d;
+          load16_to_lds(p.q + (t.q0 + token) * p.q_stride_token + head * p.q_stride_head + 8 * k_piece<D>(r, lane % kPieces), q_lds + i * 1024);
+        }
+      }
       if (kLooksUp) {
         look_up(key_base(s_begin) + lane, s_begin & 1);
         wait_loads<0>();
@@ -648,9 +651,11 @@ __global__ __launch_bounds__(kRaThreads, D == 64 ? 3 : 2) void ragged_attention_
       load_k(s_begin);
       exist = there;
       load_v(s_begin);
-    }
-    wait_for_queries();
-    if (s_begin < s_end) {
+      wait_loads<0>();
+      if (!idle) {
+#pragma unroll
+        for (int ks = 0; ks < kSteps; ++ks) qf[ks] = read_k(q_lds, 0, ks);
+      }
       __syncthreads();
       if (s_begin + 1 < s_end) load_k(s_begin + 1);
     }
@@ -744,6 +749,11 @@ __global__ __launch_bounds__(kRaThreads, D == 64 ? 3 : 2) void ragged_attention_
   };
   const int u_end = 2 * s_end;
   int u = 2 * s_begin + wave;
+  {
+    const uint16_t* src = p.q + (t.q0 + row.token) * p.q_stride_token + row.head * p.q_stride_head + 8 * lh;
+#pragma unroll
+    for (int ks = 0; ks < kSteps; ++ks) qf[ks] = *reinterpret_cast<const short8v*>(src + 16 * ks);
+  }
   if (u < u_end) {
     if (kLooksUp) {
       look_up(group_base(u) + l32, 0);
@@ -754,7 +764,9 @@ __global__ __launch_bounds__(kRaThreads, D == 64 ? 3 : 2) void ragged_attention_
     if (kLooksUp) look_up(group_base(min(u + 4, u_end - 1)) + l32, 1);
     load_group(true);
   }
-  wait_for_queries();
+  // Ahead of the loop and where the compiler sees it: it would otherwise count the loads of the queries as under way for good, and wait
+  // for the keys' loads in their place ahead of every product.  0x0F70 = vmcnt(0), other counters untouched.
+  __builtin_amdgcn_s_waitcnt(0x0F70);
   if (u < u_end) {
     for (int slot = 1; u < u_end; u += 4, slot ^= 1) {
       const uint64_t exist = there;
