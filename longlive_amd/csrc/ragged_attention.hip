@@ -561,7 +561,7 @@ __global__ __launch_bounds__(kRaThreads, D == 64 ? 3 : 2) void ragged_attention_
     float x[2][2], e[2][2], mx = -INFINITY;
     auto fetch_k = [&](auto tag) __attribute__((always_inline)) {
       constexpr int i = decltype(tag)::value;
-      fk[i % kRing] = read_k(next_k, i / kSteps, i % kSteps);
+      fk[i % kRing] = read_k(next_k, i % 2, i / 2);
     };
     each_index(fetch_k, std::make_integer_sequence<int, kAhead>{});
     __builtin_amdgcn_sched_barrier(0);
@@ -574,7 +574,7 @@ __global__ __launch_bounds__(kRaThreads, D == 64 ? 3 : 2) void ragged_attention_
       }
       __builtin_amdgcn_sched_barrier(0);
       if constexpr (slot < kS) {
-        constexpr int kt = slot / kSteps, ks = slot % kSteps;
+        constexpr int kt = slot % 2, ks = slot / 2;
         const float16v zero = {0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f};
         nx[kt] = T::mfma(fk[slot % kRing], qf[ks], ks == 0 ? zero : nx[kt]);
       } else {
