@@ -33,6 +33,7 @@ constexpr int kRaThreads = 256;
 constexpr int kRaTileRows = 128;  // rows of a workgroup, 32 a wave
 constexpr int kRaKeys = 64;       // keys of a step
 constexpr int kRaClearGroups = 16;
+constexpr float kLog2E = 1.4426950408889634f;
 constexpr uint32_t kRaJoinGroups = 512;
 
 // Where keys lie: in the pages of a table, in rows one behind the other, in such rows with a mask.
@@ -884,7 +885,7 @@ static int check_ragged(const ll_ragged_attention_args* a) {
   LL_REQUIRE(a->n_queries <= 0x7fffffffll / a->num_heads, "ll_ragged_attention: %lld queries of %d heads are more than 2^31 rows",
              (long long)a->n_queries, a->num_heads);
   LL_REQUIRE(a->streams <= 0xfffffff / a->num_kv_heads, "ll_ragged_attention: %lld streams", (long long)a->streams);
-  LL_REQUIRE(a->softmax_scale > 0.0f && std::isfinite(a->softmax_scale), "ll_ragged_attention: softmax_scale has to be positive");
+  LL_REQUIRE(a->softmax_scale > 0.0f && std::isfinite(a->softmax_scale * kLog2E), "ll_ragged_attention: softmax_scale has to be positive");
   LL_REQUIRE(a->max_q_len >= 0 && a->max_kv_len >= 0, "ll_ragged_attention: negative longest lengths");
   if (a->page_table || a->page_size) {
     LL_REQUIRE(a->page_size > 0 && a->table_width >= 0 && a->n_pages >= 0 && a->n_pages <= 0x7fffffffll,
@@ -1055,7 +1056,7 @@ extern "C" int ll_ragged_attention(const ll_ragged_attention_args* a, void* stre
   p.k_lens = a->k_lens;
   p.key_mask = a->key_mask;
   p.n_keys = a->n_keys;
-  p.scale_log2 = a->softmax_scale * 1.4426950408889634f;
+  p.scale_log2 = a->softmax_scale * kLog2E;
   p.causal = a->causal;
   p.heads = a->num_heads;
   p.kv_heads = a->num_kv_heads;

@@ -181,6 +181,41 @@ def test_a_few_tokens_each_over_long_caches(gpu, new):
     check_paged(gpu, batch(41, new, [5000, 777, 2500], 16, 4, 128, 32, BF16), max_q_len=max(new), max_kv_len=5000)
 
 
+@pytest.mark.parametrize("D,dtype", [(64, F16), (128, BF16)])
+@pytest.mark.parametrize("causal,window,sink", [(True, None, 0), (False, None, 0), (True, 3000, 130), (False, 2500, 70)])
+@pytest.mark.parametrize("new,keys,Hq,Hk,page", [([150, 40, 1], [5000, 3000, 4500], 2, 1, 16), ([200], [6000], 3, 1, 24), ([1, 2], [9000, 6400], 4, 2, 880),
+                                                 ([300, 2, 33, 129], [1700, 3333, 33, 2500], 5, 1, 8)])
+def test_tiles_whose_keys_are_cut(gpu, new, keys, Hq, Hk, page, causal, window, sink, D, dtype):
+    b = batch(45, new, keys, Hq, Hk, D, page, dtype, fill=float("nan"))
+    check_paged(gpu, b, causal=causal, window=window, sink=sink, max_q_len=max(new), max_kv_len=max(keys))
+
+
+@pytest.mark.parametrize("most_keys", [200, 2600])
+def test_more_streams_than_a_wave_has_lanes(gpu, most_keys):
+    g = torch.Generator().manual_seed(3)
+    new = (torch.randint(0, 5, (200,), generator=g) ** 2).tolist()
+    new[7], new[64], new[130], new[199] = 150, 0, 77, 3
+    keys = [max(n, int(k)) for n, k in zip(new, torch.randint(0, most_keys // 8, (200,), generator=g))]
+    keys[7], keys[63], keys[130], keys[199] = most_keys, most_keys - 1, 140, most_keys // 2
+    check_paged(gpu, batch(46, new, keys, 4, 2, 64, 16, BF16, fill=float("nan")), max_q_len=max(new), max_kv_len=max(keys))
+
+
+def test_streams_that_find_no_records_left_stay_whole(gpu):
+    # 64 kv heads leave a stream fewer records than its 16 tiles would take; the smaller one before it is cut
+    new, keys, H, D = [20, 2048], [4000, 5300], 64, 64
+    q, cache, table, lens, q_starts = batch(47, new, keys, H, H, D, 16, F16)
+    dev = {n: t.to(gpu) for n, t in cache.items()}
+    got = paged_attention(q.to(gpu), dev, table.to(gpu), lens.to(gpu), q_starts.to(gpu), max_q_len=2048, max_kv_len=5300)
+    keys_of, seen_of = ref.paged_keys({n: t[:, :, [0, 63]] for n, t in cache.items()}, table, lens)
+    rows = torch.cat([torch.arange(20), torch.tensor([20, 21, 900, 2066, 2067])])
+    for h, head in enumerate((0, 63)):
+        for b, first in ((0, 0), (1, 20)):
+            k, v = (t[:, h] for t in keys_of(b))
+            at = rows[(rows >= first) & (rows < first + new[b])]
+            want, error = ref.attend(q[at, head], k, v, seen_of()(b, new[b], len(k))[at - first], D ** -0.5)
+            close(got[at.to(gpu), head], want, error, f"stream {b} head {head}")
+
+
 def test_rows_that_see_nothing_are_zeros(gpu):
     # more new tokens than keys: the first of them sit before the stream's beginning; no keys at all; a table of holes
     b = batch(51, [5, 3, 4], [2, 0, 20], 4, 2, 64, 8, BF16, fill=float("nan"))
@@ -373,6 +408,20 @@ def check_cross(gpu, q, k, v, q_starts, k_starts, k_lens=None, key_mask=None, **
     ([2, 1], [3000, 2], 8, 8)])
 def test_cross_attention(gpu, new, states, Hq, Hk, D, dtype):
     check_cross(gpu, *cross(201, new, states, Hq, Hk, D, dtype), max_q_len=max(new), max_k_len=max(states))
+
+
+def test_no_states_at_all(gpu):
+    q, k, _, q_starts, _ = cross(205, [3, 4], [1, 0], 4, 2, 64, BF16)
+    none = torch.zeros(3, dtype=torch.int32, device=gpu)
+    assert (ragged_cross_attention(q.to(gpu), k[:0].to(gpu), k[:0].to(gpu), q_starts.to(gpu), none) == 0).all()
+
+
+@pytest.mark.parametrize("masked", [False, True])
+@pytest.mark.parametrize("new,states", [([300, 130, 2, 70], [2000, 40, 1500, 700]), ([1, 3], [3000, 2500])])
+def test_many_states(gpu, new, states, masked):
+    q, k, v, q_starts, k_starts = cross(206, new, states, 6, 2, 128, BF16)
+    mask = torch.rand(k.shape[0], generator=torch.Generator().manual_seed(1)) < 0.7 if masked else None
+    check_cross(gpu, q, k, v, q_starts, k_starts, key_mask=mask, max_q_len=max(new), max_k_len=max(states))
 
 
 @pytest.mark.parametrize("new", [[1, 1, 1, 1], [100, 3, 40, 7]])

@@ -154,3 +154,23 @@ def test_c_abi_refuses_bad_arguments_before_touching_the_gpu():
     assert call(tokens=0) == 0
     none = row(num_heads=0)
     assert call(q=none, k=none) == 0
+
+
+def test_memory_that_launches_ask_for():
+    lib = _native.load()
+
+    def need(cus=256, **kw):
+        a = _native.RaggedAttentionStruct(**{**dict(dtype=0, head_dim=128, num_heads=32, num_kv_heads=8, n_queries=32, streams=32, softmax_scale=0.1, page_size=16,
+                                                    table_width=1024, n_pages=32768, max_q_len=1, max_kv_len=16384), **kw})
+        n = ctypes.c_size_t()
+        assert lib.ll_ragged_attention_workspace(ctypes.byref(a), cus, ctypes.byref(n)) == 0
+        return n.value
+
+    assert need(n_queries=0) == need(streams=0) == 0
+    assert need(max_kv_len=300) == 0                       # one part
+    assert 0 < need() <= 256 << 20                         # single tokens over long caches: parts
+    assert need(n_queries=65536, streams=16, max_q_len=8192) <= 256 << 20
+    assert need(streams=1, n_queries=2640, max_q_len=2640, num_heads=24, num_kv_heads=24, max_kv_len=13200, page_size=880, table_width=15) == 0
+    assert need(streams=1, n_queries=1, num_heads=8) > 0   # one stream's token: its keys over the whole device
+    for cus in (1, 64, 304):
+        assert need(cus=cus) <= 256 << 20
