@@ -12,6 +12,7 @@ typedef _Float16 f16x8_hw __attribute__((ext_vector_type(8)));
 typedef _Float16 f16x2_hw __attribute__((ext_vector_type(2)));
 
 struct Bf16 {
+  static constexpr uint32_t kInfinity = 0x7F80;  // magnitudes from here on are not finite
   static __device__ __forceinline__ void unpack2(uint32_t w, float& a, float& b) {
     a = __uint_as_float(w << 16);
     b = __uint_as_float(w & 0xFFFF0000u);
@@ -29,6 +30,7 @@ struct Bf16 {
 };
 
 struct F16 {
+  static constexpr uint32_t kInfinity = 0x7C00;
   static __device__ __forceinline__ void unpack2(uint32_t w, float& a, float& b) {
     const f16x2_hw h = __builtin_bit_cast(f16x2_hw, w);
     a = (float)h[0];

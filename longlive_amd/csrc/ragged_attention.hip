@@ -362,6 +362,7 @@ __global__ __launch_bounds__(kRaThreads, D == 64 ? 3 : 2) void ragged_attention_
 #pragma unroll
     for (int r = 0; r < 16; ++r) o[dt][r] = 0.0f;
   float m = -INFINITY, l = 0.0f;
+  bool finite = true;  // V where rows of the wave see different keys
 
   // ---- where the keys of 64 lanes lie
   uint8_t* const looked_up = smem + 4 * kStepBytes + wave * 512;
@@ -460,6 +461,8 @@ __global__ __launch_bounds__(kRaThreads, D == 64 ? 3 : 2) void ragged_attention_
   // S^T: register r of sc[kt] is key 32 kt + 8 (r / 4) + 4 lh + r % 4
   typedef const __attribute__((address_space(3))) short8v* lds_short8;
   typedef __attribute__((address_space(3))) short4v* lds_short4;
+  typedef uint32_t uint2v __attribute__((ext_vector_type(2)));
+  typedef const __attribute__((address_space(3))) uint2v* lds_uint2;
   const uint32_t lds0 = lds_at(smem);
   // where the lane's fragments begin in LDS rows; a fragment's number turns bits of the piece's position
   const uint32_t k_lane = (uint32_t)(l32 * kRowBytes + k_piece<D>(l32, lh) * 16);
@@ -478,13 +481,19 @@ __global__ __launch_bounds__(kRaThreads, D == 64 ? 3 : 2) void ragged_attention_
       }
     }
   };
+  // Whether there are keys from `base` to `end` that a row of the wave does not see.
+  auto uneven = [&](int base, int end) __attribute__((always_inline)) {
+    return KIND == kRaPaged && (min(end, t.len) > last0 || (base < from1 && end > (int)p.sink));
+  };
+  auto seen_from = [&](int base) __attribute__((always_inline)) {  // of 64 keys from `base` on, those that the lane's row may see
+    return low_bits(last - base) & (~low_bits(from - base) | low_bits((int)p.sink - base));
+  };
   auto mask = [&](auto& sc, int base, uint64_t exist) __attribute__((always_inline)) {  // whether it hides any
     constexpr int NT = std::extent<std::remove_reference_t<decltype(sc)>>::value;
     constexpr uint64_t kAll = NT == 2 ? ~0ull : 0xFFFFFFFFull;
     const int end = base + 32 * NT;
-    if ((exist & kAll) == kAll && end <= last0 && (base >= from1 || end <= (int)p.sink)) return false;
-    // one bit a key: it exists, it lies below `last`, and from `from` on or below the sink
-    const uint64_t seen = exist & low_bits(last - base) & (~low_bits(from - base) | low_bits((int)p.sink - base));
+    if ((exist & kAll) == kAll && !uneven(base, end)) return false;
+    const uint64_t seen = exist & seen_from(base);  // one bit a key
     const uint32_t bits[2] = {(uint32_t)seen >> (4 * lh), (uint32_t)(seen >> 32) >> (4 * lh)};
 #pragma unroll
     for (int kt = 0; kt < NT; ++kt)
@@ -550,6 +559,72 @@ __global__ __launch_bounds__(kRaThreads, D == 64 ? 3 : 2) void ragged_attention_
         o[dt] = T::mfma(__builtin_shufflevector(part[0], part[1], 0, 1, 2, 3, 4, 5, 6, 7), pb, o[dt]);
       }
     }
+  };
+  // A key that some rows of the wave see and others do not: its weight of zero keeps it out of the others' sums, unless its V is not finite.
+  // So where rows differ, V is looked through, and if it is not finite the item is done once more, rows of V that are not finite then being
+  // added to the rows that see them alone.  (In a loop of its own: in the others it would take registers that they do not have.)
+  auto all_finite = [&](uint32_t v_rows, int n_rows) __attribute__((always_inline)) {
+    typedef unsigned short ushort2v __attribute__((ext_vector_type(2)));
+    ushort2v top = {0, 0};
+    for (int i = 0; i < n_rows * kRowBytes / 1024; ++i) {
+      const u32x4 w = *(lds_uint4)(uintptr_t)(v_rows + i * 1024 + lane * 16);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) top = __builtin_elementwise_max(top, __builtin_bit_cast(ushort2v, w[j] & 0x7FFF7FFFu));
+    }
+    return __builtin_amdgcn_ballot_w64(top[0] >= T::kInfinity || top[1] >= T::kInfinity) == 0;
+  };
+  auto weigh_apart = [&](auto& sc, uint32_t v_rows, int base) __attribute__((always_inline)) {
+    constexpr int NT = std::extent<std::remove_reference_t<decltype(sc)>>::value;
+#pragma unroll
+    for (int step = 0; step < 2 * NT; ++step) {
+      __builtin_amdgcn_sched_barrier(0);
+      uint32_t w[4];
+#pragma unroll
+      for (int u = 0; u < 4; ++u) {
+        const float p0 = __builtin_amdgcn_exp2f(fmaf(sc[step >> 1][8 * (step & 1) + 2 * u], p.scale_log2, neg));
+        const float p1 = __builtin_amdgcn_exp2f(fmaf(sc[step >> 1][8 * (step & 1) + 2 * u + 1], p.scale_log2, neg));
+        w[u] = T::pack2(p0, p1);
+        l = T::add2(w[u], l);
+      }
+      const short8v pb = __builtin_bit_cast(short8v, make_uint4(w[0], w[1], w[2], w[3]));
+#pragma unroll
+      for (int dt = 0; dt < kDTiles; ++dt) {
+        short4v part[2];
+        read_v(v_rows, step, dt, part);
+        short8v a = __builtin_shufflevector(part[0], part[1], 0, 1, 2, 3, 4, 5, 6, 7);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) a[j] = (uint32_t)(a[j] & 0x7FFF) >= T::kInfinity ? (short)0 : a[j];
+        o[dt] = T::mfma(a, pb, o[dt]);
+      }
+    }
+    int ln = lane;
+    asm volatile("" : "+v"(ln));  // formed here, not kept over the loops
+    const uint64_t seen = seen_from(base);
+#pragma unroll 1
+    for (int j = 0; j < 32 * NT; ++j) {
+      const bool sees = seen >> j & 1;
+      const uint32_t row = v_rows + j * kRowBytes + (ln >> 5) * 8;
+#pragma unroll
+      for (int dt = 0; dt < kDTiles; ++dt)
+#pragma unroll
+        for (int g = 0; g < 4; ++g) {  // columns 32 dt + 8 g + 4 lh + 0 .. 3
+          const uint2v v = *(lds_uint2)(uintptr_t)(row + v_piece<D>(j, 4 * dt + g) * 16);
+          float x[4];
+          T::unpack2(v[0], x[0], x[1]);
+          T::unpack2(v[1], x[2], x[3]);
+#pragma unroll
+          for (int i = 0; i < 4; ++i) o[dt][4 * g + i] += sees && !(fabsf(x[i]) < INFINITY) ? x[i] : 0.0f;
+        }
+      __builtin_amdgcn_sched_barrier(0);
+    }
+  };
+  auto once_more = [&]() __attribute__((always_inline)) {
+    m = -INFINITY;
+    l = neg = 0.0f;
+#pragma unroll
+    for (int dt = 0; dt < kDTiles; ++dt)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) o[dt][r] = 0.0f;
   };
   // One step of a tile of more than 32 rows and the scores of the next: every slot one MFMA (S^T of the next step, then O^T of this one) with
   // what runs beside it, held in place by scheduling barriers: the LDS reads of MFMAs some slots later, and the probabilities, a pair
@@ -668,11 +743,37 @@ __global__ __launch_bounds__(kRaThreads, D == 64 ? 3 : 2) void ragged_attention_
       load_v(s + 1);  // from the places of the last load_k
       if (s + 2 < s_end) load_k(s + 2);
     };
+    // The item once more, step by step (see all_finite).
+    auto apart = [&]() __attribute__((always_inline)) {
+      once_more();
+#pragma unroll 1
+      for (int s = s_begin; s < s_end; ++s) {
+        __syncthreads();
+        if (kLooksUp) {
+          look_up(key_base(s) + lane, 0);
+          wait_loads<0>();
+        }
+        take_places(key_base(s), lane, 0);
+        load_rows(false, wave * 16, k_lds, false);
+        load_rows(true, wave * 16, v_lds, false);
+        wait_loads<0>();
+        __syncthreads();
+        if (idle) continue;
+        float16v sc[2];
+        scores(sc, k_rows);
+        mask(sc, key_base(s), there);
+        follow(largest(sc));
+        weigh_apart(sc, v_rows, key_base(s));
+      }
+      __syncthreads();
+    };
+    const bool may_differ = KIND == kRaPaged && (p.causal || p.window);
     if (idle) {
       if (s_begin < s_end) {
         for (int s = s_begin; s + 1 < s_end; ++s) move_keys(s);
         wait_loads<0>();
         __syncthreads();
+        if (may_differ && __syncthreads_or(0)) apart();
       }
       continue;
     }
@@ -684,7 +785,9 @@ __global__ __launch_bounds__(kRaThreads, D == 64 ? 3 : 2) void ragged_attention_
       auto iteration = [&](int s, auto from_tag) __attribute__((always_inline)) {
         constexpr int from_buffer = decltype(from_tag)::value;
         move_keys(s);
-        float mx = step_and_next(sc[from_buffer], sc[from_buffer ^ 1], k_rows + ((s + 1) & 1) * kStepBytes, v_rows + (s & 1) * kStepBytes);
+        const uint32_t next_k = k_rows + ((s + 1) & 1) * kStepBytes, this_v = v_rows + (s & 1) * kStepBytes;
+        if (uneven(key_base(s), key_base(s) + kRaKeys)) finite = finite && all_finite(this_v, kRaKeys);
+        float mx = step_and_next(sc[from_buffer], sc[from_buffer ^ 1], next_k, this_v);
         if (mask(sc[from_buffer ^ 1], key_base(s + 1), exist)) mx = largest(sc[from_buffer ^ 1]);
         follow(mx);
       };
@@ -701,7 +804,10 @@ __global__ __launch_bounds__(kRaThreads, D == 64 ? 3 : 2) void ragged_attention_
       }
       wait_loads<0>();
       __syncthreads();
-      weigh(sc[0], v_rows + (s & 1) * kStepBytes);
+      const uint32_t this_v = v_rows + (s & 1) * kStepBytes;
+      if (uneven(key_base(s), key_base(s) + kRaKeys)) finite = finite && all_finite(this_v, kRaKeys);
+      weigh(sc[0], this_v);
+      if (may_differ && __syncthreads_or(!finite)) apart();
     }
     l = exchange_sum(l);
     if (t.n_parts > 1) {
@@ -785,11 +891,33 @@ __global__ __launch_bounds__(kRaThreads, D == 64 ? 3 : 2) void ragged_attention_
       follow(largest(sc));
       if (more) wait_loads<kLoads + (kLooksUp ? 1 : 0)>();
       else wait_loads<0>();
-      weigh(sc, rows_lds + 32 * kRowBytes);
+      const uint32_t this_v = rows_lds + 32 * kRowBytes;
+      if (uneven(group_base(u), group_base(u) + 32)) finite = finite && all_finite(this_v, 32);
+      weigh(sc, this_v);
       if (more) {
         wait_lds_reads();
         load_group(true);
       }
+    }
+  }
+  if (KIND == kRaPaged && !finite) {  // once more, group by group (see all_finite)
+    once_more();
+#pragma unroll 1
+    for (u = 2 * s_begin + wave; u < u_end; u += 4) {
+      if (kLooksUp) {
+        look_up(group_base(u) + l32, 0);
+        wait_loads<0>();
+      }
+      take_places(group_base(u), l32, 0);
+      wait_lds_reads();
+      load_group(false);
+      load_group(true);
+      wait_loads<0>();
+      float16v sc[1];
+      scores(sc, rows_lds);
+      mask(sc, group_base(u), there);
+      follow(largest(sc));
+      weigh_apart(sc, rows_lds + 32 * kRowBytes, group_base(u));
     }
   }
   // The four waves' results, joined: each wave takes a quarter of the columns.

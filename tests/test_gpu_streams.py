@@ -383,6 +383,32 @@ def test_nan_and_infinities_reach_the_rows_that_see_them(gpu):
     assert torch.isfinite(got[:50]).all() and got[50:70].isnan().all() and torch.isfinite(got[70:]).all()
 
 
+@pytest.mark.parametrize("D,dtype", [(64, F16), (128, BF16)])
+@pytest.mark.parametrize("window,sink", [(None, 0), (40, 3)])
+@pytest.mark.parametrize("bad", ["k_pages", "v_pages"])
+@pytest.mark.parametrize("new,keys", [([150, 1, 9], [400, 300, 70]), ([1, 20], [900, 2000])])
+def test_what_is_not_finite_stays_with_the_rows_that_see_it(gpu, new, keys, bad, window, sink, D, dtype):
+    """NaN and infinities at keys that are later than a row or lie behind its window: they have no part in that row."""
+    b = batch(136, new, keys, 4, 2, D, 16, dtype)
+    q, cache, table, lens, q_starts = b
+    clean = {n: t.clone() for n, t in cache.items()}
+    at = [{keys[i] - n + j for j in (n // 3, n - 1)} | ({keys[i] - n - 60, keys[i] - 41, 7} if window else set()) for i, n in enumerate(new)]
+    values = [float("nan"), float("inf"), -float("inf")]
+    for i, places in enumerate(at):
+        for j, place in enumerate(sorted(p for p in places if p >= 0)):
+            cache[bad][table[i, place // 16], place % 16, :, 3 * j] = values[j % 3]
+    got = paged_attention(q.to(gpu), {n: t.to(gpu) for n, t in cache.items()}, table.to(gpu), lens.to(gpu), q_starts.to(gpu), window=window, sink_tokens=sink).cpu()
+    keys_of, seen_of = ref.paged_keys(clean, table, lens)
+    want, error, _ = ref.ragged_attention(q, q_starts, D ** -0.5, keys_of, seen_of(True, window, sink))
+    seen_at = [seen_of(True, window, sink)(i, n, keys[i])[:, sorted(p for p in at[i] if p >= 0)].any(1) for i, n in enumerate(new)]
+    touched = torch.cat(seen_at)
+    close(got[~touched], want[~touched], error[~touched])
+    assert touched.any()
+    if bad == "v_pages":   # the rows that see it have it, in the columns concerned (a score of -inf would weigh nothing, so not with K)
+        assert not torch.isfinite(got[touched]).flatten(1).all(1).any()
+        close(got[touched][:, :, 20:], want[touched][:, :, 20:], error[touched][:, :, 20:])
+
+
 # ------------------------------------------------------------------------------------------------ cross attention
 def cross(seed, new, states, Hq, Hk, D, dtype):
     q = randn(seed, sum(new), Hq, D, dtype=dtype, scale=1.5)
