@@ -1046,6 +1046,16 @@ def _page_rows(pages: torch.Tensor) -> int | None:
     return _stride(pages, 1) or _stride(pages, 0)
 
 
+def _apart(t: torch.Tensor) -> bool:
+    """Whether no two elements of a tensor to be written lie in one place (by strides that grow past one another's extent)."""
+    end = 1
+    for step, n in sorted((s, n) for n, s in zip(t.shape, t.stride()) if n > 1):
+        if step < end:
+            return False
+        end = step * n
+    return True
+
+
 def _check_rows(what: str, name: str, t: torch.Tensor, dtype=None) -> None:
     if t.ndim != 3 or t.dtype not in (torch.bfloat16, torch.float16) or (dtype is not None and t.dtype != dtype):
         raise ValueError(f"{what}: {name} must be [rows, heads, head_dim] in bfloat16 or float16, all tensors in one type; got "
@@ -1058,8 +1068,8 @@ def _check_index(what: str, name: str, t: torch.Tensor, dtype, shape) -> None:
 
 
 def _check_out(what: str, out: torch.Tensor, like: torch.Tensor) -> None:
-    if out.shape != like.shape or out.dtype != like.dtype or not _rows16(out):
-        raise ValueError(f"{what}: out must be a {like.dtype} tensor of shape {tuple(like.shape)} with whole, 16-byte aligned rows")
+    if out.shape != like.shape or out.dtype != like.dtype or not _rows16(out) or not _apart(out):
+        raise ValueError(f"{what}: out must be a {like.dtype} tensor of shape {tuple(like.shape)} with whole, 16-byte aligned rows, each in a place of its own")
 
 
 def check_pages(what: str, cache: dict) -> tuple[torch.Tensor, torch.Tensor]:
@@ -1128,8 +1138,8 @@ def head_norm_rope(q, k, v, q_weight, k_weight, eps, cos, sin, positions, interl
         k_pages, v_pages = pages
         if k_pages.shape[2:] != k.shape[1:] or k_pages.dtype != q.dtype:
             raise ValueError(f"{what}: pages of {k_pages.dtype} {tuple(k_pages.shape[2:])} do not take rows of {q.dtype} {tuple(k.shape[1:])}")
-        if any(t.numel() and _page_rows(t) is None for t in pages):
-            raise ValueError(f"{what}: pages must lie one behind the other")
+        if any(t.numel() and (_page_rows(t) is None or not _apart(t)) for t in pages):
+            raise ValueError(f"{what}: pages must lie one behind the other, each row in a place of its own")
         _check_index(what, "slots", slots, torch.int64, (T,))
         v = v if _rows16(v) else v.contiguous().clone()
         n_slots = k_pages.shape[0] * k_pages.shape[1]

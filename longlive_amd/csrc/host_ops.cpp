@@ -1021,6 +1021,16 @@ const Tensor* as_rows(PyObject* o, int dev, int64_t dims, const Tensor* like) {
     if (t->size(i) > 1 && t->stride(i) % 8 != 0) return nullptr;
   return t;
 }
+// Whether no two rows of a tensor to be written (as_rows) lie in one place; false also for dimensions in another order than their strides'.
+bool apart(const Tensor& t) {
+  int64_t end = 1;
+  for (int64_t i = t.dim(); i-- > 0;) {
+    if (t.size(i) == 1) continue;
+    if (t.stride(i) < end) return false;
+    end = t.stride(i) * t.size(i);
+  }
+  return true;
+}
 // The stride of a dimension, 0 where it is never taken.
 inline int64_t stride_of(const Tensor* t, int64_t d) { return t->size(d) > 1 ? t->stride(d) : 0; }
 // A contiguous tensor of a type and so many elements.
@@ -1095,7 +1105,7 @@ PyObject* py_ragged_attention(PyObject*, PyObject* const* args, Py_ssize_t n) {
     a.clear_rest = 1;
   } else {
     const Tensor* given = as_rows(args[5], dev, 3, q);
-    if (!given || given->sizes() != q->sizes()) Py_RETURN_NONE;
+    if (!given || given->sizes() != q->sizes() || !apart(*given)) Py_RETURN_NONE;
     out = *given;
   }
   a.dtype = half_code(*q);
@@ -1169,7 +1179,7 @@ PyObject* py_head_norm_rope(PyObject*, PyObject* const* args, Py_ssize_t n) {
     q_out = empty(q->sizes(), q->scalar_type(), dev);
   } else {
     const Tensor* given = as_rows(args[13], dev, 3, q);
-    if (!given || given->sizes() != q->sizes()) Py_RETURN_NONE;
+    if (!given || given->sizes() != q->sizes() || !apart(*given)) Py_RETURN_NONE;
     q_out = *given;
   }
   const auto rows = [](const Tensor* x, const Tensor* weight, void* out, int64_t out_token, int64_t out_head) {
@@ -1185,10 +1195,10 @@ PyObject* py_head_norm_rope(PyObject*, PyObject* const* args, Py_ssize_t n) {
     const Tensor* at = as_list(args[12], dev, at::kLong, T);
     if (!kp || !vp || !v || !at || v->sizes() != k->sizes() || kp->sizes() != vp->sizes() || kp->size(2) != k->size(1) || kp->size(3) != D) Py_RETURN_NONE;
     for (const Tensor* t : {kp, vp})  // the cache's rows all as far apart
-      if (t->size(0) > 1 && t->size(1) > 1 && t->stride(0) != t->size(1) * t->stride(1)) Py_RETURN_NONE;
-    const auto apart = [](const Tensor* t) { return t->size(1) > 1 ? t->stride(1) : stride_of(t, 0); };
-    k_rows = rows(k, weights[1], kp->data_ptr(), apart(kp), stride_of(kp, 2));
-    v_rows = rows(v, nullptr, vp->data_ptr(), apart(vp), stride_of(vp, 2));
+      if (!apart(*t) || (t->size(0) > 1 && t->size(1) > 1 && t->stride(0) != t->size(1) * t->stride(1))) Py_RETURN_NONE;
+    const auto step = [](const Tensor* t) { return t->size(1) > 1 ? t->stride(1) : stride_of(t, 0); };
+    k_rows = rows(k, weights[1], kp->data_ptr(), step(kp), stride_of(kp, 2));
+    v_rows = rows(v, nullptr, vp->data_ptr(), step(vp), stride_of(vp, 2));
     slots = at->data_ptr<int64_t>();
     n_slots = kp->size(0) * kp->size(1);
   } else {

@@ -300,6 +300,26 @@ def test_queries_outputs_and_pages_with_strides(gpu):
     assert torch.equal(paged_attention(odd, paged, tables, lens.to(gpu), q_starts.to(gpu)), want)
 
 
+@pytest.mark.parametrize("new,keys", [([1, 1], [9000, 40]), ([150, 1, 9], [400, 3000, 70]), ([260], [9000])])
+def test_results_in_place_of_the_queries(gpu, new, keys):
+    q, cache, table, lens, q_starts = (t if isinstance(t, dict) else t.to(gpu) for t in batch(102, new, keys, 8, 2, 128, 16, BF16))
+    cache = {n: t.to(gpu) for n, t in cache.items()}
+    want = paged_attention(q, cache, table, lens, q_starts)
+    assert paged_attention(q, cache, table, lens, q_starts, out=q) is q
+    inside = slice(int(q_starts[0]), int(q_starts[-1]))
+    assert torch.equal(q[inside], want[inside])
+
+
+def test_inputs_that_repeat_their_rows(gpu):
+    q, k, v = (randn(s, *shape).to(gpu) for s, shape in ((5, (1, 2, 64)), (6, (1, 2, 64)), (7, (300, 1, 64))))
+    q_starts, k_starts = starts([3, 90]).to(gpu), starts([200, 100]).to(gpu)
+    a, b, c = q.expand(93, 2, 64), k.expand(300, 2, 64), v.expand(300, 2, 64)
+    want = ragged_cross_attention(a.contiguous(), b.contiguous(), c.contiguous(), q_starts, k_starts)
+    assert torch.equal(ragged_cross_attention(a, b, c, q_starts, k_starts), want)
+    for x, y in zip(head_norm_rope(a, c[:93], None, None, 1e-6, None, None), head_norm_rope(a.contiguous(), c[:93].contiguous(), None, None, 1e-6, None, None)):
+        assert torch.equal(x, y)
+
+
 def test_dimensions_of_one_with_any_stride(gpu):
     """Torch leaves anything in the stride of a dimension of size one: one row, one head, one page, pages of one row."""
     def odd(t, *dims):

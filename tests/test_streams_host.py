@@ -118,6 +118,23 @@ def test_refusals_of_cross_attention(no_gpu_needed):
             ragged_cross_attention(**{**ok, **bad})
 
 
+def test_outputs_whose_elements_share_a_place_are_refused(no_gpu_needed):
+    x, i32 = torch.zeros(3, 4, 64, dtype=BF16), lambda *s: torch.zeros(s, dtype=torch.int32)
+    cache = initialize_paged_kv_cache(1, 4, 16, 4, 64, "cpu")[0]
+    slots = torch.zeros(3, dtype=torch.int64)
+    row = torch.zeros(64, dtype=BF16)
+    for out in (row.expand(3, 4, 64), torch.zeros(3, 1, 64, dtype=BF16).expand(3, 4, 64), torch.zeros(500, dtype=BF16).as_strided((3, 4, 64), (64, 64, 1))):
+        with pytest.raises(ValueError, match="place of its own"):
+            paged_attention(x, cache, i32(2, 5), i32(2), i32(3), out=out)
+        with pytest.raises(ValueError, match="place of its own"):
+            ragged_cross_attention(x, x, x, i32(3), i32(3), out=out)
+        with pytest.raises(ValueError, match="place of its own"):
+            head_norm_rope_paged(x, x, x, cache, slots, None, None, 1e-6, None, None, out=out)
+    for pages in (row.expand(4, 16, 4, 64), torch.zeros(64, 1, 64, dtype=BF16).expand(64, 4, 64).unflatten(0, (4, 16))):
+        with pytest.raises(ValueError, match="place of its own"):
+            head_norm_rope_paged(x, x, x, {**cache, "v_pages": pages}, slots, None, None, 1e-6, None, None)
+
+
 def test_c_abi_refuses_bad_arguments_before_touching_the_gpu():
     lib, need = _native.load(), ctypes.c_size_t()
     ok = dict(dtype=0, head_dim=64, num_heads=4, num_kv_heads=2, n_queries=3, streams=2, softmax_scale=0.125, page_size=16, table_width=5, n_pages=4)
