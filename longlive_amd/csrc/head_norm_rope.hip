@@ -7,7 +7,11 @@
 // in the rotation: 4 l and 4 l + R / 2 for pairs of halves, 8 l and 8 l + 4 for neighbouring pairs (and for columns that are not
 // rotated).  Either way pair j of lane l is j = 4 l .. 4 l + 3, so that the angles are one load of 16 bytes each and nothing
 // passes between lanes but the sum of squares.  A wave takes heads of one token and one of q, k and v: position, slot, pointers and
-// strides are scalars, loaded once for up to kHeadsEach heads per lane, all of whose loads are under way before the first is used.
+// strides are scalars, loaded once for up to two heads per lane, all of whose loads are under way before the first is used.  (With a wave
+// across q, k and v, the pointers came per lane out of the argument segment, which lies in host memory: 2640 x (24 + 24) heads of 128 182 us.)
+//
+// Bound by memory: 2640 x (24 + 24) heads of 128 columns, 66 MB, 13.0 us, 5.1 TB/s (half of it out of the last-level cache when repeated);
+// 16381 x (40 + 8 + 8) of 64, 237 MB, 53 us, 4.4 TB/s; 24 x (16 + 4 + 4), a decoding step, 3.3 us of the GPU, 5.6 us a call.
 #include "ll_types16.h"
 
 namespace ll {
@@ -57,6 +61,8 @@ __device__ __forceinline__ void unpack4(uint2 w, float* f) {
 }
 
 constexpr int kHeadNormThreads = 256;
+// Two heads a lane once the device has waves enough: us with one / two, 1000 tokens x (32 + 8 + 8) heads 8.6 / 9.0, 2640 x (24 + 24) 14.9 / 14.1,
+// 16000 x (32 + 8 + 8) 92.9 / 72.4, 16381 x (40 + 8 + 8) of 64 columns 57.0 / 46.2 (four: 74.2 and 44.3).
 constexpr int64_t kManyWaves = 8192;
 
 // LANES hold a head, a wave 64 / LANES heads side by side, HEADS times.
@@ -138,7 +144,7 @@ __global__ __launch_bounds__(kHeadNormThreads) void head_norm_rope_kernel(HeadNo
 #pragma unroll
       for (int j = 0; j < 8; ++j) y[j] = y[j] * scale * f[j];
     }
-    if (rotate && 8 * l < p.R) {  // nothing is turned by angles of zero, but a product with an infinity would be NaN
+    if (rotate && 8 * l < p.R) {
       const bool apart = halves;
 #pragma unroll
       for (int j = 0; j < 4; ++j) {

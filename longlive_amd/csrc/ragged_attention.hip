@@ -8,11 +8,13 @@
 // these items in turn and find them by prefix sums over the streams, whose lengths only the device knows.  A workgroup of four
 // waves multiplies
 //   S^T = K Q^T  and  O^T = V^T P^T   (v_mfma_f32_32x32x16),
-// so that a lane owns one row: its maximum and sum need one exchange between the wave's halves, its mask two comparisons per
-// score with bounds of its own, and its rescaling is a multiplication by a scalar.  The probabilities leave the first product in
-// the registers in which the second one wants them, keys permuted; V^T is read permuted alike by the LDS read that transposes.
+// so that a lane owns one row: its maximum and sum need one exchange between the wave's halves, its mask is a word of bits, and its
+// rescaling is a multiplication by a scalar.  The probabilities leave the first product in the registers in which the second one
+// wants them, keys permuted; V^T is read permuted alike by the LDS read that transposes.
 //
-//   * Tiles of more than 32 rows: a wave owns 32 rows, and all four walk the same keys, 64 a step, through two stages in LDS.
+//   * Tiles of more than 32 rows: a wave owns 32 rows, and all four walk the same keys, 64 a step, through two stages in LDS, scores a
+//     step ahead of probabilities: under the 16 products of S^T of the next step and the 16 of O^T of this one run this step's
+//     exponentials and the next one's maximum.
 //   * Tiles of up to 32 rows (single tokens, drafts): all waves own the same rows, and each walks every fourth group of 32 keys
 //     with LDS of its own and no barrier, K of the next group on its way from the moment the scores are done, V from the moment
 //     they are used; the four results are merged at the end.
@@ -20,6 +22,13 @@
 //
 // K and V go straight from memory to LDS, 1024 bytes a load.  Where the rows lie is looked up one step ahead, an entry of the
 // page table per lane, also straight to LDS, so that no register load stands between the loads under way and their wait.
+//
+// What bounds it (bf16, 128 columns; the card's own copy of 2 GiB runs at 4.9 TB/s, the library's 8192^3 product at 1219 TFLOP/s):
+// single tokens of 32 streams over 500 to 16384 keys take 102 to 108 us, 4.6 to 4.9 TB/s of K and V; 2640 x 24 heads over 13200 keys
+// take 430 to 440 us, 0.97 to 1.0 PFLOP/s, where the matrix unit is busy for half of the cycles, 6.7 vector instructions go with each of
+// its instructions and the clock is down at 2.0 GHz.  With fewer steps per item its beginning shows (places, then keys, then the first
+// scores, one behind the other, some 5 us beside the other workgroup of the unit): 532 x 40 heads over 9000 keys 0.77 PFLOP/s, 3 x
+// 2640 x 24 over 60 to 512 encoder states 43 us, 0.56 PFLOP/s.
 #include "ll_types16.h"
 
 #include <algorithm>
@@ -333,6 +342,8 @@ __global__ __launch_bounds__(kRaThreads, D == 64 ? 3 : 2) void ragged_attention_
   const int s_begin = t.s_begin, s_end = t.s_end;
   const int tile_rows = min(kRaTileRows, t.rows - t.first);
   const uint16_t *k_head = p.k + kv_head * p.k_stride_head, *v_head = p.v + kv_head * p.v_stride_head;
+  // As wider tiles, with three waves idle, up to 32 rows take longer: single tokens of 3 streams over up to 300 keys 9.7 us, so 7.8; of 32
+  // streams over up to 16384 keys 118 us, so 108.
   const bool narrow = tile_rows <= 32;
   const int own = narrow ? 0 : wave * 32;  // the wave's first row in the tile
 
@@ -404,7 +415,9 @@ __global__ __launch_bounds__(kRaThreads, D == 64 ? 3 : 2) void ragged_attention_
   const uint32_t k_row = (uint32_t)(lane / kPieces) * p.k_stride_row * 2, v_row = (uint32_t)(lane / kPieces) * p.v_stride_row * 2;
   auto turn = [](bool values, int i) { return (values ? v_piece<D>(i * kRowsPerLoad, 0) : k_piece<D>(i * kRowsPerLoad, 0)) * 16; };
   typedef __attribute__((address_space(3))) u32x4* lds_uint4;
-  const bool whole_pages = KIND == kRaPaged && p.page.d % 16 == 0;  // 16 rows from a multiple of 16 on lie one behind the other
+  // 16 rows from a multiple of 16 on lie one behind the other, and take one address for a wave in place of one for a lane: 532 x 40 heads
+  // over 9000 keys in pages of 32 rows 124 us, of 24 rows 148.
+  const bool whole_pages = KIND == kRaPaged && p.page.d % 16 == 0;
   // counted: as many loads whatever keys there are, for waits that leave some under way.
   auto load_rows = [&](bool values, int r0, uint32_t lds, bool counted) __attribute__((always_inline)) {
     const uint16_t* base = values ? v_head : k_head;
@@ -1030,6 +1043,11 @@ static int check_ragged(const ll_ragged_attention_args* a) {
 
 // How a launch is divided (host arithmetic): as many workgroups as the device holds, and the steps of a part.  Only the device knows
 // the streams' lengths; the host knows the longest, if it is told, and how many rows there are in all.
+// Parts make items alike and cost a record each, written and read: 66 KB for a tile of 128 rows of 128 columns, 15 us of a workgroup's share
+// of the memory's rate.  us by steps of a part, 12 streams of 1 to 700 tokens x 40 heads over 300 to 9000 keys: 10 241, 16 200, 24 183, 48
+// 176, whole tiles 256 (the rule: 50); 17 streams of 3 to 900 x 20 over 100 to 2400 masked states: 10 61, 16 74, 24 and more 85 (the rule:
+// 10).  Narrow tiles, 32 single tokens x 32 heads over 500 to 16384 keys: 8 135, 12 130, 16 123, 24 132, 32 126 (the rule: 16); 4 over
+// 4000: 8 20.4, 16 23.6, 32 34.3 (the rule: 8).  One stream, 532 x 40 over 9000: 7 parts 170, 3 parts, one round of the workgroups, 143.
 struct RaPlan {
   uint32_t groups, part_steps, narrow_part_steps, records;
   size_t bytes;

@@ -75,6 +75,6 @@ def paged_attention(q: torch.Tensor, cache: dict, page_table: torch.Tensor, kv_l
 
     ``max_q_len`` / ``max_kv_len``: the longest stream's new tokens and keys, if the caller knows them; any value gives the right result,
     true ones a division of the work that fits.  Returns ``out`` [T, H, D]: rows outside every stream are zeros in a new tensor and
-    stay as they were in a given one."""
+    stay as they were in a given one, which may be q itself."""
     return _native.ragged_attention("paged_attention", q, q_starts, softmax_scale, max_q_len, max_kv_len, out, cache=cache, page_table=page_table,
                                     kv_lens=kv_lens, causal=causal, window=window, sink_tokens=sink_tokens)
