@@ -1054,7 +1054,7 @@ struct RaPlan {
 };
 constexpr int64_t kRaPartCost = 3;          // what an item costs beside its steps, in steps
 constexpr int64_t kRaCutCost = 7;           // ... and where it leaves a record, with the joining of it
-constexpr int64_t kRaLeastWideSteps = 10, kRaLeastNarrowSteps = 8, kRaMostNarrowSteps = 16;
+constexpr int64_t kRaLeastWideSteps = 10, kRaLeastNarrowSteps = 8, kRaMostNarrowSteps = 16, kRaMostWholeSteps = 32;
 constexpr size_t kRaMostBytes = (size_t)256 << 20;  // of records
 
 static RaPlan plan_ragged(const ll_ragged_attention_args& a, int cus) {
@@ -1090,8 +1090,15 @@ static RaPlan plan_ragged(const ll_ragged_attention_args& a, int cus) {
     r.part_steps = (uint32_t)std::min<int64_t>(std::max(busy * mean * 5 / (4 * slots), kRaLeastWideSteps), 1 << 24);
   }
   const bool all_narrow = longest * group <= 32;
-  // Beside wider tiles, streams of few rows are worth a second launch only where they are long.
-  if (!all_narrow && (a.streams == 1 || steps <= 2 * kRaMostNarrowSteps)) r.narrow_part_steps = 1u << 24;
+  // Beside wider tiles, streams of few rows are worth a second launch only where they are long.  By themselves, where the steps that they
+  // save, one behind the other, are more than the second launch costs; the memory serves half as many items as there are units at full pace,
+  // more of them take as long cut or whole.  us whole / cut, single tokens: 8 streams x 16 heads of 64 columns over 640 keys 8.7 / 11.2, over
+  // 1280 12.7 / 15.7; 1 x 8 of 128 over 640 12.4 / 13.9, over 1024 16.9 / 15.4; 32 x 8 of 128 over 100 to 1024 19.4 / 22.0, to 1600 26.0 / 24.7,
+  // to 2048 30.9 / 32.5.
+  const int64_t served = 2 * busy * steps / cus;
+  if (all_narrow ? steps <= kRaMostWholeSteps && std::max(steps, served) <= kRaCutCost + std::max(kRaLeastNarrowSteps, served)
+                 : a.streams == 1 || steps <= 2 * kRaMostNarrowSteps)
+    r.narrow_part_steps = 1u << 24;
   const int64_t part = all_narrow ? r.narrow_part_steps : std::min(r.part_steps, r.narrow_part_steps);
   const int64_t parts = (steps + part - 1) / part;
   if (parts > 1) {

@@ -189,5 +189,6 @@ def test_memory_that_launches_ask_for():
     assert need(n_queries=65536, streams=16, max_q_len=8192) <= 256 << 20
     assert need(streams=1, n_queries=2640, max_q_len=2640, num_heads=24, num_kv_heads=24, max_kv_len=13200, page_size=880, table_width=15) == 0
     assert need(streams=1, n_queries=1, num_heads=8) > 0   # one stream's token: its keys over the whole device
+    assert need(max_kv_len=640) == need(max_kv_len=1024) == 0    # a second launch would cost more than it saves
     for cus in (1, 64, 304):
         assert need(cus=cus) <= 256 << 20
