@@ -1047,14 +1047,20 @@ static int check_ragged(const ll_ragged_attention_args* a) {
 // of the memory's rate.  us by steps of a part, 12 streams of 1 to 700 tokens x 40 heads over 300 to 9000 keys: 10 241, 16 200, 24 183, 48
 // 176, whole tiles 256 (the rule: 50); 17 streams of 3 to 900 x 20 over 100 to 2400 masked states: 10 61, 16 74, 24 and more 85 (the rule:
 // 10).  Narrow tiles, 32 single tokens x 32 heads over 500 to 16384 keys: 8 135, 12 130, 16 123, 24 132, 32 126 (the rule: 16); 4 over
-// 4000: 8 20.4, 16 23.6, 32 34.3 (the rule: 8).  One stream, 532 x 40 over 9000: 7 parts 170, 3 parts, one round of the workgroups, 143.
+// 4000: 8 20.4, 16 23.6, 32 34.3 (the rule: 8).
+// Where tiles are alike, the number of parts follows from their cost, in sixteenths of a step of a full unit: steps are faster by themselves
+// (kRaStepCost), an item's beginning and a record are paid for by the share of the device that they keep busy.  us by steps of a part, one
+// stream of 100 x 32 / 8 heads of 128 columns over 1000 keys: 3 22.6, 4 23.2, 6 23.7, 8 27.6, whole 30.9 (the rule: 4); over 4000: 6 37.9, 8
+// 31.8, 10 33.9, 16 38.8 (8); 500 x 12 heads of 64 over 9500: 10 47.4, 16 44.3, 24 53.1 (15); 532 x 40 / 8 over 9000: 20 170, 47 143 (47).
 struct RaPlan {
   uint32_t groups, part_steps, narrow_part_steps, records;
   size_t bytes;
 };
-constexpr int64_t kRaPartCost = 3;          // what an item costs beside its steps, in steps
-constexpr int64_t kRaCutCost = 7;           // ... and where it leaves a record, with the joining of it
+constexpr int64_t kRaStepCost[2][3] = {{9, 12, 16}, {12, 16, 16}};  // 64 and 128 columns: with one, two or three workgroups to a unit
+constexpr int64_t kRaItemCost = 48, kRaRecordCost = 109;            // of items as many as the device holds: their beginnings, their records
+constexpr int64_t kRaJoinCost = 40;                                 // of the second launch
 constexpr int64_t kRaLeastWideSteps = 10, kRaLeastNarrowSteps = 8, kRaMostNarrowSteps = 16, kRaMostWholeSteps = 32;
+constexpr int64_t kRaNarrowJoin = 7;                                // of the second launch behind narrow tiles, in their steps
 constexpr size_t kRaMostBytes = (size_t)256 << 20;  // of records
 
 static RaPlan plan_ragged(const ll_ragged_attention_args& a, int cus) {
@@ -1075,16 +1081,22 @@ static RaPlan plan_ragged(const ll_ragged_attention_args& a, int cus) {
   const int64_t steps = std::max<int64_t>((keys + kRaKeys - 1) / kRaKeys, 1), busy = tiles * a.num_kv_heads;
   // Narrow tiles are bound by memory: parts short enough to keep the device busy to the end whatever the lengths are.
   r.narrow_part_steps = (uint32_t)std::min(std::max((steps * busy + 4 * slots - 1) / (4 * slots), kRaLeastNarrowSteps), kRaMostNarrowSteps);
-  if (alike) {  // the number of parts for which the rounds of all of them, one behind the other, are shortest
+  // So are tiles too few to fill half of the device, whose longest one counts, and streams that leave no room for others than long ones.
+  const int64_t room = a.streams * keys;
+  if (alike || 2 * busy <= cus || (5 * rows_of_keys >= 4 * room && 4 * rows_of_keys <= 5 * room)) {
     int64_t best = 1, least = -1;
-    for (int64_t parts = 1; parts <= 64 && (parts == 1 || steps / parts >= kRaLeastNarrowSteps); ++parts) {
-      const int64_t each = (steps + parts - 1) / parts, cost = (busy * parts + slots - 1) / slots * (each + (parts > 1 ? kRaCutCost : kRaPartCost)) + (parts > 1 ? kRaCutCost : 0);
+    for (int64_t parts = 1; parts <= 64 && (parts == 1 || steps / parts >= 3); ++parts) {
+      const int64_t each = (steps + parts - 1) / parts, items = busy * parts, rounds = (items + slots - 1) / slots;
+      const int64_t step = kRaStepCost[a.head_dim == 128][items <= cus ? 0 : items <= 2 * cus ? 1 : 2];
+      const int64_t cost = rounds * (each * step + kRaItemCost * std::min(items, slots) / slots) + (parts > 1 ? kRaJoinCost + kRaRecordCost * items / slots : 0);
       if (least < 0 || cost < least) {
         least = cost;
         best = parts;
       }
     }
     r.part_steps = best == 1 ? 1u << 24 : (uint32_t)((steps + best - 1) / best);
+  } else if (steps <= 16) {  // 12 x 20 to 300 tokens x 16 heads of 64 columns over 300 to 1000 keys whole 24.2 us, by 10 steps 26.4
+    r.part_steps = 1u << 24;
   } else {  // about what a workgroup has to do in all, if the mean stream has half of the keys that there is room for
     const int64_t mean = std::min(steps, (rows_of_keys / a.streams + kRaKeys - 1) / kRaKeys + 1) / 2 + 1;
     r.part_steps = (uint32_t)std::min<int64_t>(std::max(busy * mean * 5 / (4 * slots), kRaLeastWideSteps), 1 << 24);
@@ -1096,7 +1108,7 @@ static RaPlan plan_ragged(const ll_ragged_attention_args& a, int cus) {
   // 1280 12.7 / 15.7; 1 x 8 of 128 over 640 12.4 / 13.9, over 1024 16.9 / 15.4; 32 x 8 of 128 over 100 to 1024 19.4 / 22.0, to 1600 26.0 / 24.7,
   // to 2048 30.9 / 32.5.
   const int64_t served = 2 * busy * steps / cus;
-  if (all_narrow ? steps <= kRaMostWholeSteps && std::max(steps, served) <= kRaCutCost + std::max(kRaLeastNarrowSteps, served)
+  if (all_narrow ? steps <= kRaMostWholeSteps && std::max(steps, served) <= kRaNarrowJoin + std::max(kRaLeastNarrowSteps, served)
                  : a.streams == 1 || steps <= 2 * kRaMostNarrowSteps)
     r.narrow_part_steps = 1u << 24;
   const int64_t part = all_narrow ? r.narrow_part_steps : std::min(r.part_steps, r.narrow_part_steps);
