@@ -43,7 +43,9 @@ constexpr int kRaTileRows = 128;  // rows of a workgroup, 32 a wave
 constexpr int kRaKeys = 64;       // keys of a step
 constexpr int kRaClearGroups = 16;
 constexpr float kLog2E = 1.4426950408889634f;
-constexpr uint32_t kRaJoinGroups = 512;
+// Of the joining launch, times two passes over a tile's rows: 17 streams over 100 to 2400 masked states 59.6 us, with 512 and four 61.0, with
+// 512 and one 64.9.
+constexpr uint32_t kRaJoinGroups = 256;
 
 // Where keys lie: in the pages of a table, in rows one behind the other, in such rows with a mask.
 constexpr int kRaPaged = 0, kRaRows = 1, kRaMaskedRows = 2;
@@ -1153,7 +1155,7 @@ static int launch_ragged(const RaParams& p, uint32_t grid, hipStream_t stream) {
   LL_CHECK_LAUNCH("ll_ragged_attention");
   if (p.records) {
     const uint32_t each = kRaThreads * 4 / D;
-    ragged_join_kernel<T, D, KIND><<<dim3(kRaJoinGroups, kRaTileRows / each / 4), kRaThreads, 0, stream>>>(p);
+    ragged_join_kernel<T, D, KIND><<<dim3(kRaJoinGroups, kRaTileRows / each / 2), kRaThreads, 0, stream>>>(p);
     LL_CHECK_LAUNCH("ll_ragged_attention (join)");
   }
   return LL_OK;
