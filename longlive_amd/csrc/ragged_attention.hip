@@ -42,6 +42,7 @@ constexpr int kRaThreads = 256;
 constexpr int kRaTileRows = 128;  // rows of a workgroup, 32 a wave
 constexpr int kRaKeys = 64;       // keys of a step
 constexpr int kRaClearGroups = 16;
+constexpr uint32_t kRaLeastWideSteps = 10;  // of a part, where tiles are not alike
 constexpr float kLog2E = 1.4426950408889634f;
 // Of the joining launch, times two passes over a tile's rows: 17 streams over 100 to 2400 masked states 59.6 us, with 512 and four 61.0, with
 // 512 and one 64.9.
@@ -76,6 +77,7 @@ struct RaParams {
   uint32_t groups;        // workgroups that take the items
   // Steps of a part, for tiles of more rows and for streams of up to 32 rows.  0 records: nothing is cut.
   uint32_t part_steps, narrow_part_steps;
+  float part_share;       // not 0: part_steps follow from the streams, this times the steps of all wide tiles of a head
   uint32_t records;       // of a kv head, 32 rows each
   float* record_mem;      // [kv head][records]: 32 x D columns, then maximum and sum of each row
 };
@@ -172,7 +174,6 @@ __device__ __forceinline__ RaSpan span_of(const RaParams& p, int len, int pos0, 
   s.n_steps = min(s.sink_steps, end_step) + max(end_step - s.from_step, 0);
   return s;
 }
-__device__ __forceinline__ uint32_t part_steps_of(const RaParams& p, int rows) { return rows <= 32 ? p.narrow_part_steps : p.part_steps; }
 // Records of a tile's part.
 __device__ __forceinline__ int record_groups(int rows) { return rows <= 32 ? 1 : kRaTileRows / 32; }
 
@@ -192,7 +193,7 @@ __device__ __forceinline__ uint32_t sum_upto(uint32_t v) {
 // What is known of 64 streams, loaded at once; `items` and `records`: of the streams before.  A stream whose records would go beyond
 // what there is stays whole.  COUNT_TILES: the items are the tiles that were cut.
 template <int KIND, bool COUNT_TILES>
-__device__ __forceinline__ RaStreams load_streams(const RaParams& p, int b0, uint32_t items, uint32_t records) {
+__device__ __forceinline__ RaStreams load_streams(const RaParams& p, int b0, uint32_t items, uint32_t records, uint32_t& part_steps) {
   const int lane = threadIdx.x & 63, b = min(b0 + lane, p.streams - 1);
   const int start = p.q_starts[b], next = p.q_starts[b + 1];
   int64_t key0 = 0, len;
@@ -215,11 +216,20 @@ __device__ __forceinline__ RaStreams load_streams(const RaParams& p, int b0, uin
   s.records_upto = 0;
   if (p.records) {
     uint32_t mine = 0;
+    int steps = 0;
     if (s.tiles) {
       // the first tile that sees the stream's last key sees most: where there is a window, up to a tile's tokens more than it
       const int pos1 = s.len - 1, pos0 = pos1 - min(s.n - 1, (int)((uint32_t)(kRaTileRows - 1) / p.group) + 1);
-      const int steps = p.window ? span_of(p, s.len, pos0, pos1).n_steps + 1 : (s.len + kRaKeys - 1) / kRaKeys;
-      const uint32_t per_part = part_steps_of(p, rows);
+      steps = p.window ? span_of(p, s.len, pos0, pos1).n_steps + 1 : (s.len + kRaKeys - 1) / kRaKeys;
+    }
+    if (p.part_share != 0.0f) {  // up to 64 streams, which are all here
+      const int mean = p.causal && !p.window ? max(steps - s.n / (2 * kRaKeys), 1) : steps;
+      const uint32_t of_tiles = rows > 32 ? (uint32_t)min((int64_t)s.tiles * mean, (int64_t)1 << 25) : 0;
+      const uint32_t all = (uint32_t)__builtin_amdgcn_readlane((int)sum_upto(of_tiles), 63);
+      part_steps = max((uint32_t)__builtin_amdgcn_readfirstlane((int)((float)all * p.part_share)), kRaLeastWideSteps);
+    }
+    if (s.tiles) {
+      const uint32_t per_part = rows <= 32 ? p.narrow_part_steps : part_steps;
       s.parts = max((int)((steps + per_part - 1) / per_part), 1);
       if (s.parts > 1) mine = (uint32_t)min((int64_t)s.tiles * s.parts * record_groups(rows), (int64_t)p.records + 1);
     }
@@ -236,9 +246,11 @@ template <int KIND, bool COUNT_TILES>
 struct RaCursor {
   int b0 = 0;
   uint32_t items = 0, records = 0;  // of the streams before b0
+  uint32_t part_steps;              // of a part of a wide tile
   RaStreams s;                      // streams from b0 on
   __device__ __forceinline__ void start(const RaParams& p) {
-    if (p.streams > 0) s = load_streams<KIND, COUNT_TILES>(p, 0, 0, 0);
+    part_steps = p.part_steps;
+    if (p.streams > 0) s = load_streams<KIND, COUNT_TILES>(p, 0, 0, 0, part_steps);
   }
   // Item `index` of a kv head, which is no smaller than the last one asked for.  All lanes call it together.  False: there are fewer.
   __device__ __forceinline__ bool find(const RaParams& p, uint32_t index, RaItem& t) {
@@ -265,7 +277,7 @@ struct RaCursor {
         const RaSpan span = span_of(p, t.len, base + (int)((uint32_t)t.first / p.group), base + (int)((uint32_t)last_row / p.group));
         t.sink_steps = span.sink_steps;
         t.from_step = span.from_step;
-        const uint32_t per_part = part_steps_of(p, t.rows);
+        const uint32_t per_part = t.rows <= 32 ? p.narrow_part_steps : part_steps;
         t.n_parts = parts > 1 ? max(min((int)((span.n_steps + per_part - 1) / per_part), parts), 1) : 1;
         const int each = (span.n_steps + t.n_parts - 1) / t.n_parts;  // equal parts
         t.s_begin = min(t.part * each, span.n_steps);
@@ -277,7 +289,7 @@ struct RaCursor {
       if (b0 >= p.streams) return false;
       items = (uint32_t)__builtin_amdgcn_readlane((int)s.items_upto, 63);
       records = min((uint32_t)__builtin_amdgcn_readlane((int)s.records_upto, 63), p.records + 1);
-      s = load_streams<KIND, COUNT_TILES>(p, b0, items, records);
+      s = load_streams<KIND, COUNT_TILES>(p, b0, items, records, part_steps);
     }
   }
 };
@@ -1057,16 +1069,22 @@ static int check_ragged(const ll_ragged_attention_args* a) {
 struct RaPlan {
   uint32_t groups, part_steps, narrow_part_steps, records;
   size_t bytes;
+  float part_share;
 };
 constexpr int64_t kRaStepCost[2][3] = {{9, 12, 16}, {12, 16, 16}};  // 64 and 128 columns: with one, two or three workgroups to a unit
 constexpr int64_t kRaItemCost = 48, kRaRecordCost = 109;            // of items as many as the device holds: their beginnings, their records
 constexpr int64_t kRaJoinCost = 40;                                 // of the second launch
-constexpr int64_t kRaLeastWideSteps = 10, kRaLeastNarrowSteps = 8, kRaMostNarrowSteps = 16, kRaMostWholeSteps = 32;
+constexpr int64_t kRaLeastNarrowSteps = 8, kRaMostNarrowSteps = 16, kRaMostWholeSteps = 32;
+// Of what a workgroup has to do in all, a part: by the device, of up to 64 streams, where the launch is not so long that the last items do not
+// count.  us with 0.5 / 0.75 / 0.9 / 1.1 / by the host's guess, pages for eight times the streams' keys: 12 streams of 1 to 700 tokens x 40 / 8
+// heads over 300 to 9000 keys 207 / 216 / 204 / 199 / 274; 16 of 5 to 600 x 24 over 600 to 4600 173 / 176 / 173 / 173 / 196; 30 of 1 to 300 x
+// 32 / 8 over 300 to 4000 97 / 99 / 89 / 96 / 100; prompts of 5 times 100 to 2000 x 16 / 4, causal, 82 / 101 / 84 / 83 / 74 (there whole).
+constexpr float kRaShare = 0.9f;
 constexpr int64_t kRaNarrowJoin = 7;                                // of the second launch behind narrow tiles, in their steps
 constexpr size_t kRaMostBytes = (size_t)256 << 20;  // of records
 
 static RaPlan plan_ragged(const ll_ragged_attention_args& a, int cus) {
-  RaPlan r{0, 0, 0, 0, 0};
+  RaPlan r{0, 0, 0, 0, 0, 0.0f};
   if (a.n_queries == 0 || a.streams == 0) return r;
   const bool paged = a.page_table || a.page_size;
   const int64_t group = a.num_heads / a.num_kv_heads, slots = (a.head_dim == 64 ? 3 : 2) * cus;
@@ -1099,9 +1117,10 @@ static RaPlan plan_ragged(const ll_ragged_attention_args& a, int cus) {
     r.part_steps = best == 1 ? 1u << 24 : (uint32_t)((steps + best - 1) / best);
   } else if (steps <= 16) {  // 12 x 20 to 300 tokens x 16 heads of 64 columns over 300 to 1000 keys whole 24.2 us, by 10 steps 26.4
     r.part_steps = 1u << 24;
-  } else {  // about what a workgroup has to do in all, if the mean stream has half of the keys that there is room for
+  } else {  // about what a workgroup has to do in all (kRaShare), or if the mean stream has half of the keys that there is room for
     const int64_t mean = std::min(steps, (rows_of_keys / a.streams + kRaKeys - 1) / kRaKeys + 1) / 2 + 1;
-    r.part_steps = (uint32_t)std::min<int64_t>(std::max(busy * mean * 5 / (4 * slots), kRaLeastWideSteps), 1 << 24);
+    r.part_steps = (uint32_t)std::min<int64_t>(std::max<int64_t>(busy * mean * 5 / (4 * slots), kRaLeastWideSteps), 1 << 24);
+    if (a.streams <= 64 && busy <= 8 * slots) r.part_share = kRaShare * a.num_kv_heads / slots;
   }
   const bool all_narrow = longest * group <= 32;
   // Beside wider tiles, streams of few rows are worth a second launch only where they are long.  By themselves, where the steps that they
@@ -1114,11 +1133,13 @@ static RaPlan plan_ragged(const ll_ragged_attention_args& a, int cus) {
                  : a.streams == 1 || steps <= 2 * kRaMostNarrowSteps)
     r.narrow_part_steps = 1u << 24;
   const int64_t part = all_narrow ? r.narrow_part_steps : std::min(r.part_steps, r.narrow_part_steps);
-  const int64_t parts = (steps + part - 1) / part;
+  const int64_t parts = r.part_share != 0.0f && !all_narrow ? (steps + kRaLeastWideSteps - 1) / kRaLeastWideSteps : (steps + part - 1) / part;
   if (parts > 1) {
     // Every tile in as many parts, or what is allowed; streams that find no records left stay whole.
     const size_t record = 32 * (size_t)(a.head_dim + 2) * sizeof(float);
-    const int64_t want = tiles * parts * (all_narrow ? 1 : kRaTileRows / 32);
+    int64_t want = tiles * parts * (all_narrow ? 1 : kRaTileRows / 32);
+    if (r.part_share != 0.0f && !all_narrow)  // parts as many as the share makes, and one more of every tile
+      want = std::min(want, (int64_t)((1.0f / r.part_share + 1 + tiles) * (kRaTileRows / 32)) + a.streams * ((steps + r.narrow_part_steps - 1) / r.narrow_part_steps));
     r.records = (uint32_t)std::min<int64_t>(want, (int64_t)(kRaMostBytes / record) / a.num_kv_heads);
     r.bytes = r.records * record * a.num_kv_heads;
   }
@@ -1232,6 +1253,7 @@ extern "C" int ll_ragged_attention(const ll_ragged_attention_args* a, void* stre
   p.sink = (uint32_t)std::min<int64_t>(a->sink_keys, 0x7fffffff);
   p.groups = plan.groups;
   p.part_steps = plan.part_steps;
+  p.part_share = plan.part_share;
   p.narrow_part_steps = plan.narrow_part_steps;
   p.records = plan.records;
   p.record_mem = static_cast<float*>(a->workspace);

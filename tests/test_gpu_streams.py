@@ -218,14 +218,14 @@ def test_streams_that_find_no_records_left_stay_whole(gpu):
 
 def test_one_long_stream_among_short_ones_finds_no_records_left(gpu):
     # room for 496 records of a head; 16 tiles in 8 parts want 512, the stream before them is cut in two
-    new, keys, H, D = [20, 2048] + [1] * 60, [2000, 12000] + [16] * 60, 64, 64
+    new, keys, H, D = [20, 2048] + [1] * 70, [2000, 13000] + [16] * 70, 64, 64   # more than 64 streams: parts by the host
     q, cache, table, lens, q_starts = batch(48, new, keys, H, H, D, 16, F16)
     dev = {n: t.to(gpu) for n, t in cache.items()}
-    got = paged_attention(q.to(gpu), dev, table.to(gpu), lens.to(gpu), q_starts.to(gpu), max_q_len=2048, max_kv_len=12000)
+    got = paged_attention(q.to(gpu), dev, table.to(gpu), lens.to(gpu), q_starts.to(gpu), max_q_len=2048, max_kv_len=13000)
     keys_of, seen_of = ref.paged_keys({n: t[:, :, [0, 63]] for n, t in cache.items()}, table, lens)
     firsts = q_starts.tolist()
     for h, head in enumerate((0, 63)):
-        for b, at in ((0, torch.arange(20)), (1, torch.tensor([0, 1, 900, 2046, 2047])), (2, torch.tensor([0])), (61, torch.tensor([0]))):
+        for b, at in ((0, torch.arange(20)), (1, torch.tensor([0, 1, 900, 2046, 2047])), (2, torch.tensor([0])), (71, torch.tensor([0]))):
             k, v = (t[:, h] for t in keys_of(b))
             want, error = ref.attend(q[firsts[b] + at, head], k, v, seen_of()(b, new[b], len(k))[at], D ** -0.5)
             close(got[(firsts[b] + at).to(gpu), head], want, error, f"stream {b} head {head}")
