@@ -226,7 +226,7 @@ __device__ __forceinline__ RaStreams load_streams(const RaParams& p, int b0, uin
       const int mean = p.causal && !p.window ? max(steps - s.n / (2 * kRaKeys), 1) : steps;
       const uint32_t of_tiles = rows > 32 ? (uint32_t)min((int64_t)s.tiles * mean, (int64_t)1 << 25) : 0;
       const uint32_t all = (uint32_t)__builtin_amdgcn_readlane((int)sum_upto(of_tiles), 63);
-      part_steps = max((uint32_t)__builtin_amdgcn_readfirstlane((int)((float)all * p.part_share)), kRaLeastWideSteps);
+      part_steps = max((uint32_t)__builtin_amdgcn_readfirstlane((int)fminf((float)all * p.part_share, 1e9f)), kRaLeastWideSteps);
     }
     if (s.tiles) {
       const uint32_t per_part = rows <= 32 ? p.narrow_part_steps : part_steps;
@@ -1059,8 +1059,8 @@ static int check_ragged(const ll_ragged_attention_args* a) {
 // the streams' lengths; the host knows the longest, if it is told, and how many rows there are in all.
 // Parts make items alike and cost a record each, written and read: 66 KB for a tile of 128 rows of 128 columns, 15 us of a workgroup's share
 // of the memory's rate.  us by steps of a part, 12 streams of 1 to 700 tokens x 40 heads over 300 to 9000 keys: 10 241, 16 200, 24 183, 48
-// 176, whole tiles 256 (the rule: 50); 17 streams of 3 to 900 x 20 over 100 to 2400 masked states: 10 61, 16 74, 24 and more 85 (the rule:
-// 10).  Narrow tiles, 32 single tokens x 32 heads over 500 to 16384 keys: 8 135, 12 130, 16 123, 24 132, 32 126 (the rule: 16); 4 over
+// 176, whole tiles 256 (the rule: 56); 17 streams of 3 to 900 x 20 over 100 to 2400 masked states: 10 61, 16 74, 24 and more 85 (the rule:
+// 11).  Narrow tiles, 32 single tokens x 32 heads over 500 to 16384 keys: 8 135, 12 130, 16 123, 24 132, 32 126 (the rule: 16); 4 over
 // 4000: 8 20.4, 16 23.6, 32 34.3 (the rule: 8).
 // Where tiles are alike, the number of parts follows from their cost, in sixteenths of a step of a full unit: steps are faster by themselves
 // (kRaStepCost), an item's beginning and a record are paid for by the share of the device that they keep busy.  us by steps of a part, one
@@ -1090,7 +1090,7 @@ static RaPlan plan_ragged(const ll_ragged_attention_args& a, int cus) {
   const int64_t group = a.num_heads / a.num_kv_heads, slots = (a.head_dim == 64 ? 3 : 2) * cus;
   const int64_t longest = a.max_q_len > 0 && a.max_q_len < a.n_queries ? a.max_q_len : a.n_queries;
   const int64_t tiles = std::min(a.n_queries * group / kRaTileRows + a.streams, a.streams * ((longest * group + kRaTileRows - 1) / kRaTileRows));
-  const int64_t all_keys = paged ? a.table_width * a.page_size : a.n_keys, rows_of_keys = paged ? a.n_pages * a.page_size : a.n_keys;
+  const int64_t all_keys = paged ? a.table_width * a.page_size : a.n_keys, rows_of_keys = paged ? std::min<int64_t>(a.n_pages * a.page_size, 1ll << 60) : a.n_keys;
   int64_t keys = a.max_kv_len > 0 && a.max_kv_len < all_keys ? a.max_kv_len : all_keys;
   bool alike = a.streams == 1;  // whether all tiles see about as many keys
   if (a.window > 0 && a.window < keys && a.sink_keys < keys) {
@@ -1101,7 +1101,7 @@ static RaPlan plan_ragged(const ll_ragged_attention_args& a, int cus) {
   const int64_t steps = std::max<int64_t>((keys + kRaKeys - 1) / kRaKeys, 1), busy = tiles * a.num_kv_heads;
   // Narrow tiles are bound by memory: parts short enough to keep the device busy to the end whatever the lengths are.
   r.narrow_part_steps = (uint32_t)std::min(std::max((steps * busy + 4 * slots - 1) / (4 * slots), kRaLeastNarrowSteps), kRaMostNarrowSteps);
-  // So are tiles too few to fill half of the device, whose longest one counts, and streams that leave no room for others than long ones.
+  // As alike count tiles too few to fill half of the device, whose longest ones decide, and streams in a cache with room for long ones alone.
   const int64_t room = a.streams * keys;
   if (alike || 2 * busy <= cus || (5 * rows_of_keys >= 4 * room && 4 * rows_of_keys <= 5 * room)) {
     int64_t best = 1, least = -1;

@@ -190,5 +190,10 @@ def test_memory_that_launches_ask_for():
     assert need(streams=1, n_queries=2640, max_q_len=2640, num_heads=24, num_kv_heads=24, max_kv_len=13200, page_size=880, table_width=15) == 0
     assert need(streams=1, n_queries=1, num_heads=8) > 0   # one stream's token: its keys over the whole device
     assert need(max_kv_len=640) == need(max_kv_len=1024) == 0    # a second launch would cost more than it saves
+    most = 0x7fffffff                                            # sizes at the ends of their ranges
+    for kw in (dict(n_pages=most, page_size=most, table_width=1), dict(n_pages=most, page_size=most, table_width=1, n_queries=1 << 25, max_q_len=0, max_kv_len=0),
+               dict(streams=0xfffffff // 8, n_queries=1 << 25, page_size=1, table_width=most, n_pages=most, max_q_len=0, max_kv_len=0),
+               dict(page_size=0, n_keys=most, max_q_len=0, max_kv_len=0, n_queries=1 << 25)):
+        assert 0 <= need(**kw) <= 256 << 20
     for cus in (1, 64, 304):
         assert need(cus=cus) <= 256 << 20
