@@ -604,8 +604,8 @@ int ll_head_norm_rope(int dtype, int64_t tokens, int head_dim, const ll_head_row
  * outside every stream get zeros (clear_rest) or stay as they are.  Keys:
  *   page_table given: stream b's key j < kv_lens[b] is row j % page_size of page page_table[b, j / page_size]; entries outside
  *     0 .. n_pages - 1 are holes, whose keys nobody sees, and so is what lies behind the table's width.  The stream's new tokens are
- *     its last keys: row i of n sits at position p = kv_lens[b] - n + i and sees key j where (j <= p, if causal) and (j > p - window
- *     or j < sink_keys, if window > 0).
+ *     its last keys: row i of n = q_starts[b + 1] - q_starts[b] sits at position p = kv_lens[b] - n + i, wherever the table and the rows
+ *     of q end, and sees key j where (j <= p, if causal) and (j > p - window or j < sink_keys, if window > 0).
  *   else: rows k_starts[b] + j of k and v, j < k_lens[b], or without k_lens up to k_starts[b + 1]; within n_keys; key_mask (one
  *     byte a row, or NULL) leaves out keys whose byte is zero.  Every row sees all of them; causal and window are 0.
  * A key has no part in a row that does not see it, whatever lies in its K and V, NaN included (unfilled rows of a page, masked

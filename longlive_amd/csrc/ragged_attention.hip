@@ -143,8 +143,9 @@ __device__ __forceinline__ uint64_t low_bits(int n) { return n <= 0 ? 0 : n >= 6
 // What a workgroup does next: a part of a tile.
 struct RaItem {
   int64_t q0;               // first row of q of the stream
-  int n, rows, first;       // tokens of the stream; rows of the stream (token, head of the group), the tile's first
-  int len;                  // keys of the stream
+  int rows, first;          // rows of the stream (token, head of the group), the tile's first
+  int len;                  // keys of the stream that there is a place for
+  int base;                 // paged: the position of its first token
   int key0;                 // rows of keys: row of key 0
   const int32_t* pages;     // paged: the stream's row of the table
   int sink_steps, from_step;  // the tile's steps: 0 .. sink_steps - 1, and then from from_step on
@@ -155,8 +156,8 @@ struct RaItem {
 
 // The streams b0 .. b0 + 63, one a lane.
 struct RaStreams {
-  int q0, n, len, key0;
-  int tiles, parts;                  // parts at most: of the tile that sees most keys
+  int q0, n, len, base, key0;
+  int parts;                          // at most: of the tile that sees most keys
   uint32_t items_upto, records_upto;  // of these and the streams before
 };
 
@@ -174,6 +175,8 @@ __device__ __forceinline__ RaSpan span_of(const RaParams& p, int len, int pos0, 
   s.n_steps = min(s.sink_steps, end_step) + max(end_step - s.from_step, 0);
   return s;
 }
+// Tiles of a stream's rows.
+__device__ __forceinline__ int tiles_of(int rows) { return rows > 0 ? (rows - 1) / kRaTileRows + 1 : 0; }
 // Records of a tile's part.
 __device__ __forceinline__ int record_groups(int rows) { return rows <= 32 ? 1 : kRaTileRows / 32; }
 
@@ -196,48 +199,52 @@ template <int KIND, bool COUNT_TILES>
 __device__ __forceinline__ RaStreams load_streams(const RaParams& p, int b0, uint32_t items, uint32_t records, uint32_t& part_steps) {
   const int lane = threadIdx.x & 63, b = min(b0 + lane, p.streams - 1);
   const int start = p.q_starts[b], next = p.q_starts[b + 1];
+  const int limit = (int)p.n_queries;
+  RaStreams s;
+  s.q0 = min(max(start, 0), limit);
+  s.n = b0 + lane < p.streams ? max(min(max(next, 0), limit) - s.q0, 0) : 0;
+  s.base = 0;
   int64_t key0 = 0, len;
   if constexpr (KIND == kRaPaged) {
-    len = min(max((int64_t)p.kv_lens[b], (int64_t)0), p.table_keys);
+    // positions count from the stream's last token, wherever the table and the rows of q end
+    const int64_t given = max((int64_t)p.kv_lens[b], (int64_t)0);
+    len = min(given, p.table_keys);
+    s.base = (int)(given - ((int64_t)next - s.q0));
   } else {
     const int64_t first = p.k_starts[b], given = p.k_lens ? p.k_lens[b] : p.k_starts[b + 1];
     key0 = min(max(first, (int64_t)0), p.n_keys);
     len = min(max(p.k_lens ? given : given - key0, (int64_t)0), p.n_keys - key0);
   }
-  const int limit = (int)p.n_queries;
-  RaStreams s;
-  s.q0 = min(max(start, 0), limit);
-  s.n = b0 + lane < p.streams ? max(min(max(next, 0), limit) - s.q0, 0) : 0;
   s.len = (int)len;
   s.key0 = (int)key0;
   const int rows = s.n * (int)p.group.d;
-  s.tiles = (int)(((int64_t)rows + kRaTileRows - 1) / kRaTileRows);
+  const int tiles = tiles_of(rows);
   s.parts = 1;
   s.records_upto = 0;
   if (p.records) {
     uint32_t mine = 0;
     int steps = 0;
-    if (s.tiles) {
+    if (tiles) {
       // the first tile that sees the stream's last key sees most: where there is a window, up to a tile's tokens more than it
-      const int pos1 = s.len - 1, pos0 = pos1 - min(s.n - 1, (int)((uint32_t)(kRaTileRows - 1) / p.group) + 1);
+      const int pos1 = max(s.len - 1, s.base), pos0 = pos1 - min(s.n - 1, (int)((uint32_t)(kRaTileRows - 1) / p.group) + 1);
       steps = p.window ? span_of(p, s.len, pos0, pos1).n_steps + 1 : (s.len + kRaKeys - 1) / kRaKeys;
     }
     if (p.part_share != 0.0f) {  // up to 64 streams, which are all here
       const int mean = p.causal && !p.window ? max(steps - s.n / (2 * kRaKeys), 1) : steps;
-      const uint32_t of_tiles = rows > 32 ? (uint32_t)min((int64_t)s.tiles * mean, (int64_t)1 << 25) : 0;
+      const uint32_t of_tiles = rows > 32 ? (uint32_t)min((int64_t)tiles * mean, (int64_t)1 << 25) : 0;
       const uint32_t all = (uint32_t)__builtin_amdgcn_readlane((int)sum_upto(of_tiles), 63);
       part_steps = max((uint32_t)__builtin_amdgcn_readfirstlane((int)fminf((float)all * p.part_share, 1e9f)), kRaLeastWideSteps);
     }
-    if (s.tiles) {
+    if (tiles) {
       const uint32_t per_part = rows <= 32 ? p.narrow_part_steps : part_steps;
       s.parts = max((int)((steps + per_part - 1) / per_part), 1);
-      if (s.parts > 1) mine = (uint32_t)min((int64_t)s.tiles * s.parts * record_groups(rows), (int64_t)p.records + 1);
+      if (s.parts > 1) mine = (uint32_t)min((int64_t)tiles * s.parts * record_groups(rows), (int64_t)p.records + 1);
     }
     // sums that do not pass 32 bits: a stream adds at most records + 1, the streams before at most as much
     s.records_upto = records + sum_upto(mine);
     if (s.records_upto > p.records) s.parts = 1;
   }
-  s.items_upto = items + sum_upto(COUNT_TILES ? (s.parts > 1 ? s.tiles : 0) : s.tiles * s.parts);
+  s.items_upto = items + sum_upto(COUNT_TILES ? (s.parts > 1 ? tiles : 0) : tiles * s.parts);
   return s;
 }
 
@@ -260,21 +267,21 @@ struct RaCursor {
       if (before != ~0ull) {
         const int at = __builtin_amdgcn_readfirstlane(__popcll(before));
         auto of = [&](int v) { return __builtin_amdgcn_readlane(v, at); };
-        const int tiles = of(s.tiles), parts = of(s.parts);
+        const int parts = of(s.parts);
         const uint32_t records_end = (uint32_t)of((int)s.records_upto);
         // the last tile of a stream, which sees most keys, first, and all its parts
         uint32_t left = (uint32_t)of((int)s.items_upto) - 1 - index;
         const uint32_t tile = COUNT_TILES ? left : left / (uint32_t)parts;
         t.part = COUNT_TILES ? 0 : (int)(left - tile * (uint32_t)parts);
         t.q0 = of(s.q0);
-        t.n = of(s.n);
-        t.rows = t.n * (int)p.group.d;
+        t.rows = of(s.n) * (int)p.group.d;
         t.first = (int)tile * kRaTileRows;
         t.len = of(s.len);
+        t.base = of(s.base);
         t.key0 = of(s.key0);
         t.pages = KIND == kRaPaged ? p.page_table + (int64_t)(b0 + at) * p.table_stride : nullptr;
-        const int last_row = min(t.first + kRaTileRows, t.rows) - 1, base = t.len - t.n;
-        const RaSpan span = span_of(p, t.len, base + (int)((uint32_t)t.first / p.group), base + (int)((uint32_t)last_row / p.group));
+        const int last_row = min(t.first + kRaTileRows, t.rows) - 1;
+        const RaSpan span = span_of(p, t.len, t.base + (int)((uint32_t)t.first / p.group), t.base + (int)((uint32_t)last_row / p.group));
         t.sink_steps = span.sink_steps;
         t.from_step = span.from_step;
         const uint32_t per_part = t.rows <= 32 ? p.narrow_part_steps : part_steps;
@@ -282,7 +289,7 @@ struct RaCursor {
         const int each = (span.n_steps + t.n_parts - 1) / t.n_parts;  // equal parts
         t.s_begin = min(t.part * each, span.n_steps);
         t.s_end = min(t.s_begin + each, span.n_steps);
-        t.record = records_end - (uint32_t)((tiles - (int)tile) * parts * record_groups(t.rows));
+        t.record = records_end - (uint32_t)((tiles_of(t.rows) - (int)tile) * parts * record_groups(t.rows));
         return true;
       }
       b0 += 64;
@@ -373,7 +380,7 @@ __global__ __launch_bounds__(kRaThreads, D == 64 ? 3 : 2) void ragged_attention_
   };
   const Row row = own_row();
   // what it sees: keys below `last`, from `from` on or below the sink
-  const int pos = t.len - t.n + row.token;
+  const int pos = t.base + row.token;
   const int last = p.causal ? min(pos + 1, t.len) : t.len;
   const int from = p.window && pos >= (int)p.window ? pos - (int)p.window + 1 : 0;
   // the same for the wave's first and last row, which bound the others

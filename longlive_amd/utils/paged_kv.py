@@ -70,7 +70,7 @@ def paged_attention(q: torch.Tensor, cache: dict, page_table: torch.Tensor, kv_l
     q [T, H, D], D 64 or 128, H a multiple of the cache's heads; head h reads kv head ``h // (H // kv heads)``.  Token i of a stream's n
     sits at position ``p = kv_lens[b] - n + i`` and sees key j where ``j <= p`` (``causal``; else every key: a chunk whose tokens see
     one another) and, with a ``window``, ``j > p - window or j < sink_tokens``.  Keys in holes of the page table and behind its
-    width do not exist.  A token that sees no key gets zeros.  Scores, softmax statistics and sums are fp32; the probabilities enter the
+    width do not exist, but count for the positions.  A token that sees no key gets zeros.  Scores, softmax statistics and sums are fp32; the probabilities enter the
     second product in q's type.
 
     ``max_q_len`` / ``max_kv_len``: the longest stream's new tokens and keys, if the caller knows them; any value gives the right result,
