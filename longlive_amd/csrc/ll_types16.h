@@ -13,6 +13,7 @@ typedef _Float16 f16x2_hw __attribute__((ext_vector_type(2)));
 
 struct Bf16 {
   static constexpr uint32_t kInfinity = 0x7F80;  // magnitudes from here on are not finite
+  static constexpr float kWeightShift = 0.0f;    // log2 of what a softmax's probabilities are held times
   static __device__ __forceinline__ void unpack2(uint32_t w, float& a, float& b) {
     a = __uint_as_float(w << 16);
     b = __uint_as_float(w & 0xFFFF0000u);
@@ -31,6 +32,8 @@ struct Bf16 {
 
 struct F16 {
   static constexpr uint32_t kInfinity = 0x7C00;
+  // The range ends 2^24 below 1 and 2^16 above it: near its upper end, keys down to 2^-37 of the largest keep a weight.
+  static constexpr float kWeightShift = 13.0f;
   static __device__ __forceinline__ void unpack2(uint32_t w, float& a, float& b) {
     const f16x2_hw h = __builtin_bit_cast(f16x2_hw, w);
     a = (float)h[0];

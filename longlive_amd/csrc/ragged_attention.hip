@@ -79,7 +79,7 @@ struct RaParams {
   uint32_t part_steps, narrow_part_steps;
   float part_share;       // not 0: part_steps follow from the streams, this times the steps of all wide tiles of a head
   uint32_t records;       // of a kv head, 32 rows each
-  float* record_mem;      // [kv head][records]: 32 x D columns, then maximum and sum of each row
+  float* record_mem;      // [kv head][records]: 32 x D columns, then reference point and sum of each row
 };
 
 // Positions of 16-byte pieces in an LDS row of D columns.  The reads of a wave then go through all banks: 8 neighbouring rows of one
@@ -301,7 +301,7 @@ struct RaCursor {
   }
 };
 
-// Where part `part` of an item's tile has the four columns from `column` on of a row, and the row's maximum and sum.
+// Where part `part` of an item's tile has the four columns from `column` on of a row, and the row's reference point and sum.
 template <int D>
 __device__ __forceinline__ float* record_of(const RaParams& p, uint32_t head, const RaItem& t, int part, int row) {
   const int64_t at = (int64_t)head * p.records + t.record + (uint32_t)(part * record_groups(t.rows) + row / 32);
@@ -324,6 +324,19 @@ __device__ __forceinline__ void each_index(F& f, std::integer_sequence<int, I...
 
 // The reference point of the exponentials follows the maximum once it is 2^2 ahead: fewer rescalings, no further from 64 bits.
 constexpr float kRaStep = 2.0f;
+// Probabilities are exp2(score - reference + shift), so that in f16 a row's sums keep many keys that are each far below the largest (at a
+// reference of 1, of 200000 keys 17.5 nats below one not a single one).  Sums and outputs of a row are all times 2^shift.  None where the
+// reference, scaled, has no bits left for it: its rounding, the same for all keys of a row, would carry the largest beyond f16.
+template <typename T>
+__device__ __forceinline__ float weight_shift(float reference) {
+  return T::kWeightShift != 0.0f && fabsf(reference) < 4194304.0f ? T::kWeightShift : 0.0f;
+}
+// Results at different reference points are joined by factors 2^((one - other) * unit): references are maxima, or with a shift the negative
+// constants of the exponents.
+template <typename T>
+__device__ __forceinline__ float reference_unit(float scale_log2) {
+  return T::kWeightShift == 0.0f ? scale_log2 : 1.0f;
+}
 
 template <typename T, int D, int KIND>
 __global__ __launch_bounds__(kRaThreads, D == 64 ? 3 : 2) void ragged_attention_kernel(RaParams p) {
@@ -552,10 +565,18 @@ __global__ __launch_bounds__(kRaThreads, D == 64 ? 3 : 2) void ragged_attention_
     mx = exchange_max(mx);
     const bool raise = (mx - m) * p.scale_log2 > kRaStep;
     if (__builtin_amdgcn_ballot_w64(raise) != 0) {
-      const float alpha = raise ? __builtin_amdgcn_exp2f((m - mx) * p.scale_log2) : 1.0f;
-      m = raise ? mx : m;
+      float alpha;
       // a row that has seen nothing yet stays at -inf; 0 stands for it in the exponents, where -inf - -inf would be NaN
-      neg = m == -INFINITY ? 0.0f : -m * p.scale_log2;
+      if constexpr (T::kWeightShift == 0.0f) {
+        alpha = raise ? __builtin_amdgcn_exp2f((m - mx) * p.scale_log2) : 1.0f;
+        m = raise ? mx : m;
+        neg = m == -INFINITY ? 0.0f : -m * p.scale_log2;
+      } else {
+        const float to = fmaf(-mx, p.scale_log2, weight_shift<T>(mx * p.scale_log2));
+        alpha = raise && m != -INFINITY ? __builtin_amdgcn_exp2f(to - neg) : 1.0f;  // nothing seen: sums of zero stay what they are
+        m = raise ? mx : m;
+        neg = raise ? to : neg;
+      }
       l *= alpha;
 #pragma unroll
       for (int dt = 0; dt < kDTiles; ++dt)
@@ -563,6 +584,8 @@ __global__ __launch_bounds__(kRaThreads, D == 64 ? 3 : 2) void ragged_attention_
         for (int r = 0; r < 16; ++r) o[dt][r] *= alpha;
     }
   };
+  // What the row's sums and outputs refer to, -inf for a row that has seen nothing.
+  auto reference = [&]() __attribute__((always_inline)) { return T::kWeightShift == 0.0f || m == -INFINITY ? m : -neg; };
   // V^T of 16 keys and 32 columns: a lane needs column 32 dt + l32 of the keys 8 j + 4 lh + 0 .. 3 (j = 0, 1: the order of the scores'
   // registers).  A read serves 16 lanes: lane i points at row i / 4, columns 4 (i % 4) .. + 3, and each receives a column of the four rows.
   const uint32_t v_lane = (uint32_t)((4 * lh + ((lane & 15) >> 2)) * kRowBytes +
@@ -582,7 +605,7 @@ __global__ __launch_bounds__(kRaThreads, D == 64 ? 3 : 2) void ragged_attention_
       for (int u = 0; u < 4; ++u) {
         const float p0 = __builtin_amdgcn_exp2f(fmaf(sc[step >> 1][8 * (step & 1) + 2 * u], p.scale_log2, neg));
         const float p1 = __builtin_amdgcn_exp2f(fmaf(sc[step >> 1][8 * (step & 1) + 2 * u + 1], p.scale_log2, neg));
-        w[u] = T::pack2(p0, p1);  // at most 2^kRaStep: no overflow, and half a step's error each, as small as the result's own
+        w[u] = T::pack2(p0, p1);  // at most 2^(kRaStep + kWeightShift): no overflow, and half a step's error each, as small as the result's own
         l = T::add2(w[u], l);     // the sum, in fp32, is of what the product weighs with
       }
       const short8v pb = __builtin_bit_cast(short8v, make_uint4(w[0], w[1], w[2], w[3]));
@@ -697,7 +720,7 @@ __global__ __launch_bounds__(kRaThreads, D == 64 ? 3 : 2) void ragged_attention_
       auto pairs = [&](auto pair_tag) __attribute__((always_inline)) {
         constexpr int pair = decltype(pair_tag)::value, begin = pair * kSlots * 3 / 64;
         if constexpr (slot == begin + 2) {
-          pw[pair] = T::pack2(e[pair & 1][0], e[pair & 1][1]);  // at most 2^kRaStep, see weigh
+          pw[pair] = T::pack2(e[pair & 1][0], e[pair & 1][1]);  // no overflow, see weigh
           asm volatile("" : "+v"(pw[pair]));                    // here, and not sunk to the MFMA that reads it
           l = T::add2(pw[pair], l);
         }
@@ -851,7 +874,7 @@ __global__ __launch_bounds__(kRaThreads, D == 64 ? 3 : 2) void ragged_attention_
 #pragma unroll
           for (int g = 0; g < 4; ++g) {
             const float v[4] = {o[dt][4 * g], o[dt][4 * g + 1], o[dt][4 * g + 2], o[dt][4 * g + 3]};
-            write_record(own + l32, 32 * dt + 8 * g + 4 * lh, v, m, l);
+            write_record(own + l32, 32 * dt + 8 * g + 4 * lh, v, reference(), l);
           }
       }
       continue;
@@ -957,7 +980,7 @@ __global__ __launch_bounds__(kRaThreads, D == 64 ? 3 : 2) void ragged_attention_
   // The four waves' results, joined: each wave takes a quarter of the columns.
   l = exchange_sum(l);
   float2* const ml = reinterpret_cast<float2*>(smem + 4 * kStepBytes + 4 * 512);
-  if (lh == 0) ml[wave * 32 + l32] = make_float2(m, l);
+  if (lh == 0) ml[wave * 32 + l32] = make_float2(reference(), l);
   {
     float4* mine = reinterpret_cast<float4*>(smem + wave * kStepBytes);
 #pragma unroll
@@ -973,8 +996,8 @@ __global__ __launch_bounds__(kRaThreads, D == 64 ? 3 : 2) void ragged_attention_
 #pragma unroll
   for (int w = 0; w < 4; ++w) {
     const float2 e = ml[w * 32 + l32];
-    weight[w] = e.x == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f((e.x - all_m) * p.scale_log2);
-    // a row without a maximum of which the sum is NaN has met NaN only
+    weight[w] = e.x == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f((e.x - all_m) * reference_unit<T>(p.scale_log2));
+    // a row without a reference point of which the sum is NaN has met NaN only
     all_l += e.x == -INFINITY ? e.y : e.y * weight[w];
   }
   const float inv = all_l == 0.0f ? 0.0f : 1.0f / all_l;
@@ -1019,9 +1042,9 @@ __global__ __launch_bounds__(kRaThreads) void ragged_join_kernel(RaParams p) {
         const float2 e = *record_sums<D>(p, kv_head, t, part, row);
         const float4 y = *reinterpret_cast<const float4*>(record_of<D>(p, kv_head, t, part, row) + column);
         const float top = fmaxf(m, e.x);
-        const float a = m == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f((m - top) * p.scale_log2);
-        const float b = e.x == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f((e.x - top) * p.scale_log2);
-        // a sum beside a maximum of -inf is zero, or NaN where NaN was all that was met
+        const float a = m == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f((m - top) * reference_unit<T>(p.scale_log2));
+        const float b = e.x == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f((e.x - top) * reference_unit<T>(p.scale_log2));
+        // a sum beside a reference of -inf is zero, or NaN where NaN was all that was met
         l = (m == -INFINITY ? l : l * a) + (e.x == -INFINITY ? e.y : e.y * b);
         v[0] = fmaf(y.x, b, v[0] * a);
         v[1] = fmaf(y.y, b, v[1] * a);
