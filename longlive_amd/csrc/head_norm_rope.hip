@@ -12,6 +12,7 @@
 //
 // Bound by memory: 2640 x (24 + 24) heads of 128 columns, 66 MB, 13.0 us, 5.1 TB/s (half of it out of the last-level cache when repeated);
 // 16381 x (40 + 8 + 8) of 64, 237 MB, 53 us, 4.4 TB/s; 24 x (16 + 4 + 4), a decoding step, 3.3 us of the GPU, 5.6 us a call.
+#include "head_norm_split.h"
 #include "ll_types16.h"
 
 namespace ll {
@@ -60,7 +61,6 @@ __device__ __forceinline__ void unpack4(uint2 w, float* f) {
   T::unpack2(w.y, f[2], f[3]);
 }
 
-constexpr int kHeadNormThreads = 256;
 // Two heads a lane once the device has waves enough: us with one / two, 1000 tokens x (32 + 8 + 8) heads 8.6 / 9.0, 2640 x (24 + 24) 14.9 / 14.1,
 // 16000 x (32 + 8 + 8) 92.9 / 72.4, 16381 x (40 + 8 + 8) of 64 columns 57.0 / 46.2 (four: 74.2 and 44.3).
 constexpr int64_t kManyWaves = 8192;
@@ -178,12 +178,11 @@ static void launch_head_norm(HeadNormParams p, int64_t tokens, hipStream_t strea
   p.units_kv = waves_for(p.rows[1].heads, LANES, HEADS);
   const uint32_t per_token = p.units_q + p.units_kv + waves_for(p.rows[2].heads, LANES, HEADS);
   p.per_token = divisor(per_token);
-  const int64_t most = (1ll << 30) / per_token;  // waves are numbered in 32 bits
+  const int64_t most = head_norm_tokens(per_token);
   for (int64_t first = 0; first < tokens; first += most) {
     p.first_token = first;
     p.tokens = (uint32_t)(tokens - first < most ? tokens - first : most);
-    const uint32_t per_wg = kHeadNormThreads / 64, groups = (p.tokens * per_token + per_wg - 1) / per_wg;
-    head_norm_rope_kernel<T, LANES, HEADS><<<groups, kHeadNormThreads, 0, stream>>>(p);
+    head_norm_rope_kernel<T, LANES, HEADS><<<head_norm_groups(p.tokens, per_token), kHeadNormThreads, 0, stream>>>(p);
   }
 }
 

@@ -9,6 +9,7 @@
 
 #include "attention_split.h"
 #include "gemm_split.h"
+#include "head_norm_split.h"
 #include "scratch_sets.h"
 
 __global__ void convert_kernel(const float* __restrict__ in, int64_t n, int mode, uint8_t* __restrict__ out) {
@@ -149,6 +150,12 @@ extern "C" void ll_test_gemm_plan(int64_t M, int64_t N, int64_t Kp, int n_produc
 // How a small product is divided: workgroups that share a tile's K range.
 extern "C" int ll_test_small_gemm_parts(int64_t M, int64_t N, int64_t Kp, int n_products, int cus) {
   return ll::plan_small_gemm(M, N, Kp, n_products, cus).parts;
+}
+
+// Tokens that a launch of ll_head_norm_rope takes at most, and its threads for so many.
+extern "C" int64_t ll_test_head_norm_tokens(uint32_t per_token) { return ll::head_norm_tokens(per_token); }
+extern "C" int64_t ll_test_head_norm_threads(int64_t tokens, uint32_t per_token) {
+  return (int64_t)ll::head_norm_groups(tokens, per_token) * ll::kHeadNormThreads;
 }
 
 // A sequence of launches on one stream through the bookkeeping of its memory (scratch_sets.h).  ops: triples (0 ordinary launch,
