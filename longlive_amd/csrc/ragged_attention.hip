@@ -225,8 +225,10 @@ __device__ __forceinline__ RaStreams load_streams(const RaParams& p, int b0, uin
     uint32_t mine = 0;
     int steps = 0;
     if (tiles) {
-      // the first tile that sees the stream's last key sees most: where there is a window, up to a tile's tokens more than it
-      const int pos1 = max(s.len - 1, s.base), pos0 = pos1 - min(s.n - 1, (int)((uint32_t)(kRaTileRows - 1) / p.group) + 1);
+      // Where there is a window, the first tile that sees the stream's last key sees most: up to a tile's tokens more than it, and without
+      // causal order, where every tile sees that key, as many more as there are tokens (for several streams: see plan_ragged).
+      const int pos1 = max(s.len - 1, s.base);
+      const int pos0 = p.causal || p.streams > 1 ? pos1 - min(s.n - 1, (int)((uint32_t)(kRaTileRows - 1) / p.group) + 1) : s.base;
       steps = p.window ? span_of(p, s.len, pos0, pos1).n_steps + 1 : (s.len + kRaKeys - 1) / kRaKeys;
     }
     if (p.part_share != 0.0f) {  // up to 64 streams, which are all here
@@ -1124,7 +1126,11 @@ static RaPlan plan_ragged(const ll_ragged_attention_args& a, int cus) {
   int64_t keys = a.max_kv_len > 0 && a.max_kv_len < all_keys ? a.max_kv_len : all_keys;
   bool alike = a.streams == 1;  // whether all tiles see about as many keys
   if (a.window > 0 && a.window < keys && a.sink_keys < keys) {
-    const int64_t seen = a.window + a.sink_keys + kRaTileRows / group + kRaKeys;
+    // Without causal order a tile sees from its window's beginning to the last key.  Of several streams only the windows count all the same:
+    // parts of the longer tiles cost more than they save, 3 of 900 to 2640 x 12 heads of 128 columns over 5000 to 13200 keys, window 1024, 117
+    // us, so cut 148; 9 of 100 to 2640 x 8 of 64, window 512, 67 and 80.  A single stream, 2640 x 4 of 128 over 13200 keys: by the window alone
+    // 48 us (1024) and 68 (64), by all that is seen 41 and 39; 1500 x 16 of 64 over 9000, window 2000, 70 and 74; 2640 x 24 of 128, 4096, 215 and 216.
+    const int64_t seen = a.window + a.sink_keys + (a.causal || a.streams > 1 ? kRaTileRows / group : longest) + kRaKeys;
     alike = alike || 2 * seen < keys;
     keys = std::min(keys, seen);
   }
