@@ -2,8 +2,9 @@
 import pytest
 import torch
 
-from longlive_amd.utils.paged_kv import head_norm_rope_paged
-from test_gpu_streams import BF16, angles
+import streams_reference as ref
+from longlive_amd.utils.paged_kv import head_norm_rope_paged, paged_attention
+from test_gpu_streams import BF16, F16, angles, batch, close
 
 pytestmark = pytest.mark.gpu
 
@@ -26,3 +27,23 @@ def test_head_norms_of_more_tokens_than_a_launch_takes(gpu):
     for n in whole:
         assert torch.equal(whole[n], pieces[n])
     assert (whole["v_pages"].flatten(0, 1)[slots[-1000:]] == v[-1000:]).all()
+
+
+@pytest.mark.parametrize("new,keys,Hq,Hk,D,dtype", [([2000, 2000], [2000, 2000], 8, 2, 128, BF16), ([4000, 300], [4000, 300], 16, 4, 64, F16),
+                                                    ([600, 2000, 50, 900], [700, 2000, 3000, 2100], 16, 4, 128, BF16)])
+def test_prompts_of_which_some_find_no_records_left(gpu, new, keys, Hq, Hk, D, dtype):
+    """Causal prompts in a cache of 4096 pages, cut by the device: the first streams are cut, the last ones stay whole for want of records (or the
+    only one to be cut does)."""
+    q, cache, table, lens, q_starts = batch(211, new, keys, Hq, Hk, D, 16, dtype)
+    held = cache["k_pages"].shape[0]
+    dev = {n: torch.cat([t, torch.full((4096 - held, *t.shape[1:]), float("nan"), dtype=dtype)]).to(gpu) for n, t in cache.items()}
+    table = table[:, :-(-max(keys) // 16)].contiguous()
+    got = paged_attention(q.to(gpu), dev, table.to(gpu), lens.to(gpu), q_starts.to(gpu), max_q_len=max(new), max_kv_len=max(keys)).cpu()
+    keys_of, _ = ref.paged_keys(cache, table, lens)
+    for b, (n, m) in enumerate(zip(new, keys)):
+        k, v = keys_of(b)
+        at = torch.cat([torch.arange(0, n, 97), torch.tensor([n - 1])])
+        seen = torch.arange(m) <= (m - n + at)[:, None]
+        for h in (0, Hq - 1):
+            want, error = ref.attend(q[int(q_starts[b]) + at, h], k[:, h * Hk // Hq], v[:, h * Hk // Hq], seen, D ** -0.5)
+            close(got[int(q_starts[b]) + at, h], want, error, f"stream {b} head {h}")

@@ -40,3 +40,23 @@ def test_a_window_without_causal_order_reaches_to_the_last_key():
     assert need(**chunk, causal=1) == 0
     assert need(**chunk, causal=0) > 0
     assert need(**{**chunk, "n_queries": 20, "max_q_len": 20}, causal=0) == 0
+
+
+def taken(new, keys, heads, kv_heads, D):
+    """Records of a kv head that the wide tiles of each of several causal streams would take where the device forms the size of a part from
+    their lengths (up to 64 streams that are not alike, in a cache with room to spare)."""
+    group, share = heads // kv_heads, 0.9 * kv_heads / (256 * (3 if D == 64 else 2))
+    tiles, steps = [-(-n * group // 128) for n in new], [-(-m // 64) for m in keys]
+    part = max(int(sum(t * max(s - n // 128, 1) for t, s, n in zip(tiles, steps, new)) * share), 10)
+    return [t * -(-s // part) * 4 if s > part else 0 for t, s in zip(tiles, steps)]
+
+
+@pytest.mark.parametrize("new,keys,heads,kv_heads,D,found", [
+    ([2000, 2000], [2000, 2000], 8, 2, 128, [True, False]), ([4000, 300], [4000, 300], 16, 4, 64, [False]), ([1500, 1900, 700], [1500, 1900, 700], 8, 2, 128, [True] * 3),
+    ([600, 2000, 50, 900], [700, 2000, 3000, 2100], 16, 4, 128, [True, True, False])])
+def test_which_streams_find_records(new, keys, heads, kv_heads, D, found):
+    """Of the streams that are to be cut, in order, those that find records for all their parts: what the GPU test of streams that find none rests on."""
+    records = need(head_dim=D, num_heads=heads, num_kv_heads=kv_heads, streams=len(new), n_queries=sum(new), max_q_len=max(new), max_kv_len=max(keys), page_size=16,
+                   table_width=-(-max(keys) // 16), n_pages=4096, causal=1) // (kv_heads * 32 * (D + 2) * 4)
+    want = taken(new, keys, heads, kv_heads, D)
+    assert [sum(want[:i + 1]) <= records for i, w in enumerate(want) if w] == found
