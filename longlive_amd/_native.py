@@ -1166,7 +1166,7 @@ def ragged_attention(what, q, q_starts, softmax_scale, max_q_len, max_kv_len, ou
                      window=None, sink_tokens=0, k=None, v=None, k_starts=None, k_lens=None, key_mask=None):
     """The queries q [T, H, D] of several streams over the keys of a paged ``cache`` or over rows of k and v [n, Hk, D]
     (``ll_ragged_attention``)."""
-    if q.is_cuda and (window is None or window):
+    if q.is_cuda and q.ndim == 3 and q.shape[2] and (window is None or window):
         keys = (k, v) if cache is None else (cache["k_pages"], cache["v_pages"])
         done = host().ragged_attention(q, q_starts, q.shape[-1] ** -0.5 if softmax_scale is None else float(softmax_scale), max_q_len or 0, max_kv_len or 0,
                                        out, *keys, page_table, kv_lens, bool(causal), window or 0, sink_tokens, k_starts, k_lens, key_mask)

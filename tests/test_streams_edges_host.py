@@ -6,6 +6,8 @@ import pytest
 import torch
 
 from longlive_amd import _native
+from longlive_amd.utils.cross_attention import ragged_cross_attention
+from longlive_amd.utils.paged_kv import initialize_paged_kv_cache, paged_attention
 
 
 @pytest.fixture(scope="module")
@@ -60,3 +62,28 @@ def test_which_streams_find_records(new, keys, heads, kv_heads, D, found):
                    table_width=-(-max(keys) // 16), n_pages=4096, causal=1) // (kv_heads * 32 * (D + 2) * 4)
     want = taken(new, keys, heads, kv_heads, D)
     assert [sum(want[:i + 1]) <= records for i, w in enumerate(want) if w] == found
+
+
+class OnGpu(torch.Tensor):
+    """A tensor that says it is on the GPU, so that calls take the way that they take there."""
+    is_cuda = True
+
+
+@pytest.fixture
+def no_gpu_needed(monkeypatch):
+    """The checks of the Python layer with the check of the device taken out, a native host path that takes nothing, and a library that must
+    not be reached."""
+    monkeypatch.setattr(_native, "_require_cuda", lambda *t: None)
+    monkeypatch.setattr(_native, "host", lambda: _native._NoHostPath())
+    monkeypatch.setattr(_native, "load", lambda: pytest.fail("the call was not refused"))
+
+
+@pytest.mark.parametrize("shape", [(), (64,), (3, 4, 0), (3, 0, 0), (3, 4, 64, 1)])
+def test_queries_without_columns_or_dimensions_are_refused(no_gpu_needed, shape):
+    q, i32 = torch.zeros(shape, dtype=torch.bfloat16).as_subclass(OnGpu), lambda *s: torch.zeros(s, dtype=torch.int32)
+    cache = initialize_paged_kv_cache(1, 4, 16, 2, 64, "cpu")[0]
+    k = torch.zeros(9, 2, 64, dtype=torch.bfloat16)
+    with pytest.raises(ValueError):
+        paged_attention(q, cache, i32(2, 5), i32(2), i32(3))
+    with pytest.raises(ValueError):
+        ragged_cross_attention(q, k, k, i32(3), i32(3))
