@@ -1194,7 +1194,7 @@ def ragged_attention(what, q, q_starts, softmax_scale, max_q_len, max_kv_len, ou
     if cache is not None:
         k, v = pages
         _check_index(what, "kv_lens", kv_lens, torch.int32, (streams,))
-        if page_table.dtype != torch.int32 or page_table.ndim != 2 or page_table.shape[0] != streams or (page_table.numel() and page_table.stride(1) != 1):
+        if page_table.dtype != torch.int32 or page_table.ndim != 2 or page_table.shape[0] != streams or (page_table.numel() and page_table.shape[1] > 1 and page_table.stride(1) != 1):
             raise ValueError(f"{what}: page_table must be int32 [{streams}, pages of the longest stream] with contiguous rows")
         a.page_table, a.table_stride, a.table_width = page_table.data_ptr(), _stride(page_table, 0), page_table.shape[1]
         a.n_pages, a.page_size, a.kv_lens, a.causal = k.shape[0], k.shape[1], kv_lens.data_ptr(), int(bool(causal))

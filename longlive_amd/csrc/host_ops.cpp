@@ -1070,7 +1070,7 @@ PyObject* py_ragged_attention(PyObject*, PyObject* const* args, Py_ssize_t n) {
     const Tensor* table = plain(args[8]) ? &THPVariable_Unpack(args[8]) : nullptr;
     const Tensor* lens = as_list(args[9], dev, at::kInt, a.streams);
     if (!table || !lens || !on_device(*table, dev) || table->scalar_type() != at::kInt || table->dim() != 2 || table->size(0) != a.streams ||
-        table->numel() == 0 || table->stride(1) != 1)
+        table->numel() == 0 || (table->size(1) > 1 && table->stride(1) != 1))
       Py_RETURN_NONE;
     a.page_table = table->data_ptr<int32_t>();
     a.table_stride = table->stride(0);

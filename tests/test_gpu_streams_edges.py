@@ -47,3 +47,23 @@ def test_prompts_of_which_some_find_no_records_left(gpu, new, keys, Hq, Hk, D, d
         for h in (0, Hq - 1):
             want, error = ref.attend(q[int(q_starts[b]) + at, h], k[:, h * Hk // Hq], v[:, h * Hk // Hq], seen, D ** -0.5)
             close(got[int(q_starts[b]) + at, h], want, error, f"stream {b} head {h}")
+
+
+@pytest.mark.parametrize("native", [True, False])
+def test_a_page_table_of_one_column_with_any_stride(gpu, native, monkeypatch):
+    from longlive_amd import _native
+
+    if not native:
+        monkeypatch.setattr(_native, "_host", _native._NoHostPath())
+    q, cache, table, lens, q_starts = batch(221, [3, 1], [14, 16], 4, 2, 64, 16, BF16)
+    cache = {n: t.to(gpu) for n, t in cache.items()}
+    rest = (lens.to(gpu), q_starts.to(gpu))
+    want = paged_attention(q.to(gpu), cache, table[:, :1].contiguous().to(gpu), *rest)
+    wide = torch.full((2, 5, 3), 1 << 30, dtype=torch.int32)
+    wide[:, 2, 1] = table[:, 0]
+    wide = wide.to(gpu)[:, 2:3, 1]
+    assert wide.shape == (2, 1) and wide.stride() == (15, 3)
+    assert torch.equal(paged_attention(q.to(gpu), cache, wide, *rest), want)
+    for bad in (table[:, :1].to(gpu).expand(2, 2), table[:, :2].to(gpu).T):   # columns that are taken lie one behind the other
+        with pytest.raises(ValueError, match="page_table"):
+            paged_attention(q.to(gpu), cache, bad, *rest)

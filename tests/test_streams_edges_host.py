@@ -87,3 +87,22 @@ def test_queries_without_columns_or_dimensions_are_refused(no_gpu_needed, shape)
         paged_attention(q, cache, i32(2, 5), i32(2), i32(3))
     with pytest.raises(ValueError):
         ragged_cross_attention(q, k, k, i32(3), i32(3))
+
+
+def test_a_page_table_of_one_column_may_have_any_stride(no_gpu_needed, monkeypatch):
+    class Reached(Exception):
+        pass
+
+    def load():
+        raise Reached
+
+    q, i32 = torch.zeros(3, 4, 64, dtype=torch.bfloat16), lambda *s: torch.zeros(s, dtype=torch.int32)
+    cache = initialize_paged_kv_cache(1, 4, 16, 2, 64, "cpu")[0]
+    for bad in (i32(5, 2).T, i32(2, 1).expand(2, 5)):
+        with pytest.raises(ValueError, match="page_table"):
+            paged_attention(q, cache, bad, i32(2), i32(3))
+    monkeypatch.setattr(_native, "load", load)
+    monkeypatch.setattr(torch.cuda, "device", lambda d: torch.no_grad())
+    for good in (i32(2, 1), i32(2, 5, 3)[:, 2:3, 1], i32(2, 5)):
+        with pytest.raises(Reached):
+            paged_attention(q, cache, good, i32(2), i32(3))
