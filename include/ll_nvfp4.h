@@ -610,7 +610,8 @@ int ll_head_norm_rope(int dtype, int64_t tokens, int head_dim, const ll_head_row
  *     byte a row, or NULL) leaves out keys whose byte is zero.  Every row sees all of them; causal and window are 0.
  * A key has no part in a row that does not see it, whatever lies in its K and V, NaN included (unfilled rows of a page, masked
  * states, later tokens); what a row does see follows IEEE arithmetic.  The probabilities are rounded to dtype (in f16 those down to 2^-37
- * of a row's largest count), the sums are fp32.
+ * of a row's largest count), the sums are fp32.  Scores times softmax_scale lie within +-2^27 in f16 and +-2^30 in bf16: beyond, what their
+ * rounding leaves may be NaN.  A row whose scores are all -infinity gets zeros.
  * Rows of k and v lie less than 2^26 elements apart, pages up to 2^32.
  * max_q_len, max_kv_len: the longest stream's new tokens and keys as far as the host knows them, by which the launch is divided;
  * right for any value, fast for true ones.  workspace: ll_ragged_attention_workspace bytes, 16-byte aligned, used by this launch

@@ -71,7 +71,7 @@ def paged_attention(q: torch.Tensor, cache: dict, page_table: torch.Tensor, kv_l
     sits at position ``p = kv_lens[b] - n + i`` and sees key j where ``j <= p`` (``causal``; else every key: a chunk whose tokens see
     one another) and, with a ``window``, ``j > p - window or j < sink_tokens``.  Keys in holes of the page table and behind its
     width do not exist, but count for the positions.  A token that sees no key gets zeros.  Scores, softmax statistics and sums are fp32; the probabilities enter the
-    second product in q's type.
+    second product in q's type.  Scores times the scale lie within 2^27 (float16) or 2^30 (bfloat16) of zero.
 
     ``max_q_len`` / ``max_kv_len``: the longest stream's new tokens and keys, if the caller knows them; any value gives the right result,
     true ones a division of the work that fits.  Returns ``out`` [T, H, D]: rows outside every stream are zeros in a new tensor and

@@ -3,8 +3,9 @@ import pytest
 import torch
 
 import streams_reference as ref
+from longlive_amd.utils.cross_attention import ragged_cross_attention
 from longlive_amd.utils.paged_kv import head_norm_rope_paged, paged_attention
-from test_gpu_streams import BF16, F16, angles, batch, close
+from test_gpu_streams import BF16, F16, angles, batch, close, starts
 
 pytestmark = pytest.mark.gpu
 
@@ -67,3 +68,30 @@ def test_a_page_table_of_one_column_with_any_stride(gpu, native, monkeypatch):
     for bad in (table[:, :1].to(gpu).expand(2, 2), table[:, :2].to(gpu).T):   # columns that are taken lie one behind the other
         with pytest.raises(ValueError, match="page_table"):
             paged_attention(q.to(gpu), cache, bad, *rest)
+
+
+@pytest.mark.parametrize("n", [2, 80])
+@pytest.mark.parametrize("dtype,size", [(F16, 2.0 ** 27), (BF16, 2.0 ** 27), (BF16, 2.0 ** 30)])
+def test_scores_as_large_as_may_be(gpu, dtype, size, n):
+    """Scores whose steps are many powers of two, of both signs: the largest alone has a weight."""
+    m, D = 100, 64
+    q, k = torch.zeros(n, D, dtype=dtype), torch.zeros(m, D, dtype=dtype)
+    q[:, 0], k[:, 0] = size ** 0.5 * 0.999, torch.linspace(-1, 0.9, m) * size ** 0.5
+    v = torch.randn(m, D, generator=torch.Generator().manual_seed(2)).to(dtype)
+    for sign in (1, -1):
+        got = ragged_cross_attention(sign * q[:, None].to(gpu), k[:, None].to(gpu), v[:, None].to(gpu), starts([n]).to(gpu), starts([m]).to(gpu), softmax_scale=1.0)
+        assert torch.equal(got[:, 0].cpu(), v[m - 1 if sign > 0 else 0].expand(n, D))
+
+
+@pytest.mark.parametrize("n", [2, 80])
+@pytest.mark.parametrize("dtype", [F16, BF16])
+def test_rows_whose_scores_are_all_minus_infinity_are_zeros(gpu, dtype, n):
+    m, D = 300, 64
+    q, k = torch.zeros(n, 1, D, dtype=dtype), torch.zeros(m, 1, D, dtype=dtype)
+    q[:, 0, 0], k[:, 0, 0] = 1.0, -float("inf")
+    v = torch.ones(m, 1, D, dtype=dtype)
+    got = ragged_cross_attention(q.to(gpu), k.to(gpu), v.to(gpu), starts([n]).to(gpu), starts([m]).to(gpu))
+    assert (got == 0).all()
+    k[m - 1] = 0.0   # one key that counts
+    got = ragged_cross_attention(q.to(gpu), k.to(gpu), v.to(gpu), starts([n]).to(gpu), starts([m]).to(gpu))
+    assert (got == 1).all()
