@@ -25,10 +25,13 @@
 //
 // What bounds it (bf16, 128 columns; the card's own copy of 2 GiB runs at 4.9 TB/s, the library's 8192^3 product at 1219 TFLOP/s):
 // single tokens of 32 streams over 500 to 16384 keys take 102 to 108 us, 4.6 to 4.9 TB/s of K and V; 2640 x 24 heads over 13200 keys
-// take 430 to 440 us, 0.97 to 1.0 PFLOP/s, where the matrix unit is busy for half of the cycles, 6.7 vector instructions go with each of
-// its instructions and the clock is down at 2.0 GHz.  With fewer steps per item its beginning shows (places, then keys, then the first
-// scores, one behind the other, some 5 us beside the other workgroup of the unit): 532 x 40 heads over 9000 keys 0.77 PFLOP/s, 3 x
-// 2640 x 24 over 60 to 512 encoder states 43 us, 0.56 PFLOP/s.
+// take 424 to 442 us, 0.97 to 1.0 PFLOP/s, where the matrix unit is busy for half of the cycles, 6.1 other vector instructions go with each
+// of its instructions and the clock is down at 2.0 GHz.  Over the same keys as rows one behind the other it is 388, next to 380 of the dense
+// kernel (ll_attention_bf16): a tenth goes into where pages lie.  With fewer steps per item its beginning shows (places, then keys, then
+// the first scores, one behind the other, some 5 us beside the other workgroup of the unit): 532 x 40 / 8 heads over 9000 keys 118 us, 0.81
+// PFLOP/s, 3 x 2640 x 24 over 60 to 512 encoder states 43 us, 0.56 PFLOP/s.
+// Registers: with 64 columns three workgroups of a unit leave 168 a lane, of which 4 to 8 more would be needed (20 to 36 bytes of scratch
+// memory); with 128 columns 230 to 246 and none.  41 to 82 scalars are kept in lanes of vector registers.
 #include "ll_types16.h"
 
 #include <algorithm>
@@ -326,8 +329,8 @@ __device__ __forceinline__ void each_index(F& f, std::integer_sequence<int, I...
 
 // The reference point of the exponentials follows the maximum once it is 2^2 ahead: fewer rescalings, no further from 64 bits.
 constexpr float kRaStep = 2.0f;
-// Probabilities are exp2(score - reference + shift), so that in f16 a row's sums keep many keys that are each far below the largest (at a
-// reference of 1, of 200000 keys 17.5 nats below one not a single one).  Sums and outputs of a row are all times 2^shift.  None where the
+// Probabilities are exp2(score - reference + shift), so that in f16 a row's sums keep keys that are far below the largest: with none, 200000 keys
+// 17.5 nats below one, half a percent of the weight, would each weigh nothing.  Sums and outputs of a row are all times 2^shift.  None where the
 // reference, scaled, has no bits left for it: its rounding, the same for all keys of a row, would carry the largest beyond f16.
 template <typename T>
 __device__ __forceinline__ float weight_shift(float reference) {
@@ -451,8 +454,8 @@ __global__ __launch_bounds__(kRaThreads, D == 64 ? 3 : 2) void ragged_attention_
   const uint32_t k_row = (uint32_t)(lane / kPieces) * p.k_stride_row * 2, v_row = (uint32_t)(lane / kPieces) * p.v_stride_row * 2;
   auto turn = [](bool values, int i) { return (values ? v_piece<D>(i * kRowsPerLoad, 0) : k_piece<D>(i * kRowsPerLoad, 0)) * 16; };
   typedef __attribute__((address_space(3))) u32x4* lds_uint4;
-  // 16 rows from a multiple of 16 on lie one behind the other, and take one address for a wave in place of one for a lane: 532 x 40 heads
-  // over 9000 keys in pages of 32 rows 124 us, of 24 rows 148.
+  // 16 rows from a multiple of 16 on lie one behind the other, and take one address for a wave in place of one for a lane: 532 x 40 / 8 heads
+  // over 9000 keys in pages of 32 rows 118 us, of 24 rows 143.
   const bool whole_pages = KIND == kRaPaged && p.page.d % 16 == 0;
   // counted: as many loads whatever keys there are, for waits that leave some under way.
   auto load_rows = [&](bool values, int r0, uint32_t lds, bool counted) __attribute__((always_inline)) {
@@ -1097,7 +1100,8 @@ static int check_ragged(const ll_ragged_attention_args* a) {
 // Where tiles are alike, the number of parts follows from their cost, in sixteenths of a step of a full unit: steps are faster by themselves
 // (kRaStepCost), an item's beginning and a record are paid for by the share of the device that they keep busy.  us by steps of a part, one
 // stream of 100 x 32 / 8 heads of 128 columns over 1000 keys: 3 22.6, 4 23.2, 6 23.7, 8 27.6, whole 30.9 (the rule: 4); over 4000: 6 37.9, 8
-// 31.8, 10 33.9, 16 38.8 (8); 500 x 12 heads of 64 over 9500: 10 47.4, 16 44.3, 24 53.1 (15); 532 x 40 / 8 over 9000: 20 170, 47 143 (47).
+// 31.8, 10 33.9, 16 38.8 (8); 500 x 12 heads of 64 over 9500: 10 47.4, 16 44.3, 24 53.1 (15); 532 x 40 / 8 over 9000 in pages of 24: 20 170, 47
+// 143 (47).
 struct RaPlan {
   uint32_t groups, part_steps, narrow_part_steps, records;
   size_t bytes;
@@ -1110,7 +1114,8 @@ constexpr int64_t kRaLeastNarrowSteps = 8, kRaMostNarrowSteps = 16, kRaMostWhole
 // Of what a workgroup has to do in all, a part: by the device, of up to 64 streams, where the launch is not so long that the last items do not
 // count.  us with 0.5 / 0.75 / 0.9 / 1.1 / by the host's guess, pages for eight times the streams' keys: 12 streams of 1 to 700 tokens x 40 / 8
 // heads over 300 to 9000 keys 207 / 216 / 204 / 199 / 274; 16 of 5 to 600 x 24 over 600 to 4600 173 / 176 / 173 / 173 / 196; 30 of 1 to 300 x
-// 32 / 8 over 300 to 4000 97 / 99 / 89 / 96 / 100; prompts of 5 times 100 to 2000 x 16 / 4, causal, 82 / 101 / 84 / 83 / 74 (there whole).
+// 32 / 8 over 300 to 4000 97 / 99 / 89 / 96 / 100; prompts of 5 times 100 to 2000 x 16 / 4, causal, 82 / 101 / 84 / 83 / 74 (there whole; 74
+// also with 0.9 and the records that the plan has for them).
 constexpr float kRaShare = 0.9f;
 constexpr int64_t kRaNarrowJoin = 7;                                // of the second launch behind narrow tiles, in their steps
 constexpr size_t kRaMostBytes = (size_t)256 << 20;  // of records

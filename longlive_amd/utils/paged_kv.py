@@ -58,7 +58,9 @@ def head_norm_rope_paged(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cach
                          positions: torch.Tensor | None = None, interleaved: bool = True, out: torch.Tensor | None = None) -> torch.Tensor:
     """:func:`longlive_amd.utils.rope.head_norm_rope` of q and k whose K, with the V beside it, goes to the cache in the same launch:
     rows ``slots`` (int64 [T], :func:`paged_slots`) of ``k_pages`` / ``v_pages``; a slot outside the cache (-1) is written nowhere,
-    and two tokens must not have one slot.  Returns the rotated q, in ``out`` if given."""
+    and two tokens must not have one slot.  Returns the rotated q, in ``out`` if given, which may be q itself.
+
+    Pages of any head_dim that the norm takes are written (multiples of 8 up to 256); :func:`paged_attention` reads 64 and 128."""
     return _native.head_norm_rope(q, k, v, q_weight, k_weight, eps, cos_f32, sin_f32, positions, interleaved, cache, slots, out)
 
 
