@@ -599,6 +599,63 @@ int ll_head_norm_rope(int dtype, int64_t tokens, int head_dim, const ll_head_row
                       int interleaved, const int64_t* slots, int64_t n_slots, void* stream);
 
 /*
+ * ll_rotate_by_position: ll_head_norm_rope with angles that the launch forms from positions of any size: pair j of row t turns by
+ * angle = x * frequencies[j] radians, formed in 64 bits, and cosine and sine are multiplied by amplitude.  x is the row's position p =
+ * positions[t] (t without positions, negative ones turn the other way), or with a grid of grid_rows x grid_columns tokens to a video frame
+ * the frame p / (rows * columns), rounded down, for the first frame_pairs pairs, the row in it for row_pairs more and the column for the
+ * rest.  Every row is rotated.  With frequencies up to 1, positions below 2^31 in
+ * magnitude lose 2^-20 radians at most; 2^53 is the end.
+ */
+typedef struct ll_position_angles {
+  const double* frequencies; /* f64 [rotary_dim / 2], radians per position, 16-byte aligned */
+  int rotary_dim;            /* as in ll_head_norm_rope */
+  float amplitude;
+  int64_t grid_rows, grid_columns; /* 0 and 0: positions on a line; else their product is below 2^31 */
+  int frame_pairs, row_pairs;
+} ll_position_angles;
+int ll_rotate_by_position(int dtype, int64_t tokens, int head_dim, const ll_head_rows* q, const ll_head_rows* k, const ll_head_rows* v,
+                          float eps, const ll_position_angles* angles, const int64_t* positions, int interleaved, const int64_t* slots,
+                          int64_t n_slots, void* stream);
+
+/*
+ * ll_step_layout: what the kernels of a step read, from the lengths of its streams, in one launch (two where lengths are replaced and there are
+ * many tokens).  With m[b] = max(kv_lens[b], 0) keys held and n[b] = max(new_lens[b], 0) new tokens of stream b:
+ *   q_starts[b] = n[0] + .. + n[b - 1], kv_lens_out[b] = m[b] + n[b].  Tokens for which `tokens` has no row left, and those that would bring a
+ *     stream beyond 2^31 - 1 keys, are not laid out: n[b] is that much smaller.
+ *   page_table: a stream's pages are entries 0 .. ceil(m[b] / page_size) - 1 of its row; those up to ceil((m[b] + n[b]) / page_size) - 1 that
+ *     the table is wide enough for are written, with the pages free_pages[c], [c + 1], .. in order of streams and entries, c = *cursor (0 below 0, or
+ *     without a cursor); -1 where the list has come to its end.  pages_wanted: how many were to be written.  *cursor moves on by as many,
+ *     to n_free at most.
+ *   positions[t] = m[b] + i of the i-th token of stream b, row t, and with groups the length of its group's shared beginning more;
+ *     slots[t] = page * page_size + (m[b] + i) % page_size, or -1 where its entry is negative or behind the table.
+ *     Rows behind the last stream's get 0 and -1.
+ *   groups: group g is the streams group_starts[g] .. group_starts[g + 1] - 1 (one group may go without, all streams then), and shares
+ *     prefix_lens[g] keys (0 below 0) that are not in its streams' tables; starts do not decrease.  Streams outside every group share none.
+ * kv_lens_out may be kv_lens; apart from that outputs must not overlap inputs or each other.  workspace: ll_step_layout_workspace bytes, 4-byte
+ * aligned, used by this call alone while it runs (NULL where that is 0).
+ */
+typedef struct ll_step_layout_args {
+  int64_t streams;            /* below 2^31, like all sizes here */
+  const int32_t *new_lens, *kv_lens; /* [streams] */
+  int32_t* page_table;        /* [streams, table_width], rows table_stride apart */
+  int64_t table_stride, table_width;
+  int page_size;
+  const int32_t* free_pages;  /* [n_free] */
+  int64_t n_free;
+  int32_t* cursor;            /* [1] or NULL */
+  int64_t groups;             /* 0: none */
+  const int32_t *group_starts, *prefix_lens; /* [groups + 1] or NULL with one group, [groups] */
+  int64_t tokens;
+  int32_t *q_starts, *kv_lens_out; /* [streams + 1], [streams] */
+  int64_t *positions, *slots; /* [tokens] */
+  int32_t* pages_wanted;      /* [1] */
+  void* workspace;
+  size_t workspace_bytes;
+} ll_step_layout_args;
+int ll_step_layout_workspace(const ll_step_layout_args* args, size_t* bytes);
+int ll_step_layout(const ll_step_layout_args* args, void* stream);
+
+/*
  * ll_ragged_attention: out[t, h] = sum_j w_j v_j / sum_j w_j,  w_j = exp(softmax_scale * (q[t, h] . k_j - max)), over the keys
  * of t's stream that t may see; zeros for a row that sees none.  Head h reads kv head h / (num_heads / num_kv_heads).  Rows of q
  * outside every stream get zeros (clear_rest) or stay as they are.  Keys:
@@ -648,6 +705,26 @@ typedef struct ll_ragged_attention_args {
  * `compute_units` (host arithmetic only), or, if 0, on the current device. */
 int ll_ragged_attention_workspace(const ll_ragged_attention_args* args, int compute_units, size_t* bytes);
 int ll_ragged_attention(const ll_ragged_attention_args* args, void* stream);
+
+/*
+ * ll_shared_prefix_attention: ll_ragged_attention over pages for streams in groups that share a beginning, whose keys are read once for all rows of
+ * a group where that is cheaper.  Group g is the streams group_starts[g] .. group_starts[g + 1] - 1 (starts do not decrease; a single group may go
+ * without, all streams then; streams outside every group share nothing), and its first prefix_lens[g] keys lie in the pages of row g of
+ * prefix_table.  Every row of a group's streams sees them all; behind them come the stream's own keys, row b of page_table and kv_lens[b] as in
+ * ll_ragged_attention, positions counted from the first of them, with the causal order if `own.causal`.  Holes, rows that see no key, what is not
+ * finite, types, workspace and aliasing as there.  own.page_table is needed (or table_width 0: no own keys); own.window and own.sink_keys are 0;
+ * tables reach at most 2^30 keys.  own.max_kv_len is the longest stream's own keys, max_prefix_len the longest beginning.
+ */
+typedef struct ll_shared_prefix_args {
+  ll_ragged_attention_args own;
+  int64_t groups;                              /* 0: nothing is shared */
+  const int32_t *group_starts, *prefix_lens;   /* [groups + 1] or NULL with one group, [groups] */
+  const int32_t* prefix_table;                 /* [groups, prefix_width], rows prefix_stride apart */
+  int64_t prefix_stride, prefix_width;
+  int64_t max_prefix_len;
+} ll_shared_prefix_args;
+int ll_shared_prefix_attention_workspace(const ll_shared_prefix_args* args, int compute_units, size_t* bytes);
+int ll_shared_prefix_attention(const ll_shared_prefix_args* args, void* stream);
 
 #ifdef __cplusplus
 }

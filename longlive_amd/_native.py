@@ -117,6 +117,12 @@ _SIGNATURES = {
     "ll_kv_attention_release": (c_int, [c_void_p]),
     "ll_head_norm_rope": (c_int, [c_int, c_int64, c_int, c_void_p, c_void_p, c_void_p, c_float, c_void_p, c_void_p, c_int64, c_int, c_void_p,
                                   c_int, c_void_p, c_int64, c_void_p]),
+    "ll_rotate_by_position": (c_int, [c_int, c_int64, c_int, c_void_p, c_void_p, c_void_p, c_float, c_void_p, c_void_p, c_int, c_void_p, c_int64,
+                                      c_void_p]),
+    "ll_step_layout": (c_int, [c_void_p, c_void_p]),
+    "ll_step_layout_workspace": (c_int, [c_void_p, c_void_p]),
+    "ll_shared_prefix_attention": (c_int, [c_void_p, c_void_p]),
+    "ll_shared_prefix_attention_workspace": (c_int, [c_void_p, c_int, c_void_p]),
     "ll_ragged_attention": (c_int, [c_void_p, c_void_p]),
     "ll_ragged_attention_workspace": (c_int, [c_void_p, c_int, c_void_p]),
     "ll_nvfp4_quantize_noalloc_max_elements": (c_int64, []),
@@ -1021,6 +1027,26 @@ class RaggedAttentionStruct(ctypes.Structure):
                 ("max_q_len", c_int64), ("max_kv_len", c_int64), ("workspace", c_void_p), ("workspace_bytes", c_size_t)]
 
 
+class SharedPrefixStruct(ctypes.Structure):
+    """struct ll_shared_prefix_args of include/ll_nvfp4.h."""
+    _fields_ = [("own", RaggedAttentionStruct), ("groups", c_int64), ("group_starts", c_void_p), ("prefix_lens", c_void_p), ("prefix_table", c_void_p),
+                ("prefix_stride", c_int64), ("prefix_width", c_int64), ("max_prefix_len", c_int64)]
+
+
+class PositionAnglesStruct(ctypes.Structure):
+    """struct ll_position_angles of include/ll_nvfp4.h."""
+    _fields_ = [("frequencies", c_void_p), ("rotary_dim", c_int), ("amplitude", c_float), ("grid_rows", c_int64), ("grid_columns", c_int64),
+                ("frame_pairs", c_int), ("row_pairs", c_int)]
+
+
+class StepLayoutStruct(ctypes.Structure):
+    """struct ll_step_layout_args of include/ll_nvfp4.h."""
+    _fields_ = [("streams", c_int64), ("new_lens", c_void_p), ("kv_lens", c_void_p), ("page_table", c_void_p), ("table_stride", c_int64),
+                ("table_width", c_int64), ("page_size", c_int), ("free_pages", c_void_p), ("n_free", c_int64), ("cursor", c_void_p), ("groups", c_int64),
+                ("group_starts", c_void_p), ("prefix_lens", c_void_p), ("tokens", c_int64), ("q_starts", c_void_p), ("kv_lens_out", c_void_p),
+                ("positions", c_void_p), ("slots", c_void_p), ("pages_wanted", c_void_p), ("workspace", c_void_p), ("workspace_bytes", c_size_t)]
+
+
 def _one_device(what: str, *tensors) -> None:
     """All of them on the GPU, and on the same one."""
     _require_cuda(*tensors)
@@ -1090,6 +1116,51 @@ def _head_rows(x, weight, out, out_strides) -> HeadRowsStruct:
                           int(weight is not None and weight.dtype == torch.float32), out.data_ptr(), *out_strides)
 
 
+def _head_norm_rows(what, q, k, v, q_weight, k_weight, positions, cache, slots, q_out):
+    """What the kernels that norm and rotate heads take, checked: (q, k and v rows, q and k results (k None for pages), slots, and what has to
+    live until the launch)."""
+    paged = cache is not None
+    pages = check_pages(what, cache) if paged else ()
+    T, Hq, D = (*q.shape, 0, 0, 0)[:3]
+    for name, t in (("q", q), ("k", k)) + ((("v", v),) if paged else ()):
+        _check_rows(what, name, t, q.dtype)
+        if t.shape[0] != T or t.shape[2] != D or (name == "v" and t.shape != k.shape):
+            raise ValueError(f"{what}: q, k and v must have as many rows, one head_dim, and k and v as many heads; got {tuple(t.shape)} for {name} "
+                             f"beside q {tuple(q.shape)}, k {tuple(k.shape)}")
+    if D % 8 or not 8 <= D <= 256:
+        raise ValueError(f"{what}: head_dim {D} is not a multiple of 8 up to 256")
+    for name, w in (("q_weight", q_weight), ("k_weight", k_weight)):
+        if w is not None and (w.shape != (D,) or w.dtype not in (q.dtype, torch.float32)):
+            raise ValueError(f"{what}: {name} must be [{D}] in {q.dtype} or float32")
+    if positions is not None:
+        _check_index(what, "positions", positions, torch.int64, (T,))
+    q, k = (t if _rows16(t) else t.contiguous().clone() for t in (q, k))
+    q_weight, k_weight = (w if w is None or (w.is_contiguous() and w.data_ptr() % 16 == 0) else w.contiguous().clone() for w in (q_weight, k_weight))
+    if q_out is None:
+        q_out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+    else:
+        _check_out(what, q_out, q)
+    v_rows, n_slots, k_out = None, 0, None
+    if paged:
+        k_pages, v_pages = pages
+        if k_pages.shape[2:] != k.shape[1:] or k_pages.dtype != q.dtype:
+            raise ValueError(f"{what}: pages of {k_pages.dtype} {tuple(k_pages.shape[2:])} do not take rows of {q.dtype} {tuple(k.shape[1:])}")
+        if any(t.numel() and (_page_rows(t) is None or not _apart(t)) for t in pages):
+            raise ValueError(f"{what}: pages must lie one behind the other, each row in a place of its own")
+        _check_index(what, "slots", slots, torch.int64, (T,))
+        v = v if _rows16(v) else v.contiguous().clone()
+        n_slots = k_pages.shape[0] * k_pages.shape[1]
+        k_rows = _head_rows(k, k_weight, k_pages, (_page_rows(k_pages), _stride(k_pages, 2)))
+        v_rows = _head_rows(v, None, v_pages, (_page_rows(v_pages), _stride(v_pages, 2)))
+    else:
+        k_out = torch.empty(k.shape, dtype=k.dtype, device=k.device)
+        k_rows = _head_rows(k, k_weight, k_out, (_stride(k_out, 0), _stride(k_out, 1)))
+    q_rows = _head_rows(q, q_weight, q_out, (_stride(q_out, 0), _stride(q_out, 1)))
+    if n_slots == 0 and paged:   # a cache without pages: nothing to write to
+        k_rows.num_heads, v_rows = 0, None
+    return q_rows, k_rows, v_rows, q_out, k_out, n_slots, (q, k, v, q_weight, k_weight)
+
+
 def head_norm_rope(q, k, v, q_weight, k_weight, eps, cos, sin, positions, interleaved, cache=None, slots=None, q_out=None):
     """q [T, Hq, D], k [T, Hk, D] through a norm per head and the rotation: (q, k) in fresh tensors, or with a paged ``cache`` q alone, k
     and v [T, Hk, D] then going to the cache's rows ``slots``."""
@@ -1102,19 +1173,9 @@ def head_norm_rope(q, k, v, q_weight, k_weight, eps, cos, sin, positions, interl
             return done
     pages = check_pages(what, cache) if paged else ()
     _one_device(what, q, k, v, q_weight, k_weight, cos, sin, positions, slots, q_out, *pages)
-    T, Hq, D = (*q.shape, 0, 0, 0)[:3]
-    for name, t in (("q", q), ("k", k)) + ((("v", v),) if paged else ()):
-        _check_rows(what, name, t, q.dtype)
-        if t.shape[0] != T or t.shape[2] != D or (name == "v" and t.shape != k.shape):
-            raise ValueError(f"{what}: q, k and v must have as many rows, one head_dim, and k and v as many heads; got {tuple(t.shape)} for {name} "
-                             f"beside q {tuple(q.shape)}, k {tuple(k.shape)}")
-    if D % 8 or not 8 <= D <= 256:
-        raise ValueError(f"{what}: head_dim {D} is not a multiple of 8 up to 256")
-    for name, w in (("q_weight", q_weight), ("k_weight", k_weight)):
-        if w is not None and (w.shape != (D,) or w.dtype not in (q.dtype, torch.float32)):
-            raise ValueError(f"{what}: {name} must be [{D}] in {q.dtype} or float32")
     if (cos is None) != (sin is None):
         raise ValueError(f"{what}: cos and sin go together")
+    D = q.shape[-1] if q.ndim else 0
     R, table = 0, 0
     if cos is not None:
         if cos.ndim != 2 or cos.shape != sin.shape or cos.dtype != torch.float32 or sin.dtype != torch.float32:
@@ -1125,55 +1186,137 @@ def head_norm_rope(q, k, v, q_weight, k_weight, eps, cos, sin, positions, interl
         cos, sin = cos.contiguous(), sin.contiguous()
         if cos.data_ptr() % 16 or sin.data_ptr() % 16:
             cos, sin = cos.clone(), sin.clone()
-    if positions is not None:
-        _check_index(what, "positions", positions, torch.int64, (T,))
-    q, k = (t if _rows16(t) else t.contiguous().clone() for t in (q, k))
-    q_weight, k_weight = (w if w is None or (w.is_contiguous() and w.data_ptr() % 16 == 0) else w.contiguous().clone() for w in (q_weight, k_weight))
-    if q_out is None:
-        q_out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
-    else:
-        _check_out(what, q_out, q)
-    v_rows, n_slots = None, 0
-    if paged:
-        k_pages, v_pages = pages
-        if k_pages.shape[2:] != k.shape[1:] or k_pages.dtype != q.dtype:
-            raise ValueError(f"{what}: pages of {k_pages.dtype} {tuple(k_pages.shape[2:])} do not take rows of {q.dtype} {tuple(k.shape[1:])}")
-        if any(t.numel() and (_page_rows(t) is None or not _apart(t)) for t in pages):
-            raise ValueError(f"{what}: pages must lie one behind the other, each row in a place of its own")
-        _check_index(what, "slots", slots, torch.int64, (T,))
-        v = v if _rows16(v) else v.contiguous().clone()
-        n_slots = k_pages.shape[0] * k_pages.shape[1]
-        k_rows = _head_rows(k, k_weight, k_pages, (_page_rows(k_pages), _stride(k_pages, 2)))
-        v_rows = _head_rows(v, None, v_pages, (_page_rows(v_pages), _stride(v_pages, 2)))
-        k_out = None
-    else:
-        k_out = torch.empty(k.shape, dtype=k.dtype, device=k.device)
-        k_rows = _head_rows(k, k_weight, k_out, (_stride(k_out, 0), _stride(k_out, 1)))
-    if T == 0:
-        return q_out if paged else (q_out, k_out)
-    q_rows = _head_rows(q, q_weight, q_out, (_stride(q_out, 0), _stride(q_out, 1)))
-    if n_slots == 0 and paged:   # a cache without pages: nothing to write to
-        k_rows.num_heads, v_rows = 0, None
-    with torch.cuda.device(q.device):
-        code = load().ll_head_norm_rope(DTYPE_CODES[q.dtype], T, D, ctypes.byref(q_rows), ctypes.byref(k_rows),
-                                        None if v_rows is None else ctypes.byref(v_rows), float(eps), _ptr(cos), _ptr(sin), table, R,
-                                        _ptr(positions), int(interleaved), _ptr(slots), n_slots, _stream())
-    _check(code, "ll_head_norm_rope")
+    q_rows, k_rows, v_rows, q_out, k_out, n_slots, alive = _head_norm_rows(what, q, k, v, q_weight, k_weight, positions, cache, slots, q_out)
+    if q.shape[0]:
+        with torch.cuda.device(q.device):
+            code = load().ll_head_norm_rope(DTYPE_CODES[q.dtype], q.shape[0], D, ctypes.byref(q_rows), ctypes.byref(k_rows),
+                                            None if v_rows is None else ctypes.byref(v_rows), float(eps), _ptr(cos), _ptr(sin), table, R,
+                                            _ptr(positions), int(interleaved), _ptr(slots), n_slots, _stream())
+        _check(code, "ll_head_norm_rope")
     return q_out if paged else (q_out, k_out)
 
 
+def rotate_by_position(q, k, v, q_weight, k_weight, eps, frequencies, amplitude, positions, interleaved, grid, sections, cache=None, slots=None, q_out=None):
+    """:func:`head_norm_rope` with angles formed from positions and frequencies (``ll_rotate_by_position``)."""
+    what = "rotate_by_position"
+    paged = cache is not None
+    if (grid is None) != (sections is None):
+        raise ValueError(f"{what}: a grid of a frame's tokens goes with the pairs that frames, rows and columns turn")
+    rows, columns, frame_pairs, row_pairs = 0, 0, 0, 0
+    if grid is not None:
+        if len(grid) != 2 or len(sections) != 3 or min(grid) < 1 or min(sections) < 0 or grid[0] * grid[1] >= 1 << 31 or sum(sections) != frequencies.numel():
+            raise ValueError(f"{what}: a grid {tuple(grid)} of rows and columns, pairs {tuple(sections)} of frames, rows and columns for {frequencies.numel()} frequencies")
+        (rows, columns), (frame_pairs, row_pairs, _) = grid, sections
+    if not abs(float(amplitude)) < float("inf"):
+        raise ValueError(f"{what}: amplitude {amplitude}")
+    if q.is_cuda:
+        pages = (cache["k_pages"], cache["v_pages"]) if paged else (None, None)
+        done = host().rotate_by_position(q, k, v, q_weight, k_weight, float(eps), frequencies, float(amplitude), positions, bool(interleaved), rows, columns,
+                                         frame_pairs, row_pairs, *pages, slots, q_out)
+        if done is not None:
+            return done
+    pages = check_pages(what, cache) if paged else ()
+    _one_device(what, q, k, v, q_weight, k_weight, frequencies, positions, slots, q_out, *pages)
+    D = q.shape[-1] if q.ndim else 0
+    if frequencies.ndim != 1 or frequencies.dtype != torch.float64 or frequencies.numel() % 4 or 2 * frequencies.numel() > D:
+        raise ValueError(f"{what}: frequencies must be float64 [rotated columns / 2], the columns a multiple of 8 up to head_dim {D}; got "
+                         f"{frequencies.dtype} {tuple(frequencies.shape)}")
+    frequencies = frequencies.contiguous()
+    if frequencies.data_ptr() % 16:
+        frequencies = frequencies.clone()
+    q_rows, k_rows, v_rows, q_out, k_out, n_slots, alive = _head_norm_rows(what, q, k, v, q_weight, k_weight, positions, cache, slots, q_out)
+    if q.shape[0]:
+        angles = PositionAnglesStruct(frequencies.data_ptr(), 2 * frequencies.numel(), float(amplitude), rows, columns, frame_pairs, row_pairs)
+        with torch.cuda.device(q.device):
+            code = load().ll_rotate_by_position(DTYPE_CODES[q.dtype], q.shape[0], D, ctypes.byref(q_rows), ctypes.byref(k_rows),
+                                                None if v_rows is None else ctypes.byref(v_rows), float(eps), ctypes.byref(angles), _ptr(positions),
+                                                int(interleaved), _ptr(slots), n_slots, _stream())
+        _check(code, "ll_rotate_by_position")
+    return q_out if paged else (q_out, k_out)
+
+
+def _check_table(what: str, name: str, table: torch.Tensor, rows: int) -> None:
+    if table.dtype != torch.int32 or table.ndim != 2 or table.shape[0] != rows or (table.numel() and table.shape[1] > 1 and table.stride(1) != 1):
+        raise ValueError(f"{what}: {name} must be int32 [{rows}, pages of the longest] with contiguous rows")
+
+
+def _check_groups(what: str, streams: int, group_starts, prefix_lens) -> int:
+    """The number of groups of streams that share a beginning."""
+    groups = prefix_lens.numel()
+    _check_index(what, "prefix_lens", prefix_lens, torch.int32, (groups,))
+    if group_starts is None:
+        if groups != 1:
+            raise ValueError(f"{what}: {groups} groups need group_starts; without it all streams are one group")
+    else:
+        _check_index(what, "group_starts", group_starts, torch.int32, (groups + 1,))
+    return groups
+
+
+def step_layout(new_lens, kv_lens, page_table, free_pages, page_size, num_tokens, prefix_lens, group_starts, cursor, kv_lens_out):
+    """(q_starts, kv_lens, positions, slots, pages_wanted) of a step, ``page_table`` with its new pages (``ll_step_layout``)."""
+    what = "lay_out_step"
+    if new_lens.is_cuda:
+        done = host().step_layout(new_lens, kv_lens, page_table, free_pages, page_size, num_tokens, prefix_lens, group_starts, cursor, kv_lens_out)
+        if done is not None:
+            return done
+    _one_device(what, new_lens, kv_lens, page_table, free_pages, prefix_lens, group_starts, cursor, kv_lens_out)
+    streams = kv_lens.numel()
+    _check_index(what, "new_lens", new_lens, torch.int32, (streams,))
+    _check_index(what, "kv_lens", kv_lens, torch.int32, (streams,))
+    _check_table(what, "page_table", page_table, streams)
+    if not _apart(page_table):
+        raise ValueError(f"{what}: every entry of page_table has a place of its own")
+    _check_index(what, "free_pages", free_pages, torch.int32, (free_pages.numel(),))
+    for name, n, least in (("page_size", page_size, 1), ("num_tokens", num_tokens, 0)):
+        if int(n) != n or not least <= n < 1 << 31:
+            raise ValueError(f"{what}: {name} {n}")
+    if prefix_lens is None and group_starts is not None:
+        raise ValueError(f"{what}: group_starts goes with prefix_lens")
+    groups = 0 if prefix_lens is None else _check_groups(what, streams, group_starts, prefix_lens)
+    if cursor is not None:
+        _check_index(what, "cursor", cursor, torch.int32, (1,))
+    if kv_lens_out is not None:
+        _check_index(what, "kv_lens_out", kv_lens_out, torch.int32, (streams,))
+    device = kv_lens.device
+    if kv_lens_out is None:
+        kv_lens_out = torch.empty(streams, dtype=torch.int32, device=device)
+    q_starts, wanted = (torch.empty(n, dtype=torch.int32, device=device) for n in (streams + 1, 1))
+    positions, slots = (torch.empty(num_tokens, dtype=torch.int64, device=device) for _ in range(2))
+    a = StepLayoutStruct(streams=streams, new_lens=new_lens.data_ptr(), kv_lens=kv_lens.data_ptr(), page_table=page_table.data_ptr(),
+                         table_stride=_stride(page_table, 0), table_width=page_table.shape[1], page_size=page_size, free_pages=free_pages.data_ptr(),
+                         n_free=free_pages.numel(), cursor=_ptr(cursor), groups=groups, group_starts=_ptr(group_starts), prefix_lens=_ptr(prefix_lens),
+                         tokens=num_tokens, q_starts=q_starts.data_ptr(), kv_lens_out=kv_lens_out.data_ptr(), positions=positions.data_ptr(),
+                         slots=slots.data_ptr(), pages_wanted=wanted.data_ptr())
+    with torch.cuda.device(device):
+        lib, need = load(), c_size_t()
+        _check(lib.ll_step_layout_workspace(ctypes.byref(a), ctypes.byref(need)), what)
+        if need.value:
+            workspace = torch.empty(need.value, dtype=torch.uint8, device=device)
+            a.workspace, a.workspace_bytes = workspace.data_ptr(), need.value
+        code = lib.ll_step_layout(ctypes.byref(a), _stream())
+    _check(code, what)
+    return q_starts, kv_lens_out, positions, slots, wanted
+
+
 def ragged_attention(what, q, q_starts, softmax_scale, max_q_len, max_kv_len, out, *, cache=None, page_table=None, kv_lens=None, causal=False,
-                     window=None, sink_tokens=0, k=None, v=None, k_starts=None, k_lens=None, key_mask=None):
+                     window=None, sink_tokens=0, k=None, v=None, k_starts=None, k_lens=None, key_mask=None, prefix=None):
     """The queries q [T, H, D] of several streams over the keys of a paged ``cache`` or over rows of k and v [n, Hk, D]
-    (``ll_ragged_attention``)."""
-    if q.is_cuda and q.ndim == 3 and q.shape[2] and (window is None or window):
+    (``ll_ragged_attention``), or with ``prefix``, (table, lengths, where groups start or None, the longest or None), over beginnings that groups of
+    streams share and their own keys in the cache (``ll_shared_prefix_attention``)."""
+    if prefix is not None and q.is_cuda and q.ndim == 3 and q.shape[2]:
+        done = host().shared_prefix_attention(q, q_starts, q.shape[-1] ** -0.5 if softmax_scale is None else float(softmax_scale), max_q_len or 0, max_kv_len or 0,
+                                              out, cache["k_pages"], cache["v_pages"], page_table, kv_lens, bool(causal), prefix[0], prefix[1], prefix[2],
+                                              prefix[3] or 0)
+        if done is not None:
+            return done
+    if prefix is None and q.is_cuda and q.ndim == 3 and q.shape[2] and (window is None or window):
         keys = (k, v) if cache is None else (cache["k_pages"], cache["v_pages"])
         done = host().ragged_attention(q, q_starts, q.shape[-1] ** -0.5 if softmax_scale is None else float(softmax_scale), max_q_len or 0, max_kv_len or 0,
                                        out, *keys, page_table, kv_lens, bool(causal), window or 0, sink_tokens, k_starts, k_lens, key_mask)
         if done is not None:
             return done
     pages = check_pages(what, cache) if cache is not None else ()
-    _one_device(what, q, q_starts, out, page_table, kv_lens, k, v, k_starts, k_lens, key_mask, *pages)
+    _one_device(what, q, q_starts, out, page_table, kv_lens, k, v, k_starts, k_lens, key_mask, *pages, *(prefix or ())[:3])
     _check_rows(what, "q", q)
     T, H, D = q.shape
     if D not in (64, 128):
@@ -1194,8 +1337,7 @@ def ragged_attention(what, q, q_starts, softmax_scale, max_q_len, max_kv_len, ou
     if cache is not None:
         k, v = pages
         _check_index(what, "kv_lens", kv_lens, torch.int32, (streams,))
-        if page_table.dtype != torch.int32 or page_table.ndim != 2 or page_table.shape[0] != streams or (page_table.numel() and page_table.shape[1] > 1 and page_table.stride(1) != 1):
-            raise ValueError(f"{what}: page_table must be int32 [{streams}, pages of the longest stream] with contiguous rows")
+        _check_table(what, "page_table", page_table, streams)
         a.page_table, a.table_stride, a.table_width = page_table.data_ptr(), _stride(page_table, 0), page_table.shape[1]
         a.n_pages, a.page_size, a.kv_lens, a.causal = k.shape[0], k.shape[1], kv_lens.data_ptr(), int(bool(causal))
         a.window, a.sink_keys = window or 0, sink_tokens
@@ -1203,6 +1345,14 @@ def ragged_attention(what, q, q_starts, softmax_scale, max_q_len, max_kv_len, ou
         a.v_stride_page, a.v_stride_row, a.v_stride_head = (_stride(v, i) for i in range(3))
         if a.table_width * a.page_size >= 1 << 31:
             raise ValueError(f"{what}: a table of {a.table_width} pages of {a.page_size} rows reaches beyond 2^31 keys")
+        if prefix is not None:
+            prefix_table, prefix_lens, group_starts, longest = prefix
+            groups = _check_groups(what, streams, group_starts, prefix_lens)
+            _check_table(what, "prefix_table", prefix_table, groups)
+            if longest is not None and (int(longest) != longest or longest < 0):
+                raise ValueError(f"{what}: max_prefix_len {longest}")
+            if max(a.table_width, prefix_table.shape[1]) * a.page_size > 1 << 30:
+                raise ValueError(f"{what}: tables of {a.table_width} and {prefix_table.shape[1]} pages of {a.page_size} rows reach beyond 2^30 keys")
     else:
         _check_rows(what, "k", k, q.dtype)
         _check_rows(what, "v", v, q.dtype)
@@ -1236,10 +1386,16 @@ def ragged_attention(what, q, q_starts, softmax_scale, max_q_len, max_kv_len, ou
     a.out_stride_token, a.out_stride_head = _stride(out, 0), _stride(out, 1)
     with torch.cuda.device(q.device):
         lib, need = load(), c_size_t()
-        _check(lib.ll_ragged_attention_workspace(ctypes.byref(a), 0, ctypes.byref(need)), what)
+        size, launch, args = lib.ll_ragged_attention_workspace, lib.ll_ragged_attention, a
+        if prefix is not None:
+            size, launch = lib.ll_shared_prefix_attention_workspace, lib.ll_shared_prefix_attention
+            args = SharedPrefixStruct(own=a, groups=groups, group_starts=_ptr(group_starts), prefix_lens=prefix_lens.data_ptr(), prefix_table=prefix_table.data_ptr(),
+                                      prefix_stride=_stride(prefix_table, 0), prefix_width=prefix_table.shape[1], max_prefix_len=longest or 0)
+            a = args.own
+        _check(size(ctypes.byref(args), 0, ctypes.byref(need)), what)
         if need.value:
             workspace = torch.empty(need.value, dtype=torch.uint8, device=q.device)
             a.workspace, a.workspace_bytes = workspace.data_ptr(), need.value
-        code = lib.ll_ragged_attention(ctypes.byref(a), _stream())
+        code = launch(ctypes.byref(args), _stream())
     _check(code, what)
     return out

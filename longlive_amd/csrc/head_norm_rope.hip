@@ -1,5 +1,5 @@
 // Every head of q and k of a batch of tokens through its own RMS norm and the position rotation, K and V on to the rows of a
-// paged cache, in one pass (ll_head_norm_rope).
+// paged cache, in one pass: by angles from a table (ll_head_norm_rope) or formed from positions and frequencies (ll_rotate_by_position).
 //
 //   y = x * rsqrt(mean(x^2) + eps) * w over a head's D columns;  (a, b) -> (a cos - b sin, b cos + a sin) over pairs of columns
 //
@@ -25,6 +25,14 @@ struct HeadRows {
   int heads, weight_f32;
 };
 
+// Angles formed in the kernel.
+struct FormedAngles {
+  const double* frequencies;
+  float amplitude;
+  Divisor frame, columns;    // tokens of a video frame and of a row in it; 0: positions on a line
+  int frame_pairs, row_pairs;  // pairs turned by frames, by rows; the others by columns
+};
+
 struct HeadNormParams {
   HeadRows rows[3];  // q, k, v
   int64_t first_token;
@@ -37,6 +45,7 @@ struct HeadNormParams {
   int64_t table_rows;
   const int64_t *positions, *slots;
   int64_t n_slots;
+  FormedAngles formed;
 };
 
 // Sum over LANES neighbouring lanes, in every one of them.
@@ -65,8 +74,48 @@ __device__ __forceinline__ void unpack4(uint2 w, float* f) {
 // 16000 x (32 + 8 + 8) 92.9 / 72.4, 16381 x (40 + 8 + 8) of 64 columns 57.0 / 46.2 (four: 74.2 and 44.3).
 constexpr int64_t kManyWaves = 8192;
 
-// LANES hold a head, a wave 64 / LANES heads side by side, HEADS times.
-template <typename T, int LANES, int HEADS>
+// Cosines and sines of pairs 4 l .. 4 l + 3 at a position, which is the wave's.  A position times a frequency takes 64 bits: at position
+// 2^20 its rounding to 32 would turn the fastest pairs by 2^-4.  The matter is settled in turns, of which the whole ones are dropped; what is
+// left is exact to 2^-26 of a turn in 32 bits, and the hardware's sine and cosine of it
+// are off by no more than 2^-22, a thousandth of the rounding to f16 that follows.
+__device__ __forceinline__ void form_angles(const FormedAngles& a, int64_t pos, int l, float (&cs)[4], float (&sn)[4]) {
+  double f[4];
+  *reinterpret_cast<double2*>(f) = *reinterpret_cast<const double2*>(a.frequencies + 4 * l);
+  *reinterpret_cast<double2*>(f + 2) = *reinterpret_cast<const double2*>(a.frequencies + 4 * l + 2);
+  double at[3] = {(double)pos, 0.0, 0.0};
+  if (a.frame.d) {
+    int64_t frame;
+    uint32_t in_frame;
+    if ((uint64_t)pos >> 32 == 0) {
+      frame = (uint32_t)pos / a.frame;
+      in_frame = (uint32_t)pos - (uint32_t)frame * a.frame.d;
+    } else {  // rounded down, also below zero
+      frame = pos / (int64_t)a.frame.d;
+      int64_t rest = pos - frame * a.frame.d;
+      if (rest < 0) {
+        rest += a.frame.d;
+        --frame;
+      }
+      in_frame = (uint32_t)rest;
+    }
+    const uint32_t row = in_frame / a.columns;
+    at[0] = (double)frame;
+    at[1] = (double)row;
+    at[2] = (double)(in_frame - row * a.columns.d);
+  }
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    const int pair = 4 * l + j;
+    const double x = !a.frame.d || pair < a.frame_pairs ? at[0] : pair < a.frame_pairs + a.row_pairs ? at[1] : at[2];
+    const double turns = x * (f[j] * 0.15915494309189533577);  // 1 / (2 pi)
+    const float part = (float)(turns - rint(turns));
+    cs[j] = a.amplitude * __builtin_amdgcn_cosf(part);  // of a part of a turn
+    sn[j] = a.amplitude * __builtin_amdgcn_sinf(part);
+  }
+}
+
+// LANES hold a head, a wave 64 / LANES heads side by side, HEADS times.  FORMED: by angles formed from positions.
+template <typename T, int LANES, int HEADS, bool FORMED>
 __global__ __launch_bounds__(kHeadNormThreads) void head_norm_rope_kernel(HeadNormParams p) {
   constexpr int kSide = 64 / LANES;
   const uint32_t unit = __builtin_amdgcn_readfirstlane(blockIdx.x * (kHeadNormThreads / 64) + threadIdx.x / 64);
@@ -118,8 +167,8 @@ __global__ __launch_bounds__(kHeadNormThreads) void head_norm_rope_kernel(HeadNo
       w[1] = *reinterpret_cast<const uint2*>(static_cast<const uint16_t*>(r.weight) + c1);
     }
   }
-  const bool rotate = kind != 2 && p.R != 0 && (uint64_t)pos < (uint64_t)p.table_rows;
-  if (rotate && 8 * l < p.R) {
+  const bool rotate = kind != 2 && p.R != 0 && (FORMED || (uint64_t)pos < (uint64_t)p.table_rows);
+  if (!FORMED && rotate && 8 * l < p.R) {
     cs = *reinterpret_cast<const float4*>(p.cos + pos * (p.R / 2) + 4 * l);
     sn = *reinterpret_cast<const float4*>(p.sin + pos * (p.R / 2) + 4 * l);
   }
@@ -128,7 +177,10 @@ __global__ __launch_bounds__(kHeadNormThreads) void head_norm_rope_kernel(HeadNo
     unpack4<T>(w[0], f);
     unpack4<T>(w[1], f + 4);
   }
-  const float cc[4] = {cs.x, cs.y, cs.z, cs.w}, ss[4] = {sn.x, sn.y, sn.z, sn.w};
+  float cc[4] = {cs.x, cs.y, cs.z, cs.w}, ss[4] = {sn.x, sn.y, sn.z, sn.w};
+  if constexpr (FORMED) {
+    if (rotate && 8 * l < p.R) form_angles(p.formed, pos, l, cc, ss);
+  }
   uint16_t* dst = r.out + row * r.out_stride_token;
 #pragma unroll
   for (int i = 0; i < HEADS; ++i) {
@@ -172,7 +224,7 @@ static uint32_t waves_for(int num_heads, int lanes, int heads) {
   return (uint32_t)((num_heads + each - 1) / each);
 }
 
-template <typename T, int LANES, int HEADS>
+template <typename T, int LANES, int HEADS, bool FORMED>
 static void launch_head_norm(HeadNormParams p, int64_t tokens, hipStream_t stream) {
   p.units_q = waves_for(p.rows[0].heads, LANES, HEADS);
   p.units_kv = waves_for(p.rows[1].heads, LANES, HEADS);
@@ -182,52 +234,65 @@ static void launch_head_norm(HeadNormParams p, int64_t tokens, hipStream_t strea
   for (int64_t first = 0; first < tokens; first += most) {
     p.first_token = first;
     p.tokens = (uint32_t)(tokens - first < most ? tokens - first : most);
-    head_norm_rope_kernel<T, LANES, HEADS><<<head_norm_groups(p.tokens, per_token), kHeadNormThreads, 0, stream>>>(p);
+    head_norm_rope_kernel<T, LANES, HEADS, FORMED><<<head_norm_groups(p.tokens, per_token), kHeadNormThreads, 0, stream>>>(p);
   }
 }
 
-template <typename T, int LANES>
+template <typename T, int LANES, bool FORMED>
 static void launch_head_norm(const HeadNormParams& p, int64_t tokens, hipStream_t stream) {
   const int64_t waves = tokens * (waves_for(p.rows[0].heads, LANES, 1) + 2 * waves_for(p.rows[1].heads, LANES, 1));
   if (waves > kManyWaves)
-    launch_head_norm<T, LANES, 2>(p, tokens, stream);
+    launch_head_norm<T, LANES, 2, FORMED>(p, tokens, stream);
   else
-    launch_head_norm<T, LANES, 1>(p, tokens, stream);
+    launch_head_norm<T, LANES, 1, FORMED>(p, tokens, stream);
 }
 
-static int check_rows(const ll_head_rows* r, const char* name, bool may_norm) {
-  LL_REQUIRE(r, "ll_head_norm_rope: %s is NULL", name);
-  LL_REQUIRE(r->num_heads >= 0 && r->num_heads <= 65536, "ll_head_norm_rope: %s has %d heads", name, r->num_heads);
+template <bool FORMED>
+static void launch_head_norm(const HeadNormParams& p, int dtype, int64_t tokens, hipStream_t stream) {
+#define LL_LAUNCH(T)                                   \
+  if (p.D <= 64) {                                     \
+    launch_head_norm<T, 8, FORMED>(p, tokens, stream);   \
+  } else if (p.D <= 128) {                             \
+    launch_head_norm<T, 16, FORMED>(p, tokens, stream);  \
+  } else {                                             \
+    launch_head_norm<T, 32, FORMED>(p, tokens, stream);  \
+  }
+  if (dtype == LL_DTYPE_BF16) {
+    LL_LAUNCH(Bf16)
+  } else {
+    LL_LAUNCH(F16)
+  }
+#undef LL_LAUNCH
+}
+
+static int check_rows(const char* what, const ll_head_rows* r, const char* name, bool may_norm) {
+  LL_REQUIRE(r, "%s: %s is NULL", what, name);
+  LL_REQUIRE(r->num_heads >= 0 && r->num_heads <= 65536, "%s: %s has %d heads", what, name, r->num_heads);
   if (r->num_heads == 0) return LL_OK;
-  LL_REQUIRE(r->x && r->out, "ll_head_norm_rope: null pointer in %s", name);
-  LL_REQUIRE(((uintptr_t)r->x | (uintptr_t)r->out | (uintptr_t)r->weight) % 16 == 0, "ll_head_norm_rope: pointers of %s must be 16-byte aligned", name);
+  LL_REQUIRE(r->x && r->out, "%s: null pointer in %s", what, name);
+  LL_REQUIRE(((uintptr_t)r->x | (uintptr_t)r->out | (uintptr_t)r->weight) % 16 == 0, "%s: pointers of %s must be 16-byte aligned", what, name);
   LL_REQUIRE((r->stride_token | r->stride_head | r->out_stride_token | r->out_stride_head) % 8 == 0,
-             "ll_head_norm_rope: strides of %s must be multiples of 8", name);
-  LL_REQUIRE(may_norm || !r->weight, "ll_head_norm_rope: %s has no norm", name);
+             "%s: strides of %s must be multiples of 8", what, name);
+  LL_REQUIRE(may_norm || !r->weight, "%s: %s has no norm", what, name);
   return LL_OK;
 }
 
-}  // namespace ll
-
-extern "C" int ll_head_norm_rope(int dtype, int64_t tokens, int head_dim, const ll_head_rows* q, const ll_head_rows* k, const ll_head_rows* v,
-                                 float eps, const float* cos, const float* sin, int64_t table_rows, int rotary_dim, const int64_t* positions,
-                                 int interleaved, const int64_t* slots, int64_t n_slots, void* stream) {
-  using namespace ll;
-  LL_REQUIRE(dtype == LL_DTYPE_BF16 || dtype == LL_DTYPE_F16, "ll_head_norm_rope: dtype %d is not bf16 or f16", dtype);
-  LL_REQUIRE(tokens >= 0 && tokens < (1ll << 40), "ll_head_norm_rope: %lld tokens", (long long)tokens);
-  LL_REQUIRE(head_dim > 0 && head_dim <= 256 && head_dim % 8 == 0, "ll_head_norm_rope: head_dim %d is not a multiple of 8 up to 256", head_dim);
+// What both entry points take.
+static int head_norm_params(const char* what, int dtype, int64_t tokens, int head_dim, const ll_head_rows* q, const ll_head_rows* k,
+                            const ll_head_rows* v, float eps, int rotary_dim, const int64_t* positions, int interleaved, const int64_t* slots,
+                            int64_t n_slots, HeadNormParams& p) {
+  LL_REQUIRE(dtype == LL_DTYPE_BF16 || dtype == LL_DTYPE_F16, "%s: dtype %d is not bf16 or f16", what, dtype);
+  LL_REQUIRE(tokens >= 0 && tokens < (1ll << 40), "%s: %lld tokens", what, (long long)tokens);
+  LL_REQUIRE(head_dim > 0 && head_dim <= 256 && head_dim % 8 == 0, "%s: head_dim %d is not a multiple of 8 up to 256", what, head_dim);
   LL_REQUIRE(rotary_dim >= 0 && rotary_dim <= head_dim && rotary_dim % 8 == 0,
-             "ll_head_norm_rope: rotary_dim %d is not a multiple of 8 up to head_dim %d", rotary_dim, head_dim);
-  LL_REQUIRE(rotary_dim == 0 || (cos && sin && table_rows >= 0), "ll_head_norm_rope: no angles to rotate by");
-  LL_REQUIRE(((uintptr_t)cos | (uintptr_t)sin) % 16 == 0, "ll_head_norm_rope: cos and sin must be 16-byte aligned");
+             "%s: rotary_dim %d is not a multiple of 8 up to head_dim %d", what, rotary_dim, head_dim);
   const ll_head_rows none{};
   if (!v) v = &none;
-  if (int rc = check_rows(q, "q", true)) return rc;
-  if (int rc = check_rows(k, "k", true)) return rc;
-  if (int rc = check_rows(v, "v", false)) return rc;
-  LL_REQUIRE(v->num_heads == 0 || (slots && v->num_heads == k->num_heads), "ll_head_norm_rope: v goes with slots and has as many heads as k");
-  LL_REQUIRE(!slots || n_slots >= 0, "ll_head_norm_rope: %lld slots", (long long)n_slots);
-  HeadNormParams p{};
+  if (int rc = check_rows(what, q, "q", true)) return rc;
+  if (int rc = check_rows(what, k, "k", true)) return rc;
+  if (int rc = check_rows(what, v, "v", false)) return rc;
+  LL_REQUIRE(v->num_heads == 0 || (slots && v->num_heads == k->num_heads), "%s: v goes with slots and has as many heads as k", what);
+  LL_REQUIRE(!slots || n_slots >= 0, "%s: %lld slots", what, (long long)n_slots);
   const ll_head_rows* given[3] = {q, k, v};
   for (int i = 0; i < 3; ++i) {
     const ll_head_rows& r = *given[i];
@@ -239,28 +304,55 @@ extern "C" int ll_head_norm_rope(int dtype, int64_t tokens, int head_dim, const 
   p.interleaved = interleaved;
   p.eps = eps;
   p.inv_D = 1.0f / (float)head_dim;
-  p.cos = cos;
-  p.sin = sin;
-  p.table_rows = table_rows;
   p.positions = positions;
   p.slots = slots;
   p.n_slots = n_slots;
+  return LL_OK;
+}
+
+}  // namespace ll
+
+extern "C" int ll_head_norm_rope(int dtype, int64_t tokens, int head_dim, const ll_head_rows* q, const ll_head_rows* k, const ll_head_rows* v,
+                                 float eps, const float* cos, const float* sin, int64_t table_rows, int rotary_dim, const int64_t* positions,
+                                 int interleaved, const int64_t* slots, int64_t n_slots, void* stream) {
+  using namespace ll;
+  HeadNormParams p{};
+  if (int rc = head_norm_params("ll_head_norm_rope", dtype, tokens, head_dim, q, k, v, eps, rotary_dim, positions, interleaved, slots, n_slots, p)) return rc;
+  LL_REQUIRE(rotary_dim == 0 || (cos && sin && table_rows >= 0), "ll_head_norm_rope: no angles to rotate by");
+  LL_REQUIRE(((uintptr_t)cos | (uintptr_t)sin) % 16 == 0, "ll_head_norm_rope: cos and sin must be 16-byte aligned");
+  p.cos = cos;
+  p.sin = sin;
+  p.table_rows = table_rows;
   if (tokens == 0 || q->num_heads + k->num_heads == 0) return LL_OK;
-  const hipStream_t s = static_cast<hipStream_t>(stream);
-#define LL_LAUNCH(T)                           \
-  if (head_dim <= 64) {                        \
-    launch_head_norm<T, 8>(p, tokens, s);      \
-  } else if (head_dim <= 128) {                \
-    launch_head_norm<T, 16>(p, tokens, s);     \
-  } else {                                     \
-    launch_head_norm<T, 32>(p, tokens, s);     \
-  }
-  if (dtype == LL_DTYPE_BF16) {
-    LL_LAUNCH(Bf16)
-  } else {
-    LL_LAUNCH(F16)
-  }
-#undef LL_LAUNCH
+  launch_head_norm<false>(p, dtype, tokens, static_cast<hipStream_t>(stream));
   LL_CHECK_LAUNCH("ll_head_norm_rope");
+  return LL_OK;
+}
+
+extern "C" int ll_rotate_by_position(int dtype, int64_t tokens, int head_dim, const ll_head_rows* q, const ll_head_rows* k, const ll_head_rows* v,
+                                     float eps, const ll_position_angles* angles, const int64_t* positions, int interleaved, const int64_t* slots,
+                                     int64_t n_slots, void* stream) {
+  using namespace ll;
+  LL_REQUIRE(angles, "ll_rotate_by_position: no angles to rotate by");
+  HeadNormParams p{};
+  if (int rc = head_norm_params("ll_rotate_by_position", dtype, tokens, head_dim, q, k, v, eps, angles->rotary_dim, positions, interleaved, slots, n_slots, p))
+    return rc;
+  LL_REQUIRE(p.R == 0 || (angles->frequencies && (uintptr_t)angles->frequencies % 16 == 0), "ll_rotate_by_position: frequencies must be 16-byte aligned");
+  const int64_t rows = angles->grid_rows, columns = angles->grid_columns;
+  LL_REQUIRE(rows >= 0 && columns >= 0 && (rows > 0) == (columns > 0) && rows <= 0x7fffffffll && columns <= 0x7fffffffll && rows * columns <= 0x7fffffffll,
+             "ll_rotate_by_position: a grid of %lld x %lld", (long long)rows, (long long)columns);
+  if (rows > 0) {
+    LL_REQUIRE(angles->frame_pairs >= 0 && angles->row_pairs >= 0 && angles->frame_pairs <= p.R / 2 && angles->row_pairs <= p.R / 2 - angles->frame_pairs,
+               "ll_rotate_by_position: %d and %d of %d pairs", angles->frame_pairs, angles->row_pairs, p.R / 2);
+    p.formed.frame = divisor((uint32_t)(rows * columns));
+    p.formed.columns = divisor((uint32_t)columns);
+    p.formed.frame_pairs = angles->frame_pairs;
+    p.formed.row_pairs = angles->row_pairs;
+  }
+  p.formed.frequencies = angles->frequencies;
+  p.formed.amplitude = angles->amplitude;
+  if (tokens == 0 || q->num_heads + k->num_heads == 0) return LL_OK;
+  launch_head_norm<true>(p, dtype, tokens, static_cast<hipStream_t>(stream));
+  LL_CHECK_LAUNCH("ll_rotate_by_position");
   return LL_OK;
 }

@@ -1045,44 +1045,118 @@ inline bool as_count(PyObject* o, int64_t& n) {
   return n >= 0;
 }
 
-// ragged_attention(q, q_starts, scale, max_q_len, max_kv_len, out or None, k, v, page_table, kv_lens, causal, window, sink, k_starts, k_lens,
-// key_mask) -> [T, H, D]: over pages k, v [pages, page_size, Hk, D] with a page table, else over rows k, v [n, Hk, D] (page_table None).
-PyObject* py_ragged_attention(PyObject*, PyObject* const* args, Py_ssize_t n) {
-  HANDLE_TH_ERRORS
-  if (n != 16 || !plain(args[0])) Py_RETURN_NONE;
-  const int dev = current_device_of(THPVariable_Unpack(args[0]));
-  if (dev < 0) Py_RETURN_NONE;
-  const Tensor* q = as_rows(args[0], dev, 3, nullptr);
-  const bool paged = args[8] != Py_None;
-  const Tensor *k = q ? as_rows(args[6], dev, paged ? 4 : 3, q) : nullptr, *v = q ? as_rows(args[7], dev, paged ? 4 : 3, q) : nullptr;
-  if (!q || !k || !v || k->sizes() != v->sizes()) Py_RETURN_NONE;
-  const int64_t T = q->size(0), H = q->size(1), D = q->size(2), last = paged ? 3 : 2;
-  if ((D != 64 && D != 128) || k->size(last) != D || H % k->size(last - 1) != 0) Py_RETURN_NONE;
-  const Tensor* starts = plain(args[1]) ? &THPVariable_Unpack(args[1]) : nullptr;
-  if (!starts || !as_list(args[1], dev, at::kInt, starts->numel()) || starts->numel() < 2) Py_RETURN_NONE;
+// An int32 table of so many rows, their entries one behind the other.
+const Tensor* as_table(PyObject* o, int dev, int64_t rows) {
+  const Tensor* t = plain(o) ? &THPVariable_Unpack(o) : nullptr;
+  return t && on_device(*t, dev) && t->scalar_type() == at::kInt && t->dim() == 2 && t->size(0) == rows && t->numel() > 0 &&
+                 (t->size(1) <= 1 || t->stride(1) == 1)
+             ? t
+             : nullptr;
+}
+
+// What the attentions of several streams have in common: queries, their starts, keys (pages, or rows), sizes and the result.
+struct RaggedCall {
+  int dev = -1;
+  const Tensor *q = nullptr, *k = nullptr, *v = nullptr;
+  PyObject* given_out = nullptr;
+  Tensor out;
   ll_ragged_attention_args a{};
-  a.streams = starts->numel() - 1;
-  if (!PyFloat_Check(args[2]) || !as_count(args[3], a.max_q_len) || !as_count(args[4], a.max_kv_len) || !as_count(args[11], a.window) ||
-      !as_count(args[12], a.sink_keys))
-    Py_RETURN_NONE;
-  a.softmax_scale = (float)PyFloat_AsDouble(args[2]);
-  if (paged) {
-    const Tensor* table = plain(args[8]) ? &THPVariable_Unpack(args[8]) : nullptr;
-    const Tensor* lens = as_list(args[9], dev, at::kInt, a.streams);
-    if (!table || !lens || !on_device(*table, dev) || table->scalar_type() != at::kInt || table->dim() != 2 || table->size(0) != a.streams ||
-        table->numel() == 0 || (table->size(1) > 1 && table->stride(1) != 1))
-      Py_RETURN_NONE;
+
+  bool take(PyObject* queries, PyObject* starts_of, PyObject* scale, PyObject* max_q_len, PyObject* max_kv_len, PyObject* to, PyObject* keys, PyObject* values,
+            bool paged) {
+    if (!plain(queries)) return false;
+    dev = current_device_of(THPVariable_Unpack(queries));
+    if (dev < 0) return false;
+    q = as_rows(queries, dev, 3, nullptr);
+    if (!q) return false;
+    k = as_rows(keys, dev, paged ? 4 : 3, q);
+    v = as_rows(values, dev, paged ? 4 : 3, q);
+    if (!k || !v || k->sizes() != v->sizes()) return false;
+    const int64_t T = q->size(0), H = q->size(1), D = q->size(2), last = paged ? 3 : 2;
+    if ((D != 64 && D != 128) || k->size(last) != D || H % k->size(last - 1) != 0) return false;
+    const Tensor* starts = plain(starts_of) ? &THPVariable_Unpack(starts_of) : nullptr;
+    if (!starts || !as_list(starts_of, dev, at::kInt, starts->numel()) || starts->numel() < 2) return false;
+    a.streams = starts->numel() - 1;
+    if (!PyFloat_Check(scale) || !as_count(max_q_len, a.max_q_len) || !as_count(max_kv_len, a.max_kv_len)) return false;
+    a.softmax_scale = (float)PyFloat_AsDouble(scale);
+    if (to == Py_None) {
+      out = empty(q->sizes(), q->scalar_type(), dev);
+      a.clear_rest = 1;
+    } else {
+      const Tensor* given = as_rows(to, dev, 3, q);
+      if (!given || given->sizes() != q->sizes() || !apart(*given)) return false;
+      out = *given;
+      given_out = to;
+    }
+    a.dtype = half_code(*q);
+    a.head_dim = (int)D;
+    a.num_heads = (int)H;
+    a.num_kv_heads = (int)k->size(last - 1);
+    a.n_queries = T;
+    a.q = q->data_ptr();
+    a.q_stride_token = stride_of(q, 0);
+    a.q_stride_head = stride_of(q, 1);
+    a.out = out.data_ptr();
+    a.out_stride_token = stride_of(&out, 0);
+    a.out_stride_head = stride_of(&out, 1);
+    a.q_starts = starts->data_ptr<int32_t>();
+    a.k = k->data_ptr();
+    a.v = v->data_ptr();
+    a.k_stride_row = stride_of(k, last - 2);
+    a.v_stride_row = stride_of(v, last - 2);
+    a.k_stride_head = stride_of(k, last - 1);
+    a.v_stride_head = stride_of(v, last - 1);
+    return true;
+  }
+
+  bool take_pages(PyObject* page_table, PyObject* kv_lens, PyObject* causal) {
+    const Tensor *table = as_table(page_table, dev, a.streams), *lens = as_list(kv_lens, dev, at::kInt, a.streams);
+    if (!table || !lens || k->size(1) > 0x7fffffff) return false;
     a.page_table = table->data_ptr<int32_t>();
     a.table_stride = table->stride(0);
     a.table_width = table->size(1);
     a.n_pages = k->size(0);
-    if (k->size(1) > 0x7fffffff) Py_RETURN_NONE;
     a.page_size = (int)k->size(1);
     a.kv_lens = lens->data_ptr<int32_t>();
-    a.causal = args[10] == Py_True;
+    a.causal = causal == Py_True;
     a.k_stride_page = stride_of(k, 0);
     a.v_stride_page = stride_of(v, 0);
+    return true;
+  }
+
+  // Memory for parts, freed for work behind this call's launches on the stream.
+  Tensor workspace(size_t need) {
+    Tensor w;
+    if (need) {
+      w = empty({(int64_t)need}, at::kByte, dev);
+      a.workspace = w.data_ptr();
+      a.workspace_bytes = need;
+    }
+    return w;
+  }
+
+  PyObject* result() {
+    if (!given_out) return THPVariable_Wrap(out);
+    Py_INCREF(given_out);
+    return given_out;
+  }
+};
+
+// ragged_attention(q, q_starts, scale, max_q_len, max_kv_len, out or None, k, v, page_table, kv_lens, causal, window, sink, k_starts, k_lens,
+// key_mask) -> [T, H, D]: over pages k, v [pages, page_size, Hk, D] with a page table, else over rows k, v [n, Hk, D] (page_table None).
+PyObject* py_ragged_attention(PyObject*, PyObject* const* args, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  if (n != 16) Py_RETURN_NONE;
+  const bool paged = args[8] != Py_None;
+  RaggedCall call;
+  ll_ragged_attention_args& a = call.a;
+  if (!call.take(args[0], args[1], args[2], args[3], args[4], args[5], args[6], args[7], paged) || !as_count(args[11], a.window) ||
+      !as_count(args[12], a.sink_keys))
+    Py_RETURN_NONE;
+  if (paged) {
+    if (!call.take_pages(args[8], args[9], args[10])) Py_RETURN_NONE;
   } else {
+    const int dev = call.dev;
     const Tensor* k_starts = args[14] == Py_None ? as_list(args[13], dev, at::kInt, a.streams + 1)
                                                  : plain(args[13]) ? &THPVariable_Unpack(args[13]) : nullptr;
     if (!k_starts || k_starts->numel() < a.streams || !as_list(args[13], dev, at::kInt, k_starts->numel())) Py_RETURN_NONE;
@@ -1092,138 +1166,265 @@ PyObject* py_ragged_attention(PyObject*, PyObject* const* args, Py_ssize_t n) {
       if (!lens) Py_RETURN_NONE;
       a.k_lens = lens->data_ptr<int32_t>();
     }
-    a.n_keys = k->size(0);
+    a.n_keys = call.k->size(0);
     if (args[15] != Py_None) {
       const Tensor* mask = as_list(args[15], dev, at::kBool, a.n_keys);
       if (!mask) Py_RETURN_NONE;
       a.key_mask = static_cast<const uint8_t*>(mask->data_ptr());
     }
   }
-  Tensor out;
-  if (args[5] == Py_None) {
-    out = empty(q->sizes(), q->scalar_type(), dev);
-    a.clear_rest = 1;
-  } else {
-    const Tensor* given = as_rows(args[5], dev, 3, q);
-    if (!given || given->sizes() != q->sizes() || !apart(*given)) Py_RETURN_NONE;
-    out = *given;
-  }
-  a.dtype = half_code(*q);
-  a.head_dim = (int)D;
-  a.num_heads = (int)H;
-  a.num_kv_heads = (int)k->size(last - 1);
-  a.n_queries = T;
-  a.q = q->data_ptr();
-  a.q_stride_token = stride_of(q, 0);
-  a.q_stride_head = stride_of(q, 1);
-  a.out = out.data_ptr();
-  a.out_stride_token = stride_of(&out, 0);
-  a.out_stride_head = stride_of(&out, 1);
-  a.q_starts = starts->data_ptr<int32_t>();
-  a.k = k->data_ptr();
-  a.v = v->data_ptr();
-  a.k_stride_row = stride_of(k, last - 2);
-  a.v_stride_row = stride_of(v, last - 2);
-  a.k_stride_head = stride_of(k, last - 1);
-  a.v_stride_head = stride_of(v, last - 1);
   size_t need = 0;
   const char* what = paged ? "paged_attention" : "ragged_cross_attention";
   if (failed(ll_ragged_attention_workspace(&a, 0, &need), what)) return nullptr;
-  Tensor workspace;  // freed for work behind this call's launches on the stream
+  const Tensor workspace = call.workspace(need);
+  if (failed(ll_ragged_attention(&a, stream_of(call.dev)), what)) return nullptr;
+  return call.result();
+  END_HANDLE_TH_ERRORS
+}
+
+// shared_prefix_attention(q, q_starts, scale, max_q_len, max_kv_len, out or None, k, v, page_table, kv_lens, causal, prefix_table, prefix_lens,
+// group_starts or None, max_prefix_len) -> [T, H, D]
+PyObject* py_shared_prefix_attention(PyObject*, PyObject* const* args, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  if (n != 15) Py_RETURN_NONE;
+  RaggedCall call;
+  if (!call.take(args[0], args[1], args[2], args[3], args[4], args[5], args[6], args[7], true) || !call.take_pages(args[8], args[9], args[10])) Py_RETURN_NONE;
+  const int dev = call.dev;
+  ll_shared_prefix_args p{};
+  const Tensor* lens = plain(args[12]) ? &THPVariable_Unpack(args[12]) : nullptr;
+  if (!lens || !as_list(args[12], dev, at::kInt, lens->numel()) || !as_count(args[14], p.max_prefix_len)) Py_RETURN_NONE;
+  p.groups = lens->numel();
+  const Tensor* table = as_table(args[11], dev, p.groups);
+  if (!table || (args[13] == Py_None && p.groups != 1)) Py_RETURN_NONE;
+  if (args[13] != Py_None) {
+    const Tensor* starts = as_list(args[13], dev, at::kInt, p.groups + 1);
+    if (!starts) Py_RETURN_NONE;
+    p.group_starts = starts->data_ptr<int32_t>();
+  }
+  p.prefix_lens = lens->data_ptr<int32_t>();
+  p.prefix_table = table->data_ptr<int32_t>();
+  p.prefix_stride = table->stride(0);
+  p.prefix_width = table->size(1);
+  p.own = call.a;
+  size_t need = 0;
+  const char* what = "shared_prefix_attention";
+  if (failed(ll_shared_prefix_attention_workspace(&p, 0, &need), what)) return nullptr;
+  const Tensor workspace = call.workspace(need);
+  p.own = call.a;
+  if (failed(ll_shared_prefix_attention(&p, stream_of(dev)), what)) return nullptr;
+  return call.result();
+  END_HANDLE_TH_ERRORS
+}
+
+// step_layout(new_lens, kv_lens, page_table, free_pages, page_size, num_tokens, prefix_lens, group_starts, cursor, kv_lens_out) -> (q_starts, kv_lens,
+// positions, slots, pages_wanted); the last four arguments may be None.
+PyObject* py_step_layout(PyObject*, PyObject* const* args, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  if (n != 10 || !plain(args[1])) Py_RETURN_NONE;
+  const int dev = current_device_of(THPVariable_Unpack(args[1]));
+  if (dev < 0) Py_RETURN_NONE;
+  ll_step_layout_args a{};
+  a.streams = THPVariable_Unpack(args[1]).numel();
+  const auto list = [&](PyObject* o, int64_t numel) -> int32_t* {
+    const Tensor* t = as_list(o, dev, at::kInt, numel);
+    return t ? t->data_ptr<int32_t>() : nullptr;
+  };
+  const Tensor* table = a.streams ? as_table(args[2], dev, a.streams) : nullptr;
+  int64_t page_size = 0;
+  if (!table || !apart(*table) || !plain(args[3]) || !as_count(args[4], page_size) || page_size < 1 || page_size > 0x7fffffff || !as_count(args[5], a.tokens) ||
+      a.tokens > 0x7fffffff)
+    Py_RETURN_NONE;
+  a.n_free = THPVariable_Unpack(args[3]).numel();
+  a.new_lens = list(args[0], a.streams);
+  a.kv_lens = list(args[1], a.streams);
+  a.free_pages = list(args[3], a.n_free);
+  if (!a.new_lens || !a.kv_lens || (!a.free_pages && a.n_free)) Py_RETURN_NONE;
+  a.page_table = table->data_ptr<int32_t>();
+  a.table_stride = stride_of(table, 0);
+  a.table_width = table->size(1);
+  a.page_size = (int)page_size;
+  if (args[6] != Py_None) {
+    const Tensor* lens = plain(args[6]) ? &THPVariable_Unpack(args[6]) : nullptr;
+    a.groups = lens ? lens->numel() : 0;
+    a.prefix_lens = lens ? list(args[6], a.groups) : nullptr;
+    if (!a.prefix_lens || (args[7] == Py_None && a.groups != 1)) Py_RETURN_NONE;
+    if (args[7] != Py_None && !(a.group_starts = list(args[7], a.groups + 1))) Py_RETURN_NONE;
+  } else if (args[7] != Py_None) {
+    Py_RETURN_NONE;
+  }
+  if (args[8] != Py_None && !(a.cursor = list(args[8], 1))) Py_RETURN_NONE;
+  if (args[9] != Py_None && !(a.kv_lens_out = list(args[9], a.streams))) Py_RETURN_NONE;
+  Tensor made[5];
+  made[0] = empty({a.streams + 1}, at::kInt, dev);
+  if (!a.kv_lens_out) {
+    made[1] = empty({a.streams}, at::kInt, dev);
+    a.kv_lens_out = made[1].data_ptr<int32_t>();
+  }
+  for (int i : {2, 3}) made[i] = empty({a.tokens}, at::kLong, dev);
+  made[4] = empty({1}, at::kInt, dev);
+  a.q_starts = made[0].data_ptr<int32_t>();
+  a.positions = made[2].data_ptr<int64_t>();
+  a.slots = made[3].data_ptr<int64_t>();
+  a.pages_wanted = made[4].data_ptr<int32_t>();
+  size_t need = 0;
+  if (failed(ll_step_layout_workspace(&a, &need), "lay_out_step")) return nullptr;
+  Tensor workspace;
   if (need) {
     workspace = empty({(int64_t)need}, at::kByte, dev);
     a.workspace = workspace.data_ptr();
     a.workspace_bytes = need;
   }
-  if (failed(ll_ragged_attention(&a, stream_of(dev)), what)) return nullptr;
-  if (args[5] != Py_None) {
-    Py_INCREF(args[5]);
-    return args[5];
+  if (failed(ll_step_layout(&a, stream_of(dev)), "lay_out_step")) return nullptr;
+  PyObject* r = PyTuple_New(5);
+  if (!r) return nullptr;
+  for (int i = 0; i < 5; ++i) {
+    PyObject* o;
+    if (i == 1 && args[9] != Py_None) {
+      Py_INCREF(args[9]);
+      o = args[9];
+    } else {
+      o = THPVariable_Wrap(made[i]);
+    }
+    PyTuple_SET_ITEM(r, i, o);
   }
-  return THPVariable_Wrap(out);
+  return r;
   END_HANDLE_TH_ERRORS
 }
+
+// What the kernels that norm and rotate heads take: the rows of q, k and, with pages, v, and where they go.
+struct HeadNormCall {
+  int dev = -1;
+  const Tensor *q = nullptr, *positions = nullptr;
+  int64_t T = 0, D = 0, n_slots = 0;
+  ll_head_rows q_rows{}, k_rows{}, v_rows{};
+  const int64_t* slots = nullptr;
+  bool paged = false;
+  PyObject* given_out = nullptr;
+  Tensor q_out, k_out;
+
+  bool take(PyObject* queries, PyObject* keys, PyObject* values, PyObject* const weights_of[2], PyObject* positions_of, PyObject* k_pages, PyObject* v_pages,
+            PyObject* slots_of, PyObject* to) {
+    if (!plain(queries)) return false;
+    dev = current_device_of(THPVariable_Unpack(queries));
+    if (dev < 0) return false;
+    q = as_rows(queries, dev, 3, nullptr);
+    const Tensor* k = q ? as_rows(keys, dev, 3, q) : nullptr;
+    if (!q || !k || k->size(0) != q->size(0) || k->size(2) != q->size(2)) return false;
+    T = q->size(0);
+    D = q->size(2);
+    if (D % 8 != 0 || D > 256) return false;
+    paged = k_pages != Py_None;
+    const Tensor* weights[2] = {nullptr, nullptr};
+    for (int i = 0; i < 2; ++i) {
+      if (weights_of[i] == Py_None) continue;
+      const Tensor* w = as_tensor(weights_of[i]);
+      if (!w || !as_list(weights_of[i], dev, w->scalar_type(), D) || (w->scalar_type() != q->scalar_type() && w->scalar_type() != at::kFloat) ||
+          !aligned16(w->data_ptr()))
+        return false;
+      weights[i] = w;
+    }
+    if (positions_of != Py_None && !(positions = as_list(positions_of, dev, at::kLong, T))) return false;
+    const Tensor *kp = nullptr, *vp = nullptr, *v = nullptr;
+    if (paged) {
+      kp = as_rows(k_pages, dev, 4, q);
+      vp = as_rows(v_pages, dev, 4, q);
+      v = as_rows(values, dev, 3, q);
+      const Tensor* at = as_list(slots_of, dev, at::kLong, T);
+      if (!kp || !vp || !v || !at || v->sizes() != k->sizes() || kp->sizes() != vp->sizes() || kp->size(2) != k->size(1) || kp->size(3) != D) return false;
+      for (const Tensor* t : {kp, vp})  // the cache's rows all as far apart
+        if (!apart(*t) || (t->size(0) > 1 && t->size(1) > 1 && t->stride(0) != t->size(1) * t->stride(1))) return false;
+      slots = at->data_ptr<int64_t>();
+      n_slots = kp->size(0) * kp->size(1);
+    }
+    if (to == Py_None) {
+      q_out = empty(q->sizes(), q->scalar_type(), dev);
+    } else {
+      const Tensor* given = as_rows(to, dev, 3, q);
+      if (!given || given->sizes() != q->sizes() || !apart(*given)) return false;
+      q_out = *given;
+      given_out = to;
+    }
+    const auto rows = [](const Tensor* x, const Tensor* weight, void* out, int64_t out_token, int64_t out_head) {
+      return ll_head_rows{x->data_ptr(), stride_of(x, 0), stride_of(x, 1), (int)x->size(1), weight ? weight->data_ptr() : nullptr,
+                          weight && weight->scalar_type() == at::kFloat, out, out_token, out_head};
+    };
+    q_rows = rows(q, weights[0], q_out.data_ptr(), stride_of(&q_out, 0), stride_of(&q_out, 1));
+    if (paged) {
+      const auto step = [](const Tensor* t) { return t->size(1) > 1 ? t->stride(1) : stride_of(t, 0); };
+      k_rows = rows(k, weights[1], kp->data_ptr(), step(kp), stride_of(kp, 2));
+      v_rows = rows(v, nullptr, vp->data_ptr(), step(vp), stride_of(vp, 2));
+    } else {
+      k_out = empty(k->sizes(), k->scalar_type(), dev);
+      k_rows = rows(k, weights[1], k_out.data_ptr(), stride_of(&k_out, 0), stride_of(&k_out, 1));
+    }
+    return true;
+  }
+
+  PyObject* result() {
+    PyObject* first = given_out;
+    if (first) Py_INCREF(first);
+    else first = THPVariable_Wrap(q_out);
+    if (paged) return first;
+    PyObject* both = PyTuple_New(2);
+    if (!both) return nullptr;
+    PyTuple_SET_ITEM(both, 0, first);
+    PyTuple_SET_ITEM(both, 1, THPVariable_Wrap(k_out));
+    return both;
+  }
+};
 
 // head_norm_rope(q, k, v or None, q_weight, k_weight, eps, cos, sin, positions, interleaved, k_pages, v_pages, slots, q_out) -> (q, k), or with
 // pages q; the weights, cos and sin, positions, pages (with v and slots) and q_out may be None.
 PyObject* py_head_norm_rope(PyObject*, PyObject* const* args, Py_ssize_t n) {
   HANDLE_TH_ERRORS
-  if (n != 14 || !plain(args[0])) Py_RETURN_NONE;
-  const int dev = current_device_of(THPVariable_Unpack(args[0]));
-  if (dev < 0) Py_RETURN_NONE;
-  const Tensor* q = as_rows(args[0], dev, 3, nullptr);
-  const Tensor* k = q ? as_rows(args[1], dev, 3, q) : nullptr;
-  if (!q || !k || k->size(0) != q->size(0) || k->size(2) != q->size(2) || !PyFloat_Check(args[5])) Py_RETURN_NONE;
-  const int64_t T = q->size(0), D = q->size(2);
-  if (D % 8 != 0 || D > 256) Py_RETURN_NONE;
-  const bool paged = args[10] != Py_None;
-  const Tensor *cos = nullptr, *sin = nullptr, *positions = nullptr, *weights[2] = {nullptr, nullptr};
-  for (int i = 0; i < 2; ++i) {
-    if (args[3 + i] == Py_None) continue;
-    const Tensor* w = as_tensor(args[3 + i]);
-    if (!w || !as_list(args[3 + i], dev, w->scalar_type(), D) || (w->scalar_type() != q->scalar_type() && w->scalar_type() != at::kFloat) || !aligned16(w->data_ptr()))
-      Py_RETURN_NONE;
-    weights[i] = w;
-  }
+  if (n != 14 || !PyFloat_Check(args[5])) Py_RETURN_NONE;
+  HeadNormCall call;
+  if (!call.take(args[0], args[1], args[2], args + 3, args[8], args[10], args[11], args[12], args[13])) Py_RETURN_NONE;
+  const Tensor *cos = nullptr, *sin = nullptr;
   if (args[6] != Py_None || args[7] != Py_None) {
     cos = as_tensor(args[6]);
     sin = as_tensor(args[7]);
     for (const Tensor* t : {cos, sin})
-      if (!t || !on_device(*t, dev) || t->scalar_type() != at::kFloat || t->dim() != 2 || t->sizes() != cos->sizes() || !t->is_contiguous() || !aligned16(t->data_ptr()))
+      if (!t || !on_device(*t, call.dev) || t->scalar_type() != at::kFloat || t->dim() != 2 || t->sizes() != cos->sizes() || !t->is_contiguous() ||
+          !aligned16(t->data_ptr()))
         Py_RETURN_NONE;
-    if (2 * cos->size(1) % 8 != 0 || 2 * cos->size(1) > D || cos->numel() == 0) Py_RETURN_NONE;
+    if (2 * cos->size(1) % 8 != 0 || 2 * cos->size(1) > call.D || cos->numel() == 0) Py_RETURN_NONE;
   }
-  if (args[8] != Py_None && !(positions = as_list(args[8], dev, at::kLong, T))) Py_RETURN_NONE;
-  Tensor q_out, k_out;
-  if (args[13] == Py_None) {
-    q_out = empty(q->sizes(), q->scalar_type(), dev);
-  } else {
-    const Tensor* given = as_rows(args[13], dev, 3, q);
-    if (!given || given->sizes() != q->sizes() || !apart(*given)) Py_RETURN_NONE;
-    q_out = *given;
-  }
-  const auto rows = [](const Tensor* x, const Tensor* weight, void* out, int64_t out_token, int64_t out_head) {
-    return ll_head_rows{x->data_ptr(), stride_of(x, 0), stride_of(x, 1), (int)x->size(1), weight ? weight->data_ptr() : nullptr,
-                        weight && weight->scalar_type() == at::kFloat, out, out_token, out_head};
-  };
-  const ll_head_rows q_rows = rows(q, weights[0], q_out.data_ptr(), stride_of(&q_out, 0), stride_of(&q_out, 1));
-  ll_head_rows k_rows{}, v_rows{};
-  const int64_t* slots = nullptr;
-  int64_t n_slots = 0;
-  if (paged) {
-    const Tensor *kp = as_rows(args[10], dev, 4, q), *vp = as_rows(args[11], dev, 4, q), *v = as_rows(args[2], dev, 3, q);
-    const Tensor* at = as_list(args[12], dev, at::kLong, T);
-    if (!kp || !vp || !v || !at || v->sizes() != k->sizes() || kp->sizes() != vp->sizes() || kp->size(2) != k->size(1) || kp->size(3) != D) Py_RETURN_NONE;
-    for (const Tensor* t : {kp, vp})  // the cache's rows all as far apart
-      if (!apart(*t) || (t->size(0) > 1 && t->size(1) > 1 && t->stride(0) != t->size(1) * t->stride(1))) Py_RETURN_NONE;
-    const auto step = [](const Tensor* t) { return t->size(1) > 1 ? t->stride(1) : stride_of(t, 0); };
-    k_rows = rows(k, weights[1], kp->data_ptr(), step(kp), stride_of(kp, 2));
-    v_rows = rows(v, nullptr, vp->data_ptr(), step(vp), stride_of(vp, 2));
-    slots = at->data_ptr<int64_t>();
-    n_slots = kp->size(0) * kp->size(1);
-  } else {
-    k_out = empty(k->sizes(), k->scalar_type(), dev);
-    k_rows = rows(k, weights[1], k_out.data_ptr(), stride_of(&k_out, 0), stride_of(&k_out, 1));
-  }
-  if (failed(ll_head_norm_rope(half_code(*q), T, (int)D, &q_rows, &k_rows, paged ? &v_rows : nullptr, (float)PyFloat_AsDouble(args[5]),
-                               cos ? cos->data_ptr<float>() : nullptr, sin ? sin->data_ptr<float>() : nullptr, cos ? cos->size(0) : 0,
-                               cos ? (int)(2 * cos->size(1)) : 0, positions ? positions->data_ptr<int64_t>() : nullptr, args[9] == Py_True, slots, n_slots,
-                               stream_of(dev)),
+  if (failed(ll_head_norm_rope(half_code(*call.q), call.T, (int)call.D, &call.q_rows, &call.k_rows, call.paged ? &call.v_rows : nullptr,
+                               (float)PyFloat_AsDouble(args[5]), cos ? cos->data_ptr<float>() : nullptr, sin ? sin->data_ptr<float>() : nullptr,
+                               cos ? cos->size(0) : 0, cos ? (int)(2 * cos->size(1)) : 0, call.positions ? call.positions->data_ptr<int64_t>() : nullptr,
+                               args[9] == Py_True, call.slots, call.n_slots, stream_of(call.dev)),
              "head_norm_rope"))
     return nullptr;
-  PyObject* first;
-  if (args[13] != Py_None) {
-    Py_INCREF(args[13]);
-    first = args[13];
-  } else {
-    first = THPVariable_Wrap(q_out);
-  }
-  if (paged) return first;
-  PyObject* both = PyTuple_New(2);
-  if (!both) return nullptr;
-  PyTuple_SET_ITEM(both, 0, first);
-  PyTuple_SET_ITEM(both, 1, THPVariable_Wrap(k_out));
-  return both;
+  return call.result();
+  END_HANDLE_TH_ERRORS
+}
+
+// rotate_by_position(q, k, v or None, q_weight, k_weight, eps, frequencies, amplitude, positions, interleaved, grid rows, grid columns, pairs of
+// frames, pairs of rows, k_pages, v_pages, slots, q_out) -> as head_norm_rope
+PyObject* py_rotate_by_position(PyObject*, PyObject* const* args, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  if (n != 18 || !PyFloat_Check(args[5]) || !PyFloat_Check(args[7])) Py_RETURN_NONE;
+  HeadNormCall call;
+  if (!call.take(args[0], args[1], args[2], args + 3, args[8], args[14], args[15], args[16], args[17])) Py_RETURN_NONE;
+  const Tensor* f = as_tensor(args[6]);
+  int64_t pairs[2];
+  ll_position_angles angles{};
+  if (!f || !as_list(args[6], call.dev, at::kDouble, f->numel()) || f->numel() == 0 || f->numel() % 4 != 0 || 2 * f->numel() > call.D || !aligned16(f->data_ptr()) ||
+      !as_count(args[10], angles.grid_rows) || !as_count(args[11], angles.grid_columns) || !as_count(args[12], pairs[0]) || !as_count(args[13], pairs[1]) ||
+      pairs[0] + pairs[1] > f->numel())
+    Py_RETURN_NONE;
+  angles.frequencies = f->data_ptr<double>();
+  angles.rotary_dim = (int)(2 * f->numel());
+  angles.amplitude = (float)PyFloat_AsDouble(args[7]);
+  angles.frame_pairs = (int)pairs[0];
+  angles.row_pairs = (int)pairs[1];
+  if (failed(ll_rotate_by_position(half_code(*call.q), call.T, (int)call.D, &call.q_rows, &call.k_rows, call.paged ? &call.v_rows : nullptr,
+                                   (float)PyFloat_AsDouble(args[5]), &angles, call.positions ? call.positions->data_ptr<int64_t>() : nullptr,
+                                   args[9] == Py_True, call.slots, call.n_slots, stream_of(call.dev)),
+             "rotate_by_position"))
+    return nullptr;
+  return call.result();
   END_HANDLE_TH_ERRORS
 }
 
@@ -1237,6 +1438,9 @@ PyMethodDef methods[] = {
     {"head", (PyCFunction)(void (*)(void))py_head, METH_FASTCALL, nullptr},
     {"unipc_step", (PyCFunction)(void (*)(void))py_unipc_step, METH_FASTCALL, nullptr},
     {"ragged_attention", (PyCFunction)(void (*)(void))py_ragged_attention, METH_FASTCALL, nullptr},
+    {"shared_prefix_attention", (PyCFunction)(void (*)(void))py_shared_prefix_attention, METH_FASTCALL, nullptr},
+    {"step_layout", (PyCFunction)(void (*)(void))py_step_layout, METH_FASTCALL, nullptr},
+    {"rotate_by_position", (PyCFunction)(void (*)(void))py_rotate_by_position, METH_FASTCALL, nullptr},
     {"head_norm_rope", (PyCFunction)(void (*)(void))py_head_norm_rope, METH_FASTCALL, nullptr},
     {"recording", py_recording, METH_O, nullptr},
     {"current_stream", py_current_stream, METH_NOARGS, nullptr},

@@ -52,7 +52,8 @@ constexpr float kLog2E = 1.4426950408889634f;
 constexpr uint32_t kRaJoinGroups = 256;
 
 // Where keys lie: in the pages of a table, in rows one behind the other, in such rows with a mask.
-constexpr int kRaPaged = 0, kRaRows = 1, kRaMaskedRows = 2;
+// Shared: in the pages of a table, behind those of a beginning that a group of streams shares.
+constexpr int kRaPaged = 0, kRaRows = 1, kRaMaskedRows = 2, kRaShared = 3;
 
 struct RaParams {
   const uint16_t* q;
@@ -83,6 +84,12 @@ struct RaParams {
   float part_share;       // not 0: part_steps follow from the streams, this times the steps of all wide tiles of a head
   uint32_t records;       // of a kv head, 32 rows each
   float* record_mem;      // [kv head][records]: 32 x D columns, then reference point and sum of each row
+  // Shared beginnings.  `records` is not used: results of parts lie by row, [prefix_parts + own_parts][n_queries][heads] of D columns, then
+  // as many reference points and sums.
+  const int32_t *group_starts, *prefix_lens, *prefix_table;
+  int64_t prefix_stride, prefix_keys;  // keys that a row of the table reaches
+  int n_groups;
+  uint32_t prefix_part_steps, prefix_parts, own_parts;  // steps of a part, and how many there are at most; 0 prefix_parts: none is joined
 };
 
 // Positions of 16-byte pieces in an LDS row of D columns.  The reads of a wave then go through all banks: 8 neighbouring rows of one
@@ -143,6 +150,42 @@ __device__ __forceinline__ int64_t stream_start(const RaParams& p, int b) { retu
 // The lowest n of 64 bits, for any n.
 __device__ __forceinline__ uint64_t low_bits(int n) { return n <= 0 ? 0 : n >= 64 ? ~0ull : ~(~0ull << n); }
 
+// A group of streams, its rows of q and the keys that it shares.
+struct RaGroup {
+  int q0, n, len;
+  bool joined;  // its rows attend the beginning together, each stream's rows then its own keys, and the two are joined; else one behind the other
+};
+// Going together saves a group of m streams about m / 2 tiles of every step of the beginning, what its streams' last tiles lack, and costs two
+// records of every row: it is done from this many steps times streams to a tile on.
+constexpr int kRaJoinedCost = 28;
+__device__ __forceinline__ RaGroup group_of(const RaParams& p, int g) {
+  const int from = p.group_starts ? min(max(p.group_starts[g], 0), p.streams) : 0;
+  const int to = p.group_starts ? min(max(p.group_starts[g + 1], from), p.streams) : p.streams;
+  RaGroup r;
+  const int limit = (int)p.n_queries;
+  r.q0 = min(max(p.q_starts[from], 0), limit);
+  r.n = max(min(max(p.q_starts[to], 0), limit) - r.q0, 0);
+  r.len = (int)min((int64_t)max(p.prefix_lens[g], 0), p.prefix_keys);
+  r.joined = p.prefix_parts > 0 && to - from > 1 &&
+             (int64_t)(to - from) * (r.len / kRaKeys) >= (int64_t)kRaJoinedCost * (((uint32_t)r.n * p.group.d + kRaTileRows - 1) / kRaTileRows);
+  return r;
+}
+// The group of a stream, -1 for none.
+__device__ __forceinline__ int group_of_stream(const RaParams& p, int b) {
+  if (p.n_groups == 0) return -1;
+  if (!p.group_starts) return 0;
+  int g = 0, end = p.n_groups + 1;  // the last that begins at or before it
+  while (end - g > 1) {
+    const int at = (g + end) >> 1;
+    if (p.group_starts[at] <= b) g = at;
+    else end = at;
+  }
+  return g < p.n_groups && p.group_starts[g] <= b ? g : -1;
+}
+__device__ __forceinline__ int steps_of(int keys) { return (keys + kRaKeys - 1) / kRaKeys; }
+// Parts of a tile that takes so many steps.
+__device__ __forceinline__ int shared_parts(uint32_t steps, uint32_t per_part, uint32_t most) { return (int)min((steps + per_part - 1) / per_part, most); }
+
 // What a workgroup does next: a part of a tile.
 struct RaItem {
   int64_t q0;               // first row of q of the stream
@@ -155,6 +198,10 @@ struct RaItem {
   int s_begin, s_end;       // of these, the part's
   int n_parts, part;
   uint32_t record;          // of part 0; the others follow, each as many records as the tile has groups of 32 rows
+  // Shared: of the tile's steps the first go over the beginning, whose keys have the numbers -64 prefix_steps and up.
+  const int32_t* prefix_pages;
+  int prefix_steps, prefix_len;
+  bool to_record;           // the part's results are joined with others
 };
 
 // The streams b0 .. b0 + 63, one a lane.
@@ -162,6 +209,7 @@ struct RaStreams {
   int q0, n, len, base, key0;
   int parts;                          // at most: of the tile that sees most keys
   uint32_t items_upto, records_upto;  // of these and the streams before
+  int shares, prefix_len, joined;     // shared: the group, or -1; keys of its beginning that the items go over; whether others are joined with them
 };
 
 // Steps of a tile whose first and last token sit at pos0 and pos1, of a stream of len keys.
@@ -253,6 +301,50 @@ __device__ __forceinline__ RaStreams load_streams(const RaParams& p, int b0, uin
   return s;
 }
 
+// With shared beginnings: first the groups, whose items are the beginnings that are attended together, then the streams.
+__device__ __forceinline__ RaStreams load_shared(const RaParams& p, int b0, uint32_t items) {
+  const int at = b0 + (threadIdx.x & 63);
+  RaStreams s{};
+  s.shares = -1;
+  int steps = 0;
+  uint32_t per_part = 1, most = 1;
+  if (at < p.n_groups) {
+    const RaGroup g = group_of(p, at);
+    if (g.joined) {
+      s.q0 = g.q0;
+      s.n = g.n;
+      s.shares = at;
+      s.joined = 1;
+      s.prefix_len = g.len;
+      steps = steps_of(g.len);
+      per_part = p.prefix_part_steps;
+      most = p.prefix_parts;
+    }
+  } else if (at < p.n_groups + p.streams) {
+    const int b = at - p.n_groups, limit = (int)p.n_queries;
+    const int next = p.q_starts[b + 1];
+    s.q0 = min(max(p.q_starts[b], 0), limit);
+    s.n = max(min(max(next, 0), limit) - s.q0, 0);
+    const int64_t given = max((int64_t)p.kv_lens[b], (int64_t)0);
+    s.len = (int)min(given, p.table_keys);
+    s.base = (int)(given - ((int64_t)next - s.q0));
+    s.shares = group_of_stream(p, b);
+    if (s.shares >= 0) {
+      const RaGroup g = group_of(p, s.shares);
+      s.joined = g.joined;
+      if (!g.joined) s.prefix_len = g.len;
+    }
+    steps = steps_of(s.prefix_len) + steps_of(s.len);
+    per_part = s.n * (int)p.group.d <= 32 ? p.narrow_part_steps : p.part_steps;
+    most = p.own_parts;
+  }
+  const int tiles = tiles_of(s.n * (int)p.group.d);
+  // a joined stream without keys of its own has nothing to add, one that is not has its zeros to write
+  s.parts = max(shared_parts((uint32_t)steps, per_part, most), s.joined ? 0 : 1);
+  s.items_upto = items + sum_upto((uint32_t)(tiles * s.parts));
+  return s;
+}
+
 // Finds items one behind the other.
 template <int KIND, bool COUNT_TILES>
 struct RaCursor {
@@ -262,7 +354,11 @@ struct RaCursor {
   RaStreams s;                      // streams from b0 on
   __device__ __forceinline__ void start(const RaParams& p) {
     part_steps = p.part_steps;
-    if (p.streams > 0) s = load_streams<KIND, COUNT_TILES>(p, 0, 0, 0, part_steps);
+    if constexpr (KIND == kRaShared) {
+      if (p.streams > 0) s = load_shared(p, 0, 0);
+    } else {
+      if (p.streams > 0) s = load_streams<KIND, COUNT_TILES>(p, 0, 0, 0, part_steps);
+    }
   }
   // Item `index` of a kv head, which is no smaller than the last one asked for.  All lanes call it together.  False: there are fewer.
   __device__ __forceinline__ bool find(const RaParams& p, uint32_t index, RaItem& t) {
@@ -286,6 +382,26 @@ struct RaCursor {
         t.key0 = of(s.key0);
         t.pages = KIND == kRaPaged ? p.page_table + (int64_t)(b0 + at) * p.table_stride : nullptr;
         const int last_row = min(t.first + kRaTileRows, t.rows) - 1;
+        if constexpr (KIND == kRaShared) {
+          const int b = b0 + at - p.n_groups, shares = of(s.shares);  // b below 0: a beginning
+          t.prefix_len = of(s.prefix_len);
+          t.prefix_steps = steps_of(t.prefix_len);
+          t.prefix_pages = p.prefix_table + (int64_t)max(shares, 0) * p.prefix_stride;
+          t.pages = p.page_table + (int64_t)max(b, 0) * p.table_stride;
+          const int end = p.causal ? min(t.base + (int)((uint32_t)last_row / p.group) + 1, t.len) : t.len;
+          const int steps = t.prefix_steps + (end > 0 ? steps_of(end) : 0);
+          // As the joining launch counts them.  A tile that sees fewer keys than the stream's last leaves parts out.
+          const uint32_t per_part = b < 0 ? p.prefix_part_steps : t.rows <= 32 ? p.narrow_part_steps : p.part_steps;
+          t.n_parts = min(shared_parts((uint32_t)steps, per_part, (uint32_t)parts), parts);
+          const bool joined = of(s.joined) != 0;
+          if (!joined) t.n_parts = max(t.n_parts, 1);
+          const int each = t.n_parts > 0 ? (steps + t.n_parts - 1) / t.n_parts : 0;
+          t.s_begin = min(t.part * each, steps);
+          t.s_end = min(t.s_begin + each, steps);
+          t.record = b < 0 ? 0 : p.prefix_parts;
+          t.to_record = joined || t.n_parts > 1;
+          return true;
+        }
         const RaSpan span = span_of(p, t.len, t.base + (int)((uint32_t)t.first / p.group), t.base + (int)((uint32_t)last_row / p.group));
         t.sink_steps = span.sink_steps;
         t.from_step = span.from_step;
@@ -298,8 +414,12 @@ struct RaCursor {
         return true;
       }
       b0 += 64;
-      if (b0 >= p.streams) return false;
+      if (b0 >= p.streams + (KIND == kRaShared ? p.n_groups : 0)) return false;
       items = (uint32_t)__builtin_amdgcn_readlane((int)s.items_upto, 63);
+      if constexpr (KIND == kRaShared) {
+        s = load_shared(p, b0, items);
+        continue;
+      }
       records = min((uint32_t)__builtin_amdgcn_readlane((int)s.records_upto, 63), p.records + 1);
       s = load_streams<KIND, COUNT_TILES>(p, b0, items, records, part_steps);
     }
@@ -316,6 +436,17 @@ template <int D>
 __device__ __forceinline__ float2* record_sums(const RaParams& p, uint32_t head, const RaItem& t, int part, int row) {
   const int64_t at = (int64_t)head * p.records + t.record + (uint32_t)(part * record_groups(t.rows) + row / 32);
   return reinterpret_cast<float2*>(p.record_mem + at * 32 * (D + 2) + 32 * D) + row % 32;
+}
+
+// Shared: where part `slot` of all has a row's columns, and its reference point and sum.
+template <int D>
+__device__ __forceinline__ float* shared_record(const RaParams& p, uint32_t slot, int64_t token, int head) {
+  return p.record_mem + (((int64_t)slot * p.n_queries + token) * p.heads + head) * D;
+}
+template <int D>
+__device__ __forceinline__ float2* shared_sums(const RaParams& p, uint32_t slot, int64_t token, int head) {
+  const int64_t rows = p.n_queries * p.heads;
+  return reinterpret_cast<float2*>(p.record_mem + (int64_t)(p.prefix_parts + p.own_parts) * rows * D) + ((int64_t)slot * p.n_queries + token) * p.heads + head;
 }
 
 template <int D>
@@ -348,7 +479,7 @@ __global__ __launch_bounds__(kRaThreads, D == 64 ? 3 : 2) void ragged_attention_
   constexpr int kRowBytes = 2 * D, kPieces = D / 8, kDTiles = D / 32, kSteps = D / 16;
   constexpr int kRowsPerLoad = 1024 / kRowBytes, kGroupLoads = 16 / kRowsPerLoad;  // loads of 16 rows
   constexpr int kStepBytes = kRaKeys * kRowBytes;                                  // K or V of a step
-  constexpr bool kLooksUp = KIND != kRaRows;
+  constexpr bool kLooksUp = KIND != kRaRows, kPages = KIND == kRaPaged || KIND == kRaShared;
   extern __shared__ __attribute__((aligned(1024))) uint8_t smem[];
   if (blockIdx.x >= p.groups) {  // rows outside every stream
     const int64_t first = p.streams ? stream_start(p, 0) : 0, end = p.streams ? max(stream_start(p, p.streams), first) : 0;
@@ -399,8 +530,10 @@ __global__ __launch_bounds__(kRaThreads, D == 64 ? 3 : 2) void ragged_attention_
   const Row row = own_row();
   // what it sees: keys below `last`, from `from` on or below the sink
   const int pos = t.base + row.token;
-  const int last = p.causal ? min(pos + 1, t.len) : t.len;
-  const int from = p.window && pos >= (int)p.window ? pos - (int)p.window + 1 : 0;
+  // (shared: keys of the beginning have numbers below zero, and every row sees them)
+  int last = p.causal ? min(pos + 1, t.len) : t.len;
+  if constexpr (KIND == kRaShared) last = max(last, 0);
+  const int from = KIND == kRaShared ? -(1 << 30) : p.window && pos >= (int)p.window ? pos - (int)p.window + 1 : 0;
   // the same for the wave's first and last row, which bound the others
   const int last0 = __builtin_amdgcn_readfirstlane(last), from1 = __builtin_amdgcn_readlane(from, 31);
   const bool idle = own >= tile_rows;  // a wave without rows only moves keys
@@ -417,10 +550,20 @@ __global__ __launch_bounds__(kRaThreads, D == 64 ? 3 : 2) void ragged_attention_
   // ---- where the keys of 64 lanes lie
   uint8_t* const looked_up = smem + 4 * kStepBytes + wave * 512;
   const uint32_t looked_up_lds = lds_at(looked_up);
-  auto key_base = [&](int s) __attribute__((always_inline)) { return (s < t.sink_steps ? s : t.from_step + s - t.sink_steps) * kRaKeys; };
+  auto key_base = [&](int s) __attribute__((always_inline)) {
+    if constexpr (KIND == kRaShared) return (s - t.prefix_steps) * kRaKeys;
+    return (s < t.sink_steps ? s : t.from_step + s - t.sink_steps) * kRaKeys;
+  };
   uint32_t next_row = 0;
   auto look_up = [&](int key, int slot) __attribute__((always_inline)) {
-    const uint32_t k = (uint32_t)min(key, t.len - 1);
+    uint32_t k = (uint32_t)min(key, t.len - 1);
+    if constexpr (KIND == kRaShared) {  // all 64 keys of a step lie on one side
+      const bool shared = __builtin_amdgcn_readfirstlane(key) < 0;
+      k = (uint32_t)min(shared ? key + t.prefix_steps * kRaKeys : key, (shared ? t.prefix_len : t.len) - 1);
+      const uint32_t page = k / p.page;
+      next_row = k - page * p.page.d;
+      load4_to_lds((shared ? t.prefix_pages : t.pages) + page, looked_up_lds + slot * 256);
+    }
     if constexpr (KIND == kRaPaged) {
       const uint32_t page = k / p.page;
       next_row = k - page * p.page.d;
@@ -435,8 +578,9 @@ __global__ __launch_bounds__(kRaThreads, D == 64 ? 3 : 2) void ragged_attention_
   auto take_places = [&](int base, int at, int slot) __attribute__((always_inline)) {
     const int key = base + at;
     bool ok = key < t.len;
+    if constexpr (KIND == kRaShared) ok = base < 0 ? key + t.prefix_steps * kRaKeys < t.prefix_len : ok;
     first_key = base;
-    if constexpr (KIND == kRaPaged) {
+    if constexpr (kPages) {
       at_page = *reinterpret_cast<const uint32_t*>(looked_up + slot * 256 + lane * 4);
       at_row = next_row;  // of the key that was looked up last, which is this one where it exists
       ok = ok && at_page < p.n_pages;
@@ -456,7 +600,7 @@ __global__ __launch_bounds__(kRaThreads, D == 64 ? 3 : 2) void ragged_attention_
   typedef __attribute__((address_space(3))) u32x4* lds_uint4;
   // 16 rows from a multiple of 16 on lie one behind the other, and take one address for a wave in place of one for a lane: 532 x 40 / 8 heads
   // over 9000 keys in pages of 32 rows 118 us, of 24 rows 143.
-  const bool whole_pages = KIND == kRaPaged && p.page.d % 16 == 0;
+  const bool whole_pages = kPages && p.page.d % 16 == 0;
   // counted: as many loads whatever keys there are, for waits that leave some under way.
   auto load_rows = [&](bool values, int r0, uint32_t lds, bool counted) __attribute__((always_inline)) {
     const uint16_t* base = values ? v_head : k_head;
@@ -466,7 +610,7 @@ __global__ __launch_bounds__(kRaThreads, D == 64 ? 3 : 2) void ragged_attention_
     // 16 rows one behind the other that may be read, whether they hold keys or not.
     bool in_line;
     uint64_t at;
-    if constexpr (KIND == kRaPaged) {
+    if constexpr (kPages) {
       in_line = whole_pages && (exist & 1);
       at = (uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)at_page, r0) * per_page + (uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)at_row, r0) * per_row;
     } else {
@@ -498,7 +642,7 @@ __global__ __launch_bounds__(kRaThreads, D == 64 ? 3 : 2) void ragged_attention_
 #pragma unroll
       for (int i = 0; i < kGroupLoads; ++i) {
         const int in_group = i * kRowsPerLoad + row0, row = r0 + in_group;
-        if constexpr (KIND == kRaPaged) {
+        if constexpr (kPages) {
           at = (uint64_t)(uint32_t)__shfl((int)at_page, row) * per_page + (uint64_t)(uint32_t)__shfl((int)at_row, row) * per_row;
         } else {
           at = (uint64_t)(uint32_t)(t.key0 + first_key + row) * per_row;
@@ -535,6 +679,7 @@ __global__ __launch_bounds__(kRaThreads, D == 64 ? 3 : 2) void ragged_attention_
   };
   // Whether there are keys from `base` to `end` that a row of the wave does not see.
   auto uneven = [&](int base, int end) __attribute__((always_inline)) {
+    if constexpr (KIND == kRaShared) return min(end, t.len) > last0;
     return KIND == kRaPaged && (min(end, t.len) > last0 || (base < from1 && end > (int)p.sink));
   };
   auto seen_from = [&](int base) __attribute__((always_inline)) {  // of 64 keys from `base` on, those that the lane's row may see
@@ -753,8 +898,16 @@ __global__ __launch_bounds__(kRaThreads, D == 64 ? 3 : 2) void ragged_attention_
     return mx;
   };
 
+  const bool to_record = KIND == kRaShared ? t.to_record : t.n_parts > 1;
   auto write_record = [&](int row_in_tile, int column, const float (&v)[4], float mm, float ll) __attribute__((always_inline)) {
     // four columns of a row of this part's record
+    if constexpr (KIND == kRaShared) {
+      const int f = t.first + row_in_tile, token = (uint32_t)f / p.group, head = kv_head * p.group.d + (f - token * p.group.d);
+      const uint32_t slot = t.record + t.part;
+      *reinterpret_cast<float4*>(shared_record<D>(p, slot, t.q0 + token, head) + column) = make_float4(v[0], v[1], v[2], v[3]);
+      if (column == 0) *shared_sums<D>(p, slot, t.q0 + token, head) = make_float2(mm, ll);
+      return;
+    }
     *reinterpret_cast<float4*>(record_of<D>(p, kv_head, t, t.part, row_in_tile) + column) = make_float4(v[0], v[1], v[2], v[3]);
     if (column == 0) *record_sums<D>(p, kv_head, t, t.part, row_in_tile) = make_float2(mm, ll);
   };
@@ -829,7 +982,7 @@ __global__ __launch_bounds__(kRaThreads, D == 64 ? 3 : 2) void ragged_attention_
       }
       __syncthreads();
     };
-    const bool may_differ = KIND == kRaPaged && (p.causal || p.window);
+    const bool may_differ = kPages && (p.causal || p.window);
     if (idle) {
       if (s_begin < s_end) {
         for (int s = s_begin; s + 1 < s_end; ++s) move_keys(s);
@@ -872,7 +1025,7 @@ __global__ __launch_bounds__(kRaThreads, D == 64 ? 3 : 2) void ragged_attention_
       if (may_differ && __syncthreads_or(!finite)) apart();
     }
     l = exchange_sum(l);
-    if (t.n_parts > 1) {
+    if (to_record) {
       if (own + l32 < tile_rows) {
 #pragma unroll
         for (int dt = 0; dt < kDTiles; ++dt)
@@ -962,7 +1115,7 @@ __global__ __launch_bounds__(kRaThreads, D == 64 ? 3 : 2) void ragged_attention_
       }
     }
   }
-  if (KIND == kRaPaged && !finite) {  // once more, group by group (see all_finite)
+  if (kPages && !finite) {  // once more, group by group (see all_finite)
     once_more();
 #pragma unroll 1
     for (u = 2 * s_begin + wave; u < u_end; u += 4) {
@@ -1019,8 +1172,8 @@ __global__ __launch_bounds__(kRaThreads, D == 64 ? 3 : 2) void ragged_attention_
       v[3] = fmaf(e.w, weight[w], v[3]);
     }
     const int column = 32 * dt + 8 * g + 4 * lh;
-    if (l32 < tile_rows && t.n_parts > 1) write_record(l32, column, v, all_m, all_l);
-    if (l32 < tile_rows && t.n_parts == 1)
+    if (l32 < tile_rows && to_record) write_record(l32, column, v, all_m, all_l);
+    if (l32 < tile_rows && !to_record)
       *reinterpret_cast<uint2*>(p.out + (t.q0 + to.token) * p.out_stride_token + to.head * p.out_stride_head + column) =
           make_uint2(T::pack2(v[0] * inv, v[1] * inv), T::pack2(v[2] * inv, v[3] * inv));
   }
@@ -1061,6 +1214,68 @@ __global__ __launch_bounds__(kRaThreads) void ragged_join_kernel(RaParams p) {
       const int f = t.first + row, token = (uint32_t)f / p.group, head = kv_head * p.group.d + (f - token * p.group.d);
       uint16_t* dst = p.out + (t.q0 + token) * p.out_stride_token + head * p.out_stride_head + column;
       *reinterpret_cast<uint2*>(dst) = make_uint2(T::pack2(v[0] * inv, v[1] * inv), T::pack2(v[2] * inv, v[3] * inv));
+    }
+  }
+}
+
+// Joins, row by row, the parts of what a group attended together with the parts of the streams' own keys, and the parts of tiles that were cut:
+// D / 4 lanes a row, the heads of one token to a workgroup, or some of them.
+template <typename T, int D>
+__global__ __launch_bounds__(kRaThreads) void shared_join_kernel(RaParams p) {
+  constexpr int kRows = kRaThreads * 4 / D;
+  const int lane = threadIdx.x & 63, column = threadIdx.x % (D / 4) * 4;
+  for (int64_t token = blockIdx.x; token < p.n_queries; token += gridDim.x) {
+    // the last stream that begins at or before the token: 64 of what is left at a time
+    int b = 0, left = p.streams + 1;
+    while (left > 1) {
+      const int step = (left + 63) / 64, at = lane * step;
+      const int before = __popcll(__builtin_amdgcn_ballot_w64(at < left && p.q_starts[min(b + at, p.streams)] <= token));
+      const int found = max(before - 1, 0) * step;
+      b += found;
+      left = min(step, left - found);
+    }
+    b = __builtin_amdgcn_readfirstlane(b);
+    if (b >= p.streams || p.q_starts[b] > token) continue;
+    const int limit = (int)p.n_queries, next = p.q_starts[b + 1];
+    const int q0 = min(max(p.q_starts[b], 0), limit), n = max(min(max(next, 0), limit) - q0, 0);
+    const int64_t given = max((int64_t)p.kv_lens[b], (int64_t)0);
+    const int len = (int)min(given, p.table_keys), base = (int)(given - ((int64_t)next - q0));
+    const int g = group_of_stream(p, b);
+    int of_group = 0, ahead = 0;  // parts of the beginning; or its steps, ahead of the stream's own
+    bool joined = false;
+    if (g >= 0) {
+      const RaGroup r = group_of(p, g);
+      joined = r.joined;
+      if (joined) of_group = shared_parts((uint32_t)steps_of(r.len), p.prefix_part_steps, p.prefix_parts);
+      else ahead = steps_of(r.len);
+    }
+    const int rows = n * (int)p.group.d;
+    const uint32_t per_part = rows <= 32 ? p.narrow_part_steps : p.part_steps;
+    for (int head = blockIdx.y * kRows + threadIdx.x / (D / 4); head < p.heads; head += gridDim.y * kRows) {
+      const int f = (int)(token - q0) * (int)p.group.d + (int)((uint32_t)head - (uint32_t)head / p.group * p.group.d);
+      const int last_row = min(f / kRaTileRows * kRaTileRows + kRaTileRows, rows) - 1;
+      const int end = p.causal ? min(base + (int)((uint32_t)last_row / p.group) + 1, len) : len;
+      const int parts = shared_parts((uint32_t)(ahead + (end > 0 ? steps_of(end) : 0)), per_part, p.own_parts);
+      if (!joined && parts <= 1) continue;  // its results are where they belong
+      float m = -INFINITY, l = 0.0f, v[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll 4
+      for (int i = 0; i < of_group + parts; ++i) {
+        const uint32_t slot = i < of_group ? i : p.prefix_parts + i - of_group;
+        const float2 e = *shared_sums<D>(p, slot, token, head);
+        const float4 y = *reinterpret_cast<const float4*>(shared_record<D>(p, slot, token, head) + column);
+        const float top = fmaxf(m, e.x);
+        const float a = m == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f((m - top) * reference_unit<T>(p.scale_log2));
+        const float c = e.x == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f((e.x - top) * reference_unit<T>(p.scale_log2));
+        l = (m == -INFINITY ? l : l * a) + (e.x == -INFINITY ? e.y : e.y * c);  // as in the other joining launch
+        v[0] = fmaf(y.x, c, v[0] * a);
+        v[1] = fmaf(y.y, c, v[1] * a);
+        v[2] = fmaf(y.z, c, v[2] * a);
+        v[3] = fmaf(y.w, c, v[3] * a);
+        m = top;
+      }
+      const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+      *reinterpret_cast<uint2*>(p.out + token * p.out_stride_token + head * p.out_stride_head + column) =
+          make_uint2(T::pack2(v[0] * inv, v[1] * inv), T::pack2(v[2] * inv, v[3] * inv));
     }
   }
 }
@@ -1232,12 +1447,8 @@ static int launch_ragged(const RaParams& p, int kind, uint32_t grid, hipStream_t
   if (kind == kRaRows) return launch_ragged<T, D, kRaRows>(p, grid, stream);
   return launch_ragged<T, D, kRaMaskedRows>(p, grid, stream);
 }
-}  // namespace ll
 
-extern "C" int ll_ragged_attention(const ll_ragged_attention_args* a, void* stream) {
-  using namespace ll;
-  if (int rc = check_ragged(a)) return rc;
-  if (a->n_queries == 0) return LL_OK;
+static int check_ragged_pointers(const ll_ragged_attention_args* a) {
   const bool paged = a->page_table || a->page_size;
   const bool has_keys = paged ? a->n_pages > 0 && a->table_width > 0 : a->n_keys > 0;
   LL_REQUIRE(a->q && a->out, "ll_ragged_attention: null q or out");
@@ -1252,15 +1463,12 @@ extern "C" int ll_ragged_attention(const ll_ragged_attention_args* a, void* stre
   LL_REQUIRE(a->k_stride_page >= 0 && a->v_stride_page >= 0 && a->k_stride_page <= 0xffffffffll && a->v_stride_page <= 0xffffffffll &&
                  a->k_stride_row >= 0 && a->v_stride_row >= 0 && a->k_stride_row < (1ll << 26) && a->v_stride_row < (1ll << 26),
              "ll_ragged_attention: pages of k and v lie at most 2^32 elements apart, rows 2^26");
-  int dev = 0, cus = 0;
-  if (hipError_t e = hipGetDevice(&dev)) {
-    set_error("ll_ragged_attention: hipGetDevice failed: %s", hipGetErrorString(e));
-    return LL_ELAUNCH;
-  }
-  if (int rc = compute_units_of(dev, cus, "ll_ragged_attention")) return rc;
-  const RaPlan plan = plan_ragged(*a, cus);
-  LL_REQUIRE(plan.bytes == 0 || (a->workspace && (uintptr_t)a->workspace % 16 == 0 && a->workspace_bytes >= plan.bytes),
-             "ll_ragged_attention: a workspace of %zu bytes, 16-byte aligned, is needed", plan.bytes);
+  return LL_OK;
+}
+
+static RaParams ragged_params(const ll_ragged_attention_args* a) {
+  const bool paged = a->page_table || a->page_size;
+  const bool has_keys = paged ? a->n_pages > 0 && a->table_width > 0 : a->n_keys > 0;
   RaParams p{};
   p.q = static_cast<const uint16_t*>(a->q);
   p.out = static_cast<uint16_t*>(a->out);
@@ -1296,6 +1504,25 @@ extern "C" int ll_ragged_attention(const ll_ragged_attention_args* a, void* stre
   p.group = divisor((uint32_t)(a->num_heads / a->num_kv_heads));
   p.window = (uint32_t)std::min<int64_t>(a->window, 0x7fffffff);  // keys are fewer
   p.sink = (uint32_t)std::min<int64_t>(a->sink_keys, 0x7fffffff);
+  return p;
+}
+}  // namespace ll
+
+extern "C" int ll_ragged_attention(const ll_ragged_attention_args* a, void* stream) {
+  using namespace ll;
+  if (int rc = check_ragged(a)) return rc;
+  if (a->n_queries == 0) return LL_OK;
+  if (int rc = check_ragged_pointers(a)) return rc;
+  int dev = 0, cus = 0;
+  if (hipError_t e = hipGetDevice(&dev)) {
+    set_error("ll_ragged_attention: hipGetDevice failed: %s", hipGetErrorString(e));
+    return LL_ELAUNCH;
+  }
+  if (int rc = compute_units_of(dev, cus, "ll_ragged_attention")) return rc;
+  const RaPlan plan = plan_ragged(*a, cus);
+  LL_REQUIRE(plan.bytes == 0 || (a->workspace && (uintptr_t)a->workspace % 16 == 0 && a->workspace_bytes >= plan.bytes),
+             "ll_ragged_attention: a workspace of %zu bytes, 16-byte aligned, is needed", plan.bytes);
+  RaParams p = ragged_params(a);
   p.groups = plan.groups;
   p.part_steps = plan.part_steps;
   p.part_share = plan.part_share;
@@ -1304,9 +1531,150 @@ extern "C" int ll_ragged_attention(const ll_ragged_attention_args* a, void* stre
   p.record_mem = static_cast<float*>(a->workspace);
   const uint32_t grid = p.groups + (a->clear_rest ? kRaClearGroups : 0);
   if (grid == 0) return LL_OK;
+  const bool paged = a->page_table || a->page_size;
   const int kind = paged ? kRaPaged : a->key_mask ? kRaMaskedRows : kRaRows;
   const hipStream_t s = static_cast<hipStream_t>(stream);
   if (a->dtype == LL_DTYPE_BF16)
     return a->head_dim == 128 ? launch_ragged<Bf16, 128>(p, kind, grid, s) : launch_ragged<Bf16, 64>(p, kind, grid, s);
   return a->head_dim == 128 ? launch_ragged<F16, 128>(p, kind, grid, s) : launch_ragged<F16, 64>(p, kind, grid, s);
+}
+
+namespace ll {
+static int check_shared(const ll_shared_prefix_args* a) {
+  LL_REQUIRE(a, "ll_shared_prefix_attention: no arguments");
+  if (int rc = check_ragged(&a->own)) return rc;
+  LL_REQUIRE(a->own.page_size > 0, "ll_shared_prefix_attention: keys lie in pages");
+  LL_REQUIRE(a->own.window == 0 && a->own.sink_keys == 0, "ll_shared_prefix_attention: there are no windows");
+  LL_REQUIRE(a->groups >= 0 && a->groups <= 0xfffffff, "ll_shared_prefix_attention: %lld groups", (long long)a->groups);
+  LL_REQUIRE(a->max_prefix_len >= 0, "ll_shared_prefix_attention: negative longest beginning");
+  LL_REQUIRE(a->prefix_width >= 0 && a->prefix_width <= (1ll << 30) / a->own.page_size && a->own.table_width <= (1ll << 30) / a->own.page_size,
+             "ll_shared_prefix_attention: tables of %lld and %lld pages of %d rows reach beyond 2^30 keys", (long long)a->prefix_width,
+             (long long)a->own.table_width, a->own.page_size);
+  return LL_OK;
+}
+
+// How a launch over shared beginnings is divided (host arithmetic).
+struct SharedPlan {
+  uint32_t groups, part_steps, narrow_part_steps, prefix_part_steps, prefix_parts, own_parts;
+  size_t bytes;
+};
+constexpr size_t kRaMostSharedBytes = (size_t)1 << 30;  // of records
+constexpr int64_t kRaLeastPrefixSteps = 6, kRaMostParts = 64;
+
+static SharedPlan plan_shared(const ll_shared_prefix_args& s, int cus) {
+  const ll_ragged_attention_args& a = s.own;
+  SharedPlan r{0, 1u << 24, 1u << 24, 1u << 24, 0, 1, 0};
+  if (a.n_queries == 0 || a.streams == 0) return r;
+  const int64_t group = a.num_heads / a.num_kv_heads, slots = (a.head_dim == 64 ? 3 : 2) * cus;
+  const int64_t longest = a.max_q_len > 0 && a.max_q_len < a.n_queries ? a.max_q_len : a.n_queries;
+  const int64_t tiles = std::min(a.n_queries * group / kRaTileRows + a.streams, a.streams * ((longest * group + kRaTileRows - 1) / kRaTileRows));
+  const auto steps_within = [&](int64_t told, int64_t width) {
+    const int64_t reach = width * a.page_size, keys = told > 0 && told < reach ? told : reach;
+    return (keys + kRaKeys - 1) / kRaKeys;
+  };
+  const int64_t own_steps = steps_within(a.max_kv_len, a.n_pages ? a.table_width : 0);
+  const int64_t prefix_steps = s.groups && a.n_pages ? steps_within(s.max_prefix_len, s.prefix_width) : 0;
+  const int64_t together = a.n_queries * group / kRaTileRows + std::min(s.groups, a.streams);  // tiles of whole groups
+  const size_t part_bytes = (size_t)a.n_queries * a.num_heads * (a.head_dim + 2) * sizeof(float);
+  int64_t most_parts = std::min<int64_t>(kRaMostParts, (int64_t)(kRaMostSharedBytes / part_bytes));
+  if (a.streams > 1 && prefix_steps > 0 && most_parts >= 2 && a.streams * prefix_steps >= kRaJoinedCost * (a.n_queries * group / kRaTileRows)) {
+    // What all workgroups have to do, in steps, and a workgroup's share of it.
+    const int64_t narrow = tiles * a.num_kv_heads, all = together * a.num_kv_heads * prefix_steps + narrow * ((own_steps + 1) / 2 + 3);
+    const int64_t share = std::max((all + slots - 1) / slots, kRaLeastPrefixSteps);
+    r.prefix_parts = (uint32_t)std::min((prefix_steps + share - 1) / share, most_parts - 1);
+    r.own_parts = (uint32_t)std::min((own_steps + 2 * share - 1) / (2 * share), most_parts - (int64_t)r.prefix_parts);
+    r.own_parts = std::max(r.own_parts, 1u);
+    r.prefix_part_steps = (uint32_t)((prefix_steps + r.prefix_parts - 1) / r.prefix_parts);
+    r.part_steps = r.narrow_part_steps = (uint32_t)std::max<int64_t>((own_steps + r.own_parts - 1) / r.own_parts, 1);
+  } else {
+    const int64_t steps = std::max<int64_t>(prefix_steps + own_steps, 1), busy = tiles * a.num_kv_heads;
+    int64_t best = 1, least = -1;
+    for (int64_t parts = 1; parts <= most_parts && (parts == 1 || steps / parts >= 3); ++parts) {
+      const int64_t each = (steps + parts - 1) / parts, items = busy * parts, rounds = (items + slots - 1) / slots;
+      const int64_t step = kRaStepCost[a.head_dim == 128][items <= cus ? 0 : items <= 2 * cus ? 1 : 2];
+      const int64_t cost = rounds * (each * step + kRaItemCost * std::min(items, slots) / slots) + (parts > 1 ? kRaJoinCost + kRaRecordCost * items / slots : 0);
+      if (least < 0 || cost < least) {
+        least = cost;
+        best = parts;
+      }
+    }
+    r.own_parts = (uint32_t)best;
+    if (best > 1) r.part_steps = r.narrow_part_steps = (uint32_t)((steps + best - 1) / best);
+  }
+  if (r.prefix_parts + r.own_parts > 1) r.bytes = part_bytes * (r.prefix_parts + r.own_parts);
+  r.groups = (uint32_t)std::min(slots, (together * r.prefix_parts + (a.n_queries * group / kRaTileRows + a.streams) * r.own_parts) * a.num_kv_heads);
+  return r;
+}
+
+template <typename T, int D>
+static int launch_shared(const RaParams& p, uint32_t grid, hipStream_t stream) {
+  static std::atomic<uint64_t> allowed{0};
+  const void* kernel = reinterpret_cast<const void*>(&ragged_attention_kernel<T, D, kRaShared>);
+  if (int rc = allow_dynamic_lds(kernel, kRaLds<D>, allowed, "ll_shared_prefix_attention")) return rc;
+  ragged_attention_kernel<T, D, kRaShared><<<grid, kRaThreads, kRaLds<D>, stream>>>(p);
+  LL_CHECK_LAUNCH("ll_shared_prefix_attention");
+  if (p.prefix_parts + p.own_parts > 1) {
+    const uint32_t rows = kRaThreads * 4 / D;
+    const dim3 join((uint32_t)std::min<int64_t>(p.n_queries, 4096), ((uint32_t)p.heads + rows - 1) / rows);
+    shared_join_kernel<T, D><<<join, kRaThreads, 0, stream>>>(p);
+    LL_CHECK_LAUNCH("ll_shared_prefix_attention (join)");
+  }
+  return LL_OK;
+}
+}  // namespace ll
+
+extern "C" int ll_shared_prefix_attention_workspace(const ll_shared_prefix_args* a, int compute_units, size_t* bytes) {
+  using namespace ll;
+  if (int rc = check_shared(a)) return rc;
+  LL_REQUIRE(bytes && compute_units >= 0, "ll_shared_prefix_attention_workspace: nowhere to put the answer");
+  if (compute_units == 0) {
+    int dev = 0;
+    if (hipError_t e = hipGetDevice(&dev)) {
+      set_error("ll_shared_prefix_attention_workspace: hipGetDevice failed: %s", hipGetErrorString(e));
+      return LL_ELAUNCH;
+    }
+    if (int rc = compute_units_of(dev, compute_units, "ll_shared_prefix_attention_workspace")) return rc;
+  }
+  *bytes = plan_shared(*a, compute_units).bytes;
+  return LL_OK;
+}
+
+extern "C" int ll_shared_prefix_attention(const ll_shared_prefix_args* args, void* stream) {
+  using namespace ll;
+  if (int rc = check_shared(args)) return rc;
+  const ll_ragged_attention_args* a = &args->own;
+  if (a->n_queries == 0) return LL_OK;
+  if (int rc = check_ragged_pointers(a)) return rc;
+  const bool shares = args->groups > 0 && args->prefix_width > 0 && a->n_pages > 0;
+  LL_REQUIRE(!shares || (args->prefix_lens && args->prefix_table), "ll_shared_prefix_attention: null lengths or table of what is shared");
+  LL_REQUIRE(args->groups <= 1 || args->group_starts, "ll_shared_prefix_attention: %lld groups without their beginnings", (long long)args->groups);
+  LL_REQUIRE(!shares || (a->k && a->v), "ll_shared_prefix_attention: null k or v");
+  int dev = 0, cus = 0;
+  if (hipError_t e = hipGetDevice(&dev)) {
+    set_error("ll_shared_prefix_attention: hipGetDevice failed: %s", hipGetErrorString(e));
+    return LL_ELAUNCH;
+  }
+  if (int rc = compute_units_of(dev, cus, "ll_shared_prefix_attention")) return rc;
+  const SharedPlan plan = plan_shared(*args, cus);
+  LL_REQUIRE(plan.bytes == 0 || (a->workspace && (uintptr_t)a->workspace % 16 == 0 && a->workspace_bytes >= plan.bytes),
+             "ll_shared_prefix_attention: a workspace of %zu bytes, 16-byte aligned, is needed", plan.bytes);
+  RaParams p = ragged_params(a);
+  p.groups = plan.groups;
+  p.part_steps = plan.part_steps;
+  p.narrow_part_steps = plan.narrow_part_steps;
+  p.prefix_part_steps = plan.prefix_part_steps;
+  p.prefix_parts = plan.prefix_parts;
+  p.own_parts = plan.own_parts;
+  p.record_mem = static_cast<float*>(a->workspace);
+  p.n_groups = shares ? (int)args->groups : 0;
+  p.group_starts = args->group_starts;
+  p.prefix_lens = args->prefix_lens;
+  p.prefix_table = args->prefix_table;
+  p.prefix_stride = args->prefix_stride;
+  p.prefix_keys = shares ? args->prefix_width * a->page_size : 0;
+  const uint32_t grid = p.groups + (a->clear_rest ? kRaClearGroups : 0);
+  if (grid == 0) return LL_OK;
+  const hipStream_t st = static_cast<hipStream_t>(stream);
+  if (a->dtype == LL_DTYPE_BF16) return a->head_dim == 128 ? launch_shared<Bf16, 128>(p, grid, st) : launch_shared<Bf16, 64>(p, grid, st);
+  return a->head_dim == 128 ? launch_shared<F16, 128>(p, grid, st) : launch_shared<F16, 64>(p, grid, st);
 }

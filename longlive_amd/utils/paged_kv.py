@@ -11,8 +11,14 @@ What a step of a batch looks like on the device, all int32 (one launch recorded 
 * ``kv_lens`` [streams]: keys of each stream, its new tokens included;
 * ``page_table`` [streams, pages of the longest stream]: key j of stream b is row ``j % page_size`` of page
   ``page_table[b, j // page_size]``.
+
+:func:`lay_out_step` makes these on the device from the streams' lengths and hands out free pages.  Groups of streams that begin alike (many
+answers to one prompt, several continuations of one video) may keep what they share outside their own tables, in a row of a
+``prefix_table``: :func:`shared_prefix_attention` reads it once for a whole group.
 """
 from __future__ import annotations
+
+from typing import NamedTuple
 
 import torch
 
@@ -53,6 +59,34 @@ def paged_slots(page_table: torch.Tensor, kv_lens: torch.Tensor, q_starts: torch
     return torch.where(inside & (page >= 0), page * page_size + place % page_size, -1)
 
 
+class StepLayout(NamedTuple):
+    """What :func:`lay_out_step` makes, on the device."""
+    q_starts: torch.Tensor      # int32 [streams + 1]
+    kv_lens: torch.Tensor       # int32 [streams], the new tokens included
+    positions: torch.Tensor     # int64 [num_tokens]
+    slots: torch.Tensor         # int64 [num_tokens]
+    pages_wanted: torch.Tensor  # int32 [1]
+
+
+def lay_out_step(new_lens: torch.Tensor, kv_lens: torch.Tensor, page_table: torch.Tensor, free_pages: torch.Tensor, page_size: int, num_tokens: int, *,
+                 prefix_lens: torch.Tensor | None = None, group_starts: torch.Tensor | None = None, cursor: torch.Tensor | None = None,
+                 kv_lens_out: torch.Tensor | None = None) -> StepLayout:
+    """What the operators of a step read, from ``new_lens`` [streams], the streams' new tokens, and ``kv_lens`` [streams], the keys that they hold
+    before them: int32 on the device, where nothing is waited for.  One launch, to be recorded into a graph or not.
+
+    A stream's rows follow those of the stream before; its keys go on where they ended.  Pages that they need are taken from ``free_pages`` (int32 [n])
+    in order of streams and keys and written into ``page_table``; where the list has come to its end, -1, a hole.  ``pages_wanted`` says how
+    many were to be written: more than the list holds, and some tokens have no place.  With a ``cursor`` (int32 [1]) the list is taken from
+    that entry on, and the cursor moves behind what was taken; with ``kv_lens_out``, which may be ``kv_lens``, the new lengths go there: steps
+    that a graph replays go on from one another.
+
+    ``positions`` count from the stream's first key, and with ``prefix_lens`` (int32 [groups]) from the beginning that its group shares:
+    group g is streams ``group_starts[g] .. group_starts[g + 1] - 1`` (int32 [groups + 1]; all streams are one group without).  ``slots`` is -1 for
+    tokens in holes and behind the table's width.  Tokens for which ``num_tokens`` has no row left are not laid out: their streams' lengths do not
+    count them.  Rows behind the last stream's have position 0 and slot -1."""
+    return StepLayout(*_native.step_layout(new_lens, kv_lens, page_table, free_pages, page_size, num_tokens, prefix_lens, group_starts, cursor, kv_lens_out))
+
+
 def head_norm_rope_paged(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cache: dict, slots: torch.Tensor, q_weight: torch.Tensor | None,
                          k_weight: torch.Tensor | None, eps: float, cos_f32: torch.Tensor | None, sin_f32: torch.Tensor | None,
                          positions: torch.Tensor | None = None, interleaved: bool = True, out: torch.Tensor | None = None) -> torch.Tensor:
@@ -62,6 +96,15 @@ def head_norm_rope_paged(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cach
 
     Pages of any head_dim that the norm takes are written (multiples of 8 up to 256); :func:`paged_attention` reads 64 and 128."""
     return _native.head_norm_rope(q, k, v, q_weight, k_weight, eps, cos_f32, sin_f32, positions, interleaved, cache, slots, out)
+
+
+def rotate_by_position_paged(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cache: dict, slots: torch.Tensor, positions: torch.Tensor | None,
+                             frequencies: torch.Tensor, *, interleaved: bool = True, amplitude: float = 1.0, grid: tuple[int, int] | None = None,
+                             sections: tuple[int, int, int] | None = None, q_weight: torch.Tensor | None = None, k_weight: torch.Tensor | None = None,
+                             eps: float = 1e-6, out: torch.Tensor | None = None) -> torch.Tensor:
+    """:func:`longlive_amd.utils.rope.rotate_by_position` of q and k whose K, with the V beside it, goes to the cache in the same launch, as in
+    :func:`head_norm_rope_paged`.  Returns the rotated q, in ``out`` if given, which may be q itself."""
+    return _native.rotate_by_position(q, k, v, q_weight, k_weight, eps, frequencies, amplitude, positions, interleaved, grid, sections, cache, slots, out)
 
 
 def paged_attention(q: torch.Tensor, cache: dict, page_table: torch.Tensor, kv_lens: torch.Tensor, q_starts: torch.Tensor, causal: bool = True,
@@ -80,3 +123,21 @@ def paged_attention(q: torch.Tensor, cache: dict, page_table: torch.Tensor, kv_l
     stay as they were in a given one, which may be q itself."""
     return _native.ragged_attention("paged_attention", q, q_starts, softmax_scale, max_q_len, max_kv_len, out, cache=cache, page_table=page_table,
                                     kv_lens=kv_lens, causal=causal, window=window, sink_tokens=sink_tokens)
+
+
+def shared_prefix_attention(q: torch.Tensor, cache: dict, prefix_table: torch.Tensor, prefix_lens: torch.Tensor, page_table: torch.Tensor,
+                            kv_lens: torch.Tensor, q_starts: torch.Tensor, group_starts: torch.Tensor | None = None, causal: bool = True,
+                            softmax_scale: float | None = None, max_q_len: int | None = None, max_kv_len: int | None = None,
+                            max_prefix_len: int | None = None, out: torch.Tensor | None = None) -> torch.Tensor:
+    """:func:`paged_attention` of streams in groups that share a beginning, which is read once for a group's rows where that is cheaper.
+
+    Group g is streams ``group_starts[g] .. group_starts[g + 1] - 1`` (int32 [groups + 1], not decreasing; without it all streams are one group;
+    streams outside every group share nothing).  The ``prefix_lens[g]`` keys (int32 [groups]) that it shares lie in the pages of ``prefix_table[g]``
+    (int32 [groups, pages of the longest]), and every token of its streams sees all of them.  ``page_table`` and ``kv_lens`` are of the keys behind,
+    each stream's own: token i of n sees own key j where ``j <= kv_lens[b] - n + i`` (``causal``; else every one).  A common beginning of whole
+    pages at the front of every row of one table is handed on as views: ``table[:1, :w]`` and ``table[:, w:]``, with lengths that count from there.
+
+    ``max_prefix_len``: the longest beginning, like ``max_q_len`` and ``max_kv_len`` (the longest stream's own keys).  The rest as in
+    :func:`paged_attention`."""
+    return _native.ragged_attention("shared_prefix_attention", q, q_starts, softmax_scale, max_q_len, max_kv_len, out, cache=cache, page_table=page_table,
+                                    kv_lens=kv_lens, causal=causal, prefix=(prefix_table, prefix_lens, group_starts, max_prefix_len))

@@ -6,6 +6,8 @@ Mirrors ``rope_params`` (wan_5b/modules/model.py:29-36), the table layout of
 """
 from __future__ import annotations
 
+import math
+
 import torch
 
 from .. import _native
@@ -96,6 +98,62 @@ def head_norm_rope(q: torch.Tensor, k: torch.Tensor, q_weight: torch.Tensor | No
     rotation.  Rows whose position (int64) lies outside the table are normed and not rotated.  Where the norm runs over whole
     rows of all heads, as in the reference's model, ``_native.qk_norm_rope_pair`` is the call."""
     return _native.head_norm_rope(q, k, None, q_weight, k_weight, eps, cos_f32, sin_f32, positions, interleaved)
+
+
+def rotary_frequencies(rotary_dim: int, base: float = 10000.0, scaling: str | None = None, factor: float = 1.0, trained_positions: int | None = None,
+                       slow: float = 1.0, fast: float = 32.0, device: torch.device | str | None = None) -> torch.Tensor:
+    """Radians per position of a head's ``rotary_dim / 2`` pairs, ``base ** (-2 j / rotary_dim)``, float64; for contexts ``factor`` times as long as
+    a model was trained on, with ``scaling``
+
+    * ``"positions"``: all divided by ``factor`` (positions interpolated);
+    * ``"base"``: ``base`` times ``factor ** (rotary_dim / (rotary_dim - 2))``: the slowest pair divided by ``factor``, the fastest as it was;
+    * ``"parts"``: pairs that make ``fast`` turns or more over ``trained_positions`` as they were, those that make ``slow`` or fewer divided, a
+      linear passage between them.  Models trained so often have cosines and sines multiplied by ``0.1 * log(factor) + 1``
+      (``amplitude`` of :func:`rotate_by_position`)."""
+    if rotary_dim < 2 or rotary_dim % 2:
+        raise ValueError(f"rotary_frequencies: {rotary_dim} rotated columns")
+    if not (0.0 < base < float("inf") and 0.0 < factor < float("inf")):
+        raise ValueError(f"rotary_frequencies: base {base}, factor {factor}")
+    if scaling not in (None, "positions", "base", "parts"):
+        raise ValueError(f"rotary_frequencies: scaling {scaling!r} is not 'positions', 'base' or 'parts'")
+    if scaling is None and factor != 1.0:
+        raise ValueError(f"rotary_frequencies: a factor of {factor} needs a scaling")
+    if scaling == "base":
+        if rotary_dim == 2:
+            raise ValueError("rotary_frequencies: a single pair has no other base")
+        base = base * factor ** (rotary_dim / (rotary_dim - 2))
+    f = base ** (-torch.arange(0, rotary_dim, 2, dtype=torch.float64) / rotary_dim)
+    if scaling == "positions":
+        f = f / factor
+    if scaling == "parts":
+        if not trained_positions or trained_positions < 1 or not slow < fast:
+            raise ValueError(f"rotary_frequencies: parts by turns over {trained_positions} trained positions, between {slow} and {fast}")
+        kept = ((f * (trained_positions / (2.0 * math.pi)) - slow) / (fast - slow)).clamp(0.0, 1.0)
+        f = f * (kept + (1.0 - kept) / factor)
+    return f.to(device) if device is not None else f
+
+
+def video_frequencies(head_dim: int = 128, theta: float = 10000.0, device: torch.device | str | None = None) -> tuple[torch.Tensor, tuple[int, int, int]]:
+    """The frequencies of :func:`build_rope_angles`, float64 [head_dim / 2], and how many pairs frames, rows and columns turn: what
+    :func:`rotate_by_position` takes with ``grid=(rows, columns)`` of a frame's tokens."""
+    c = head_dim // 2
+    sections = (c - 2 * (c // 3), c // 3, c // 3)
+    f = torch.cat([rope_params(2, dim, theta)[1] for dim in (head_dim - 4 * (head_dim // 6), 2 * (head_dim // 6), 2 * (head_dim // 6))])
+    return (f.to(device) if device is not None else f), sections
+
+
+def rotate_by_position(q: torch.Tensor, k: torch.Tensor, positions: torch.Tensor | None, frequencies: torch.Tensor, *, interleaved: bool = True,
+                       amplitude: float = 1.0, grid: tuple[int, int] | None = None, sections: tuple[int, int, int] | None = None,
+                       q_weight: torch.Tensor | None = None, k_weight: torch.Tensor | None = None, eps: float = 1e-6) -> tuple[torch.Tensor, torch.Tensor]:
+    """:func:`head_norm_rope` without a table: pair j of row t turns by ``positions[t] * frequencies[j]`` radians (:func:`rotary_frequencies`, float64
+    [rotated / 2]), formed in 64 bits in the launch, so that positions may be any (int64; negative ones turn back, row t's is t without), and
+    cosine and sine are multiplied by ``amplitude``.
+
+    With ``grid``, (rows, columns) of the tokens of a video frame, position p is frame ``p // (rows * columns)``, row ``p // columns % rows`` and column
+    ``p % columns``, each of which turns its share of the pairs: ``sections``, three numbers (:func:`video_frequencies`).
+
+    Types, layouts, norms and results as there; without weights there is no norm."""
+    return _native.rotate_by_position(q, k, None, q_weight, k_weight, eps, frequencies, amplitude, positions, interleaved, grid, sections)
 
 
 # the reference's name for the same entry point
