@@ -52,8 +52,23 @@ constexpr float kLog2E = 1.4426950408889634f;
 constexpr uint32_t kRaJoinGroups = 256;
 
 // Where keys lie: in the pages of a table, in rows one behind the other, in such rows with a mask.
-// Shared: in the pages of a table, behind those of a beginning that a group of streams shares.
-constexpr int kRaPaged = 0, kRaRows = 1, kRaMaskedRows = 2, kRaShared = 3;
+// With shared beginnings: in the pages of a table, behind those of the beginning of the stream's group.  Listed: a launch ahead has listed the
+// items, beginnings of whole groups among them.
+constexpr int kRaPaged = 0, kRaRows = 1, kRaMaskedRows = 2, kRaPrefixed = 3, kRaListed = 4;
+
+// An item of every kv head, as listed ahead.
+struct RaListedItem {
+  int q0, rows, first, len, base, prefix_len, prefix_row, table_row, s_begin, s_end;
+  int slot;  // of the part's results, -1: they are the tile's
+  int unused;
+};
+struct RaList {
+  uint32_t prefix_items, single_items, items;  // items of beginnings; with those that take a workgroup; with those that take a wave
+  uint32_t wide_part, narrow_part;             // steps of a part of a stream's own keys, for more than 32 rows and for fewer
+};
+struct RaJoined {  // of a stream: parts of its group's beginning, or steps of it ahead of its own
+  int parts, ahead, joined;
+};
 
 struct RaParams {
   const uint16_t* q;
@@ -84,12 +99,18 @@ struct RaParams {
   float part_share;       // not 0: part_steps follow from the streams, this times the steps of all wide tiles of a head
   uint32_t records;       // of a kv head, 32 rows each
   float* record_mem;      // [kv head][records]: 32 x D columns, then reference point and sum of each row
-  // Shared beginnings.  `records` is not used: results of parts lie by row, [prefix_parts + own_parts][n_queries][heads] of D columns, then
-  // as many reference points and sums.
+  // Shared beginnings.
   const int32_t *group_starts, *prefix_lens, *prefix_table;
   int64_t prefix_stride, prefix_keys;  // keys that a row of the table reaches
   int n_groups;
-  uint32_t prefix_part_steps, prefix_parts, own_parts;  // steps of a part, and how many there are at most; 0 prefix_parts: none is joined
+  // Listed: results of parts lie by row in record_mem, [prefix_parts + own_parts][n_queries][heads] of D columns, then as many reference points
+  // and sums.
+  uint32_t prefix_parts, own_parts;    // parts of a tile at most
+  RaList* list;
+  RaListedItem* listed;
+  uint32_t most_listed;
+  RaJoined* joined;                    // [streams]
+  uint32_t* first_items;               // [groups + 1]: of a workgroup, behind the beginnings'
 };
 
 // Positions of 16-byte pieces in an LDS row of D columns.  The reads of a wave then go through all banks: 8 neighbouring rows of one
@@ -166,7 +187,7 @@ __device__ __forceinline__ RaGroup group_of(const RaParams& p, int g) {
   r.q0 = min(max(p.q_starts[from], 0), limit);
   r.n = max(min(max(p.q_starts[to], 0), limit) - r.q0, 0);
   r.len = (int)min((int64_t)max(p.prefix_lens[g], 0), p.prefix_keys);
-  r.joined = p.prefix_parts > 0 && to - from > 1 &&
+  r.joined = p.prefix_parts > 0 && to - from > 1 && r.n > 0 &&
              (int64_t)(to - from) * (r.len / kRaKeys) >= (int64_t)kRaJoinedCost * (((uint32_t)r.n * p.group.d + kRaTileRows - 1) / kRaTileRows);
   return r;
 }
@@ -183,7 +204,7 @@ __device__ __forceinline__ int group_of_stream(const RaParams& p, int b) {
   return g < p.n_groups && p.group_starts[g] <= b ? g : -1;
 }
 __device__ __forceinline__ int steps_of(int keys) { return (keys + kRaKeys - 1) / kRaKeys; }
-// Parts of a tile that takes so many steps.
+// Parts of a tile that takes so many steps, no more than `most`.
 __device__ __forceinline__ int shared_parts(uint32_t steps, uint32_t per_part, uint32_t most) { return (int)min((steps + per_part - 1) / per_part, most); }
 
 // What a workgroup does next: a part of a tile.
@@ -198,10 +219,10 @@ struct RaItem {
   int s_begin, s_end;       // of these, the part's
   int n_parts, part;
   uint32_t record;          // of part 0; the others follow, each as many records as the tile has groups of 32 rows
-  // Shared: of the tile's steps the first go over the beginning, whose keys have the numbers -64 prefix_steps and up.
+  // With shared beginnings: of the tile's steps the first go over the beginning, whose keys have the numbers -64 prefix_steps and up.
   const int32_t* prefix_pages;
   int prefix_steps, prefix_len;
-  bool to_record;           // the part's results are joined with others
+  int slot;                 // where the part's results go, to be joined with others; -1: they are the tile's
 };
 
 // The streams b0 .. b0 + 63, one a lane.
@@ -209,7 +230,7 @@ struct RaStreams {
   int q0, n, len, base, key0;
   int parts;                          // at most: of the tile that sees most keys
   uint32_t items_upto, records_upto;  // of these and the streams before
-  int shares, prefix_len, joined;     // shared: the group, or -1; keys of its beginning that the items go over; whether others are joined with them
+  int shares, prefix_len;             // with shared beginnings: the group, its keys
 };
 
 // Steps of a tile whose first and last token sit at pos0 and pos1, of a stream of len keys.
@@ -256,7 +277,8 @@ __device__ __forceinline__ RaStreams load_streams(const RaParams& p, int b0, uin
   s.n = b0 + lane < p.streams ? max(min(max(next, 0), limit) - s.q0, 0) : 0;
   s.base = 0;
   int64_t key0 = 0, len;
-  if constexpr (KIND == kRaPaged) {
+  s.shares = s.prefix_len = 0;
+  if constexpr (KIND == kRaPaged || KIND == kRaPrefixed) {
     // positions count from the stream's last token, wherever the table and the rows of q end
     const int64_t given = max((int64_t)p.kv_lens[b], (int64_t)0);
     len = min(given, p.table_keys);
@@ -268,6 +290,11 @@ __device__ __forceinline__ RaStreams load_streams(const RaParams& p, int b0, uin
   }
   s.len = (int)len;
   s.key0 = (int)key0;
+  if constexpr (KIND == kRaPrefixed) {
+    const int g = group_of_stream(p, b);
+    s.shares = max(g, 0);
+    s.prefix_len = g < 0 ? 0 : group_of(p, g).len;
+  }
   const int rows = s.n * (int)p.group.d;
   const int tiles = tiles_of(rows);
   s.parts = 1;
@@ -281,6 +308,7 @@ __device__ __forceinline__ RaStreams load_streams(const RaParams& p, int b0, uin
       const int pos1 = max(s.len - 1, s.base);
       const int pos0 = p.causal || p.streams > 1 ? pos1 - min(s.n - 1, (int)((uint32_t)(kRaTileRows - 1) / p.group) + 1) : s.base;
       steps = p.window ? span_of(p, s.len, pos0, pos1).n_steps + 1 : (s.len + kRaKeys - 1) / kRaKeys;
+      if constexpr (KIND == kRaPrefixed) steps += steps_of(s.prefix_len);
     }
     if (p.part_share != 0.0f) {  // up to 64 streams, which are all here
       const int mean = p.causal && !p.window ? max(steps - s.n / (2 * kRaKeys), 1) : steps;
@@ -301,50 +329,6 @@ __device__ __forceinline__ RaStreams load_streams(const RaParams& p, int b0, uin
   return s;
 }
 
-// With shared beginnings: first the groups, whose items are the beginnings that are attended together, then the streams.
-__device__ __forceinline__ RaStreams load_shared(const RaParams& p, int b0, uint32_t items) {
-  const int at = b0 + (threadIdx.x & 63);
-  RaStreams s{};
-  s.shares = -1;
-  int steps = 0;
-  uint32_t per_part = 1, most = 1;
-  if (at < p.n_groups) {
-    const RaGroup g = group_of(p, at);
-    if (g.joined) {
-      s.q0 = g.q0;
-      s.n = g.n;
-      s.shares = at;
-      s.joined = 1;
-      s.prefix_len = g.len;
-      steps = steps_of(g.len);
-      per_part = p.prefix_part_steps;
-      most = p.prefix_parts;
-    }
-  } else if (at < p.n_groups + p.streams) {
-    const int b = at - p.n_groups, limit = (int)p.n_queries;
-    const int next = p.q_starts[b + 1];
-    s.q0 = min(max(p.q_starts[b], 0), limit);
-    s.n = max(min(max(next, 0), limit) - s.q0, 0);
-    const int64_t given = max((int64_t)p.kv_lens[b], (int64_t)0);
-    s.len = (int)min(given, p.table_keys);
-    s.base = (int)(given - ((int64_t)next - s.q0));
-    s.shares = group_of_stream(p, b);
-    if (s.shares >= 0) {
-      const RaGroup g = group_of(p, s.shares);
-      s.joined = g.joined;
-      if (!g.joined) s.prefix_len = g.len;
-    }
-    steps = steps_of(s.prefix_len) + steps_of(s.len);
-    per_part = s.n * (int)p.group.d <= 32 ? p.narrow_part_steps : p.part_steps;
-    most = p.own_parts;
-  }
-  const int tiles = tiles_of(s.n * (int)p.group.d);
-  // a joined stream without keys of its own has nothing to add, one that is not has its zeros to write
-  s.parts = max(shared_parts((uint32_t)steps, per_part, most), s.joined ? 0 : 1);
-  s.items_upto = items + sum_upto((uint32_t)(tiles * s.parts));
-  return s;
-}
-
 // Finds items one behind the other.
 template <int KIND, bool COUNT_TILES>
 struct RaCursor {
@@ -354,11 +338,7 @@ struct RaCursor {
   RaStreams s;                      // streams from b0 on
   __device__ __forceinline__ void start(const RaParams& p) {
     part_steps = p.part_steps;
-    if constexpr (KIND == kRaShared) {
-      if (p.streams > 0) s = load_shared(p, 0, 0);
-    } else {
-      if (p.streams > 0) s = load_streams<KIND, COUNT_TILES>(p, 0, 0, 0, part_steps);
-    }
+    if (p.streams > 0) s = load_streams<KIND, COUNT_TILES>(p, 0, 0, 0, part_steps);
   }
   // Item `index` of a kv head, which is no smaller than the last one asked for.  All lanes call it together.  False: there are fewer.
   __device__ __forceinline__ bool find(const RaParams& p, uint32_t index, RaItem& t) {
@@ -380,29 +360,15 @@ struct RaCursor {
         t.len = of(s.len);
         t.base = of(s.base);
         t.key0 = of(s.key0);
-        t.pages = KIND == kRaPaged ? p.page_table + (int64_t)(b0 + at) * p.table_stride : nullptr;
+        t.pages = KIND == kRaPaged || KIND == kRaPrefixed ? p.page_table + (int64_t)(b0 + at) * p.table_stride : nullptr;
         const int last_row = min(t.first + kRaTileRows, t.rows) - 1;
-        if constexpr (KIND == kRaShared) {
-          const int b = b0 + at - p.n_groups, shares = of(s.shares);  // b below 0: a beginning
+        RaSpan span = span_of(p, t.len, t.base + (int)((uint32_t)t.first / p.group), t.base + (int)((uint32_t)last_row / p.group));
+        if constexpr (KIND == kRaPrefixed) {
           t.prefix_len = of(s.prefix_len);
           t.prefix_steps = steps_of(t.prefix_len);
-          t.prefix_pages = p.prefix_table + (int64_t)max(shares, 0) * p.prefix_stride;
-          t.pages = p.page_table + (int64_t)max(b, 0) * p.table_stride;
-          const int end = p.causal ? min(t.base + (int)((uint32_t)last_row / p.group) + 1, t.len) : t.len;
-          const int steps = t.prefix_steps + (end > 0 ? steps_of(end) : 0);
-          // As the joining launch counts them.  A tile that sees fewer keys than the stream's last leaves parts out.
-          const uint32_t per_part = b < 0 ? p.prefix_part_steps : t.rows <= 32 ? p.narrow_part_steps : p.part_steps;
-          t.n_parts = min(shared_parts((uint32_t)steps, per_part, (uint32_t)parts), parts);
-          const bool joined = of(s.joined) != 0;
-          if (!joined) t.n_parts = max(t.n_parts, 1);
-          const int each = t.n_parts > 0 ? (steps + t.n_parts - 1) / t.n_parts : 0;
-          t.s_begin = min(t.part * each, steps);
-          t.s_end = min(t.s_begin + each, steps);
-          t.record = b < 0 ? 0 : p.prefix_parts;
-          t.to_record = joined || t.n_parts > 1;
-          return true;
+          t.prefix_pages = p.prefix_table + (int64_t)of(s.shares) * p.prefix_stride;
+          span.n_steps += t.prefix_steps;
         }
-        const RaSpan span = span_of(p, t.len, t.base + (int)((uint32_t)t.first / p.group), t.base + (int)((uint32_t)last_row / p.group));
         t.sink_steps = span.sink_steps;
         t.from_step = span.from_step;
         const uint32_t per_part = t.rows <= 32 ? p.narrow_part_steps : part_steps;
@@ -414,12 +380,8 @@ struct RaCursor {
         return true;
       }
       b0 += 64;
-      if (b0 >= p.streams + (KIND == kRaShared ? p.n_groups : 0)) return false;
+      if (b0 >= p.streams) return false;
       items = (uint32_t)__builtin_amdgcn_readlane((int)s.items_upto, 63);
-      if constexpr (KIND == kRaShared) {
-        s = load_shared(p, b0, items);
-        continue;
-      }
       records = min((uint32_t)__builtin_amdgcn_readlane((int)s.records_upto, 63), p.records + 1);
       s = load_streams<KIND, COUNT_TILES>(p, b0, items, records, part_steps);
     }
@@ -438,7 +400,7 @@ __device__ __forceinline__ float2* record_sums(const RaParams& p, uint32_t head,
   return reinterpret_cast<float2*>(p.record_mem + at * 32 * (D + 2) + 32 * D) + row % 32;
 }
 
-// Shared: where part `slot` of all has a row's columns, and its reference point and sum.
+// Listed: where part `slot` of all has a row's columns, and its reference point and sum.
 template <int D>
 __device__ __forceinline__ float* shared_record(const RaParams& p, uint32_t slot, int64_t token, int head) {
   return p.record_mem + (((int64_t)slot * p.n_queries + token) * p.heads + head) * D;
@@ -479,7 +441,7 @@ __global__ __launch_bounds__(kRaThreads, D == 64 ? 3 : 2) void ragged_attention_
   constexpr int kRowBytes = 2 * D, kPieces = D / 8, kDTiles = D / 32, kSteps = D / 16;
   constexpr int kRowsPerLoad = 1024 / kRowBytes, kGroupLoads = 16 / kRowsPerLoad;  // loads of 16 rows
   constexpr int kStepBytes = kRaKeys * kRowBytes;                                  // K or V of a step
-  constexpr bool kLooksUp = KIND != kRaRows, kPages = KIND == kRaPaged || KIND == kRaShared;
+  constexpr bool kLooksUp = KIND != kRaRows, kPrefixed = KIND == kRaPrefixed || KIND == kRaListed, kPages = KIND == kRaPaged || kPrefixed;
   extern __shared__ __attribute__((aligned(1024))) uint8_t smem[];
   if (blockIdx.x >= p.groups) {  // rows outside every stream
     const int64_t first = p.streams ? stream_start(p, 0) : 0, end = p.streams ? max(stream_start(p, p.streams), first) : 0;
@@ -496,14 +458,54 @@ __global__ __launch_bounds__(kRaThreads, D == 64 ? 3 : 2) void ragged_attention_
   // Item after item: a kv head after the other, so that with a multiple of eight heads the workgroups of an XCD (consecutive ones go to
   // different XCDs) read the same, and neighbouring tiles of a stream run side by side.  (Items handed to whoever asks first, by a counter
   // of each XCD that a launch ahead clears: 12 streams of 1 to 700 tokens over 300 to 9000 keys 176 us in turn, 199 so.)
-  RaCursor<KIND, false> cursor;
-  cursor.start(p);
+  RaCursor<KIND == kRaListed ? kRaPaged : KIND, false> cursor;
+  if constexpr (KIND != kRaListed) cursor.start(p);
+  bool packed = false;  // each wave has an item of its own, of up to 32 rows
+  RaList list{};
+  uint32_t next_item = 0, end_item = 0;
+  if constexpr (KIND == kRaListed) {
+    list = *p.list;
+    next_item = p.first_items[blockIdx.x];
+    end_item = min(p.first_items[blockIdx.x + 1], list.items);
+  }
   for (uint32_t id = blockIdx.x;; id += p.groups) {
-  const uint32_t index = id / (uint32_t)p.kv_heads, kv_head = id - index * (uint32_t)p.kv_heads;
+  uint32_t index = id / (uint32_t)p.kv_heads, kv_head = id - index * (uint32_t)p.kv_heads;
   RaItem t;
+  if constexpr (KIND == kRaListed) {
+    uint32_t item = id;
+    packed = false;
+    if (item >= list.prefix_items) {
+      if (next_item >= end_item) return;
+      item = next_item;
+      packed = item >= list.single_items;
+      next_item += packed ? 4 : 1;
+      if (packed) item += threadIdx.x >> 6;
+    }
+    __syncthreads();  // no wave is at the item before any more
+    item = (uint32_t)__builtin_amdgcn_readfirstlane((int)item);
+    if (packed && item >= end_item) continue;
+    index = item / (uint32_t)p.kv_heads;
+    kv_head = item - index * (uint32_t)p.kv_heads;
+    const RaListedItem& of = p.listed[index];
+    auto uniform = [](int v) { return __builtin_amdgcn_readfirstlane(v); };
+    t.rows = uniform(of.rows);
+    t.q0 = uniform(of.q0);
+    t.first = uniform(of.first);
+    t.len = uniform(of.len);
+    t.base = uniform(of.base);
+    t.prefix_len = uniform(of.prefix_len);
+    t.prefix_steps = steps_of(t.prefix_len);
+    t.prefix_pages = p.prefix_table + (int64_t)uniform(of.prefix_row) * p.prefix_stride;
+    t.pages = p.page_table + (int64_t)uniform(of.table_row) * p.table_stride;
+    t.s_begin = uniform(of.s_begin);
+    t.s_end = uniform(of.s_end);
+    t.slot = uniform(of.slot);
+    if (t.rows == 0) continue;
+  } else {
   if (!cursor.find(p, index, t)) return;
   if (t.part >= t.n_parts) continue;  // a tile that sees fewer keys than the stream's last
   __syncthreads();                    // no wave is at the item before any more
+  }
   // The thread's coordinates, formed anew for every item: what is derived from them would otherwise be formed ahead of the loop over the
   // items and take registers throughout.
   int tid = threadIdx.x;
@@ -530,10 +532,10 @@ __global__ __launch_bounds__(kRaThreads, D == 64 ? 3 : 2) void ragged_attention_
   const Row row = own_row();
   // what it sees: keys below `last`, from `from` on or below the sink
   const int pos = t.base + row.token;
-  // (shared: keys of the beginning have numbers below zero, and every row sees them)
+  // (keys of a shared beginning have numbers below zero, and every row sees them)
   int last = p.causal ? min(pos + 1, t.len) : t.len;
-  if constexpr (KIND == kRaShared) last = max(last, 0);
-  const int from = KIND == kRaShared ? -(1 << 30) : p.window && pos >= (int)p.window ? pos - (int)p.window + 1 : 0;
+  if constexpr (kPrefixed) last = max(last, 0);
+  const int from = kPrefixed ? -(1 << 30) : p.window && pos >= (int)p.window ? pos - (int)p.window + 1 : 0;
   // the same for the wave's first and last row, which bound the others
   const int last0 = __builtin_amdgcn_readfirstlane(last), from1 = __builtin_amdgcn_readlane(from, 31);
   const bool idle = own >= tile_rows;  // a wave without rows only moves keys
@@ -551,13 +553,13 @@ __global__ __launch_bounds__(kRaThreads, D == 64 ? 3 : 2) void ragged_attention_
   uint8_t* const looked_up = smem + 4 * kStepBytes + wave * 512;
   const uint32_t looked_up_lds = lds_at(looked_up);
   auto key_base = [&](int s) __attribute__((always_inline)) {
-    if constexpr (KIND == kRaShared) return (s - t.prefix_steps) * kRaKeys;
+    if constexpr (kPrefixed) return (s - t.prefix_steps) * kRaKeys;
     return (s < t.sink_steps ? s : t.from_step + s - t.sink_steps) * kRaKeys;
   };
   uint32_t next_row = 0;
   auto look_up = [&](int key, int slot) __attribute__((always_inline)) {
     uint32_t k = (uint32_t)min(key, t.len - 1);
-    if constexpr (KIND == kRaShared) {  // all 64 keys of a step lie on one side
+    if constexpr (kPrefixed) {  // all 64 keys of a step lie on one side
       const bool shared = __builtin_amdgcn_readfirstlane(key) < 0;
       k = (uint32_t)min(shared ? key + t.prefix_steps * kRaKeys : key, (shared ? t.prefix_len : t.len) - 1);
       const uint32_t page = k / p.page;
@@ -578,7 +580,7 @@ __global__ __launch_bounds__(kRaThreads, D == 64 ? 3 : 2) void ragged_attention_
   auto take_places = [&](int base, int at, int slot) __attribute__((always_inline)) {
     const int key = base + at;
     bool ok = key < t.len;
-    if constexpr (KIND == kRaShared) ok = base < 0 ? key + t.prefix_steps * kRaKeys < t.prefix_len : ok;
+    if constexpr (kPrefixed) ok = base < 0 ? key + t.prefix_steps * kRaKeys < t.prefix_len : ok;
     first_key = base;
     if constexpr (kPages) {
       at_page = *reinterpret_cast<const uint32_t*>(looked_up + slot * 256 + lane * 4);
@@ -679,7 +681,7 @@ __global__ __launch_bounds__(kRaThreads, D == 64 ? 3 : 2) void ragged_attention_
   };
   // Whether there are keys from `base` to `end` that a row of the wave does not see.
   auto uneven = [&](int base, int end) __attribute__((always_inline)) {
-    if constexpr (KIND == kRaShared) return min(end, t.len) > last0;
+    if constexpr (kPrefixed) return min(end, t.len) > last0;
     return KIND == kRaPaged && (min(end, t.len) > last0 || (base < from1 && end > (int)p.sink));
   };
   auto seen_from = [&](int base) __attribute__((always_inline)) {  // of 64 keys from `base` on, those that the lane's row may see
@@ -898,12 +900,12 @@ __global__ __launch_bounds__(kRaThreads, D == 64 ? 3 : 2) void ragged_attention_
     return mx;
   };
 
-  const bool to_record = KIND == kRaShared ? t.to_record : t.n_parts > 1;
+  const bool to_record = KIND == kRaListed ? t.slot >= 0 : t.n_parts > 1;
   auto write_record = [&](int row_in_tile, int column, const float (&v)[4], float mm, float ll) __attribute__((always_inline)) {
     // four columns of a row of this part's record
-    if constexpr (KIND == kRaShared) {
+    if constexpr (KIND == kRaListed) {
       const int f = t.first + row_in_tile, token = (uint32_t)f / p.group, head = kv_head * p.group.d + (f - token * p.group.d);
-      const uint32_t slot = t.record + t.part;
+      const uint32_t slot = (uint32_t)t.slot;
       *reinterpret_cast<float4*>(shared_record<D>(p, slot, t.q0 + token, head) + column) = make_float4(v[0], v[1], v[2], v[3]);
       if (column == 0) *shared_sums<D>(p, slot, t.q0 + token, head) = make_float2(mm, ll);
       return;
@@ -1069,8 +1071,8 @@ __global__ __launch_bounds__(kRaThreads, D == 64 ? 3 : 2) void ragged_attention_
     load_rows(values, 0, rows_lds + (values ? 32 * kRowBytes : 0), true);
     load_rows(values, 16, rows_lds + (values ? 32 * kRowBytes : 0) + 16 * kRowBytes, true);
   };
-  const int u_end = 2 * s_end;
-  int u = 2 * s_begin + wave;
+  const int u_end = 2 * s_end, u_first = 2 * s_begin + (KIND == kRaListed && packed ? 0 : wave), u_step = KIND == kRaListed && packed ? 1 : 4;
+  int u = u_first;
   {
     const uint16_t* src = p.q + (t.q0 + row.token) * p.q_stride_token + row.head * p.q_stride_head + 8 * lh;
 #pragma unroll
@@ -1083,24 +1085,24 @@ __global__ __launch_bounds__(kRaThreads, D == 64 ? 3 : 2) void ragged_attention_
     }
     take_places(group_base(u), l32, 0);
     load_group(false);
-    if (kLooksUp) look_up(group_base(min(u + 4, u_end - 1)) + l32, 1);
+    if (kLooksUp) look_up(group_base(min(u + u_step, u_end - 1)) + l32, 1);
     load_group(true);
   }
   // Ahead of the loop and where the compiler sees it: it would otherwise count the loads of the queries as under way for good, and wait
   // for the keys' loads in their place ahead of every product.  0x0F70 = vmcnt(0), other counters untouched.
   __builtin_amdgcn_s_waitcnt(0x0F70);
   if (u < u_end) {
-    for (int slot = 1; u < u_end; u += 4, slot ^= 1) {
+    for (int slot = 1; u < u_end; u += u_step, slot ^= 1) {
       const uint64_t exist = there;
-      const bool more = u + 4 < u_end;
+      const bool more = u + u_step < u_end;
       wait_loads<kLoads>();  // K, and the places of the next group; V may be on its way
       float16v sc[1];
       scores(sc, rows_lds);
       if (more) {
-        take_places(group_base(u + 4), l32, slot);
+        take_places(group_base(u + u_step), l32, slot);
         wait_lds_reads();
         load_group(false);
-        if (kLooksUp) look_up(group_base(min(u + 8, u_end - 1)) + l32, slot ^ 1);
+        if (kLooksUp) look_up(group_base(min(u + 2 * u_step, u_end - 1)) + l32, slot ^ 1);
       }
       mask(sc, group_base(u), exist);
       follow(largest(sc));
@@ -1118,7 +1120,7 @@ __global__ __launch_bounds__(kRaThreads, D == 64 ? 3 : 2) void ragged_attention_
   if (kPages && !finite) {  // once more, group by group (see all_finite)
     once_more();
 #pragma unroll 1
-    for (u = 2 * s_begin + wave; u < u_end; u += 4) {
+    for (u = u_first; u < u_end; u += u_step) {
       if (kLooksUp) {
         look_up(group_base(u) + l32, 0);
         wait_loads<0>();
@@ -1135,8 +1137,26 @@ __global__ __launch_bounds__(kRaThreads, D == 64 ? 3 : 2) void ragged_attention_
       weigh_apart(sc, rows_lds + 32 * kRowBytes, group_base(u));
     }
   }
-  // The four waves' results, joined: each wave takes a quarter of the columns.
   l = exchange_sum(l);
+  if (KIND == kRaListed && packed) {
+    const Row to = own_row();
+    const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+    if (l32 < tile_rows) {
+#pragma unroll
+      for (int dt = 0; dt < kDTiles; ++dt)
+#pragma unroll
+        for (int g = 0; g < 4; ++g) {
+          const float v[4] = {o[dt][4 * g], o[dt][4 * g + 1], o[dt][4 * g + 2], o[dt][4 * g + 3]};
+          const int column = 32 * dt + 8 * g + 4 * lh;
+          if (to_record) write_record(l32, column, v, reference(), l);
+          else
+            *reinterpret_cast<uint2*>(p.out + (t.q0 + to.token) * p.out_stride_token + to.head * p.out_stride_head + column) =
+                make_uint2(T::pack2(v[0] * inv, v[1] * inv), T::pack2(v[2] * inv, v[3] * inv));
+        }
+    }
+    continue;
+  }
+  // The four waves' results, joined: each wave takes a quarter of the columns.
   float2* const ml = reinterpret_cast<float2*>(smem + 4 * kStepBytes + 4 * 512);
   if (lh == 0) ml[wave * 32 + l32] = make_float2(reference(), l);
   {
@@ -1218,12 +1238,290 @@ __global__ __launch_bounds__(kRaThreads) void ragged_join_kernel(RaParams p) {
   }
 }
 
+// ---- beginnings that groups attend together
+//
+// The rows of a joined group attend the beginning as tiles of their own, each stream's rows its own keys, and a last launch joins the two, row by
+// row.  What all this takes is known to the device alone, so a launch of one workgroup adds it up and lists the items: first the beginnings', in
+// parts, then the streams' own.  On a unit tiles of few rows, which wait for memory, then run beside wide ones.  A wave by itself takes two to
+// three times as long for a narrow tile as four do together, waiting for the page table, then for K, for little else: four tiles run side by
+// side, if one does not take longer than the launch does anyway.
+//
+// us of 64 single tokens x 32 / 8 heads over 16384 shared and 30 to 1000 own keys: items found by every workgroup in turn, beginnings first, in 32
+// parts 62, in 14 parts 63; so on workgroups of their own 50.
+constexpr int kRaPlanThreads = 256;   // a wave to a SIMD: 64 streams 8.6 us, with four waves, most of them idle, 10.9
+constexpr int kRaJoinedGroups = 256;  // in a launch at most: a thread each
+constexpr int kRaLeastPrefixPart = 2, kRaLeastOwnPart = 4;  // steps
+
+// us, by columns: of a wide tile's beginning, of its steps with up to one, two and three of them on a unit, of a narrow tile by four waves and by one,
+// of joining a part of a wide tile (of the whole device).
+struct RaCosts {
+  float wide, wide_step[3], narrow, narrow_step, alone, alone_step, join;
+};
+__device__ __forceinline__ constexpr RaCosts costs_of(int columns) {
+  return columns == 128 ? RaCosts{7.0f, {1.8f, 2.3f, 2.3f}, 5.5f, 1.3f, 3.4f, 3.3f, 0.0135f} : RaCosts{4.0f, {1.4f, 1.7f, 2.0f}, 4.2f, 0.95f, 4.1f, 2.65f, 0.007f};
+}
+
+struct RaSharedStream {
+  int q0, rows, len, base, shares, prefix_len, joined;
+  int parts;       // of a tile at most
+  uint32_t ticks;  // of an item
+};
+__device__ __forceinline__ RaSharedStream shared_stream(const RaParams& p, int b) {  // but for its group
+  RaSharedStream s;
+  const int limit = (int)p.n_queries;
+  const int start = p.q_starts[b], next = p.q_starts[b + 1];
+  const int64_t given = max((int64_t)p.kv_lens[b], (int64_t)0);
+  s.q0 = min(max(start, 0), limit);
+  s.rows = max(min(max(next, 0), limit) - s.q0, 0) * (int)p.group.d;
+  s.len = (int)min(given, p.table_keys);
+  s.base = (int)(given - ((int64_t)next - s.q0));
+  s.shares = -1;
+  s.prefix_len = s.joined = 0;
+  return s;
+}
+// Steps of a tile whose last row is `last_row` of its stream's, over the stream's own keys.
+__device__ __forceinline__ int own_steps_of(const RaParams& p, const RaSharedStream& s, int last_row) {
+  const int end = p.causal ? min(s.base + (int)((uint32_t)last_row / p.group) + 1, s.len) : s.len;
+  return end > 0 ? steps_of(end) : 0;
+}
+
+__device__ __forceinline__ float sum_upto(float v) {  // over this lane and those before it
+#define LL_DPP_ADD(ctrl, row_mask) v += __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, v), ctrl, row_mask, 0xF, true))
+  LL_DPP_ADD(0x111, 0xF);
+  LL_DPP_ADD(0x112, 0xF);
+  LL_DPP_ADD(0x114, 0xF);
+  LL_DPP_ADD(0x118, 0xF);
+  LL_DPP_ADD(0x142, 0xA);
+  LL_DPP_ADD(0x143, 0xC);
+#undef LL_DPP_ADD
+  return v;
+}
+template <typename V>
+__device__ __forceinline__ V of_lane(V v, int lane) {
+  return __builtin_bit_cast(V, __builtin_amdgcn_readlane(__builtin_bit_cast(int, v), lane));
+}
+// Sums over the threads of the planning workgroup, N at once: v becomes those before this thread, `all` those of all.
+template <typename V, int N>
+__device__ __forceinline__ void plan_sums(V (&v)[N], V (&all)[N], V (&of_waves)[N][kRaPlanThreads / 64]) {
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  V upto[N];
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    upto[i] = sum_upto(v[i]);
+    if (lane == 63) of_waves[i][wave] = upto[i];
+  }
+  __syncthreads();
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    const V waves = sum_upto(lane < kRaPlanThreads / 64 ? of_waves[i][lane] : (V)0);
+    all[i] = of_lane(waves, kRaPlanThreads / 64 - 1);
+    v[i] = upto[i] - v[i] + (wave ? of_lane(waves, max(wave - 1, 0)) : (V)0);
+  }
+  __syncthreads();
+}
+
+template <int D>
+__global__ __launch_bounds__(kRaPlanThreads) void shared_plan_kernel(RaParams p, uint32_t units) {
+  constexpr RaCosts cost = costs_of(D);
+  __shared__ int starts[kRaJoinedGroups + 1], lens[kRaJoinedGroups], group_q0[kRaJoinedGroups], group_rows[kRaJoinedGroups];  // lens below zero: joined
+  __shared__ uint32_t upto[kRaPlanThreads], ticks_upto[kRaPlanThreads];
+  __shared__ RaSharedStream streams[kRaPlanThreads];
+  __shared__ float floats[5][kRaPlanThreads / 64];
+  __shared__ uint32_t words[4][kRaPlanThreads / 64];
+  const int tid = threadIdx.x, lane = tid & 63;
+  const RaSharedStream early = shared_stream(p, min(tid, p.streams - 1));
+  float take[5] = {};  // beginnings; wide tiles, narrow ones by four waves, by one; how many of these
+  if (tid < p.n_groups) {
+    const RaGroup r = group_of(p, tid);
+    const int rows = r.n * (int)p.group.d;
+    starts[tid] = p.group_starts ? p.group_starts[tid] : 0;
+    if (tid == p.n_groups - 1) starts[tid + 1] = p.group_starts ? p.group_starts[tid + 1] : p.streams;
+    lens[tid] = r.joined ? -r.len : r.len;
+    group_q0[tid] = r.q0;
+    group_rows[tid] = rows;
+    if (r.joined) take[0] = (float)tiles_of(rows) * (float)steps_of(r.len) * (rows <= 32 ? cost.narrow_step : cost.wide_step[0]);
+  }
+  __syncthreads();
+  const auto with_group = [&](RaSharedStream s, int b) __attribute__((always_inline)) {
+    if (b >= p.streams) s.rows = 0;
+    int g = 0, end = p.n_groups + 1;
+    while (end - g > 1) {
+      const int at = (g + end) >> 1;
+      if (starts[at] <= b) g = at;
+      else end = at;
+    }
+    if (g == p.n_groups || starts[g] > b) return s;
+    s.shares = g;
+    s.joined = lens[g] < 0;
+    s.prefix_len = max(lens[g], 0);
+    return s;
+  };
+  const RaSharedStream first = with_group(early, tid);
+  const auto stream = [&](int b0) __attribute__((always_inline)) {  // of this thread
+    return b0 == 0 ? first : with_group(shared_stream(p, min(b0 + tid, p.streams - 1)), b0 + tid);
+  };
+  const auto steps_in = [](const RaSharedStream& s) { return steps_of(s.prefix_len) + steps_of(s.len); };
+  // ---- what there is to do, in us of a workgroup
+  for (int b0 = 0; b0 < p.streams; b0 += kRaPlanThreads) {
+    const RaSharedStream s = stream(b0);
+    const int steps = steps_in(s);
+    if (s.rows == 0 || (s.joined && steps == 0)) continue;
+    if (s.rows <= 32) {
+      take[2] += cost.narrow + cost.narrow_step * steps;
+      take[3] += cost.alone + cost.alone_step * steps;
+      take[4] += 1.0f;
+    } else {
+      take[1] += (float)tiles_of(s.rows) * (cost.wide + cost.wide_step[1] * steps);
+    }
+  }
+  float all_take[5];
+  plan_sums(take, all_take, floats);
+  const float heads = (float)p.kv_heads, prefixes = all_take[0] * heads, wide = all_take[1] * heads, narrow = all_take[2] * heads, alone = all_take[3] * heads,
+              tiles = all_take[4] * heads;
+  const bool pack = tiles > 0.0f && alone * p.groups <= 0.75f * tiles * (prefixes + wide + 0.25f * alone);
+  const float streams_take = wide + (pack ? 0.25f * alone : narrow);
+  // ---- steps of a part of a beginning: a lane to a number of them, about a workgroup's share.  Which one has all done first?
+  int best;
+  const int steps_tried = max((int)fminf((prefixes + streams_take) / p.groups / cost.wide_step[0] * (0.3f + 0.05f * lane), 1e9f), kRaLeastPrefixPart);
+  float least;
+  {
+    uint32_t items = 0;
+    int wide_part = 0, narrow_part = 0;
+    float rows = 0.0f;
+    for (int g = 0; g < p.n_groups; ++g) {
+      if (lens[g] >= 0 || group_rows[g] == 0) continue;
+      const int steps = steps_of(-lens[g]), n = shared_parts((uint32_t)steps, (uint32_t)steps_tried, p.prefix_parts), part = (steps + n - 1) / n;
+      items += (uint32_t)(tiles_of(group_rows[g]) * n);
+      rows += (float)group_rows[g] * n;
+      if (group_rows[g] <= 32) narrow_part = max(narrow_part, part);
+      else wide_part = max(wide_part, part);
+    }
+    items *= (uint32_t)p.kv_heads;
+    const float step = cost.wide_step[items <= units ? 0 : items <= 2 * units ? 1 : 2];
+    const float one = fmaxf(wide_part ? cost.wide + step * wide_part : 0.0f, narrow_part ? cost.narrow + cost.narrow_step * narrow_part : 0.0f);
+    const float takes = rows * heads * (cost.join / kRaTileRows) +
+                        (items < p.groups ? fmaxf(one, streams_take / (p.groups - items)) : one * ((items + p.groups - 1) / p.groups) + streams_take / p.groups);
+    least = takes;
+    for (int i = 1; i < 64; i <<= 1) least = fminf(least, __shfl_xor(least, i));
+    best = __builtin_ctzll(__builtin_amdgcn_ballot_w64(takes <= least) | (1ull << 63));
+  }
+  const uint32_t prefix_part = (uint32_t)__builtin_amdgcn_readlane(steps_tried, best);
+  // about a half of what a workgroup has to do, so that shares come out alike
+  const auto part_within = [&](float start, float step) { return (uint32_t)max((int)fminf((0.5f * least - start) / step, 1e9f), kRaLeastOwnPart); };
+  const uint32_t wide_own = part_within(cost.wide, cost.wide_step[1]), narrow_own = pack ? part_within(cost.alone, cost.alone_step) : part_within(cost.narrow, cost.narrow_step);
+  // ---- how many items there are, and what the streams' take: in whole numbers, so that shares begin and end at the same items.  Their sum
+  // stays below 2^31
+  const float ticks_per_us = fminf(4.0f, 0x1p28f / fmaxf(wide + narrow + alone, 1.0f));
+  const auto with_parts = [&](RaSharedStream s) __attribute__((always_inline)) {
+    const int steps = steps_in(s);
+    // a joined stream without keys of its own has nothing to add, one that is not has its zeros to write
+    s.parts = max(shared_parts((uint32_t)steps, s.rows <= 32 ? narrow_own : wide_own, p.own_parts), s.joined ? 0 : 1);
+    const int part = s.parts ? (steps + s.parts - 1) / s.parts : 0;
+    const float us = s.rows > 32 ? cost.wide + cost.wide_step[1] * part : pack ? 0.25f * (cost.alone + cost.alone_step * part) : cost.narrow + cost.narrow_step * part;
+    s.ticks = (uint32_t)(us * ticks_per_us) + 1;
+    return s;
+  };
+  const RaSharedStream first_parts = with_parts(first);
+  const auto parted_stream = [&](int b0) __attribute__((always_inline)) { return b0 == 0 ? first_parts : with_parts(stream(b0)); };
+  uint32_t count[4] = {}, all[4];  // items of beginnings; of streams, a workgroup's and a wave's; ticks of all these
+  if (tid < p.n_groups && lens[tid] < 0)
+    count[0] = (uint32_t)(tiles_of(group_rows[tid]) * shared_parts((uint32_t)steps_of(-lens[tid]), prefix_part, p.prefix_parts));
+  const uint32_t of_group = count[0];
+  for (int b0 = 0; b0 < p.streams; b0 += kRaPlanThreads) {
+    const RaSharedStream s = parted_stream(b0);
+    const uint32_t items = (uint32_t)(tiles_of(s.rows) * s.parts);
+    if (pack && s.rows <= 32) count[2] += items;
+    else count[1] += items;
+    count[3] += items * (uint32_t)p.kv_heads * s.ticks;
+    if (b0 + tid < p.streams)
+      p.joined[b0 + tid] = RaJoined{s.joined ? shared_parts((uint32_t)steps_of(-lens[s.shares]), prefix_part, p.prefix_parts) : 0, steps_of(s.prefix_len), s.joined};
+  }
+  plan_sums(count, all, words);
+  // ---- the items of the beginnings
+  const uint32_t prefix_items = min(all[0], p.most_listed);
+  if (tid < p.n_groups) upto[tid] = count[0] + of_group;
+  __syncthreads();
+  for (uint32_t i = tid; i < prefix_items; i += kRaPlanThreads) {
+    int before = -1, g = p.n_groups - 1;  // the first group whose items reach beyond it
+    while (g - before > 1) {
+      const int at = (before + g) >> 1;
+      if (upto[at] <= i) before = at;
+      else g = at;
+    }
+    const int steps = steps_of(-lens[g]), n = shared_parts((uint32_t)steps, prefix_part, p.prefix_parts), each = (steps + n - 1) / n;
+    const uint32_t at = i - (g ? upto[g - 1] : 0), tile = at / (uint32_t)n;
+    const int part = (int)(at - tile * (uint32_t)n);
+    p.listed[i] = RaListedItem{group_q0[g], group_rows[g], (int)tile * kRaTileRows, 0, 0, -lens[g], g, 0, min(part * each, steps), min((part + 1) * each, steps), part, 0};
+  }
+  // ---- the items of the streams: those of a workgroup, then those of a wave; the workgroups without a beginning share them by what they take
+  const uint32_t busy = prefix_items * (uint32_t)p.kv_heads, first_free = busy < p.groups ? busy : 0, free = p.groups - first_free, share = all[3] / free + 1;
+  const uint32_t single_items = min(prefix_items + all[1], p.most_listed) * (uint32_t)p.kv_heads;
+  const uint32_t items_in_all = min(prefix_items + all[1] + all[2], p.most_listed) * (uint32_t)p.kv_heads;  // no more, whatever the starts are
+  for (uint32_t w = tid; w <= first_free; w += kRaPlanThreads) p.first_items[w] = busy;
+  uint32_t listed = prefix_items, ticks_before = 0;
+  for (int alone_now = 0; alone_now < (all[2] ? 2 : 1); ++alone_now) {
+    for (int b0 = 0; b0 < p.streams; b0 += kRaPlanThreads) {
+      const RaSharedStream s = parted_stream(b0);
+      const uint32_t items = (pack && s.rows <= 32) == (alone_now == 1) ? (uint32_t)(tiles_of(s.rows) * s.parts) : 0;
+      const uint32_t mine = items * (uint32_t)p.kv_heads * s.ticks;
+      uint32_t sums[2] = {items, mine}, of_all[2];
+      plan_sums(sums, of_all, *reinterpret_cast<uint32_t(*)[2][kRaPlanThreads / 64]>(&words));
+      upto[tid] = sums[0] + items;
+      ticks_upto[tid] = sums[1] + mine;
+      streams[tid] = s;
+      __syncthreads();
+      const auto beyond = [&](const uint32_t* sums_upto, uint32_t at) __attribute__((always_inline)) {  // the first stream whose sum reaches beyond
+        int before = -1, of = kRaPlanThreads - 1;
+        while (of - before > 1) {
+          const int mid = (before + of) >> 1;
+          if (sums_upto[mid] <= at) before = mid;
+          else of = mid;
+        }
+        return of;
+      };
+      // workgroups whose share begins among these items; of those that a wave takes, four go together
+      for (uint32_t w = (uint32_t)tid + 1; w < free; w += kRaPlanThreads) {
+        const uint32_t begin = w * share - ticks_before;
+        if (w * share < ticks_before || begin >= of_all[1]) continue;
+        const int of = beyond(ticks_upto, begin);
+        const uint32_t each = streams[of].ticks;
+        uint32_t i = (listed + (of ? upto[of - 1] : 0)) * (uint32_t)p.kv_heads + (begin - (of ? ticks_upto[of - 1] : 0) + each - 1) / each;
+        if (alone_now == 1) i = single_items + (i - single_items + 3) / 4 * 4;
+        p.first_items[first_free + w] = i;
+      }
+      for (uint32_t i = tid; i < of_all[0] && listed + i < p.most_listed; i += kRaPlanThreads) {
+        const int of = beyond(upto, i);
+        const RaSharedStream r = streams[of];
+        const uint32_t item = i - (of ? upto[of - 1] : 0), from_last = r.parts == 1 ? item : item / (uint32_t)r.parts;
+        const int part = (int)(item - from_last * (uint32_t)r.parts), tile = tiles_of(r.rows) - 1 - (int)from_last;  // the last one sees most keys
+        const int steps = steps_of(r.prefix_len) + own_steps_of(p, r, min(tile * kRaTileRows + kRaTileRows, r.rows) - 1);
+        // as the joining launch counts them; a tile that sees fewer keys than the stream's last leaves parts out
+        const int used = r.parts == 1 ? max(min(steps, 1), r.joined ? 0 : 1)
+                                      : max(shared_parts((uint32_t)steps, r.rows <= 32 ? narrow_own : wide_own, p.own_parts), r.joined ? 0 : 1);
+        const int each = used > 1 ? (steps + used - 1) / used : steps;
+        p.listed[listed + i] = RaListedItem{r.q0, part < used ? r.rows : 0, tile * kRaTileRows, r.len, r.base, r.prefix_len, max(r.shares, 0), b0 + of,
+                                            min(part * each, steps), min((part + 1) * each, steps), r.joined || used > 1 ? (int)p.prefix_parts + part : -1, 0};
+      }
+      listed += of_all[0];
+      ticks_before += of_all[1];
+      __syncthreads();
+    }
+  }
+  for (uint32_t w = (uint32_t)tid + 1; w < free; w += kRaPlanThreads)  // shares that begin behind the last item
+    if (w * share >= ticks_before) p.first_items[first_free + w] = items_in_all;
+  if (tid == 0) {
+    p.first_items[p.groups] = items_in_all;
+    *p.list = RaList{busy, single_items, items_in_all, wide_own, narrow_own};
+  }
+}
+
 // Joins, row by row, the parts of what a group attended together with the parts of the streams' own keys, and the parts of tiles that were cut:
 // D / 4 lanes a row, the heads of one token to a workgroup, or some of them.
 template <typename T, int D>
 __global__ __launch_bounds__(kRaThreads) void shared_join_kernel(RaParams p) {
   constexpr int kRows = kRaThreads * 4 / D;
   const int lane = threadIdx.x & 63, column = threadIdx.x % (D / 4) * 4;
+  const RaList list = *p.list;
   for (int64_t token = blockIdx.x; token < p.n_queries; token += gridDim.x) {
     // the last stream that begins at or before the token: 64 of what is left at a time
     int b = 0, left = p.streams + 1;
@@ -1236,31 +1534,17 @@ __global__ __launch_bounds__(kRaThreads) void shared_join_kernel(RaParams p) {
     }
     b = __builtin_amdgcn_readfirstlane(b);
     if (b >= p.streams || p.q_starts[b] > token) continue;
-    const int limit = (int)p.n_queries, next = p.q_starts[b + 1];
-    const int q0 = min(max(p.q_starts[b], 0), limit), n = max(min(max(next, 0), limit) - q0, 0);
-    const int64_t given = max((int64_t)p.kv_lens[b], (int64_t)0);
-    const int len = (int)min(given, p.table_keys), base = (int)(given - ((int64_t)next - q0));
-    const int g = group_of_stream(p, b);
-    int of_group = 0, ahead = 0;  // parts of the beginning; or its steps, ahead of the stream's own
-    bool joined = false;
-    if (g >= 0) {
-      const RaGroup r = group_of(p, g);
-      joined = r.joined;
-      if (joined) of_group = shared_parts((uint32_t)steps_of(r.len), p.prefix_part_steps, p.prefix_parts);
-      else ahead = steps_of(r.len);
-    }
-    const int rows = n * (int)p.group.d;
-    const uint32_t per_part = rows <= 32 ? p.narrow_part_steps : p.part_steps;
+    const RaSharedStream s = shared_stream(p, b);
+    const RaJoined with = p.joined[b];
     for (int head = blockIdx.y * kRows + threadIdx.x / (D / 4); head < p.heads; head += gridDim.y * kRows) {
-      const int f = (int)(token - q0) * (int)p.group.d + (int)((uint32_t)head - (uint32_t)head / p.group * p.group.d);
-      const int last_row = min(f / kRaTileRows * kRaTileRows + kRaTileRows, rows) - 1;
-      const int end = p.causal ? min(base + (int)((uint32_t)last_row / p.group) + 1, len) : len;
-      const int parts = shared_parts((uint32_t)(ahead + (end > 0 ? steps_of(end) : 0)), per_part, p.own_parts);
-      if (!joined && parts <= 1) continue;  // its results are where they belong
+      const int f = (int)(token - s.q0) * (int)p.group.d + (int)((uint32_t)head - (uint32_t)head / p.group * p.group.d);
+      const int steps = with.ahead + own_steps_of(p, s, min(f / kRaTileRows * kRaTileRows + kRaTileRows, s.rows) - 1);
+      const int parts = shared_parts((uint32_t)steps, s.rows <= 32 ? list.narrow_part : list.wide_part, p.own_parts);
+      if (!with.joined && parts <= 1) continue;  // its results are where they belong
       float m = -INFINITY, l = 0.0f, v[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll 4
-      for (int i = 0; i < of_group + parts; ++i) {
-        const uint32_t slot = i < of_group ? i : p.prefix_parts + i - of_group;
+#pragma unroll 8
+      for (int i = 0; i < with.parts + parts; ++i) {
+        const uint32_t slot = i < with.parts ? i : p.prefix_parts + i - with.parts;
         const float2 e = *shared_sums<D>(p, slot, token, head);
         const float4 y = *reinterpret_cast<const float4*>(shared_record<D>(p, slot, token, head) + column);
         const float top = fmaxf(m, e.x);
@@ -1553,17 +1837,33 @@ static int check_shared(const ll_shared_prefix_args* a) {
   return LL_OK;
 }
 
-// How a launch over shared beginnings is divided (host arithmetic).
+// How a launch over shared beginnings is divided (host arithmetic).  Without parts of beginnings every stream goes over its group's by itself,
+// divided as keys of one table are.
 struct SharedPlan {
-  uint32_t groups, part_steps, narrow_part_steps, prefix_part_steps, prefix_parts, own_parts;
-  size_t bytes;
+  RaPlan alone;
+  uint32_t groups, prefix_parts, own_parts;  // parts of a tile at most: the device makes as many as fit
+  uint32_t most_listed;
+  size_t list, listed, joined, first_items, bytes;  // where they begin in the workspace, behind the records; all of it
 };
-constexpr size_t kRaMostSharedBytes = (size_t)1 << 30;  // of records
-constexpr int64_t kRaLeastPrefixSteps = 6, kRaMostParts = 64;
+constexpr size_t kRaMostSharedBytes = (size_t)256 << 20;  // of records, where there are more than two of a row
+constexpr int64_t kRaMostParts = 64;
+// What a launch to list the items and one to join their results have to save, in steps of wide tiles of all workgroups: some 10 us.
+constexpr int64_t kRaJoinedSteps = 5;
+
+// A stream's keys and those of its group's beginning as if they were in one table.
+static ll_ragged_attention_args one_table(const ll_shared_prefix_args& s) {
+  ll_ragged_attention_args a = s.own;
+  const int64_t own = a.table_width * a.page_size, shared = s.groups ? s.prefix_width * a.page_size : 0;
+  const auto told = [](int64_t n, int64_t reach) { return n > 0 && n < reach ? n : reach; };
+  a.max_kv_len = told(a.max_kv_len, own) + told(s.max_prefix_len, shared);
+  a.table_width += s.groups ? s.prefix_width : 0;
+  return a;
+}
 
 static SharedPlan plan_shared(const ll_shared_prefix_args& s, int cus) {
   const ll_ragged_attention_args& a = s.own;
-  SharedPlan r{0, 1u << 24, 1u << 24, 1u << 24, 0, 1, 0};
+  SharedPlan r{};
+  r.own_parts = 1;
   if (a.n_queries == 0 || a.streams == 0) return r;
   const int64_t group = a.num_heads / a.num_kv_heads, slots = (a.head_dim == 64 ? 3 : 2) * cus;
   const int64_t longest = a.max_q_len > 0 && a.max_q_len < a.n_queries ? a.max_q_len : a.n_queries;
@@ -1575,50 +1875,45 @@ static SharedPlan plan_shared(const ll_shared_prefix_args& s, int cus) {
   const int64_t own_steps = steps_within(a.max_kv_len, a.n_pages ? a.table_width : 0);
   const int64_t prefix_steps = s.groups && a.n_pages ? steps_within(s.max_prefix_len, s.prefix_width) : 0;
   const int64_t together = a.n_queries * group / kRaTileRows + std::min(s.groups, a.streams);  // tiles of whole groups
-  const size_t part_bytes = (size_t)a.n_queries * a.num_heads * (a.head_dim + 2) * sizeof(float);
-  int64_t most_parts = std::min<int64_t>(kRaMostParts, (int64_t)(kRaMostSharedBytes / part_bytes));
-  if (a.streams > 1 && prefix_steps > 0 && most_parts >= 2 && a.streams * prefix_steps >= kRaJoinedCost * (a.n_queries * group / kRaTileRows)) {
-    // What all workgroups have to do, in steps, and a workgroup's share of it.
-    const int64_t narrow = tiles * a.num_kv_heads, all = together * a.num_kv_heads * prefix_steps + narrow * ((own_steps + 1) / 2 + 3);
-    const int64_t share = std::max((all + slots - 1) / slots, kRaLeastPrefixSteps);
-    r.prefix_parts = (uint32_t)std::min((prefix_steps + share - 1) / share, most_parts - 1);
-    r.own_parts = (uint32_t)std::min((own_steps + 2 * share - 1) / (2 * share), most_parts - (int64_t)r.prefix_parts);
-    r.own_parts = std::max(r.own_parts, 1u);
-    r.prefix_part_steps = (uint32_t)((prefix_steps + r.prefix_parts - 1) / r.prefix_parts);
-    r.part_steps = r.narrow_part_steps = (uint32_t)std::max<int64_t>((own_steps + r.own_parts - 1) / r.own_parts, 1);
+  const size_t rows = (size_t)a.n_queries * a.num_heads, part_bytes = rows * (a.head_dim + 2) * sizeof(float);
+  if (a.streams > 1 && s.groups <= kRaJoinedGroups && part_bytes <= 4 * kRaMostSharedBytes &&
+      ((tiles - together) * prefix_steps - kRaJoinedCost / 2 * together) * a.num_kv_heads > kRaJoinedSteps * slots) {
+    // No tile has more parts than there are workgroups for each head, since a workgroup's share is not below that much of one tile.
+    const int64_t most = std::max<int64_t>(std::min<int64_t>(kRaMostParts, (int64_t)(kRaMostSharedBytes / part_bytes)), 2);
+    r.own_parts = (uint32_t)std::max<int64_t>(std::min<int64_t>((own_steps + kRaLeastOwnPart - 1) / kRaLeastOwnPart, most / 4), 1);
+    r.prefix_parts = (uint32_t)std::min(std::min<int64_t>((prefix_steps + kRaLeastPrefixPart - 1) / kRaLeastPrefixPart, slots / a.num_kv_heads + 1), most - r.own_parts);
+    const int64_t items = together * r.prefix_parts + (a.n_queries * group / kRaTileRows + a.streams) * r.own_parts;
+    r.groups = (uint32_t)std::min(slots, items * a.num_kv_heads);
+    r.most_listed = (uint32_t)std::min<int64_t>(items, 0xffffffffll / a.num_kv_heads);
+    const auto behind = [](size_t bytes) { return (bytes + 63) / 64 * 64; };
+    r.list = behind(part_bytes * (r.prefix_parts + r.own_parts));
+    r.listed = behind(r.list + sizeof(RaList));
+    r.joined = behind(r.listed + items * sizeof(RaListedItem));
+    r.first_items = behind(r.joined + a.streams * sizeof(RaJoined));
+    r.bytes = r.first_items + (r.groups + 1) * sizeof(uint32_t);
   } else {
-    const int64_t steps = std::max<int64_t>(prefix_steps + own_steps, 1), busy = tiles * a.num_kv_heads;
-    int64_t best = 1, least = -1;
-    for (int64_t parts = 1; parts <= most_parts && (parts == 1 || steps / parts >= 3); ++parts) {
-      const int64_t each = (steps + parts - 1) / parts, items = busy * parts, rounds = (items + slots - 1) / slots;
-      const int64_t step = kRaStepCost[a.head_dim == 128][items <= cus ? 0 : items <= 2 * cus ? 1 : 2];
-      const int64_t cost = rounds * (each * step + kRaItemCost * std::min(items, slots) / slots) + (parts > 1 ? kRaJoinCost + kRaRecordCost * items / slots : 0);
-      if (least < 0 || cost < least) {
-        least = cost;
-        best = parts;
-      }
-    }
-    r.own_parts = (uint32_t)best;
-    if (best > 1) r.part_steps = r.narrow_part_steps = (uint32_t)((steps + best - 1) / best);
+    r.alone = plan_ragged(one_table(s), cus);
+    r.groups = r.alone.groups;
+    r.bytes = r.alone.bytes;
   }
-  if (r.prefix_parts + r.own_parts > 1) r.bytes = part_bytes * (r.prefix_parts + r.own_parts);
-  r.groups = (uint32_t)std::min(slots, (together * r.prefix_parts + (a.n_queries * group / kRaTileRows + a.streams) * r.own_parts) * a.num_kv_heads);
   return r;
 }
 
 template <typename T, int D>
-static int launch_shared(const RaParams& p, uint32_t grid, hipStream_t stream) {
+static int launch_shared(const RaParams& p, uint32_t grid, uint32_t units, hipStream_t stream) {
+  if (p.prefix_parts == 0) return launch_ragged<T, D, kRaPrefixed>(p, grid, stream);
   static std::atomic<uint64_t> allowed{0};
-  const void* kernel = reinterpret_cast<const void*>(&ragged_attention_kernel<T, D, kRaShared>);
-  if (int rc = allow_dynamic_lds(kernel, kRaLds<D>, allowed, "ll_shared_prefix_attention")) return rc;
-  ragged_attention_kernel<T, D, kRaShared><<<grid, kRaThreads, kRaLds<D>, stream>>>(p);
+  constexpr size_t kLds = kRaLds<D>;
+  const void* kernel = reinterpret_cast<const void*>(&ragged_attention_kernel<T, D, kRaListed>);
+  if (int rc = allow_dynamic_lds(kernel, kLds, allowed, "ll_shared_prefix_attention")) return rc;
+  shared_plan_kernel<D><<<1, kRaPlanThreads, 0, stream>>>(p, units);
+  LL_CHECK_LAUNCH("ll_shared_prefix_attention (items)");
+  ragged_attention_kernel<T, D, kRaListed><<<grid, kRaThreads, kLds, stream>>>(p);
   LL_CHECK_LAUNCH("ll_shared_prefix_attention");
-  if (p.prefix_parts + p.own_parts > 1) {
-    const uint32_t rows = kRaThreads * 4 / D;
-    const dim3 join((uint32_t)std::min<int64_t>(p.n_queries, 4096), ((uint32_t)p.heads + rows - 1) / rows);
-    shared_join_kernel<T, D><<<join, kRaThreads, 0, stream>>>(p);
-    LL_CHECK_LAUNCH("ll_shared_prefix_attention (join)");
-  }
+  const uint32_t rows = kRaThreads * 4 / D;
+  const dim3 join((uint32_t)std::min<int64_t>(p.n_queries, 4096), ((uint32_t)p.heads + rows - 1) / rows);
+  shared_join_kernel<T, D><<<join, kRaThreads, 0, stream>>>(p);
+  LL_CHECK_LAUNCH("ll_shared_prefix_attention (join)");
   return LL_OK;
 }
 }  // namespace ll
@@ -1660,12 +1955,21 @@ extern "C" int ll_shared_prefix_attention(const ll_shared_prefix_args* args, voi
              "ll_shared_prefix_attention: a workspace of %zu bytes, 16-byte aligned, is needed", plan.bytes);
   RaParams p = ragged_params(a);
   p.groups = plan.groups;
-  p.part_steps = plan.part_steps;
-  p.narrow_part_steps = plan.narrow_part_steps;
-  p.prefix_part_steps = plan.prefix_part_steps;
+  p.part_steps = plan.alone.part_steps;
+  p.part_share = plan.alone.part_share;
+  p.narrow_part_steps = plan.alone.narrow_part_steps;
+  p.records = plan.alone.records;
   p.prefix_parts = plan.prefix_parts;
   p.own_parts = plan.own_parts;
   p.record_mem = static_cast<float*>(a->workspace);
+  if (plan.prefix_parts) {
+    uint8_t* const memory = static_cast<uint8_t*>(a->workspace);
+    p.list = reinterpret_cast<RaList*>(memory + plan.list);
+    p.listed = reinterpret_cast<RaListedItem*>(memory + plan.listed);
+    p.most_listed = plan.most_listed;
+    p.joined = reinterpret_cast<RaJoined*>(memory + plan.joined);
+    p.first_items = reinterpret_cast<uint32_t*>(memory + plan.first_items);
+  }
   p.n_groups = shares ? (int)args->groups : 0;
   p.group_starts = args->group_starts;
   p.prefix_lens = args->prefix_lens;
@@ -1675,6 +1979,6 @@ extern "C" int ll_shared_prefix_attention(const ll_shared_prefix_args* args, voi
   const uint32_t grid = p.groups + (a->clear_rest ? kRaClearGroups : 0);
   if (grid == 0) return LL_OK;
   const hipStream_t st = static_cast<hipStream_t>(stream);
-  if (a->dtype == LL_DTYPE_BF16) return a->head_dim == 128 ? launch_shared<Bf16, 128>(p, grid, st) : launch_shared<Bf16, 64>(p, grid, st);
-  return a->head_dim == 128 ? launch_shared<F16, 128>(p, grid, st) : launch_shared<F16, 64>(p, grid, st);
+  if (a->dtype == LL_DTYPE_BF16) return a->head_dim == 128 ? launch_shared<Bf16, 128>(p, grid, cus, st) : launch_shared<Bf16, 64>(p, grid, cus, st);
+  return a->head_dim == 128 ? launch_shared<F16, 128>(p, grid, cus, st) : launch_shared<F16, 64>(p, grid, cus, st);
 }

@@ -181,6 +181,9 @@ def test_memory_that_calls_ask_for():
     assert shared_bytes(shared_args(own=dict(n_queries=0))) == 0 and shared_bytes(shared_args(own=dict(streams=0))) == 0
     # results of parts for every row, whole records of fp32 columns, reference point and sum
     some = shared_bytes(shared_args(own=dict(n_queries=64, streams=64, num_heads=32, num_kv_heads=8, max_q_len=1, max_kv_len=64), prefix_width=1024))
-    assert some > 0 and some % (64 * 32 * 130 * 4) == 0
-    # several long chunks, each of which fills tiles by itself: nothing is joined
-    assert shared_bytes(shared_args(own=dict(n_queries=10560, streams=4, num_heads=24, num_kv_heads=24, max_q_len=2640, max_kv_len=2640, page_size=880), prefix_width=12)) == 0
+    assert some // (64 * 32 * 130 * 4) > 1
+    # several long chunks, each of which fills tiles by itself, go over the beginning one by one, as over keys of one table
+    chunks = dict(n_queries=10560, streams=4, num_heads=24, num_kv_heads=24, max_q_len=2640, page_size=880)
+    one = shared_args(own=dict(**chunks, table_width=15, max_kv_len=13200, causal=0)).own
+    assert lib.ll_ragged_attention_workspace(ctypes.byref(one), 256, ctypes.byref(n)) == 0
+    assert shared_bytes(shared_args(own=dict(**chunks, table_width=3, max_kv_len=2640), prefix_width=12, max_prefix_len=10560)) == n.value
