@@ -110,7 +110,6 @@ struct RaParams {
   RaListedItem* listed;
   uint32_t most_listed;
   RaJoined* joined;                    // [streams]
-  uint32_t* first_items;               // [groups + 1]: of a workgroup, behind the beginnings'
 };
 
 // Positions of 16-byte pieces in an LDS row of D columns.  The reads of a wave then go through all banks: 8 neighbouring rows of one
@@ -462,11 +461,10 @@ __global__ __launch_bounds__(kRaThreads, D == 64 ? 3 : 2) void ragged_attention_
   if constexpr (KIND != kRaListed) cursor.start(p);
   bool packed = false;  // each wave has an item of its own, of up to 32 rows
   RaList list{};
-  uint32_t next_item = 0, end_item = 0;
+  uint32_t free_from = 0, round = 0;  // listed: the first workgroup that takes streams' items, how many times it did
   if constexpr (KIND == kRaListed) {
     list = *p.list;
-    next_item = p.first_items[blockIdx.x];
-    end_item = min(p.first_items[blockIdx.x + 1], list.items);
+    free_from = list.prefix_items < p.groups ? list.prefix_items : 0;
   }
   for (uint32_t id = blockIdx.x;; id += p.groups) {
   uint32_t index = id / (uint32_t)p.kv_heads, kv_head = id - index * (uint32_t)p.kv_heads;
@@ -475,15 +473,21 @@ __global__ __launch_bounds__(kRaThreads, D == 64 ? 3 : 2) void ragged_attention_
     uint32_t item = id;
     packed = false;
     if (item >= list.prefix_items) {
-      if (next_item >= end_item) return;
-      item = next_item;
-      packed = item >= list.single_items;
-      next_item += packed ? 4 : 1;
-      if (packed) item += threadIdx.x >> 6;
+      // from the longest to the shortest, back and forth over the workgroups without a beginning
+      if (blockIdx.x < free_from) return;
+      const uint32_t free = p.groups - free_from, at = blockIdx.x - free_from;
+      item = list.prefix_items + round * free + (round & 1 ? free - 1 - at : at);
+      ++round;
+      if (item >= list.single_items) {
+        packed = true;
+        item = list.single_items + 4 * (item - list.single_items);
+        if (item >= list.items) return;
+        item += threadIdx.x >> 6;
+      }
     }
     __syncthreads();  // no wave is at the item before any more
     item = (uint32_t)__builtin_amdgcn_readfirstlane((int)item);
-    if (packed && item >= end_item) continue;
+    if (packed && item >= list.items) continue;
     index = item / (uint32_t)p.kv_heads;
     kv_head = item - index * (uint32_t)p.kv_heads;
     const RaListedItem& of = p.listed[index];
@@ -1250,7 +1254,8 @@ __global__ __launch_bounds__(kRaThreads) void ragged_join_kernel(RaParams p) {
 // parts 62, in 14 parts 63; so on workgroups of their own 50.
 constexpr int kRaPlanThreads = 256;   // a wave to a SIMD: 64 streams 8.6 us, with four waves, most of them idle, 10.9
 constexpr int kRaJoinedGroups = 256;  // in a launch at most: a thread each
-constexpr int kRaLeastPrefixPart = 2, kRaLeastOwnPart = 4;  // steps
+constexpr int kRaSizes = 64;
+constexpr int kRaLeastPrefixPart = 2, kRaLeastOwnPart = 5;  // steps
 
 // us, by columns: of a wide tile's beginning, of its steps with up to one, two and three of them on a unit, of a narrow tile by four waves and by one,
 // of joining a part of a wide tile (of the whole device).
@@ -1263,8 +1268,6 @@ __device__ __forceinline__ constexpr RaCosts costs_of(int columns) {
 
 struct RaSharedStream {
   int q0, rows, len, base, shares, prefix_len, joined;
-  int parts;       // of a tile at most
-  uint32_t ticks;  // of an item
 };
 __device__ __forceinline__ RaSharedStream shared_stream(const RaParams& p, int b) {  // but for its group
   RaSharedStream s;
@@ -1324,10 +1327,9 @@ template <int D>
 __global__ __launch_bounds__(kRaPlanThreads) void shared_plan_kernel(RaParams p, uint32_t units) {
   constexpr RaCosts cost = costs_of(D);
   __shared__ int starts[kRaJoinedGroups + 1], lens[kRaJoinedGroups], group_q0[kRaJoinedGroups], group_rows[kRaJoinedGroups];  // lens below zero: joined
-  __shared__ uint32_t upto[kRaPlanThreads], ticks_upto[kRaPlanThreads];
-  __shared__ RaSharedStream streams[kRaPlanThreads];
+  __shared__ uint32_t upto[kRaJoinedGroups], sizes[2 * kRaSizes];  // items up to a group; of so long, for a workgroup and for a wave
   __shared__ float floats[5][kRaPlanThreads / 64];
-  __shared__ uint32_t words[4][kRaPlanThreads / 64];
+  __shared__ uint32_t words[1][kRaPlanThreads / 64];
   const int tid = threadIdx.x, lane = tid & 63;
   const RaSharedStream early = shared_stream(p, min(tid, p.streams - 1));
   float take[5] = {};  // beginnings; wide tiles, narrow ones by four waves, by one; how many of these
@@ -1379,11 +1381,36 @@ __global__ __launch_bounds__(kRaPlanThreads) void shared_plan_kernel(RaParams p,
   const float heads = (float)p.kv_heads, prefixes = all_take[0] * heads, wide = all_take[1] * heads, narrow = all_take[2] * heads, alone = all_take[3] * heads,
               tiles = all_take[4] * heads;
   const bool pack = tiles > 0.0f && alone * p.groups <= 0.75f * tiles * (prefixes + wide + 0.25f * alone);
-  const float streams_take = wide + (pack ? 0.25f * alone : narrow);
+  // ---- the streams' items, of about half of what a workgroup has to do: how many there are of about as much, what they take
+  const float estimate = (prefixes + wide + (pack ? 0.25f * alone : narrow)) / p.groups, per_us = 0.75f * kRaSizes / fmaxf(estimate, 1.0f);
+  const auto part_within = [&](float start, float step) { return (uint32_t)max((int)fminf((0.5f * estimate - start) / step, 1e9f), kRaLeastOwnPart); };
+  const uint32_t wide_own = part_within(cost.wide, cost.wide_step[1]), narrow_own = pack ? part_within(cost.alone, cost.alone_step) : part_within(cost.narrow, cost.narrow_step);
+  if (tid < 2 * kRaSizes) sizes[tid] = 0;
+  __syncthreads();
+  // f(class, size, steps of the tile, its parts, steps of each, us of each) for every tile of a stream that has something to do
+  const auto each_tile = [&](const RaSharedStream& s, auto&& f) __attribute__((always_inline)) {
+    for (int tile = 0; tile < tiles_of(s.rows); ++tile) {
+      const int steps = steps_of(s.prefix_len) + own_steps_of(p, s, min(tile * kRaTileRows + kRaTileRows, s.rows) - 1);
+      if (s.joined && steps == 0) continue;  // nothing to add; one that is not joined has its zeros to write
+      const int parts = max(shared_parts((uint32_t)steps, s.rows <= 32 ? narrow_own : wide_own, p.own_parts), 1), part = parts > 1 ? (steps + parts - 1) / parts : steps;
+      const bool by_wave = pack && s.rows <= 32;
+      const float us = s.rows > 32 ? cost.wide + cost.wide_step[1] * part : by_wave ? 0.25f * (cost.alone + cost.alone_step * part) : cost.narrow + cost.narrow_step * part;
+      f(tile, by_wave ? 1 : 0, kRaSizes - 1 - min((int)((by_wave ? 4.0f : 1.0f) * us * per_us), kRaSizes - 1), steps, parts, part, us);
+    }
+  };
+  float takes_now[1] = {0.0f}, takes_all[1];
+  for (int b0 = 0; b0 < p.streams; b0 += kRaPlanThreads) {
+    const RaSharedStream s = stream(b0);
+    each_tile(s, [&](int, int by_wave, int size, int, int parts, int, float us) {
+      atomicAdd(&sizes[by_wave * kRaSizes + size], (uint32_t)parts);
+      takes_now[0] += parts * us;
+    });
+  }
+  plan_sums(takes_now, takes_all, *reinterpret_cast<float(*)[1][kRaPlanThreads / 64]>(&floats));
+  const float streams_take = takes_all[0] * heads;
   // ---- steps of a part of a beginning: a lane to a number of them, about a workgroup's share.  Which one has all done first?
-  int best;
   const int steps_tried = max((int)fminf((prefixes + streams_take) / p.groups / cost.wide_step[0] * (0.3f + 0.05f * lane), 1e9f), kRaLeastPrefixPart);
-  float least;
+  uint32_t prefix_part;
   {
     uint32_t items = 0;
     int wide_part = 0, narrow_part = 0;
@@ -1401,45 +1428,24 @@ __global__ __launch_bounds__(kRaPlanThreads) void shared_plan_kernel(RaParams p,
     const float one = fmaxf(wide_part ? cost.wide + step * wide_part : 0.0f, narrow_part ? cost.narrow + cost.narrow_step * narrow_part : 0.0f);
     const float takes = rows * heads * (cost.join / kRaTileRows) +
                         (items < p.groups ? fmaxf(one, streams_take / (p.groups - items)) : one * ((items + p.groups - 1) / p.groups) + streams_take / p.groups);
-    least = takes;
+    float least = takes;
     for (int i = 1; i < 64; i <<= 1) least = fminf(least, __shfl_xor(least, i));
-    best = __builtin_ctzll(__builtin_amdgcn_ballot_w64(takes <= least) | (1ull << 63));
+    const int best = __builtin_ctzll(__builtin_amdgcn_ballot_w64(takes <= least) | (1ull << 63));
+    prefix_part = (uint32_t)__builtin_amdgcn_readlane(steps_tried, best);
   }
-  const uint32_t prefix_part = (uint32_t)__builtin_amdgcn_readlane(steps_tried, best);
-  // about a half of what a workgroup has to do, so that shares come out alike
-  const auto part_within = [&](float start, float step) { return (uint32_t)max((int)fminf((0.5f * least - start) / step, 1e9f), kRaLeastOwnPart); };
-  const uint32_t wide_own = part_within(cost.wide, cost.wide_step[1]), narrow_own = pack ? part_within(cost.alone, cost.alone_step) : part_within(cost.narrow, cost.narrow_step);
-  // ---- how many items there are, and what the streams' take: in whole numbers, so that shares begin and end at the same items.  Their sum
-  // stays below 2^31
-  const float ticks_per_us = fminf(4.0f, 0x1p28f / fmaxf(wide + narrow + alone, 1.0f));
-  const auto with_parts = [&](RaSharedStream s) __attribute__((always_inline)) {
-    const int steps = steps_in(s);
-    // a joined stream without keys of its own has nothing to add, one that is not has its zeros to write
-    s.parts = max(shared_parts((uint32_t)steps, s.rows <= 32 ? narrow_own : wide_own, p.own_parts), s.joined ? 0 : 1);
-    const int part = s.parts ? (steps + s.parts - 1) / s.parts : 0;
-    const float us = s.rows > 32 ? cost.wide + cost.wide_step[1] * part : pack ? 0.25f * (cost.alone + cost.alone_step * part) : cost.narrow + cost.narrow_step * part;
-    s.ticks = (uint32_t)(us * ticks_per_us) + 1;
-    return s;
-  };
-  const RaSharedStream first_parts = with_parts(first);
-  const auto parted_stream = [&](int b0) __attribute__((always_inline)) { return b0 == 0 ? first_parts : with_parts(stream(b0)); };
-  uint32_t count[4] = {}, all[4];  // items of beginnings; of streams, a workgroup's and a wave's; ticks of all these
-  if (tid < p.n_groups && lens[tid] < 0)
-    count[0] = (uint32_t)(tiles_of(group_rows[tid]) * shared_parts((uint32_t)steps_of(-lens[tid]), prefix_part, p.prefix_parts));
-  const uint32_t of_group = count[0];
   for (int b0 = 0; b0 < p.streams; b0 += kRaPlanThreads) {
-    const RaSharedStream s = parted_stream(b0);
-    const uint32_t items = (uint32_t)(tiles_of(s.rows) * s.parts);
-    if (pack && s.rows <= 32) count[2] += items;
-    else count[1] += items;
-    count[3] += items * (uint32_t)p.kv_heads * s.ticks;
+    const RaSharedStream s = stream(b0);
     if (b0 + tid < p.streams)
       p.joined[b0 + tid] = RaJoined{s.joined ? shared_parts((uint32_t)steps_of(-lens[s.shares]), prefix_part, p.prefix_parts) : 0, steps_of(s.prefix_len), s.joined};
   }
-  plan_sums(count, all, words);
+  uint32_t of_groups[1] = {}, all_of_groups[1];
+  if (tid < p.n_groups && lens[tid] < 0)
+    of_groups[0] = (uint32_t)(tiles_of(group_rows[tid]) * shared_parts((uint32_t)steps_of(-lens[tid]), prefix_part, p.prefix_parts));
+  const uint32_t of_group = of_groups[0];
+  plan_sums(of_groups, all_of_groups, words);
   // ---- the items of the beginnings
-  const uint32_t prefix_items = min(all[0], p.most_listed);
-  if (tid < p.n_groups) upto[tid] = count[0] + of_group;
+  const uint32_t prefix_items = min(all_of_groups[0], p.most_listed);
+  if (tid < p.n_groups) upto[tid] = of_groups[0] + of_group;
   __syncthreads();
   for (uint32_t i = tid; i < prefix_items; i += kRaPlanThreads) {
     int before = -1, g = p.n_groups - 1;  // the first group whose items reach beyond it
@@ -1453,65 +1459,30 @@ __global__ __launch_bounds__(kRaPlanThreads) void shared_plan_kernel(RaParams p,
     const int part = (int)(at - tile * (uint32_t)n);
     p.listed[i] = RaListedItem{group_q0[g], group_rows[g], (int)tile * kRaTileRows, 0, 0, -lens[g], g, 0, min(part * each, steps), min((part + 1) * each, steps), part, 0};
   }
-  // ---- the items of the streams: those of a workgroup, then those of a wave; the workgroups without a beginning share them by what they take
-  const uint32_t busy = prefix_items * (uint32_t)p.kv_heads, first_free = busy < p.groups ? busy : 0, free = p.groups - first_free, share = all[3] / free + 1;
-  const uint32_t single_items = min(prefix_items + all[1], p.most_listed) * (uint32_t)p.kv_heads;
-  const uint32_t items_in_all = min(prefix_items + all[1] + all[2], p.most_listed) * (uint32_t)p.kv_heads;  // no more, whatever the starts are
-  for (uint32_t w = tid; w <= first_free; w += kRaPlanThreads) p.first_items[w] = busy;
-  uint32_t listed = prefix_items, ticks_before = 0;
-  for (int alone_now = 0; alone_now < (all[2] ? 2 : 1); ++alone_now) {
-    for (int b0 = 0; b0 < p.streams; b0 += kRaPlanThreads) {
-      const RaSharedStream s = parted_stream(b0);
-      const uint32_t items = (pack && s.rows <= 32) == (alone_now == 1) ? (uint32_t)(tiles_of(s.rows) * s.parts) : 0;
-      const uint32_t mine = items * (uint32_t)p.kv_heads * s.ticks;
-      uint32_t sums[2] = {items, mine}, of_all[2];
-      plan_sums(sums, of_all, *reinterpret_cast<uint32_t(*)[2][kRaPlanThreads / 64]>(&words));
-      upto[tid] = sums[0] + items;
-      ticks_upto[tid] = sums[1] + mine;
-      streams[tid] = s;
-      __syncthreads();
-      const auto beyond = [&](const uint32_t* sums_upto, uint32_t at) __attribute__((always_inline)) {  // the first stream whose sum reaches beyond
-        int before = -1, of = kRaPlanThreads - 1;
-        while (of - before > 1) {
-          const int mid = (before + of) >> 1;
-          if (sums_upto[mid] <= at) before = mid;
-          else of = mid;
-        }
-        return of;
-      };
-      // workgroups whose share begins among these items; of those that a wave takes, four go together
-      for (uint32_t w = (uint32_t)tid + 1; w < free; w += kRaPlanThreads) {
-        const uint32_t begin = w * share - ticks_before;
-        if (w * share < ticks_before || begin >= of_all[1]) continue;
-        const int of = beyond(ticks_upto, begin);
-        const uint32_t each = streams[of].ticks;
-        uint32_t i = (listed + (of ? upto[of - 1] : 0)) * (uint32_t)p.kv_heads + (begin - (of ? ticks_upto[of - 1] : 0) + each - 1) / each;
-        if (alone_now == 1) i = single_items + (i - single_items + 3) / 4 * 4;
-        p.first_items[first_free + w] = i;
-      }
-      for (uint32_t i = tid; i < of_all[0] && listed + i < p.most_listed; i += kRaPlanThreads) {
-        const int of = beyond(upto, i);
-        const RaSharedStream r = streams[of];
-        const uint32_t item = i - (of ? upto[of - 1] : 0), from_last = r.parts == 1 ? item : item / (uint32_t)r.parts;
-        const int part = (int)(item - from_last * (uint32_t)r.parts), tile = tiles_of(r.rows) - 1 - (int)from_last;  // the last one sees most keys
-        const int steps = steps_of(r.prefix_len) + own_steps_of(p, r, min(tile * kRaTileRows + kRaTileRows, r.rows) - 1);
-        // as the joining launch counts them; a tile that sees fewer keys than the stream's last leaves parts out
-        const int used = r.parts == 1 ? max(min(steps, 1), r.joined ? 0 : 1)
-                                      : max(shared_parts((uint32_t)steps, r.rows <= 32 ? narrow_own : wide_own, p.own_parts), r.joined ? 0 : 1);
-        const int each = used > 1 ? (steps + used - 1) / used : steps;
-        p.listed[listed + i] = RaListedItem{r.q0, part < used ? r.rows : 0, tile * kRaTileRows, r.len, r.base, r.prefix_len, max(r.shares, 0), b0 + of,
-                                            min(part * each, steps), min((part + 1) * each, steps), r.joined || used > 1 ? (int)p.prefix_parts + part : -1, 0};
-      }
-      listed += of_all[0];
-      ticks_before += of_all[1];
-      __syncthreads();
+  // ---- the items of the streams: those of a workgroup, then those of a wave, the longest of each first
+  uint32_t singles = 0, waves = 0;
+  if (tid < 64) {
+    static_assert(kRaSizes == 64, "a lane to a size");
+    const uint32_t single = sizes[lane], wave = sizes[kRaSizes + lane], singles_upto = sum_upto(single), waves_upto = sum_upto(wave);
+    singles = of_lane(singles_upto, 63);
+    waves = of_lane(waves_upto, 63);
+    sizes[lane] = prefix_items + singles_upto - single;
+    sizes[kRaSizes + lane] = prefix_items + singles + waves_upto - wave;
+    if (lane == 0) {  // no more than there is room for, whatever the starts are
+      const uint32_t heads_of = (uint32_t)p.kv_heads;
+      *p.list = RaList{prefix_items * heads_of, min(prefix_items + singles, p.most_listed) * heads_of, min(prefix_items + singles + waves, p.most_listed) * heads_of, wide_own,
+                       narrow_own};
     }
   }
-  for (uint32_t w = (uint32_t)tid + 1; w < free; w += kRaPlanThreads)  // shares that begin behind the last item
-    if (w * share >= ticks_before) p.first_items[first_free + w] = items_in_all;
-  if (tid == 0) {
-    p.first_items[p.groups] = items_in_all;
-    *p.list = RaList{busy, single_items, items_in_all, wide_own, narrow_own};
+  __syncthreads();
+  for (int b0 = 0; b0 < p.streams; b0 += kRaPlanThreads) {
+    const RaSharedStream s = stream(b0);
+    each_tile(s, [&](int tile, int by_wave, int size, int steps, int parts, int part, float) {
+      const uint32_t at = atomicAdd(&sizes[by_wave * kRaSizes + size], (uint32_t)parts);
+      for (int i = 0; i < parts && at + i < p.most_listed; ++i)
+        p.listed[at + i] = RaListedItem{s.q0, s.rows, tile * kRaTileRows, s.len, s.base, s.prefix_len, max(s.shares, 0), b0 + tid, min(i * part, steps), min((i + 1) * part, steps),
+                                        s.joined || parts > 1 ? (int)p.prefix_parts + i : -1, 0};
+    });
   }
 }
 
@@ -1843,7 +1814,7 @@ struct SharedPlan {
   RaPlan alone;
   uint32_t groups, prefix_parts, own_parts;  // parts of a tile at most: the device makes as many as fit
   uint32_t most_listed;
-  size_t list, listed, joined, first_items, bytes;  // where they begin in the workspace, behind the records; all of it
+  size_t list, listed, joined, bytes;  // where they begin in the workspace, behind the records; all of it
 };
 constexpr size_t kRaMostSharedBytes = (size_t)256 << 20;  // of records, where there are more than two of a row
 constexpr int64_t kRaMostParts = 64;
@@ -1889,8 +1860,7 @@ static SharedPlan plan_shared(const ll_shared_prefix_args& s, int cus) {
     r.list = behind(part_bytes * (r.prefix_parts + r.own_parts));
     r.listed = behind(r.list + sizeof(RaList));
     r.joined = behind(r.listed + items * sizeof(RaListedItem));
-    r.first_items = behind(r.joined + a.streams * sizeof(RaJoined));
-    r.bytes = r.first_items + (r.groups + 1) * sizeof(uint32_t);
+    r.bytes = r.joined + a.streams * sizeof(RaJoined);
   } else {
     r.alone = plan_ragged(one_table(s), cus);
     r.groups = r.alone.groups;
@@ -1968,7 +1938,6 @@ extern "C" int ll_shared_prefix_attention(const ll_shared_prefix_args* args, voi
     p.listed = reinterpret_cast<RaListedItem*>(memory + plan.listed);
     p.most_listed = plan.most_listed;
     p.joined = reinterpret_cast<RaJoined*>(memory + plan.joined);
-    p.first_items = reinterpret_cast<uint32_t*>(memory + plan.first_items);
   }
   p.n_groups = shares ? (int)args->groups : 0;
   p.group_starts = args->group_starts;
