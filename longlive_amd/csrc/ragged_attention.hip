@@ -1331,7 +1331,10 @@ __global__ __launch_bounds__(kRaPlanThreads) void shared_plan_kernel(RaParams p,
   __shared__ float floats[5][kRaPlanThreads / 64];
   __shared__ uint32_t words[1][kRaPlanThreads / 64];
   const int tid = threadIdx.x, lane = tid & 63;
-  const RaSharedStream early = shared_stream(p, min(tid, p.streams - 1));
+  // threads of a stream, for its tiles, and streams at a time
+  const int per_stream = p.streams <= 16 ? 16 : p.streams <= 32 ? 8 : p.streams <= 64 ? 4 : p.streams <= 128 ? 2 : 1, at_once = kRaPlanThreads / per_stream;
+  const int tile0 = tid % per_stream, mine = tid / per_stream;
+  const RaSharedStream early = shared_stream(p, min(mine, p.streams - 1));
   float take[5] = {};  // beginnings; wide tiles, narrow ones by four waves, by one; how many of these
   if (tid < p.n_groups) {
     const RaGroup r = group_of(p, tid);
@@ -1358,16 +1361,16 @@ __global__ __launch_bounds__(kRaPlanThreads) void shared_plan_kernel(RaParams p,
     s.prefix_len = max(lens[g], 0);
     return s;
   };
-  const RaSharedStream first = with_group(early, tid);
+  const RaSharedStream first = with_group(early, mine);
   const auto stream = [&](int b0) __attribute__((always_inline)) {  // of this thread
-    return b0 == 0 ? first : with_group(shared_stream(p, min(b0 + tid, p.streams - 1)), b0 + tid);
+    return b0 == 0 ? first : with_group(shared_stream(p, min(b0 + mine, p.streams - 1)), b0 + mine);
   };
   const auto steps_in = [](const RaSharedStream& s) { return steps_of(s.prefix_len) + steps_of(s.len); };
   // ---- what there is to do, in us of a workgroup
-  for (int b0 = 0; b0 < p.streams; b0 += kRaPlanThreads) {
+  for (int b0 = 0; b0 < p.streams; b0 += at_once) {
     const RaSharedStream s = stream(b0);
     const int steps = steps_in(s);
-    if (s.rows == 0 || (s.joined && steps == 0)) continue;
+    if (tile0 != 0 || s.rows == 0 || (s.joined && steps == 0)) continue;
     if (s.rows <= 32) {
       take[2] += cost.narrow + cost.narrow_step * steps;
       take[3] += cost.alone + cost.alone_step * steps;
@@ -1389,7 +1392,7 @@ __global__ __launch_bounds__(kRaPlanThreads) void shared_plan_kernel(RaParams p,
   __syncthreads();
   // f(class, size, steps of the tile, its parts, steps of each, us of each) for every tile of a stream that has something to do
   const auto each_tile = [&](const RaSharedStream& s, auto&& f) __attribute__((always_inline)) {
-    for (int tile = 0; tile < tiles_of(s.rows); ++tile) {
+    for (int tile = tile0; tile < tiles_of(s.rows); tile += per_stream) {
       const int steps = steps_of(s.prefix_len) + own_steps_of(p, s, min(tile * kRaTileRows + kRaTileRows, s.rows) - 1);
       if (s.joined && steps == 0) continue;  // nothing to add; one that is not joined has its zeros to write
       const int parts = max(shared_parts((uint32_t)steps, s.rows <= 32 ? narrow_own : wide_own, p.own_parts), 1), part = parts > 1 ? (steps + parts - 1) / parts : steps;
@@ -1399,7 +1402,7 @@ __global__ __launch_bounds__(kRaPlanThreads) void shared_plan_kernel(RaParams p,
     }
   };
   float takes_now[1] = {0.0f}, takes_all[1];
-  for (int b0 = 0; b0 < p.streams; b0 += kRaPlanThreads) {
+  for (int b0 = 0; b0 < p.streams; b0 += at_once) {
     const RaSharedStream s = stream(b0);
     each_tile(s, [&](int, int by_wave, int size, int, int parts, int, float us) {
       atomicAdd(&sizes[by_wave * kRaSizes + size], (uint32_t)parts);
@@ -1433,10 +1436,10 @@ __global__ __launch_bounds__(kRaPlanThreads) void shared_plan_kernel(RaParams p,
     const int best = __builtin_ctzll(__builtin_amdgcn_ballot_w64(takes <= least) | (1ull << 63));
     prefix_part = (uint32_t)__builtin_amdgcn_readlane(steps_tried, best);
   }
-  for (int b0 = 0; b0 < p.streams; b0 += kRaPlanThreads) {
+  for (int b0 = 0; b0 < p.streams; b0 += at_once) {
     const RaSharedStream s = stream(b0);
-    if (b0 + tid < p.streams)
-      p.joined[b0 + tid] = RaJoined{s.joined ? shared_parts((uint32_t)steps_of(-lens[s.shares]), prefix_part, p.prefix_parts) : 0, steps_of(s.prefix_len), s.joined};
+    if (tile0 == 0 && b0 + mine < p.streams)
+      p.joined[b0 + mine] = RaJoined{s.joined ? shared_parts((uint32_t)steps_of(-lens[s.shares]), prefix_part, p.prefix_parts) : 0, steps_of(s.prefix_len), s.joined};
   }
   uint32_t of_groups[1] = {}, all_of_groups[1];
   if (tid < p.n_groups && lens[tid] < 0)
@@ -1475,12 +1478,12 @@ __global__ __launch_bounds__(kRaPlanThreads) void shared_plan_kernel(RaParams p,
     }
   }
   __syncthreads();
-  for (int b0 = 0; b0 < p.streams; b0 += kRaPlanThreads) {
+  for (int b0 = 0; b0 < p.streams; b0 += at_once) {
     const RaSharedStream s = stream(b0);
     each_tile(s, [&](int tile, int by_wave, int size, int steps, int parts, int part, float) {
       const uint32_t at = atomicAdd(&sizes[by_wave * kRaSizes + size], (uint32_t)parts);
       for (int i = 0; i < parts && at + i < p.most_listed; ++i)
-        p.listed[at + i] = RaListedItem{s.q0, s.rows, tile * kRaTileRows, s.len, s.base, s.prefix_len, max(s.shares, 0), b0 + tid, min(i * part, steps), min((i + 1) * part, steps),
+        p.listed[at + i] = RaListedItem{s.q0, s.rows, tile * kRaTileRows, s.len, s.base, s.prefix_len, max(s.shares, 0), b0 + mine, min(i * part, steps), min((i + 1) * part, steps),
                                         s.joined || parts > 1 ? (int)p.prefix_parts + i : -1, 0};
     });
   }
