@@ -178,6 +178,7 @@ struct RaGroup {
 // Going together saves a group of m streams about m / 2 tiles of every step of the beginning, what its streams' last tiles lack, and costs two
 // records of every row: it is done from this many steps times streams to a tile on.
 constexpr int kRaJoinedCost = 28;
+__device__ __forceinline__ int group_len(const RaParams& p, int g) { return (int)min((int64_t)max(p.prefix_lens[g], 0), p.prefix_keys); }
 __device__ __forceinline__ RaGroup group_of(const RaParams& p, int g) {
   const int from = p.group_starts ? min(max(p.group_starts[g], 0), p.streams) : 0;
   const int to = p.group_starts ? min(max(p.group_starts[g + 1], from), p.streams) : p.streams;
@@ -185,7 +186,7 @@ __device__ __forceinline__ RaGroup group_of(const RaParams& p, int g) {
   const int limit = (int)p.n_queries;
   r.q0 = min(max(p.q_starts[from], 0), limit);
   r.n = max(min(max(p.q_starts[to], 0), limit) - r.q0, 0);
-  r.len = (int)min((int64_t)max(p.prefix_lens[g], 0), p.prefix_keys);
+  r.len = group_len(p, g);
   r.joined = p.prefix_parts > 0 && to - from > 1 && r.n > 0 &&
              (int64_t)(to - from) * (r.len / kRaKeys) >= (int64_t)kRaJoinedCost * (((uint32_t)r.n * p.group.d + kRaTileRows - 1) / kRaTileRows);
   return r;
@@ -291,8 +292,8 @@ __device__ __forceinline__ RaStreams load_streams(const RaParams& p, int b0, uin
   s.key0 = (int)key0;
   if constexpr (KIND == kRaPrefixed) {
     const int g = group_of_stream(p, b);
+    s.prefix_len = g < 0 ? 0 : group_len(p, g);
     s.shares = max(g, 0);
-    s.prefix_len = g < 0 ? 0 : group_of(p, g).len;
   }
   const int rows = s.n * (int)p.group.d;
   const int tiles = tiles_of(rows);
@@ -1383,7 +1384,10 @@ __global__ __launch_bounds__(kRaPlanThreads) void shared_plan_kernel(RaParams p,
   plan_sums(take, all_take, floats);
   const float heads = (float)p.kv_heads, prefixes = all_take[0] * heads, wide = all_take[1] * heads, narrow = all_take[2] * heads, alone = all_take[3] * heads,
               tiles = all_take[4] * heads;
-  const bool pack = tiles > 0.0f && alone * p.groups <= 0.75f * tiles * (prefixes + wide + 0.25f * alone);
+  // us with four waves to each / one: 128 single tokens of five groups x 32 / 8 heads (1024 tiles for 512 workgroups) over 20 to 2000 own keys 99.2 /
+  // 87.8, 100 x 40 / 8 over 20 to 60 30.6 / 29.4, 32 x 24 over 20 to 600 50.5 / 49.1; 64 x 32 / 8 over 30 to 1000 (512 tiles) 51.6 / 57.4, 20 of 1 to
+  // 64 tokens x 24 over 10 to 400 (some 300 narrow ones) 51.9 / 63.9.
+  const bool pack = tiles >= 1.4f * p.groups && alone * p.groups <= 2.0f * tiles * (prefixes + wide + 0.25f * alone);
   // ---- the streams' items, of about half of what a workgroup has to do: how many there are of about as much, what they take
   const float estimate = (prefixes + wide + (pack ? 0.25f * alone : narrow)) / p.groups, per_us = 0.75f * kRaSizes / fmaxf(estimate, 1.0f);
   const auto part_within = [&](float start, float step) { return (uint32_t)max((int)fminf((0.5f * estimate - start) / step, 1e9f), kRaLeastOwnPart); };
