@@ -1204,9 +1204,10 @@ def rotate_by_position(q, k, v, q_weight, k_weight, eps, frequencies, amplitude,
         raise ValueError(f"{what}: a grid of a frame's tokens goes with the pairs that frames, rows and columns turn")
     rows, columns, frame_pairs, row_pairs = 0, 0, 0, 0
     if grid is not None:
-        if len(grid) != 2 or len(sections) != 3 or min(grid) < 1 or min(sections) < 0 or grid[0] * grid[1] >= 1 << 31 or sum(sections) != frequencies.numel():
+        if len(grid) != 2 or len(sections) != 3 or any(int(n) != n for n in (*grid, *sections)) or min(grid) < 1 or min(sections) < 0 or \
+                grid[0] * grid[1] >= 1 << 31 or sum(sections) != frequencies.numel():
             raise ValueError(f"{what}: a grid {tuple(grid)} of rows and columns, pairs {tuple(sections)} of frames, rows and columns for {frequencies.numel()} frequencies")
-        (rows, columns), (frame_pairs, row_pairs, _) = grid, sections
+        rows, columns, frame_pairs, row_pairs = (int(n) for n in (*grid, *sections[:2]))
     if not abs(float(amplitude)) < float("inf"):
         raise ValueError(f"{what}: amplitude {amplitude}")
     if q.is_cuda:
@@ -1270,6 +1271,7 @@ def step_layout(new_lens, kv_lens, page_table, free_pages, page_size, num_tokens
     for name, n, least in (("page_size", page_size, 1), ("num_tokens", num_tokens, 0)):
         if int(n) != n or not least <= n < 1 << 31:
             raise ValueError(f"{what}: {name} {n}")
+    page_size, num_tokens = int(page_size), int(num_tokens)
     if prefix_lens is None and group_starts is not None:
         raise ValueError(f"{what}: group_starts goes with prefix_lens")
     groups = 0 if prefix_lens is None else _check_groups(what, streams, group_starts, prefix_lens)

@@ -98,7 +98,7 @@ def test_refusals_of_rotation(no_gpu_needed):
                 dict(positions=slots.int()), dict(positions=slots[:2]), dict(frequencies=f.float()), dict(frequencies=f[:30]), dict(frequencies=f.view(4, 8)),
                 dict(frequencies=rotary_frequencies(72)), dict(grid=(2, 3)), dict(sections=(12, 10, 10)), dict(grid=(2, 3), sections=(12, 10, 9)),
                 dict(grid=(0, 3), sections=(12, 10, 10)), dict(grid=(2, 3, 4), sections=(12, 10, 10)), dict(grid=(1 << 16, 1 << 15), sections=(12, 10, 10)),
-                dict(grid=(2, 3), sections=(42, -10, 0)), dict(amplitude=float("nan")), dict(amplitude=float("inf")),
+                dict(grid=(2, 3), sections=(42, -10, 0)), dict(grid=(2.5, 3), sections=(12, 10, 10)), dict(amplitude=float("nan")), dict(amplitude=float("inf")),
                 dict(q=torch.zeros(3, 2, 264, dtype=BF16), k=torch.zeros(3, 2, 264, dtype=BF16))):
         with pytest.raises(ValueError):
             rotate_by_position(**{**ok, **bad})
