@@ -72,12 +72,17 @@ __device__ __forceinline__ void unpack4(uint2 w, float* f) {
 
 // Two heads a lane once the device has waves enough: us with one / two, 1000 tokens x (32 + 8 + 8) heads 8.6 / 9.0, 2640 x (24 + 24) 14.9 / 14.1,
 // 16000 x (32 + 8 + 8) 92.9 / 72.4, 16381 x (40 + 8 + 8) of 64 columns 57.0 / 46.2 (four: 74.2 and 44.3).
+// With angles formed: 1000 x (32 + 8 + 8) 6.8 / 6.1, 2640 x (24 + 24) 13.2 / 13.3 (of video frames 13.1 / 14.1), 10560 x (24 + 24) 49.8 / 45.9, 10560 x
+// (32 + 8) 33.1 / 34.3, 40000 x (32 + 8 + 8) 184 / 176.
 constexpr int64_t kManyWaves = 8192;
 
 // Cosines and sines of pairs 4 l .. 4 l + 3 at a position, which is the wave's.  A position times a frequency takes 64 bits: at position
 // 2^20 its rounding to 32 would turn the fastest pairs by 2^-4.  The matter is settled in turns, of which the whole ones are dropped; what is
 // left is exact to 2^-26 of a turn in 32 bits, and the hardware's sine and cosine of it
 // are off by no more than 2^-22, a thousandth of the rounding to f16 that follows.
+// Formed once for the wave's heads, it hides behind their loads: 40000 x (32 + 8 + 8) heads of 128 columns, 983 MB, 176 us, 5.6 TB/s; 16381 x (40 + 8
+// + 8) of 64 with 32 rotated, 235 MB, 36 and 49 on two cards; 2640 x (24 + 24) by video frames, 65 MB, 14.1, without the table's 90 MB for 176 000
+// positions; 24 x (16 + 4 + 4) 3.4 on the device, 5.6 from call to call.
 __device__ __forceinline__ void form_angles(const FormedAngles& a, int64_t pos, int l, float (&cs)[4], float (&sn)[4]) {
   double f[4];
   *reinterpret_cast<double2*>(f) = *reinterpret_cast<const double2*>(a.frequencies + 4 * l);

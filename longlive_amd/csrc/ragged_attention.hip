@@ -60,7 +60,7 @@ constexpr int kRaPaged = 0, kRaRows = 1, kRaMaskedRows = 2, kRaPrefixed = 3, kRa
 struct RaListedItem {
   int q0, rows, first, len, base, prefix_len, prefix_row, table_row, s_begin, s_end;
   int slot;  // of the part's results, -1: they are the tile's
-  int unused;
+  int unused;  // to whole 16 bytes
 };
 struct RaList {
   uint32_t prefix_items, single_items, items;  // items of beginnings; with those that take a workgroup; with those that take a wave
@@ -176,7 +176,9 @@ struct RaGroup {
   bool joined;  // its rows attend the beginning together, each stream's rows then its own keys, and the two are joined; else one behind the other
 };
 // Going together saves a group of m streams about m / 2 tiles of every step of the beginning, what its streams' last tiles lack, and costs two
-// records of every row: it is done from this many steps times streams to a tile on.
+// records of every row: it is done from this many steps times streams to a tile on.  us with all groups together / with those that gain: 16 groups
+// of 4 streams x 33 to 64 tokens x 32 / 8 heads of 128 columns over 2000 shared keys 226 / 173 (none gains), 4 of 16 over 1000 143 / 111, 16 of 4
+// x 12 of 64 over 2000 76 / 76 (all do), one of 16 x 16 / 4 of 64 over 2000 36 / 43.
 constexpr int kRaJoinedCost = 28;
 __device__ __forceinline__ int group_len(const RaParams& p, int g) { return (int)min((int64_t)max(p.prefix_lens[g], 0), p.prefix_keys); }
 __device__ __forceinline__ RaGroup group_of(const RaParams& p, int g) {
@@ -1392,6 +1394,15 @@ __global__ __launch_bounds__(kRaPlanThreads) void shared_plan_kernel(RaParams p,
   const float estimate = (prefixes + wide + (pack ? 0.25f * alone : narrow)) / p.groups, per_us = 0.75f * kRaSizes / fmaxf(estimate, 1.0f);
   const auto part_within = [&](float start, float step) { return (uint32_t)max((int)fminf((0.5f * estimate - start) / step, 1e9f), kRaLeastOwnPart); };
   const uint32_t wide_own = part_within(cost.wide, cost.wide_step[1]), narrow_own = pack ? part_within(cost.alone, cost.alone_step) : part_within(cost.narrow, cost.narrow_step);
+  // What an item takes, in 65536ths of a size: whole numbers, since it has to come out the same where it is counted and where it is listed.
+  struct Size {
+    uint32_t start, step;
+  };
+  const auto sizes_of = [&](float start, float step) {
+    const auto whole = [&](float us) { return (uint32_t)__builtin_amdgcn_readfirstlane((int)(65536.0f * us * per_us)); };
+    return Size{whole(start), whole(step)};
+  };
+  const Size wide_size = sizes_of(cost.wide, cost.wide_step[1]), narrow_size = pack ? sizes_of(cost.alone, cost.alone_step) : sizes_of(cost.narrow, cost.narrow_step);
   if (tid < 2 * kRaSizes) sizes[tid] = 0;
   __syncthreads();
   // f(class, size, steps of the tile, its parts, steps of each, us of each) for every tile of a stream that has something to do
@@ -1401,8 +1412,9 @@ __global__ __launch_bounds__(kRaPlanThreads) void shared_plan_kernel(RaParams p,
       if (s.joined && steps == 0) continue;  // nothing to add; one that is not joined has its zeros to write
       const int parts = max(shared_parts((uint32_t)steps, s.rows <= 32 ? narrow_own : wide_own, p.own_parts), 1), part = parts > 1 ? (steps + parts - 1) / parts : steps;
       const bool by_wave = pack && s.rows <= 32;
+      const Size z = s.rows <= 32 ? narrow_size : wide_size;
       const float us = s.rows > 32 ? cost.wide + cost.wide_step[1] * part : by_wave ? 0.25f * (cost.alone + cost.alone_step * part) : cost.narrow + cost.narrow_step * part;
-      f(tile, by_wave ? 1 : 0, kRaSizes - 1 - min((int)((by_wave ? 4.0f : 1.0f) * us * per_us), kRaSizes - 1), steps, parts, part, us);
+      f(tile, by_wave ? 1 : 0, kRaSizes - 1 - (int)min((z.start + (uint64_t)z.step * (uint32_t)part) >> 16, (uint64_t)kRaSizes - 1), steps, parts, part, us);
     }
   };
   float takes_now[1] = {0.0f}, takes_all[1];
@@ -1825,8 +1837,13 @@ struct SharedPlan {
 };
 constexpr size_t kRaMostSharedBytes = (size_t)256 << 20;  // of records, where there are more than two of a row
 constexpr int64_t kRaMostParts = 64;
-// What a launch to list the items and one to join their results have to save, in steps of wide tiles of all workgroups: some 10 us.
-constexpr int64_t kRaJoinedSteps = 5;
+// What a launch to list the items and one to join their results have to save, in steps of all workgroups: some 10 us.  Steps of narrow tiles
+// are shorter.  A group takes as long as so many steps more, for its tile's beginning, for its records, and since keys that its streams go over one
+// after the other come from the caches but for the first time.  us joined / direct on the one side, single tokens x 24 heads of 128 columns: 16
+// streams over 1000 keys 25.5 / 26.3, over 2000 26 / 58, 16 groups of 4 over 2000 112 / 195, 4 over 4000 28 / 33, 16 of 33 to 64 tokens over 2000 57 /
+// 82; on the other: 16 over 500 22.6 / 19.3, 16 groups of 4 over 500 58 / 52, 16 of 4 x 32 / 8 heads over 1000 39 / 28, 4 x 32 / 8 over 4000 25 / 20,
+// 16 of 33 to 64 tokens x 12 of 64 over 2000 35 / 32.  Wrong by most: 4 of 33 to 64 tokens x 16 / 4 heads of 64 over 2000 stay direct, 27 / 56.
+constexpr int64_t kRaJoinedSteps = 5, kRaJoinedNarrowSteps = 7, kRaJoinedGroupSteps = 20;
 
 // A stream's keys and those of its group's beginning as if they were in one table.
 static ll_ragged_attention_args one_table(const ll_shared_prefix_args& s) {
@@ -1852,13 +1869,15 @@ static SharedPlan plan_shared(const ll_shared_prefix_args& s, int cus) {
   };
   const int64_t own_steps = steps_within(a.max_kv_len, a.n_pages ? a.table_width : 0);
   const int64_t prefix_steps = s.groups && a.n_pages ? steps_within(s.max_prefix_len, s.prefix_width) : 0;
-  const int64_t together = a.n_queries * group / kRaTileRows + std::min(s.groups, a.streams);  // tiles of whole groups
+  const int64_t groups = std::min(s.groups, a.streams), together = a.n_queries * group / kRaTileRows + groups;  // tiles of whole groups
   const size_t rows = (size_t)a.n_queries * a.num_heads, part_bytes = rows * (a.head_dim + 2) * sizeof(float);
   if (a.streams > 1 && s.groups <= kRaJoinedGroups && part_bytes <= 4 * kRaMostSharedBytes &&
-      ((tiles - together) * prefix_steps - kRaJoinedCost / 2 * together) * a.num_kv_heads > kRaJoinedSteps * slots) {
+      ((tiles - together) * prefix_steps - kRaJoinedGroupSteps * groups) * a.num_kv_heads > (longest * group <= 32 ? kRaJoinedNarrowSteps : kRaJoinedSteps) * slots) {
     // No tile has more parts than there are workgroups for each head, since a workgroup's share is not below that much of one tile.
     const int64_t most = std::max<int64_t>(std::min<int64_t>(kRaMostParts, (int64_t)(kRaMostSharedBytes / part_bytes)), 2);
-    r.own_parts = (uint32_t)std::max<int64_t>(std::min<int64_t>((own_steps + kRaLeastOwnPart - 1) / kRaLeastOwnPart, most / 4), 1);
+    // of streams whose group is not joined, over its beginning too: 16 groups of some 4 single tokens, a few of one, x 24 heads over 4000 keys 187 us;
+    // without 322
+    r.own_parts = (uint32_t)std::max<int64_t>(std::min<int64_t>((own_steps + prefix_steps + kRaLeastOwnPart - 1) / kRaLeastOwnPart, most / 4), 1);
     r.prefix_parts = (uint32_t)std::min(std::min<int64_t>((prefix_steps + kRaLeastPrefixPart - 1) / kRaLeastPrefixPart, slots / a.num_kv_heads + 1), most - r.own_parts);
     const int64_t items = together * r.prefix_parts + (a.n_queries * group / kRaTileRows + a.streams) * r.own_parts;
     r.groups = (uint32_t)std::min(slots, items * a.num_kv_heads);

@@ -64,6 +64,17 @@ def test_groups_of_which_some_are_joined(gpu):
     check(gpu, b, [1, 40, 41, 45, 45, 60, 78], causal=False)
 
 
+@pytest.mark.parametrize("D,Hk", [(64, 8), (128, 2)])
+def test_long_beginnings_of_groups_that_are_not_joined(gpu, D, Hk):
+    # single streams, of few and of many rows, over beginnings as long as those that others share: in parts, beginning and own keys in one
+    new = [1] * 40 + [1, 3, 200, 64, 1]
+    keys = [n + 50 * (i % 9) for i, n in enumerate(new)]
+    keys[44] = 0
+    b = batch(212, new, keys, [5000, 6001, 4000, 5500, 3500, 4500], Hk, Hk, D, 16, BF16, fill=float("nan"))
+    for causal in (True, False):
+        check(gpu, b, [0, 40, 41, 42, 43, 44, 45], causal)
+
+
 def test_more_groups_than_are_joined_in_a_launch(gpu):
     new = [1] * 600
     keys = [1 + 7 * i % 40 for i in range(600)]
