@@ -1,5 +1,6 @@
 // Attention of a batch of streams of different length (ll_ragged_attention): new tokens over the keys of a paged cache, or
-// queries over encoder states whose number differs from stream to stream.
+// queries over encoder states whose number differs from stream to stream; and over beginnings that groups of streams share
+// (ll_shared_prefix_attention, see "beginnings that groups attend together").
 //
 //   out[t, h] = sum_j w_j v_j / sum_j w_j,   w_j = exp(scale * (q[t, h] . k_j - max)),   j over the keys that row t may see
 //
@@ -31,7 +32,8 @@
 // the first scores, one behind the other, some 5 us beside the other workgroup of the unit): 532 x 40 / 8 heads over 9000 keys 118 us, 0.81
 // PFLOP/s, 3 x 2640 x 24 over 60 to 512 encoder states 43 us, 0.56 PFLOP/s.
 // Registers: with 64 columns three workgroups of a unit leave 168 a lane, of which 4 to 8 more would be needed (20 to 36 bytes of scratch
-// memory); with 128 columns 230 to 246 and none.  41 to 82 scalars are kept in lanes of vector registers.
+// memory); with 128 columns 230 to 246 and none.  41 to 82 scalars are kept in lanes of vector registers.  With shared beginnings 168 and 68 to 76
+// bytes, 250 to 254 and none, 62 to 111 scalars.
 #include "ll_types16.h"
 
 #include <algorithm>
@@ -1253,6 +1255,13 @@ __global__ __launch_bounds__(kRaThreads) void ragged_join_kernel(RaParams p) {
 // three times as long for a narrow tile as four do together, waiting for the page table, then for K, for little else: four tiles run side by
 // side, if one does not take longer than the launch does anyway.
 //
+// What bounds it, next to the floor of reading every key once or of all products at the library's rate: the three launches one behind the other, and
+// items whose beginning is a chain of waits (places, keys, scores), so that the shortest takes 5 us and a workgroup has three to five of them.  64
+// single tokens x 32 / 8 heads of 128 columns over 16384 shared and 30 to 1000 own keys 52 us (7 for the list, 42 for the items, 7 for joining them),
+// floor 28.5 for 140 MB; each stream over all of its keys takes 354.  100 x 4 tokens x 12 heads of 64 over 3001 and 8 to 300 keys 39 (7, 27, 7), floor
+// 8.6; 104.  41 streams of 1 to 200 tokens x 20 / 4 of 128 in four groups, over 300 to 5000 and 10 to 900, 76 (9, 60, 15), floor 16.5; 85.  4 x 2640
+// tokens x 24 over 10560 and 2640 are not joined, since their tiles are full as they are: 1740 to 1760, 0.97 to 0.98 PFLOP/s.
+//
 // us of 64 single tokens x 32 / 8 heads over 16384 shared and 30 to 1000 own keys: items found by every workgroup in turn, beginnings first, in 32
 // parts 62, in 14 parts 63; so on workgroups of their own 50.
 constexpr int kRaPlanThreads = 256;   // a wave to a SIMD: 64 streams 8.6 us, with four waves, most of them idle, 10.9
@@ -1871,7 +1880,9 @@ static SharedPlan plan_shared(const ll_shared_prefix_args& s, int cus) {
   const int64_t prefix_steps = s.groups && a.n_pages ? steps_within(s.max_prefix_len, s.prefix_width) : 0;
   const int64_t groups = std::min(s.groups, a.streams), together = a.n_queries * group / kRaTileRows + groups;  // tiles of whole groups
   const size_t rows = (size_t)a.n_queries * a.num_heads, part_bytes = rows * (a.head_dim + 2) * sizeof(float);
+  // The second line: groups of which, on average, none comes near being joined (4 x 2640 tokens x 24 heads over 10560 + 2640 keys).
   if (a.streams > 1 && s.groups <= kRaJoinedGroups && part_bytes <= 4 * kRaMostSharedBytes &&
+      a.streams * prefix_steps >= kRaJoinedCost / 2 * together &&
       ((tiles - together) * prefix_steps - kRaJoinedGroupSteps * groups) * a.num_kv_heads > (longest * group <= 32 ? kRaJoinedNarrowSteps : kRaJoinedSteps) * slots) {
     // No tile has more parts than there are workgroups for each head, since a workgroup's share is not below that much of one tile.
     const int64_t most = std::max<int64_t>(std::min<int64_t>(kRaMostParts, (int64_t)(kRaMostSharedBytes / part_bytes)), 2);
