@@ -190,6 +190,79 @@ def test_recorded_listing_follows_the_lengths(gpu):
             close(replayed, want, error, f"case {i}")
 
 
+@pytest.mark.parametrize("hints", [(1, 1, 2100), (None, 1, 4500), (10 ** 9, 10 ** 12, 10 ** 12)])
+def test_lengths_that_the_host_takes_to_be_others(gpu, hints):
+    new = [1] * 50 + [70, 3, 40]
+    b = batch(213, new, [n + 31 * i % 1100 for i, n in enumerate(new)], [4300, 4500, 700], 16, 8, 64, 16, F16)
+    check_shared(gpu, b, [0, 30, 52, 53], told=False, max_q_len=hints[0], max_kv_len=hints[1], max_prefix_len=hints[2])
+
+
+def test_lengths_beyond_the_tables(gpu):
+    b = list(batch(214, [1] * 40 + [3] * 20, [64] * 60, [3008], 8, 8, 64, 16, BF16))
+    b[4] = b[4][:, :4].contiguous()
+    assert parts_asked_for(b)
+    want = attend(gpu, b, causal=False, max_q_len=3)
+    b[3], b[5] = b[3] + 5000, b[5] + 1000
+    assert torch.equal(attend(gpu, b, causal=False, max_q_len=3), want)
+
+
+@pytest.mark.parametrize("page", [24, 16])
+def test_strides(gpu, page):
+    new = [1] * 60 + [2, 50]
+    q, cache, *tables, q_starts = b = batch(215, new, [n + 9 * i % 200 for i, n in enumerate(new)], [4000], 8, 4, 128, page, BF16)
+    want = check(gpu, b)
+    T = sum(new)
+    wide = torch.zeros(T, 11, 128, dtype=BF16, device=gpu)
+    wide[:, 2:10] = q.to(gpu)
+    both = torch.stack([cache["k_pages"], cache["v_pages"]], dim=1).transpose(2, 3).contiguous().to(gpu)   # [pages, 2, heads, rows, D]
+    paged = {"k_pages": both[:, 0].transpose(1, 2), "v_pages": both[:, 1].transpose(1, 2)}
+    out = torch.full((8, T, 128), 7.0, dtype=BF16, device=gpu).transpose(0, 1)
+    on = [t.to(gpu) for t in tables]
+    args = (paged, torch.cat([on[0], on[0]], dim=1)[:, :on[0].shape[1]], on[1], torch.cat([on[2], on[2]], dim=1)[:, :on[2].shape[1]], on[3], q_starts.to(gpu))
+    told = dict(max_q_len=max(new), max_kv_len=int(tables[3].max()), max_prefix_len=4000)
+    shared_prefix_attention(wide[:, 2:10], *args, out=out, **told)
+    assert torch.equal(out, want)
+
+
+@pytest.mark.parametrize("D,dtype", [(64, BF16), (128, F16)])
+def test_scales(gpu, D, dtype):
+    for scale in (0.01, 3.0):
+        check(gpu, batch(216, [1] * 70, [30 + i for i in range(70)], [3000], 8, 8, D, 16, dtype), softmax_scale=scale)
+
+
+def test_shared_values_that_are_not_finite(gpu):
+    # a row that sees an infinite or undefined value has it, and no other column or group has
+    new = [1] * 40 + [35] + [1] * 40
+    b = batch(217, new, [n + 5 for n in new], [3000, 2500], 8, 8, 64, 8, BF16)
+    want, error, _ = step_ref.shared_prefix(*b, int32([0, 41, 81]), True, 64 ** -0.5)
+    b[1]["v_pages"][b[2][0, 100], 3, 2, 9] = float("inf")
+    b[1]["v_pages"][b[2][1, 200], 4, 5, 11] = float("nan")
+    assert parts_asked_for(b)
+    got = attend(gpu, b, [0, 41, 81], max_q_len=35, max_kv_len=40, max_prefix_len=3000).cpu()
+    inside = 75
+    assert (got[:inside, 2, 9] == float("inf")).all() and got[inside:, 5, 11].isnan().all()
+    keep = torch.ones_like(want, dtype=torch.bool)
+    keep[:inside, 2, 9] = False
+    keep[inside:, 5, 11] = False
+    close(torch.where(keep, got.double(), 0.0), torch.where(keep, want, 0.0), torch.where(keep, error, 1.0))
+
+
+def test_a_cache_beyond_32_bits_of_offsets(gpu):
+    q, cache, *rest = b = batch(218, [1] * 60 + [40], [40 + i for i in range(61)], [3000], 8, 8, 64, 64, F16)
+    assert parts_asked_for(b)
+    pages = cache["k_pages"].shape[0]
+    apart = (1 << 31) // pages // 64 * 64 + 64 * 1024
+    far = torch.empty(pages, apart, dtype=F16, device=gpu)   # 2^31 elements and more between the first page and the last
+    size = 64 * 8 * 64
+    dev = {}
+    for i, n in enumerate(("k_pages", "v_pages")):
+        dev[n] = far[:, i * size:(i + 1) * size].unflatten(1, (64, 8, 64))
+        dev[n].copy_(cache[n])
+    got = shared_prefix_attention(q.to(gpu), dev, *(t.to(gpu) for t in rest), max_q_len=40, max_kv_len=100, max_prefix_len=3000)
+    want, error, _ = step_ref.shared_prefix(q, cache, *rest, None, True, 64 ** -0.5)
+    close(got, want, error)
+
+
 def test_layout_with_a_cursor_beyond_the_list_or_below_it(gpu):
     for cursor, pages in ((7, [-1, -1]), (3, [-1, -1]), (2, [12, -1]), (-5, [10, 11])):
         table, at = torch.full((2, 2), -1, dtype=torch.int32, device=gpu), int32([cursor], gpu)
