@@ -1871,18 +1871,19 @@ static SharedPlan plan_shared(const ll_shared_prefix_args& s, int cus) {
   if (a.n_queries == 0 || a.streams == 0) return r;
   const int64_t group = a.num_heads / a.num_kv_heads, slots = (a.head_dim == 64 ? 3 : 2) * cus;
   const int64_t longest = a.max_q_len > 0 && a.max_q_len < a.n_queries ? a.max_q_len : a.n_queries;
-  const int64_t tiles = std::min(a.n_queries * group / kRaTileRows + a.streams, a.streams * ((longest * group + kRaTileRows - 1) / kRaTileRows));
+  const int64_t streams = std::min(a.streams, a.n_queries);  // with rows
+  const int64_t tiles = std::min(a.n_queries * group / kRaTileRows + streams, streams * ((longest * group + kRaTileRows - 1) / kRaTileRows));
   const auto steps_within = [&](int64_t told, int64_t width) {
     const int64_t reach = width * a.page_size, keys = told > 0 && told < reach ? told : reach;
     return (keys + kRaKeys - 1) / kRaKeys;
   };
   const int64_t own_steps = steps_within(a.max_kv_len, a.n_pages ? a.table_width : 0);
   const int64_t prefix_steps = s.groups && a.n_pages ? steps_within(s.max_prefix_len, s.prefix_width) : 0;
-  const int64_t groups = std::min(s.groups, a.streams), together = a.n_queries * group / kRaTileRows + groups;  // tiles of whole groups
+  const int64_t groups = std::min(s.groups, streams), together = a.n_queries * group / kRaTileRows + groups;  // tiles of whole groups
   const size_t rows = (size_t)a.n_queries * a.num_heads, part_bytes = rows * (a.head_dim + 2) * sizeof(float);
   // The second line: groups of which, on average, none comes near being joined (4 x 2640 tokens x 24 heads over 10560 + 2640 keys).
-  if (a.streams > 1 && s.groups <= kRaJoinedGroups && part_bytes <= 4 * kRaMostSharedBytes &&
-      a.streams * prefix_steps >= kRaJoinedCost / 2 * together &&
+  if (streams > 1 && s.groups <= kRaJoinedGroups && part_bytes <= 4 * kRaMostSharedBytes &&
+      streams * prefix_steps >= kRaJoinedCost / 2 * together &&
       ((tiles - together) * prefix_steps - kRaJoinedGroupSteps * groups) * a.num_kv_heads > (longest * group <= 32 ? kRaJoinedNarrowSteps : kRaJoinedSteps) * slots) {
     // No tile has more parts than there are workgroups for each head, since a workgroup's share is not below that much of one tile.
     const int64_t most = std::max<int64_t>(std::min<int64_t>(kRaMostParts, (int64_t)(kRaMostSharedBytes / part_bytes)), 2);
@@ -1890,7 +1891,7 @@ static SharedPlan plan_shared(const ll_shared_prefix_args& s, int cus) {
     // without 322
     r.own_parts = (uint32_t)std::max<int64_t>(std::min<int64_t>((own_steps + prefix_steps + kRaLeastOwnPart - 1) / kRaLeastOwnPart, most / 4), 1);
     r.prefix_parts = (uint32_t)std::min(std::min<int64_t>((prefix_steps + kRaLeastPrefixPart - 1) / kRaLeastPrefixPart, slots / a.num_kv_heads + 1), most - r.own_parts);
-    const int64_t items = together * r.prefix_parts + (a.n_queries * group / kRaTileRows + a.streams) * r.own_parts;
+    const int64_t items = together * r.prefix_parts + (a.n_queries * group / kRaTileRows + streams) * r.own_parts;
     r.groups = (uint32_t)std::min(slots, items * a.num_kv_heads);
     r.most_listed = (uint32_t)std::min<int64_t>(items, 0xffffffffll / a.num_kv_heads);
     const auto behind = [](size_t bytes) { return (bytes + 63) / 64 * 64; };

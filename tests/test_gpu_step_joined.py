@@ -46,6 +46,12 @@ def test_more_streams_than_the_listing_has_threads(gpu, D, dtype, causal):
     check(gpu, b, None, causal)
 
 
+def test_many_streams_without_new_tokens(gpu):
+    new = [int(i % 37 == 5) + 2 * int(i % 211 == 9) for i in range(3000)]
+    b = batch(219, new, [(n + 17 * i % 90) * (n > 0) for i, n in enumerate(new)], [2000, 1500], 8, 8, 128, 16, BF16)
+    check(gpu, b, [0, 1800, 2990])
+
+
 @pytest.mark.parametrize("Hq,Hk,D,dtype", [(6, 3, 128, BF16), (20, 4, 64, F16), (12, 12, 64, BF16), (24, 24, 128, BF16)])
 @pytest.mark.parametrize("page", [16, 24, 880])
 def test_single_tokens_drafts_and_prompts_together(gpu, Hq, Hk, D, dtype, page):

@@ -187,3 +187,7 @@ def test_memory_that_calls_ask_for():
     one = shared_args(own=dict(**chunks, table_width=15, max_kv_len=13200, causal=0)).own
     assert lib.ll_ragged_attention_workspace(ctypes.byref(one), 256, ctypes.byref(n)) == 0
     assert shared_bytes(shared_args(own=dict(**chunks, table_width=3, max_kv_len=2640), prefix_width=12, max_prefix_len=10560)) == n.value
+    # streams without new tokens take no more than where they are listed
+    few, many = (shared_bytes(shared_args(own=dict(n_queries=64, streams=n, num_heads=32, num_kv_heads=8, max_q_len=1, max_kv_len=64), prefix_width=1024))
+                 for n in (64, 1 << 20))
+    assert few < many <= few + 12 * (1 << 20)
