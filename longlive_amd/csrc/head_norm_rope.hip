@@ -81,7 +81,7 @@ constexpr int64_t kManyWaves = 8192;
 // left is exact to 2^-26 of a turn in 32 bits, and the hardware's sine and cosine of it
 // are off by no more than 2^-22, a thousandth of the rounding to f16 that follows.
 // Formed once for the wave's heads, it hides behind their loads: 40000 x (32 + 8 + 8) heads of 128 columns, 983 MB, 176 us, 5.6 TB/s; 16381 x (40 + 8
-// + 8) of 64 with 32 rotated, 235 MB, 36 and 49 on two cards; 2640 x (24 + 24) by video frames, 65 MB, 14.1, without the table's 90 MB for 176 000
+// + 8) of 64 with 32 rotated, 235 MB, 49, and 36 out of the last-level cache; 2640 x (24 + 24) by video frames, 65 MB, 14.1, without the table's 90 MB for 176 000
 // positions; 24 x (16 + 4 + 4) 3.4 on the device, 5.6 from call to call.
 __device__ __forceinline__ void form_angles(const FormedAngles& a, int64_t pos, int l, float (&cs)[4], float (&sn)[4]) {
   double f[4];
