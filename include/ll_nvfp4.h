@@ -631,8 +631,8 @@ int ll_rotate_by_position(int dtype, int64_t tokens, int head_dim, const ll_head
  *     Rows behind the last stream's get 0 and -1.
  *   groups: group g is the streams group_starts[g] .. group_starts[g + 1] - 1 (one group may go without, all streams then), and shares
  *     prefix_lens[g] keys (0 below 0) that are not in its streams' tables; starts do not decrease.  Streams outside every group share none.
- * kv_lens_out may be kv_lens; apart from that outputs must not overlap inputs or each other.  workspace: ll_step_layout_workspace bytes, 4-byte
- * aligned, used by this call alone while it runs (NULL where that is 0).
+ * kv_lens_out may be kv_lens.  Apart from that, what is written (page_table, *cursor and workspace among it) overlaps neither inputs nor one another, or the
+ * call is refused.  workspace: ll_step_layout_workspace bytes, 4-byte aligned, used by this call alone while it runs (NULL where that is 0).
  */
 typedef struct ll_step_layout_args {
   int64_t streams;            /* below 2^31, like all sizes here */

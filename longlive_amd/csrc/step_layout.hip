@@ -18,6 +18,7 @@
 #include "ll_common.h"
 
 #include <algorithm>
+#include <utility>
 
 namespace ll {
 
@@ -171,6 +172,49 @@ static bool layout_in_parts(const ll_step_layout_args& a) { return a.tokens > kL
 // Whether several workgroups would read what one of them replaces.
 static bool layout_keeps(const ll_step_layout_args& a) { return layout_in_parts(a) && a.streams > 0 && (a.kv_lens_out == a.kv_lens || a.cursor); }
 
+// Whether two ranges of bytes share one.
+static bool meet(const void* a, int64_t a_bytes, const void* b, int64_t b_bytes) {
+  const uintptr_t at = (uintptr_t)a, bt = (uintptr_t)b;
+  return a_bytes > 0 && b_bytes > 0 && (at < bt ? bt - at < (uint64_t)a_bytes : at - bt < (uint64_t)b_bytes);
+}
+// Whether a range of bytes shares one with the table's rows; it may lie between them.
+static bool meets_table(const ll_step_layout_args& a, const void* b, int64_t bytes) {
+  const int64_t width = a.table_width * 4, stride = (a.table_stride < 0 ? -a.table_stride : a.table_stride) * 4;
+  if (bytes <= 0 || width == 0 || a.streams == 0) return false;
+  const int32_t* const low = a.table_stride < 0 ? a.page_table + (a.streams - 1) * a.table_stride : a.page_table;
+  const int64_t off = (int64_t)((uintptr_t)b - (uintptr_t)low);
+  if (off < width) return off + bytes > 0;
+  if (a.streams == 1) return false;
+  const int64_t row = off / stride, in_row = off - row * stride;
+  return row < a.streams && (in_row < width || (row + 1 < a.streams && in_row + bytes > stride));
+}
+
+// What is written lies in places of its own: with several workgroups the first replaces what later ones would still read.
+static int check_apart(const ll_step_layout_args& a) {
+  const auto list = [](const void* at, int64_t bytes) { return std::pair<const void*, int64_t>(at, at ? bytes : 0); };
+  const auto inputs = {list(a.new_lens, 4 * a.streams), list(a.kv_lens, 4 * a.streams), list(a.free_pages, 4 * a.n_free),
+                       list(a.group_starts, a.groups ? 4 * (a.groups + 1) : 0), list(a.prefix_lens, 4 * a.groups)};
+  const std::pair<const void*, int64_t> outputs[] = {list(a.kv_lens_out, 4 * a.streams),   list(a.cursor, 4),          list(a.q_starts, 4 * (a.streams + 1)),
+                                                     list(a.positions, 8 * a.tokens),      list(a.slots, 8 * a.tokens), list(a.pages_wanted, 4),
+                                                     list(a.workspace, layout_keeps(a) ? 4 * (a.streams + 1) : 0)};
+  LL_REQUIRE(a.streams <= 1 || a.table_width == 0 || a.table_stride >= a.table_width || -a.table_stride >= a.table_width,
+             "ll_step_layout: rows of the page table overlap, %lld apart for %lld entries", (long long)a.table_stride, (long long)a.table_width);
+  bool apart = true;
+  for (const auto& in : inputs) {
+    apart = apart && !meets_table(a, in.first, in.second);
+    for (const auto& out : outputs) {
+      const bool in_place = out.first == a.kv_lens_out && in.first == a.kv_lens && out.first == in.first;
+      apart = apart && (in_place || !meet(in.first, in.second, out.first, out.second));
+    }
+  }
+  for (const auto& out : outputs) {
+    apart = apart && !meets_table(a, out.first, out.second);
+    for (const auto* other = outputs; other < &out; ++other) apart = apart && !meet(other->first, other->second, out.first, out.second);
+  }
+  LL_REQUIRE(apart, "ll_step_layout: outputs (page table, cursor, new lengths, results) overlap inputs or one another; only the new lengths may replace the held ones");
+  return LL_OK;
+}
+
 static int check_layout(const ll_step_layout_args* a) {
   LL_REQUIRE(a, "ll_step_layout: no arguments");
   LL_REQUIRE(a->streams >= 0 && a->streams < 0x7fffffffll, "ll_step_layout: %lld streams", (long long)a->streams);
@@ -202,6 +246,7 @@ extern "C" int ll_step_layout(const ll_step_layout_args* a, void* stream) {
   LL_REQUIRE(a->n_free == 0 || a->free_pages, "ll_step_layout: null list of free pages");
   LL_REQUIRE(a->groups == 0 || a->prefix_lens, "ll_step_layout: groups without lengths of what they share");
   LL_REQUIRE(a->groups <= 1 || a->group_starts, "ll_step_layout: %lld groups without their beginnings", (long long)a->groups);
+  if (int rc = check_apart(*a)) return rc;
   const hipStream_t s = static_cast<hipStream_t>(stream);
   LayoutParams p{};
   p.new_lens = a->new_lens;

@@ -83,7 +83,10 @@ def lay_out_step(new_lens: torch.Tensor, kv_lens: torch.Tensor, page_table: torc
     ``positions`` count from the stream's first key, and with ``prefix_lens`` (int32 [groups]) from the beginning that its group shares:
     group g is streams ``group_starts[g] .. group_starts[g + 1] - 1`` (int32 [groups + 1]; all streams are one group without).  ``slots`` is -1 for
     tokens in holes and behind the table's width.  Tokens for which ``num_tokens`` has no row left are not laid out: their streams' lengths do not
-    count them.  Rows behind the last stream's have position 0 and slot -1."""
+    count them.  Rows behind the last stream's have position 0 and slot -1.
+
+    ``page_table``, ``cursor`` and ``kv_lens_out`` are written and share no memory with one another or with what is read, but for ``kv_lens_out``
+    in place of ``kv_lens``."""
     return StepLayout(*_native.step_layout(new_lens, kv_lens, page_table, free_pages, page_size, num_tokens, prefix_lens, group_starts, cursor, kv_lens_out))
 
 

@@ -103,6 +103,27 @@ def test_layout_without_streams_or_tokens(gpu):
     assert got.q_starts.tolist() == [0, 0] and got.kv_lens.tolist() == [3]
 
 
+@pytest.mark.parametrize("native", [True, False])
+@pytest.mark.parametrize("tokens", [4, 3000])
+def test_layouts_that_would_overwrite_what_they_read_are_refused(gpu, tokens, native, monkeypatch):
+    from longlive_amd import _native
+    if not native:   # by way of ctypes
+        monkeypatch.setattr(_native, "host", lambda: type("None", (), {"step_layout": staticmethod(lambda *a: None)}))
+    memory = torch.arange(100, dtype=torch.int32, device=gpu)
+    new, held, table, free, cursor = memory[:4], memory[4:8], memory[10:34].view(4, 6)[:, :4], memory[40:60], memory[60:61]
+    ok = dict(new_lens=new, kv_lens=held, page_table=table, free_pages=free, page_size=16, num_tokens=tokens, cursor=cursor)
+    for bad in (dict(kv_lens_out=new), dict(kv_lens_out=memory[5:9]), dict(kv_lens_out=memory[1:5]), dict(kv_lens_out=memory[57:61]), dict(kv_lens_out=memory[8:12]), dict(cursor=memory[2:3]),
+                dict(cursor=memory[6:7]), dict(cursor=memory[45:46]), dict(cursor=memory[16:17]), dict(page_table=memory[6:30].view(4, 6)[:, :4]), dict(free_pages=memory[20:40])):
+        with pytest.raises(ValueError, match="overlap"):
+            lay_out_step(**{**ok, **bad})
+    torch.cuda.synchronize()
+    assert memory.tolist() == list(range(100))
+    # side by side, the cursor between two rows of the table
+    got = lay_out_step(**{**ok, "cursor": memory[14:15], "kv_lens_out": held})
+    n = [0, 1, 2, 3] if tokens == 3000 else [0, 1, 2, 1]
+    assert got.kv_lens is held and memory[:8].tolist() == [0, 1, 2, 3] + [m + i for m, i in zip([4, 5, 6, 7], n)] and memory[40:60].tolist() == list(range(40, 60))
+
+
 @pytest.mark.parametrize("tokens", [7, 3000])
 def test_steps_that_a_graph_replays_go_on_from_one_another(gpu, tokens):
     page, new, lens = 4, [1, 0, 3, 1, 1], [0, 9, 4, 3, 2]

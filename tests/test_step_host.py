@@ -173,6 +173,46 @@ def test_library_refuses_layouts(bad):
     assert _native.load().ll_step_layout_workspace(ctypes.byref(a), ctypes.byref(n)) == -1
 
 
+# addresses that no call reaches: without a device a layout that is not refused ends at its launch, which fails
+def layout_args(**kw):
+    return _native.StepLayoutStruct(**{**dict(streams=4, new_lens=0x1000, kv_lens=0x2000, page_table=0x3000, table_stride=10, table_width=8, page_size=16, free_pages=0x4000,
+                                              n_free=5, cursor=0x4100, groups=2, group_starts=0x4200, prefix_lens=0x4300, tokens=6, q_starts=0x5000, kv_lens_out=0x6000,
+                                              positions=0x7000, slots=0x8000, pages_wanted=0x9000), **kw})
+
+
+TABLE_ENDS = 0x3000 + 4 * (3 * 10 + 8)
+
+
+@pytest.mark.parametrize("tokens", [6, 5000])
+@pytest.mark.parametrize("bad", [
+    dict(kv_lens_out=0x1000), dict(kv_lens_out=0x1000 - 12), dict(kv_lens_out=0x2004), dict(kv_lens_out=0x1FFC), dict(kv_lens_out=0x4010), dict(kv_lens_out=0x4208),
+    dict(kv_lens_out=0x4304), dict(cursor=0x1000), dict(cursor=0x200C), dict(cursor=0x4010), dict(cursor=0x4208), dict(cursor=0x4304), dict(cursor=0x6004),
+    dict(page_table=0x1000), dict(kv_lens=0x3000), dict(kv_lens=0x3000 - 4), dict(new_lens=0x3004), dict(new_lens=0x3000 + 4 * 8), dict(free_pages=0x3000 + 4 * 17),
+    dict(cursor=0x3000 + 4 * 10), dict(cursor=TABLE_ENDS - 4), dict(kv_lens_out=0x3000 + 4 * 9), dict(prefix_lens=TABLE_ENDS - 4), dict(group_starts=0x3000 - 8),
+    dict(q_starts=0x1004), dict(q_starts=0x6000 - 16), dict(positions=0x2000), dict(slots=0x7000 + 8 * 5), dict(pages_wanted=0x4100), dict(pages_wanted=0x4300),
+    dict(table_stride=7), dict(table_stride=0), dict(table_stride=-7), dict(table_stride=-10, cursor=0x3000 - 4 * 30)])
+def test_library_refuses_layouts_that_overlap(bad, tokens):
+    lib = _native.load()
+    kept = dict(workspace=0x100000, workspace_bytes=1 << 12)
+    if tokens > 6:
+        kept.update(positions=0x200000, slots=0x300000)   # long ones
+    moved = {"positions": 0x1FF8, "slots": 0x200000 + 8 * (tokens - 1)} if tokens > 6 else {}
+    bad = {n: moved.get(n, at) for n, at in bad.items()}
+    assert lib.ll_step_layout(ctypes.byref(layout_args(**{**dict(tokens=tokens), **kept, **bad})), None) == -1
+    assert b"overlap" in lib.ll_last_error()
+
+
+@pytest.mark.skipif(torch.cuda.is_available(), reason="the addresses are nobody's: only where no launch can come of them")
+@pytest.mark.parametrize("good", [
+    dict(), dict(kv_lens_out=0x2000), dict(kv_lens_out=0x1010), dict(kv_lens_out=0x2000 - 16), dict(cursor=0x2010), dict(cursor=0x2000 - 4), dict(cursor=TABLE_ENDS),
+    dict(cursor=0x3000 + 4 * 8), dict(cursor=0x3000 + 4 * 29), dict(cursor=0x3000 - 4), dict(prefix_lens=0x3000 + 4 * 18), dict(group_starts=TABLE_ENDS),
+    dict(new_lens=0x2000), dict(prefix_lens=0x1000), dict(cursor=None), dict(groups=0, group_starts=0x2000, prefix_lens=None, kv_lens_out=0x2000),
+    dict(table_width=0, cursor=0x3000), dict(streams=1, table_stride=0), dict(table_stride=-10, cursor=0x3000 + 4 * 8), dict(table_stride=-10, cursor=0x3000 - 4 * 31)])
+def test_layouts_whose_parts_lie_side_by_side_pass_the_checks(good):
+    args = layout_args(**{**dict(workspace=0x100000, workspace_bytes=1 << 12), **good})
+    assert _native.load().ll_step_layout(ctypes.byref(args), None) == -2   # as far as the launch
+
+
 def test_memory_that_calls_ask_for():
     lib, n = _native.load(), ctypes.c_size_t()
     for tokens, out, cursor, want in ((100, 8, 0, 0), (1 << 20, 8, 0, 0), (1 << 20, 16, 0, 44), (1 << 20, 8, 4, 44), (100, 16, 4, 0)):   # lengths at 16
