@@ -635,7 +635,7 @@ int ll_rotate_by_position(int dtype, int64_t tokens, int head_dim, const ll_head
  * call is refused.  workspace: ll_step_layout_workspace bytes, 4-byte aligned, used by this call alone while it runs (NULL where that is 0).
  */
 typedef struct ll_step_layout_args {
-  int64_t streams;            /* below 2^31, like all sizes here */
+  int64_t streams;            /* below 2^28, like groups; the other sizes below 2^31 */
   const int32_t *new_lens, *kv_lens; /* [streams] */
   int32_t* page_table;        /* [streams, table_width], rows table_stride apart */
   int64_t table_stride, table_width;

@@ -217,12 +217,13 @@ static int check_apart(const ll_step_layout_args& a) {
 
 static int check_layout(const ll_step_layout_args* a) {
   LL_REQUIRE(a, "ll_step_layout: no arguments");
-  LL_REQUIRE(a->streams >= 0 && a->streams < 0x7fffffffll, "ll_step_layout: %lld streams", (long long)a->streams);
+  // as many as attention takes: the kernel counts streams on by a workgroup's threads, and adds two groups' numbers, in 31 bits
+  LL_REQUIRE(a->streams >= 0 && a->streams <= 0xfffffff, "ll_step_layout: %lld streams", (long long)a->streams);
   LL_REQUIRE(a->tokens >= 0 && a->tokens <= 0x7fffffffll, "ll_step_layout: %lld tokens", (long long)a->tokens);
   LL_REQUIRE(a->page_size > 0, "ll_step_layout: pages of %d rows", a->page_size);
   LL_REQUIRE(a->table_width >= 0 && a->table_width <= 0x7fffffffll, "ll_step_layout: a table of %lld pages a stream", (long long)a->table_width);
   LL_REQUIRE(a->n_free >= 0 && a->n_free <= 0x7fffffffll, "ll_step_layout: %lld free pages", (long long)a->n_free);
-  LL_REQUIRE(a->groups >= 0 && a->groups < 0x7fffffffll, "ll_step_layout: %lld groups", (long long)a->groups);
+  LL_REQUIRE(a->groups >= 0 && a->groups <= 0xfffffff, "ll_step_layout: %lld groups", (long long)a->groups);
   return LL_OK;
 }
 

@@ -173,6 +173,14 @@ def test_library_refuses_layouts(bad):
     assert _native.load().ll_step_layout_workspace(ctypes.byref(a), ctypes.byref(n)) == -1
 
 
+def test_library_refuses_layouts_whose_numbers_pass_31_bits_in_the_kernel():
+    n = ctypes.c_size_t()
+    for more, want in ((dict(streams=(1 << 31) - 2), -1), (dict(streams=1 << 28), -1), (dict(groups=(1 << 31) - 2), -1), (dict(groups=1 << 28), -1),
+                       (dict(streams=(1 << 28) - 1, groups=(1 << 28) - 1), 0)):
+        a = _native.StepLayoutStruct(**{**dict(streams=2, page_size=16, table_width=3, tokens=4), **more})
+        assert _native.load().ll_step_layout_workspace(ctypes.byref(a), ctypes.byref(n)) == want, more
+
+
 # addresses that no call reaches: without a device a layout that is not refused ends at its launch, which fails
 def layout_args(**kw):
     return _native.StepLayoutStruct(**{**dict(streams=4, new_lens=0x1000, kv_lens=0x2000, page_table=0x3000, table_stride=10, table_width=8, page_size=16, free_pages=0x4000,
