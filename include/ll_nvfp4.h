@@ -609,7 +609,7 @@ int ll_head_norm_rope(int dtype, int64_t tokens, int head_dim, const ll_head_row
 typedef struct ll_position_angles {
   const double* frequencies; /* f64 [rotary_dim / 2], radians per position, 16-byte aligned */
   int rotary_dim;            /* as in ll_head_norm_rope */
-  float amplitude;
+  float amplitude;           /* finite */
   int64_t grid_rows, grid_columns; /* 0 and 0: positions on a line; else their product is below 2^31 */
   int frame_pairs, row_pairs;
 } ll_position_angles;

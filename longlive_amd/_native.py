@@ -1208,7 +1208,7 @@ def rotate_by_position(q, k, v, q_weight, k_weight, eps, frequencies, amplitude,
                 grid[0] * grid[1] >= 1 << 31 or sum(sections) != frequencies.numel():
             raise ValueError(f"{what}: a grid {tuple(grid)} of rows and columns, pairs {tuple(sections)} of frames, rows and columns for {frequencies.numel()} frequencies")
         rows, columns, frame_pairs, row_pairs = (int(n) for n in (*grid, *sections[:2]))
-    if not abs(float(amplitude)) < float("inf"):
+    if not abs(c_float(float(amplitude)).value) < float("inf"):   # in the kernel's 32 bits
         raise ValueError(f"{what}: amplitude {amplitude}")
     if q.is_cuda:
         pages = (cache["k_pages"], cache["v_pages"]) if paged else (None, None)

@@ -15,6 +15,8 @@
 #include "head_norm_split.h"
 #include "ll_types16.h"
 
+#include <cmath>
+
 namespace ll {
 
 struct HeadRows {
@@ -343,6 +345,7 @@ extern "C" int ll_rotate_by_position(int dtype, int64_t tokens, int head_dim, co
   if (int rc = head_norm_params("ll_rotate_by_position", dtype, tokens, head_dim, q, k, v, eps, angles->rotary_dim, positions, interleaved, slots, n_slots, p))
     return rc;
   LL_REQUIRE(p.R == 0 || (angles->frequencies && (uintptr_t)angles->frequencies % 16 == 0), "ll_rotate_by_position: frequencies must be 16-byte aligned");
+  LL_REQUIRE(std::isfinite(angles->amplitude), "ll_rotate_by_position: amplitude %g", (double)angles->amplitude);
   const int64_t rows = angles->grid_rows, columns = angles->grid_columns;
   LL_REQUIRE(rows >= 0 && columns >= 0 && (rows > 0) == (columns > 0) && rows <= 0x7fffffffll && columns <= 0x7fffffffll && rows * columns <= 0x7fffffffll,
              "ll_rotate_by_position: a grid of %lld x %lld", (long long)rows, (long long)columns);

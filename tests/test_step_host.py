@@ -110,6 +110,21 @@ def test_refusals_of_rotation(no_gpu_needed):
             rotate_by_position_paged(**{**ok, **bad})
 
 
+def test_amplitudes_beyond_32_bits_are_refused(no_gpu_needed):
+    # infinite in the kernel, they would make zeros undefined
+    x, f = torch.zeros(3, 2, 64, dtype=BF16), rotary_frequencies(64)
+    for amplitude in (1e39, -1e39, 3.5e38):
+        with pytest.raises(ValueError, match="amplitude"):
+            rotate_by_position(x, x, None, f, amplitude=amplitude)
+
+
+def test_library_refuses_amplitudes_that_are_not_finite():
+    rows = _native.HeadRowsStruct(num_heads=0)
+    for amplitude, want in ((1e39, -1), (float("nan"), -1), (3.4e38, 0)):
+        angles = _native.PositionAnglesStruct(amplitude=amplitude)
+        assert _native.load().ll_rotate_by_position(0, 1, 64, ctypes.byref(rows), ctypes.byref(rows), None, 0.0, ctypes.byref(angles), None, 1, None, 0, None) == want
+
+
 def test_refusals_of_shared_prefix_attention(no_gpu_needed):
     q = torch.zeros(3, 4, 64, dtype=BF16)
     cache = initialize_paged_kv_cache(1, 4, 16, 2, 64, "cpu")[0]
