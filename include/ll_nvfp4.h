@@ -603,8 +603,8 @@ int ll_head_norm_rope(int dtype, int64_t tokens, int head_dim, const ll_head_row
  * angle = x * frequencies[j] radians, formed in 64 bits, and cosine and sine are multiplied by amplitude.  x is the row's position p =
  * positions[t] (t without positions, negative ones turn the other way), or with a grid of grid_rows x grid_columns tokens to a video frame
  * the frame p / (rows * columns), rounded down, for the first frame_pairs pairs, the row in it for row_pairs more and the column for the
- * rest.  Every row is rotated.  With frequencies up to 1, positions below 2^31 in
- * magnitude lose 2^-20 radians at most; 2^53 is the end.
+ * rest.  Every row is rotated.  Angles are within 3 * 2^-53 of their size: with frequencies up to 1, positions below 2^31 in magnitude lose
+ * 2^-20 radians at most; beyond 2^53 nothing of an angle is left.
  */
 typedef struct ll_position_angles {
   const double* frequencies; /* f64 [rotary_dim / 2], radians per position, 16-byte aligned */
@@ -712,8 +712,11 @@ int ll_ragged_attention(const ll_ragged_attention_args* args, void* stream);
  * without, all streams then; streams outside every group share nothing), and its first prefix_lens[g] keys lie in the pages of row g of
  * prefix_table.  Every row of a group's streams sees them all; behind them come the stream's own keys, row b of page_table and kv_lens[b] as in
  * ll_ragged_attention, positions counted from the first of them, with the causal order if `own.causal`.  Holes, rows that see no key, what is not
- * finite, types, workspace and aliasing as there.  own.page_table is needed (or table_width 0: no own keys); own.window and own.sink_keys are 0;
- * tables reach at most 2^30 keys.  own.max_kv_len is the longest stream's own keys, max_prefix_len the longest beginning.
+ * finite, types, rounding of the probabilities, workspace and aliasing as there.  own.page_table is needed (or table_width 0: no own keys); own.window
+ * and own.sink_keys are 0 (a window goes with one table whose rows begin with the shared pages, by ll_ragged_attention); tables reach at most
+ * 2^30 keys.  own.max_kv_len is the longest stream's own keys, max_prefix_len the longest beginning.  More than 256 groups go over their
+ * beginnings stream by stream, and so do batches of which one part's results, num_heads * (head_dim + 2) floats a token, take more than 1 GiB.  The
+ * workspace holds 64 parts at most, as many as 256 MiB have room for or two: up to 2 GiB, and the list of items.
  */
 typedef struct ll_shared_prefix_args {
   ll_ragged_attention_args own;

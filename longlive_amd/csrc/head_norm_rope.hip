@@ -74,8 +74,11 @@ __device__ __forceinline__ void unpack4(uint2 w, float* f) {
 
 // Two heads a lane once the device has waves enough: us with one / two, 1000 tokens x (32 + 8 + 8) heads 8.6 / 9.0, 2640 x (24 + 24) 14.9 / 14.1,
 // 16000 x (32 + 8 + 8) 92.9 / 72.4, 16381 x (40 + 8 + 8) of 64 columns 57.0 / 46.2 (four: 74.2 and 44.3).
-// With angles formed: 1000 x (32 + 8 + 8) 6.8 / 6.1, 2640 x (24 + 24) 13.2 / 13.3 (of video frames 13.1 / 14.1), 10560 x (24 + 24) 49.8 / 45.9, 10560 x
-// (32 + 8) 33.1 / 34.3, 40000 x (32 + 8 + 8) 184 / 176.
+// With angles formed it depends on where the rows come from.  Out of memory: 2000 x (32 + 8 + 8) 14.5 / 14.1, 2640 x (24 + 24) 16.2 / 15.1 (of video frames
+// 16.2 / 16.1), 10560 x (24 + 24) 50.1 / 46.2 (50.9 / 47.1), 10560 x (32 + 8) 41.3 / 39.7, 16381 x (40 + 8 + 8) of 64 columns 51.0 / 50.7, 40000 x (32 + 8 + 8)
+// 190 / 182.  Where one call repeats another and finds its rows in the last-level cache, one head may be a little faster: 2640 x (24 + 24) 13.0 / 13.5 (13.5 /
+// 14.3), 10560 x (32 + 8) 33.3 / 34.4, 16381 x (40 + 8 + 8) 35.8 / 37.8, but not 2000 x (32 + 8 + 8) 9.9 / 8.8 nor 10560 x (24 + 24) 42.9 / 41.8.  The rule goes
+// by the former.
 constexpr int64_t kManyWaves = 8192;
 
 // Cosines and sines of pairs 4 l .. 4 l + 3 at a position, which is the wave's.  A position times a frequency takes 64 bits: at position

@@ -1256,11 +1256,12 @@ __global__ __launch_bounds__(kRaThreads) void ragged_join_kernel(RaParams p) {
 // side, if one does not take longer than the launch does anyway.
 //
 // What bounds it, next to the floor of reading every key once or of all products at the library's rate: the three launches one behind the other, and
-// items whose beginning is a chain of waits (places, keys, scores), so that the shortest takes 5 us and a workgroup has three to five of them.  64
-// single tokens x 32 / 8 heads of 128 columns over 16384 shared and 30 to 1000 own keys 60 us, 52 out of the last-level cache (7 for the list, 42 for the items, 7 for joining),
-// floor 28.5 for 140 MB; each stream over all of its keys takes 354.  100 x 4 tokens x 12 heads of 64 over 3001 and 8 to 300 keys 39 (7, 27, 7), floor
-// 8.6; 104.  41 streams of 1 to 200 tokens x 20 / 4 of 128 in four groups, over 300 to 5000 and 10 to 900, 76 (9, 60, 15), floor 16.5; 85.  4 x 2640
-// tokens x 24 over 10560 and 2640 are not joined, since their tiles are full as they are: 1740 to 1760, 0.97 to 0.98 PFLOP/s.
+// items whose beginning is a chain of waits (places, keys, scores), so that the shortest takes 5 us and a workgroup has three to five of them.  Calls
+// one behind the other; in brackets list, items and joining by a kernel trace, under which all three take up to an eighth longer: 64 single tokens x 32 / 8
+// heads of 128 columns over 16384 shared and 30 to 1000 own keys 60 us, 52 with keys from the last-level cache (8, 43, 8), where 140 MB copied take 28.5;
+// each stream over all of its keys takes 354.  100 x 4 tokens x 12 heads of 64 over 3001 and 8 to 300 keys 39 (7, 27, 7), copied 8.6; 104.  41 streams
+// of 1 to 200 tokens x 20 / 4 of 128 in four groups, over 300 to 5000 and 10 to 900, 76 (9, 61, 15), the library's products 16.5; 85.  4 x 2640
+// tokens x 24 over 10560 and 2640 are not joined, since their tiles are full as they are: 1740 to 1790, 0.96 to 0.98 PFLOP/s.
 //
 // us of 64 single tokens x 32 / 8 heads over 16384 shared and 30 to 1000 own keys: items found by every workgroup in turn, beginnings first, in 32
 // parts 62, in 14 parts 63; so on workgroups of their own 50.

@@ -12,9 +12,9 @@
 // belongs to streams, and nothing passes between workgroups.  Lengths that the launch replaces (kv_lens_out is kv_lens, or a cursor)
 // are then copied aside first, by a launch of its own, since workgroups that begin late still read them.
 //
-// What bounds it: the launch and one chain of dependent reads (lengths, sums, table, free pages), next to which the bytes are nothing.  24 streams
-// of one token take 2.7 us on the device, 5.8 from call to call, where a fill of one number takes 3.5; 1000 streams of 1 to 4 tokens 6.2 on the device,
-// 100 prompts of 50 to 4096 tokens 6.1.
+// What bounds it: the launch and one chain of dependent reads (lengths, sums, table, free pages), next to which the bytes are nothing.  From call to call,
+// and on the device by a kernel trace, which lengthens what is as short: 24 streams of one token 5.6 to 6.4 us and 2.7 to 3.0, where a fill of one number takes
+// 3.5 from call to call; 1000 streams of 1 to 4 tokens 6.3 to 6.6 and 6.0 to 6.3; 100 prompts of 50 to 4096 tokens 5.9 to 6.3 and 5.2 to 5.9.
 #include "ll_common.h"
 
 #include <algorithm>

@@ -140,7 +140,7 @@ def shared_prefix_attention(q: torch.Tensor, cache: dict, prefix_table: torch.Te
     each stream's own: token i of n sees own key j where ``j <= kv_lens[b] - n + i`` (``causal``; else every one).  A common beginning of whole
     pages at the front of every row of one table is handed on as views: ``table[:1, :w]`` and ``table[:, w:]``, with lengths that count from there.
 
-    ``max_prefix_len``: the longest beginning, like ``max_q_len`` and ``max_kv_len`` (the longest stream's own keys).  The rest as in
-    :func:`paged_attention`."""
+    ``max_prefix_len``: the longest beginning, like ``max_q_len`` and ``max_kv_len`` (the longest stream's own keys).  There is no window: with one,
+    streams go over one table whose rows begin with the shared pages, by :func:`paged_attention`.  The rest as there."""
     return _native.ragged_attention("shared_prefix_attention", q, q_starts, softmax_scale, max_q_len, max_kv_len, out, cache=cache, page_table=page_table,
                                     kv_lens=kv_lens, causal=causal, prefix=(prefix_table, prefix_lens, group_starts, max_prefix_len))

@@ -146,8 +146,8 @@ def rotate_by_position(q: torch.Tensor, k: torch.Tensor, positions: torch.Tensor
                        amplitude: float = 1.0, grid: tuple[int, int] | None = None, sections: tuple[int, int, int] | None = None,
                        q_weight: torch.Tensor | None = None, k_weight: torch.Tensor | None = None, eps: float = 1e-6) -> tuple[torch.Tensor, torch.Tensor]:
     """:func:`head_norm_rope` without a table: pair j of row t turns by ``positions[t] * frequencies[j]`` radians (:func:`rotary_frequencies`, float64
-    [rotated / 2]), formed in 64 bits in the launch, so that positions may be any (int64; negative ones turn back, row t's is t without), and
-    cosine and sine are multiplied by ``amplitude``.
+    [rotated / 2]), formed in 64 bits in the launch, so that positions (int64; negative ones turn back, row t's is t without) end with no table: below
+    2^31, with frequencies up to 1, an angle is right to 2^-20 radians.  Cosine and sine are multiplied by ``amplitude``, which is finite in 32 bits.
 
     With ``grid``, (rows, columns) of the tokens of a video frame, position p is frame ``p // (rows * columns)``, row ``p // columns % rows`` and column
     ``p % columns``, each of which turns its share of the pairs: ``sections``, three numbers (:func:`video_frequencies`).
