@@ -106,7 +106,7 @@ def rotate_by_position_paged(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, 
                              sections: tuple[int, int, int] | None = None, q_weight: torch.Tensor | None = None, k_weight: torch.Tensor | None = None,
                              eps: float = 1e-6, out: torch.Tensor | None = None) -> torch.Tensor:
     """:func:`longlive_amd.utils.rope.rotate_by_position` of q and k whose K, with the V beside it, goes to the cache in the same launch, as in
-    :func:`head_norm_rope_paged`.  Returns the rotated q, in ``out`` if given, which may be q itself."""
+    :func:`head_norm_rope_paged`.  Returns the rotated q, in ``out`` if given, which is q itself or memory that nothing else of the call uses."""
     return _native.rotate_by_position(q, k, v, q_weight, k_weight, eps, frequencies, amplitude, positions, interleaved, grid, sections, cache, slots, out)
 
 
@@ -123,7 +123,7 @@ def paged_attention(q: torch.Tensor, cache: dict, page_table: torch.Tensor, kv_l
 
     ``max_q_len`` / ``max_kv_len``: the longest stream's new tokens and keys, if the caller knows them; any value gives the right result,
     true ones a division of the work that fits.  Returns ``out`` [T, H, D]: rows outside every stream are zeros in a new tensor and
-    stay as they were in a given one, which may be q itself."""
+    stay as they were in a given one, which is q itself or memory that nothing else of the call uses."""
     return _native.ragged_attention("paged_attention", q, q_starts, softmax_scale, max_q_len, max_kv_len, out, cache=cache, page_table=page_table,
                                     kv_lens=kv_lens, causal=causal, window=window, sink_tokens=sink_tokens)
 
